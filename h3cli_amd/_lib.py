@@ -156,6 +156,19 @@ _SIGNATURES.update({
     "h3_hip_sha256": (_i, [_p, C.c_size_t, _p]),
     "h3_hip_fp8_pack": (_i, [_p, _p, _p, _p, C.c_size_t]),
     "h3_hip_quant_weight_from_bf16": (_p, [_p, _p, _u32, _u32]),
+    # block-scaled FP8
+    "h3_hip_fp8_block_layout": (_i, [_u32, _u32, _u32] + [C.POINTER(_sz)] * 4),
+    "h3_hip_fp8_block_new": (_p, [_p, _u32, _u32, _u32]),
+    "h3_hip_fp8_block_from_packed": (_p, [_p, _p, _p, _u32, _u32, _u32]),
+    "h3_hip_fp8_block_weight_from_bf16": (_p, [_p, _p, _u32, _u32]),
+    "h3_hip_fp8_block_pack": (_i, [_p, _p, _p, _u32, _u32]),
+    "h3_hip_fp8_block_unpack": (_i, [_p, _p, _p, _u32, _u32]),
+    "h3_hip_linear_fp8_block": (_i, [_p, _p, _p, _p, _p, _u32, _u32, _u32]),
+    "h3_hip_mlp_fp8_block": (_i, [_p, _p, _p, _p, _p, _u32, _u32, _u32, _u32]),
+    "h3_hip_swiglu_fp8_block": (_i, [_p, _p, _p, _u32, _u32]),
+    "h3_hip_adaln_fp8_block": (_i, [_p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _f]),
+    "h3_hip_gate_adaln_fp8_block": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _u32, _f]),
+    "h3_hip_add_rms_norm_fp8_block": (_i, [_p, _p, _p, _p, _p, _p, _u32, _u32, _f]),
     # the rest of the reference surface implemented here (include/h3_gpu_surface.h)
     "h3_gpu_adaln_bf16_offset": (_i, [_p, _p, _p, _sz, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _f]),
     "h3_gpu_rms_norm_bf16": (_i, [_p, _p, _p, _p, _u32, _u32, _f]),

@@ -111,6 +111,8 @@ struct h3_gpu_tensor {
     int quant_mode;
     uint32_t quant_n, quant_k;
     size_t quant_scale, quant_global;
+    // Block-scaled FP8 matrix (fp8_block.h): tile 1 an activation, 128 a weight, 0 neither.
+    uint32_t block_tile, block_rows, block_cols;
     void *quant_dequant;    // NVFP4 resident weight: BF16 code * block scale [quant_n, quant_k]
     // Streaming fences (copy stream fills, compute stream reads).
     hipEvent_t ready, released;
@@ -157,6 +159,7 @@ struct h3_gpu {
     h3_device_buffer gemm_weights;
     h3_device_buffer gemm_partials; // FP32 partial sums of the tiles split over K
     h3_device_buffer mlp_workspace; // h3_gpu_mlp_bf16: activated rows (and the fused product)
+    h3_device_buffer block_workspace; // FP8 block projections: packed BF16 inputs, the MLP's activation
     unsigned cus;                   // compute units of the device
     // What the last projection or attention launched (h3_hip_last_kernel).
     struct { const char *name; unsigned rows, shares; bool converted; } last;

@@ -65,6 +65,7 @@ int h3_require(h3_gpu *g, const h3_gpu_tensor *t, h3_gpu_dtype dtype, size_t ele
     if (!t) return h3_set_error(g, "%s: missing tensor", name);
     if (t->owner != g) return h3_set_error(g, "%s: tensor belongs to another context", name);
     if (t->q8) return h3_set_error(g, "%s: packed q8 weight is not a plain tensor", name);
+    if (t->block_tile) return h3_set_error(g, "%s: packed FP8 block matrix is not a plain tensor", name);
     if (t->dtype != dtype) return h3_set_error(g, "%s: dtype %d, expected %d", name, (int)t->dtype, (int)dtype);
     if (t->elements < elements) return h3_set_error(g, "%s: %zu elements, need %zu", name, t->elements, elements);
     return 1;
@@ -133,6 +134,7 @@ extern "C" void h3_gpu_free(h3_gpu *g) {
     h3_buffer_free(&g->gemm_weights);
     h3_buffer_free(&g->gemm_partials);
     h3_buffer_free(&g->mlp_workspace);
+    h3_buffer_free(&g->block_workspace);
     if (g->compute) hipStreamDestroy(g->compute);
     if (g->copy) hipStreamDestroy(g->copy);
     delete g;

@@ -5,6 +5,7 @@
 // keeps a row (or a head) in registers between its reduction and its output.
 #include "common.h"
 #include "internal.h"
+#include "fp8_block.h"
 #include <cmath>
 
 namespace {
@@ -31,6 +32,7 @@ struct AdaLNArgs {
     const uint32_t *row_map;
     unsigned rows, width, slots, shift_slot, scale_slot, gate_slot;
     float eps;
+    Fp8BlockRows packed;    // output in FP8 blocks instead of out
 };
 
 // One wave (W 1) or one workgroup (W 4) per row. MODE 0: AdaLN. MODE 1 (gate_adaln): the row is first gated (residual + branch * gate,
@@ -38,7 +40,10 @@ struct AdaLNArgs {
 // reference's two-kernel composition does (src/cuda/gpu_cuda.cu:1118-1120).
 // MODE 2: plain RMSNorm y = bf16(x * rsqrt(mean x^2 + eps) * w), no modulation
 // (src/cuda/cuda_kernels.cuh:805-833).
-enum { ADALN = 0, GATE_ADALN = 1, RMS_NORM = 2 };
+// MODE 3: RMSNorm of the row plus the branch, rounded to BF16 and stored like a gated row.
+// PACK: the output goes out in FP8 blocks (fp8_block.h) from its FP32 values, not rounded to
+// BF16 first; 16 neighbouring lanes hold a block, so its scale costs four exchanges.
+enum { ADALN = 0, GATE_ADALN = 1, RMS_NORM = 2, ADD_RMS_NORM = 3 };
 // CH: 16-byte chunks per lane (width <= 512 * W * CH); the row stays in registers
 // as packed BF16 between the reduction and the output pass (exact: the value
 // normalized is the BF16 input, or the BF16-rounded gated row).
@@ -50,16 +55,16 @@ enum { ADALN = 0, GATE_ADALN = 1, RMS_NORM = 2 };
 // (14.5, 14.7 / 21.8, 21.7), where bandwidth bounds both, nor at width 2048, a chunk per
 // lane (729 rows 4.6, 5.0 / 5.8, 5.1).
 constexpr unsigned ADALN_ROWS = 2048, ADALN_WIDTH = 4096;
-template <int MODE, int CH, int W>
+template <int MODE, int CH, int W, bool PACK = false>
 __global__ __launch_bounds__(256) void adaln_kernel(AdaLNArgs a) {
-    constexpr bool GATE = MODE == GATE_ADALN;
+    constexpr bool GATE = MODE == GATE_ADALN, PLAIN = MODE == RMS_NORM || MODE == ADD_RMS_NORM;
     constexpr unsigned STRIDE = 64 * W;
     const unsigned wave = threadIdx.x / 64, lane = threadIdx.x % STRIDE;
     const unsigned row = W == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
     if (row >= a.rows) return;
     const unsigned chunks = a.width / 8;
     const size_t base = (size_t)row * a.width;
-    const size_t mbase = MODE == RMS_NORM ? 0 : (size_t)a.row_map[row] * a.slots * a.width;
+    const size_t mbase = PLAIN ? 0 : (size_t)a.row_map[row] * a.slots * a.width;
     u16x8 raw[CH];
     float sumsq = 0.f;
 #pragma unroll
@@ -80,6 +85,12 @@ __global__ __launch_bounds__(256) void adaln_kernel(AdaLNArgs a) {
                 raw[i][e] = f32_to_bf16(fmaf(bf16_to_f32(br[e]), bf16_to_f32(gr[e]), bf16_to_f32(raw[i][e])));
             *reinterpret_cast<u16x8 *>(a.gated + base + c * 8) = raw[i];
         }
+        if constexpr (MODE == ADD_RMS_NORM) {
+            u16x8 br = *reinterpret_cast<const u16x8 *>(a.branch + base + c * 8);
+#pragma unroll
+            for (int e = 0; e < 8; e++) raw[i][e] = f32_to_bf16(bf16_to_f32(raw[i][e]) + bf16_to_f32(br[e]));
+            *reinterpret_cast<u16x8 *>(a.gated + base + c * 8) = raw[i];
+        }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float v = bf16_to_f32(raw[i][e]);
@@ -92,6 +103,42 @@ __global__ __launch_bounds__(256) void adaln_kernel(AdaLNArgs a) {
         if (threadIdx.x % 64 == 0) part[wave] = sumsq;
         __syncthreads();
         sumsq = part[0] + part[1] + part[2] + part[3];
+    }
+    if constexpr (PACK) {
+        // A Newton step on the reciprocal root: codes flip where a value crosses a midpoint.
+        const float mean = sumsq / (float)a.width + a.eps;
+        float inv = rsqrtf(mean);
+        inv = fmaf(0.5f * inv, fmaf(-mean * inv, inv, 1.f), inv);
+        const unsigned blocks = a.packed.stride / 8;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const unsigned c = lane + STRIDE * i;
+            if (c >= blocks) break;     // the 16 lanes of a block leave together
+            float y[8] = {};
+            unsigned amax = 0;
+            if (c < chunks) {
+                const u16x8 wr = *reinterpret_cast<const u16x8 *>(a.weight + c * 8);
+                u16x8 sh = {}, sc = {};
+                if constexpr (!PLAIN) {
+                    sh = *reinterpret_cast<const u16x8 *>(a.mod + mbase + (size_t)a.shift_slot * a.width + c * 8);
+                    sc = *reinterpret_cast<const u16x8 *>(a.mod + mbase + (size_t)a.scale_slot * a.width + c * 8);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    y[e] = bf16_to_f32(raw[i][e]) * inv * bf16_to_f32(wr[e]);
+                    if constexpr (!PLAIN) y[e] = fmaf(y[e], 1.0f + bf16_to_f32(sc[e]), bf16_to_f32(sh[e]));
+                    amax = max(amax, finite_magnitude(y[e], bad));
+                }
+            }
+            const unsigned scale = fp8_block_scale(lanes_max<16>(amax));
+            const float inverse = fp8_block_inverse(scale);
+            *reinterpret_cast<uint2 *>(a.packed.codes + (size_t)row * a.packed.stride + c * 8) =
+                make_uint2(fp8_block_encode4(y, inverse), fp8_block_encode4(y + 4, inverse));
+            if (c % 16 == 0) a.packed.scales[(size_t)row * a.packed.scale_stride + c / 16] = (uint8_t)scale;
+        }
+        if (bad) *a.packed.fault = 1u;
+        return;
     }
     const float inv = rsqrtf(sumsq / (float)a.width + a.eps);
 #pragma unroll
@@ -117,12 +164,12 @@ __global__ __launch_bounds__(256) void adaln_kernel(AdaLNArgs a) {
 }
 
 // Launch with the smallest chunk count that covers the row.
-template <int MODE>
+template <int MODE, bool PACK = false>
 void launch_adaln(h3_gpu *g, const AdaLNArgs &a) {
     const dim3 block(256);
     if (a.width >= ADALN_WIDTH && a.rows <= ADALN_ROWS) {
         switch ((a.width / 8 + 255) / 256) {
-#define H3_ADALN_CASE(n) case n: hipLaunchKernelGGL((adaln_kernel<MODE, n, 4>), dim3(a.rows), block, 0, g->compute, a); break;
+#define H3_ADALN_CASE(n) case n: hipLaunchKernelGGL((adaln_kernel<MODE, n, 4, PACK>), dim3(a.rows), block, 0, g->compute, a); break;
             H3_ADALN_CASE(2) H3_ADALN_CASE(3) default: H3_ADALN_CASE(4)
 #undef H3_ADALN_CASE
         }
@@ -130,7 +177,7 @@ void launch_adaln(h3_gpu *g, const AdaLNArgs &a) {
     }
     const unsigned per_lane = (a.width / 8 + 63) / 64;
     const dim3 grid((a.rows + 3) / 4);
-#define H3_ADALN_CASE(n) case n: hipLaunchKernelGGL((adaln_kernel<MODE, n, 1>), grid, block, 0, g->compute, a); break;
+#define H3_ADALN_CASE(n) case n: hipLaunchKernelGGL((adaln_kernel<MODE, n, 1, PACK>), grid, block, 0, g->compute, a); break;
     switch (per_lane) {
         H3_ADALN_CASE(1) H3_ADALN_CASE(2) H3_ADALN_CASE(3) H3_ADALN_CASE(4) H3_ADALN_CASE(5) H3_ADALN_CASE(6)
         H3_ADALN_CASE(7) H3_ADALN_CASE(8) H3_ADALN_CASE(9) H3_ADALN_CASE(10) H3_ADALN_CASE(11) H3_ADALN_CASE(12)
@@ -429,6 +476,74 @@ extern "C" int h3_gpu_gate_adaln_bf16(h3_gpu *g, h3_gpu_tensor *gated, h3_gpu_te
                 (const uint32_t *)map->data, rows, width, slots, shift, scale, gate_slot, eps};
     launch_adaln<GATE_ADALN>(g, a);
     return h3_launch_status(g, "gate AdaLN");
+}
+
+// The norms with their result in FP8 blocks, for projections that take it so
+// (h3_hip_linear_fp8_block, h3_hip_mlp_fp8_block).
+static int packed_norm_shape(h3_gpu *g, const h3_gpu_tensor *out, uint32_t rows, uint32_t width, const char *what) {
+    if (!rows || !width || width % 8 || width > 64 * MAX_CHUNKS * 8)
+        return h3_set_error(g, "%s: width must be a multiple of 8 up to 8192", what);
+    return h3_require_fp8_block(g, out, 1, rows, width, what);
+}
+
+extern "C" int h3_hip_adaln_fp8_block(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *w,
+                                      const h3_gpu_tensor *mod, const h3_gpu_tensor *map, uint32_t rows, uint32_t width,
+                                      uint32_t slots, uint32_t shift, uint32_t scale, float eps) {
+    const size_t n = (size_t)rows * width;
+    if (!h3_launch_ready(g)) return 0;
+    if (shift >= slots || scale >= slots) return h3_set_error(g, "FP8 block AdaLN: slots must be valid");
+    if (!packed_norm_shape(g, out, rows, width, "FP8 block AdaLN output") ||
+        !h3_require(g, in, H3_GPU_BF16, n, "AdaLN input") || !h3_require(g, w, H3_GPU_BF16, width, "AdaLN norm") ||
+        !h3_require(g, mod, H3_GPU_BF16, (size_t)slots * width, "AdaLN modulation") || !check_map(g, map, rows, "AdaLN"))
+        return 0;
+    AdaLNArgs a{nullptr, nullptr, (const uint16_t *)in->data, nullptr, (const uint16_t *)w->data,
+                (const uint16_t *)mod->data, nullptr, (const uint32_t *)map->data, rows, width, slots, shift, scale, 0, eps,
+                h3_fp8_block_rows(g, out)};
+    launch_adaln<ADALN, true>(g, a);
+    return h3_launch_status(g, "FP8 block AdaLN");
+}
+
+extern "C" int h3_hip_gate_adaln_fp8_block(h3_gpu *g, h3_gpu_tensor *gated, h3_gpu_tensor *out, const h3_gpu_tensor *res,
+                                           const h3_gpu_tensor *branch, const h3_gpu_tensor *w,
+                                           const h3_gpu_tensor *gate_mod, const h3_gpu_tensor *norm_mod,
+                                           const h3_gpu_tensor *map, uint32_t rows, uint32_t width, uint32_t slots,
+                                           uint32_t gate_slot, uint32_t shift, uint32_t scale, float eps) {
+    const size_t n = (size_t)rows * width;
+    if (!h3_launch_ready(g)) return 0;
+    if (gate_slot >= slots || shift >= slots || scale >= slots)
+        return h3_set_error(g, "FP8 block gate AdaLN: slots must be valid");
+    if (!packed_norm_shape(g, out, rows, width, "FP8 block gate AdaLN output") ||
+        !h3_require(g, res, H3_GPU_BF16, n, "gate residual") || !h3_require(g, branch, H3_GPU_BF16, n, "gate branch") ||
+        !h3_require(g, w, H3_GPU_BF16, width, "AdaLN norm") ||
+        !h3_require(g, gate_mod, H3_GPU_BF16, (size_t)slots * width, "gate modulation") ||
+        !h3_require(g, norm_mod, H3_GPU_BF16, (size_t)slots * width, "AdaLN modulation") ||
+        !check_map(g, map, rows, "gate AdaLN") || !h3_require(g, gated, H3_GPU_BF16, n, "gated residual"))
+        return 0;
+    if (gated == branch) return h3_set_error(g, "gate AdaLN: outputs must not alias the branch or each other");
+    AdaLNArgs a{nullptr, (uint16_t *)gated->data, (const uint16_t *)res->data, (const uint16_t *)branch->data,
+                (const uint16_t *)w->data, (const uint16_t *)norm_mod->data, (const uint16_t *)gate_mod->data,
+                (const uint32_t *)map->data, rows, width, slots, shift, scale, gate_slot, eps, h3_fp8_block_rows(g, out)};
+    launch_adaln<GATE_ADALN, true>(g, a);
+    return h3_launch_status(g, "FP8 block gate AdaLN");
+}
+
+extern "C" int h3_hip_add_rms_norm_fp8_block(h3_gpu *g, h3_gpu_tensor *sum, h3_gpu_tensor *out, const h3_gpu_tensor *res,
+                                             const h3_gpu_tensor *branch, const h3_gpu_tensor *w, uint32_t rows,
+                                             uint32_t width, float eps) {
+    const size_t n = (size_t)rows * width;
+    if (!h3_launch_ready(g)) return 0;
+    if (!sum != !branch) return h3_set_error(g, "FP8 block RMSNorm: a branch and its sum come together");
+    if (!packed_norm_shape(g, out, rows, width, "FP8 block RMSNorm output") ||
+        !h3_require(g, res, H3_GPU_BF16, n, "RMSNorm residual") || !h3_require(g, w, H3_GPU_BF16, width, "RMSNorm weight") ||
+        (branch && (!h3_require(g, branch, H3_GPU_BF16, n, "RMSNorm branch") ||
+                    !h3_require(g, sum, H3_GPU_BF16, n, "RMSNorm sum"))))
+        return 0;
+    AdaLNArgs a{nullptr, branch ? (uint16_t *)sum->data : nullptr, (const uint16_t *)res->data,
+                branch ? (const uint16_t *)branch->data : nullptr, (const uint16_t *)w->data, nullptr, nullptr, nullptr,
+                rows, width, 0, 0, 0, 0, eps, h3_fp8_block_rows(g, out)};
+    if (branch) launch_adaln<ADD_RMS_NORM, true>(g, a);
+    else launch_adaln<RMS_NORM, true>(g, a);
+    return h3_launch_status(g, "FP8 block RMSNorm");
 }
 
 static int qkv_rope(h3_gpu *g, h3_gpu_tensor *q, h3_gpu_tensor *k, h3_gpu_tensor *v, const h3_gpu_tensor *qkv,

@@ -1,0 +1,124 @@
+// Block-scaled FP8: the packed matrix, its encoding on the device, and the projection
+// kernels' arguments (fp8_block.hip, gemm_fp8_block.hip, elementwise.hip).
+//
+// A matrix [rows, columns] is E4M3 codes in rows of `stride` bytes (columns rounded up to
+// 128, the rest zero) and one E8M0 scale byte e + 127, value 2^e, per block of 128: an
+// activation's block (tile 1) is 128 columns of one row, a weight's (tile 128) 128 rows by
+// 128 columns. Scale rows are `scale_stride` bytes, a multiple of 16, so that the
+// scales of 16 blocks come in one load.
+//
+// Why powers of two: E4M3 is a floating-point type, so a scale's mantissa would not make its
+// codes more exact, only extend their range below by less than one binade, while
+// v_mfma_scale takes a power of two per row without a further instruction (an FP32 scale is
+// an FMA per sum and block, half as many VALU cycles as the products take). x / 2^e is exact,
+// so a code has one rounding.
+#pragma once
+#include "common.h"
+#include "gemm.h"
+
+constexpr uint32_t FP8_BLOCK = 128;
+// Least exponent of a scale: blocks below 448 * 2^-64 lose their small values, and products
+// of two scales stay in FP32's range.
+constexpr int FP8_BLOCK_LEAST = -64;
+// 256 rows of codes have 32-bit offsets.
+constexpr uint32_t FP8_BLOCK_COLUMNS = (1u << 24) - FP8_BLOCK;
+
+struct Fp8BlockLayout {
+    size_t stride, scales, scale_stride, bytes;
+};
+inline Fp8BlockLayout fp8_block_layout(uint32_t rows, uint32_t columns, uint32_t tile) {
+    const size_t blocks = (columns + FP8_BLOCK - 1) / FP8_BLOCK;
+    Fp8BlockLayout l;
+    l.stride = blocks * FP8_BLOCK;
+    l.scales = ((size_t)rows * l.stride + 255) & ~(size_t)255;
+    l.scale_stride = (blocks + 15) & ~(size_t)15;
+    l.bytes = l.scales + ((size_t)rows + tile - 1) / tile * l.scale_stride;
+    return l;
+}
+
+// Where a packing kernel writes: row r's codes at codes + r * stride, its scales at
+// scales + r * scale_stride.
+struct Fp8BlockRows {
+    uint8_t *codes, *scales;
+    unsigned stride, scale_stride;
+    unsigned *fault;      // set where a value is not finite
+};
+
+#if defined(__HIPCC__)
+// Magnitude bits of a finite value; a non-finite one counts as zero and sets bad. (The opaque
+// step keeps the compiler, which assumes that no value is NaN, from folding the test.)
+__device__ inline unsigned finite_magnitude(float v, bool &bad) {
+    unsigned u = __builtin_bit_cast(unsigned, v);
+    asm("" : "+v"(u));
+    u &= 0x7fffffffu;
+    const bool wrong = u >= 0x7f800000u;
+    bad |= wrong;
+    return wrong ? 0u : u;
+}
+// Scale byte of a block whose largest magnitude has these bits: the least e >= -64 with
+// amax <= 448 * 2^e. 448 = 1.75 * 2^8, so e = exponent - 8, one more if the mantissa is
+// above 1.75.
+__device__ inline unsigned fp8_block_scale(unsigned amax) {
+    const int e = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return (unsigned)max(e, FP8_BLOCK_LEAST + 127);
+}
+// 2^-e of a scale byte (63 to 247), for the encoding.
+__device__ inline float fp8_block_inverse(unsigned scale) { return __builtin_bit_cast(float, (254u - scale) << 23); }
+// Four codes of v * inverse: round to nearest even; |v * inverse| <= 448.
+__device__ inline unsigned fp8_block_encode4(const float *v, float inverse) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inverse, v[1] * inverse, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inverse, v[3] * inverse, w, true);
+}
+// Largest of `lanes` neighbouring lanes (a power of two up to 64).
+template <int LANES> __device__ inline unsigned lanes_max(unsigned v) {
+#pragma unroll
+    for (int off = LANES / 2; off >= 1; off >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, off, 64));
+    return v;
+}
+// silu(gate) * up = gate / (1 + exp(-gate)) * up in FP32, each step within about a unit in
+// the last place, because a code flips where the value crosses a midpoint: exp(-gate) as 2^hi
+// (1 + lo ln 2) with the product's rounding error in lo, and the reciprocal with a Newton
+// step, on (1 + exp) / 16, whose reciprocal is normal up to exp's overflow, where the result
+// is zero.
+__device__ inline float swiglu_exact(float gate, float up) {
+    constexpr float L = 1.4426950408889634f, L_LOW = 1.9259629911266175e-8f, LN2 = 0.6931471805599453f;
+    const float x = __builtin_amdgcn_fmed3f(gate, -128.f, 128.f);      // exp(-x) is 0 beside 1, or infinite, outside
+    const float hi = -x * L, lo = -fmaf(x, L, hi) - x * L_LOW;
+    float e = __builtin_amdgcn_exp2f(hi);
+    e = e < 3e38f ? fmaf(e, lo * LN2, e) : 3e38f;
+    const float d = fmaf(e, 0.0625f, 0.0625f);
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.f), r, r);
+    r = e < 3e38f ? r : 0.f;
+    return gate * 0.0625f * r * up;
+}
+#endif
+
+// y = bf16(x . w^T + bias) and its variants (h3_gemm_fp8_block).
+struct Fp8BlockGemmArgs {
+    uint16_t *y;                // [m, n], or
+    float *y32;                 // the sums as they are [m, n], or, with swiglu,
+    Fp8BlockRows out;           // silu(gate) * up packed [m, n / 2]: w holds gate rows, then up rows
+    const uint16_t *bias;       // [n], y only
+    const uint8_t *x, *w;       // codes, rows of k bytes (a multiple of 128)
+    const uint8_t *xs, *ws;     // scales, rows of scale_stride bytes; w's one per 128 rows
+    unsigned m, n, k, scale_stride;
+    bool swiglu;                // n / 2 a multiple of 128
+    TileSplit tile;             // set by the kernels' launchers
+};
+int h3_gemm_fp8_block(h3_gpu *g, const Fp8BlockGemmArgs &a);
+// Whether the SwiGLU variant is faster as one launch than as y32 and h3_launch_swiglu_fp8_block.
+bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m);
+// Packs silu(gate) * up of FP32 or BF16 rows [rows, 2 * width].
+int h3_launch_swiglu_fp8_block(h3_gpu *g, Fp8BlockRows out, const void *fused, bool f32, uint32_t rows, uint32_t width);
+
+// Entry-point helpers (fp8_block.hip): whether t is a packed matrix of this context with this
+// tile, at least `rows` rows (tile 1; a weight: exactly) and `columns` columns, else the error.
+int h3_require_fp8_block(h3_gpu *g, const h3_gpu_tensor *t, uint32_t tile, uint32_t rows, uint32_t columns,
+                         const char *name);
+Fp8BlockRows h3_fp8_block_rows(h3_gpu *g, const h3_gpu_tensor *t);
+// A projection whose weight is packed in blocks and its input BF16 (packed here) or packed.
+int h3_fp8_block_linear(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *w,
+                        const h3_gpu_tensor *bias, uint32_t rows, uint32_t k, uint32_t n);
+int h3_fp8_block_mlp(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *w1,
+                     const h3_gpu_tensor *w2, uint32_t rows, uint32_t k, uint32_t hidden, uint32_t n);

@@ -3,6 +3,7 @@
 #include "common.h"
 #include "internal.h"
 #include "gemm.h"
+#include "fp8_block.h"
 #include <algorithm>
 #include <cerrno>
 #include <cmath>
@@ -17,6 +18,11 @@ static int linear(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const 
     if (!h3_launch_ready(g)) return 0;
     if (!rows || !k || !n || !w || w->owner != g)
         return h3_set_error(g, "linear %ux%ux%u: invalid shape or weight", rows, n, k);
+    if (w->block_tile) {
+        if (activation) return h3_set_error(g, "linear: FP8 block weights take no activation");
+        if (in && in->block_tile) return h3_set_error(g, "linear input: packed FP8 block matrix (h3_hip_linear_fp8_block)");
+        return h3_fp8_block_linear(g, out, in, w, bias, rows, k, n);
+    }
     if (!h3_require(g, in, H3_GPU_BF16, (size_t)rows * k, "linear input") ||
         !h3_require(g, out, H3_GPU_BF16, (size_t)rows * (activation == H3_GEMM_SWIGLU ? n / 2 : n), "linear output") ||
         (bias && !h3_require(g, bias, H3_GPU_BF16, n, "linear bias")))
@@ -89,6 +95,10 @@ static MlpPart mlp_part(const h3_gpu_tensor *w1, size_t rows, uint32_t width, ui
 extern "C" int h3_gpu_mlp_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *w1,
                                const h3_gpu_tensor *w2, uint32_t rows, uint32_t width, uint32_t hidden, uint32_t output_dim) {
     if (!g) return 0;
+    if (w1 && w1->block_tile) {
+        if (in && in->block_tile) return h3_set_error(g, "MLP input: packed FP8 block matrix (h3_hip_mlp_fp8_block)");
+        return h3_fp8_block_mlp(g, out, in, w1, w2, rows, width, hidden, output_dim);
+    }
     // Its intermediates cannot be allocated for a graph, nor may a graph keep the workspace.
     if (h3_capturing(g)) return h3_set_error(g, "MLP: the compute stream is being captured");
     if (!rows || !hidden || hidden > UINT32_MAX / 2 ||

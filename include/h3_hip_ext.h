@@ -152,6 +152,76 @@ int h3_hip_fp8_pack(h3_gpu *gpu, const h3_gpu_tensor *x, h3_gpu_tensor *codes, h
  * h3_gpu_quant_configure(mode 1 or 2); n, k multiples of 128. */
 h3_gpu_tensor *h3_hip_quant_weight_from_bf16(h3_gpu *gpu, const h3_gpu_tensor *w, uint32_t n, uint32_t k);
 
+/* ---- block-scaled FP8 ---------------------------------------------------
+ * A packed matrix [rows, columns]: E4M3 codes with one power-of-two scale for
+ * each block of 128. tile 1, an activation: a block is 128 columns of one row;
+ * tile 128, a weight [output, input]: 128 rows by 128 columns. The last blocks
+ * may be cut off; any shape up to 2^24 - 128 columns will do. A block's scale
+ * is 2^e with the least e >= -64 for which max|x| <= 448 * 2^e, held as the
+ * byte e + 127 (E8M0); a code is x / 2^e rounded to nearest even, so it is as
+ * exact as E4M3 gets, and BF16 holds it (but for values that round to 2^128,
+ * from 1.9375 * 2^127 on: infinity when unpacked). A value that is not finite
+ * fails the next submit, like one in an FP8 projection's input. The packed
+ * type is a tensor of its own: the operators below take it, others refuse it.
+ * Work with rows <= the tensor's rows leaves the rows behind as they were.
+ *
+ * h3_hip_fp8_block_layout: where a matrix has its parts, in bytes: codes of
+ * row r from r * stride on (zeros behind `columns`), scales of row r (tile 1)
+ * or of rows 128 r to 128 r + 127 from scales + r * scale_stride on; bytes in
+ * all. h3_hip_tensor_copy_to_host, h3_hip_tensor_stream_host and
+ * h3_hip_tensor_device_pointer give that memory. 0 on an invalid shape. */
+int h3_hip_fp8_block_layout(uint32_t rows, uint32_t columns, uint32_t tile, size_t *stride,
+                            size_t *scales, size_t *scale_stride, size_t *bytes);
+/* A matrix of zeros. */
+h3_gpu_tensor *h3_hip_fp8_block_new(h3_gpu *gpu, uint32_t rows, uint32_t columns, uint32_t tile);
+/* From host memory: codes [rows, columns], scales [ceil(rows / tile)]
+ * [ceil(columns / 128)], both dense; codes and scales that are not numbers
+ * (0x7f, 0xff; 0xff) are refused. */
+h3_gpu_tensor *h3_hip_fp8_block_from_packed(h3_gpu *gpu, const uint8_t *codes, const uint8_t *scales,
+                                            uint32_t rows, uint32_t columns, uint32_t tile);
+/* A weight from rows x columns BF16 device values. Waits for the stream. */
+h3_gpu_tensor *h3_hip_fp8_block_weight_from_bf16(h3_gpu *gpu, const h3_gpu_tensor *w, uint32_t rows,
+                                                 uint32_t columns);
+/* BF16 rows into an activation, and the BF16 values of a packed matrix (an
+ * activation's first rows, or a whole weight). */
+int h3_hip_fp8_block_pack(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                          uint32_t rows, uint32_t columns);
+int h3_hip_fp8_block_unpack(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                            uint32_t rows, uint32_t columns);
+/* y[rows, output_dim] = bf16(x . W^T (+ bias)), x an activation and W a weight,
+ * FP32 sums. h3_gpu_linear_bf16 takes such a weight too and packs its BF16
+ * input per call, in a workspace of the context (refused under capture). */
+int h3_hip_linear_fp8_block(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                            const h3_gpu_tensor *weight, const h3_gpu_tensor *bias,
+                            uint32_t rows, uint32_t input_dim, uint32_t output_dim);
+/* h3_gpu_mlp_bf16 with weights in FP8 blocks: fc1 -> silu(gate) * up, packed
+ * from FP32 -> fc2. hidden_dim a multiple of 128. h3_gpu_mlp_bf16 takes such
+ * weights too, with a BF16 input. Both refuse under capture. */
+int h3_hip_mlp_fp8_block(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                         const h3_gpu_tensor *fc1_weight, const h3_gpu_tensor *fc2_weight,
+                         uint32_t rows, uint32_t input_dim, uint32_t hidden_dim, uint32_t output_dim);
+/* h3_gpu_swiglu_bf16, h3_gpu_adaln_bf16, h3_gpu_gate_adaln_bf16 and
+ * h3_gpu_rms_norm_bf16 with an activation for their (normalized) output,
+ * packed from the FP32 values. */
+int h3_hip_swiglu_fp8_block(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                            uint32_t rows, uint32_t width);
+int h3_hip_adaln_fp8_block(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                           const h3_gpu_tensor *norm_weight, const h3_gpu_tensor *modulation,
+                           const h3_gpu_tensor *row_map, uint32_t rows, uint32_t width,
+                           uint32_t slots, uint32_t shift_slot, uint32_t scale_slot, float epsilon);
+int h3_hip_gate_adaln_fp8_block(h3_gpu *gpu, h3_gpu_tensor *gated_residual, h3_gpu_tensor *output,
+                                const h3_gpu_tensor *residual, const h3_gpu_tensor *branch,
+                                const h3_gpu_tensor *norm_weight, const h3_gpu_tensor *gate_modulation,
+                                const h3_gpu_tensor *norm_modulation, const h3_gpu_tensor *row_map,
+                                uint32_t rows, uint32_t width, uint32_t slots, uint32_t gate_slot,
+                                uint32_t shift_slot, uint32_t scale_slot, float epsilon);
+/* sum = bf16(residual + branch) and its RMSNorm; sum may be the residual or
+ * the branch. Without a branch and a sum (both NULL) the residual's. */
+int h3_hip_add_rms_norm_fp8_block(h3_gpu *gpu, h3_gpu_tensor *sum, h3_gpu_tensor *output,
+                                  const h3_gpu_tensor *residual, const h3_gpu_tensor *branch,
+                                  const h3_gpu_tensor *norm_weight, uint32_t rows, uint32_t width,
+                                  float epsilon);
+
 /* Sage quantization of sequence-major BF16 Q, K, V [seq, heads, 128] into the
  * layouts the quantized attention kernel consumes (all head-major, rows padded
  * to a multiple of 64, padded rows zero):
