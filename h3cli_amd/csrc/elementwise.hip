@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void adaln_kernel(AdaLNArgs a) {
             const float inverse = fp8_block_inverse(scale);
             *reinterpret_cast<uint2 *>(a.packed.codes + (size_t)row * a.packed.stride + c * 8) =
                 make_uint2(fp8_block_encode4(y, inverse), fp8_block_encode4(y + 4, inverse));
-            if (c % 16 == 0) a.packed.scales[(size_t)row * a.packed.scale_stride + c / 16] = (uint8_t)scale;
+            if (c % 16 == 0) a.packed.scales[fp8_block_scale_at(row, c / 16, a.packed.groups)] = (uint8_t)scale;
         }
         if (bad) *a.packed.fault = 1u;
         return;

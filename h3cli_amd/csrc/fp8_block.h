@@ -4,8 +4,11 @@
 // A matrix [rows, columns] is E4M3 codes in rows of `stride` bytes (columns rounded up to
 // 128, the rest zero) and one E8M0 scale byte e + 127, value 2^e, per block of 128: an
 // activation's block (tile 1) is 128 columns of one row, a weight's (tile 128) 128 rows by
-// 128 columns. Scale rows are `scale_stride` bytes, a multiple of 16, so that the
-// scales of 16 blocks come in one load.
+// 128 columns. Scales lie as the products read them, lanes being rows: 32 scale rows by four
+// blocks are 128 bytes, a dword of four blocks for each row; the `groups` fours of a row
+// follow each other, then come the next 32 rows. (As rows of bytes, each lane's dword is in a
+// cache line of its own: a quarter more traffic from L2 than the codes', and 2.5% of the time
+// of a projection of 18225 rows, 5376 -> 28672.)
 //
 // Why powers of two: E4M3 is a floating-point type, so a scale's mantissa would not make its
 // codes more exact, only extend their range below by less than one binade, while
@@ -24,23 +27,27 @@ constexpr int FP8_BLOCK_LEAST = -64;
 constexpr uint32_t FP8_BLOCK_COLUMNS = (1u << 24) - FP8_BLOCK;
 
 struct Fp8BlockLayout {
-    size_t stride, scales, scale_stride, bytes;
+    size_t stride, scales, groups, bytes;
 };
 inline Fp8BlockLayout fp8_block_layout(uint32_t rows, uint32_t columns, uint32_t tile) {
     const size_t blocks = (columns + FP8_BLOCK - 1) / FP8_BLOCK;
     Fp8BlockLayout l;
     l.stride = blocks * FP8_BLOCK;
     l.scales = ((size_t)rows * l.stride + 255) & ~(size_t)255;
-    l.scale_stride = (blocks + 15) & ~(size_t)15;
-    l.bytes = l.scales + ((size_t)rows + tile - 1) / tile * l.scale_stride;
+    l.groups = (blocks + 3) / 4;
+    l.bytes = l.scales + (((size_t)rows + tile - 1) / tile + 31) / 32 * l.groups * 128;
     return l;
 }
 
-// Where a packing kernel writes: row r's codes at codes + r * stride, its scales at
-// scales + r * scale_stride.
+// Byte of (scale row, block).
+__host__ __device__ inline size_t fp8_block_scale_at(unsigned row, unsigned block, unsigned groups) {
+    return ((size_t)(row / 32) * groups + block / 4) * 128 + row % 32 * 4 + block % 4;
+}
+
+// Where a packing kernel writes: row r's codes at codes + r * stride.
 struct Fp8BlockRows {
     uint8_t *codes, *scales;
-    unsigned stride, scale_stride;
+    unsigned stride, groups;
     unsigned *fault;      // set where a value is not finite
 };
 
@@ -101,14 +108,14 @@ struct Fp8BlockGemmArgs {
     Fp8BlockRows out;           // silu(gate) * up packed [m, n / 2]: w holds gate rows, then up rows
     const uint16_t *bias;       // [n], y only
     const uint8_t *x, *w;       // codes, rows of k bytes (a multiple of 128)
-    const uint8_t *xs, *ws;     // scales, rows of scale_stride bytes; w's one per 128 rows
-    unsigned m, n, k, scale_stride;
+    const uint8_t *xs, *ws;     // scales; a scale row of w per 128 rows
+    unsigned m, n, k, groups;
     bool swiglu;                // n / 2 a multiple of 128
     TileSplit tile;             // set by the kernels' launchers
 };
 int h3_gemm_fp8_block(h3_gpu *g, const Fp8BlockGemmArgs &a);
 // Whether the SwiGLU variant is faster as one launch than as y32 and h3_launch_swiglu_fp8_block.
-bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m);
+bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m, uint32_t k, uint32_t hidden);
 // Packs silu(gate) * up of FP32 or BF16 rows [rows, 2 * width].
 int h3_launch_swiglu_fp8_block(h3_gpu *g, Fp8BlockRows out, const void *fused, bool f32, uint32_t rows, uint32_t width);
 

@@ -9,7 +9,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <vector>
+#include <memory>
+#include <new>
 
 namespace {
 
@@ -82,7 +83,7 @@ __global__ __launch_bounds__(256) void fp8_block_pack(const T *in, Fp8BlockRows 
     const unsigned scale = fp8_block_scale(lanes_max<LANES>(magnitude16(v, bad)));
     if (bad) *out.fault = 1u;
     *reinterpret_cast<u32x4 *>(out.codes + (size_t)row * out.stride + col) = encode16(v, scale);
-    if (id % LANES == 0) out.scales[(size_t)row * out.scale_stride + block] = (uint8_t)scale;
+    if (id % LANES == 0) out.scales[fp8_block_scale_at(row, block, out.groups)] = (uint8_t)scale;
 }
 
 // A weight's blocks of 128 x 128: a workgroup each, 32 rows at a time and eight lanes a row,
@@ -109,13 +110,13 @@ __global__ __launch_bounds__(256) void fp8_block_pack_weight(const uint16_t *in,
         load16<VEC>(in + (size_t)(r0 + at) * columns, col, columns, v);
         *reinterpret_cast<u32x4 *>(out.codes + (size_t)(r0 + at) * out.stride + col) = encode16(v, scale);
     }
-    if (threadIdx.x == 0) out.scales[(size_t)(r0 / FP8_BLOCK) * out.scale_stride + block] = (uint8_t)scale;
+    if (threadIdx.x == 0) out.scales[fp8_block_scale_at(r0 / FP8_BLOCK, block, out.groups)] = (uint8_t)scale;
 }
 
 // BF16 values code * 2^e, exact but for values below BF16's range. 16 values per lane.
 template <bool VEC>
 __global__ __launch_bounds__(256) void fp8_block_unpack(const uint8_t *codes, const uint8_t *scales, unsigned stride,
-                                                        unsigned scale_stride, unsigned tile, uint16_t *out,
+                                                        unsigned groups, unsigned tile, uint16_t *out,
                                                         unsigned rows, unsigned columns) {
     const unsigned lanes = stride / LANE;
     const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(256) void fp8_block_unpack(const uint8_t *codes, co
     if (col >= columns) return;
     const u32x4 q = *reinterpret_cast<const u32x4 *>(codes + (size_t)row * stride + col);
     // The two halves of the power of two: their product with a code has one rounding.
-    const int e = (int)scales[(size_t)(row / tile) * scale_stride + col / FP8_BLOCK] - 127;
+    const int e = (int)scales[fp8_block_scale_at(row / tile, col / FP8_BLOCK, groups)] - 127;
     uint16_t v[LANE];
 #pragma unroll
     for (int w = 0; w < 4; w++)
@@ -185,7 +186,7 @@ Fp8BlockLayout layout_of(const h3_gpu_tensor *t) { return fp8_block_layout(t->bl
 // Rows of a packed activation over workspace memory (bytes as fp8_block_layout says).
 Fp8BlockRows workspace_rows(h3_gpu *g, void *data, uint32_t rows, uint32_t columns) {
     const Fp8BlockLayout l = fp8_block_layout(rows, columns, 1);
-    return {(uint8_t *)data, (uint8_t *)data + l.scales, (unsigned)l.stride, (unsigned)l.scale_stride, g->fault + 2};
+    return {(uint8_t *)data, (uint8_t *)data + l.scales, (unsigned)l.stride, (unsigned)l.groups, g->fault + 2};
 }
 
 Fp8BlockGemmArgs gemm_args(const Fp8BlockRows &x, const h3_gpu_tensor *w, uint32_t rows, uint32_t n) {
@@ -193,7 +194,7 @@ Fp8BlockGemmArgs gemm_args(const Fp8BlockRows &x, const h3_gpu_tensor *w, uint32
     Fp8BlockGemmArgs a{};
     a.x = x.codes; a.xs = x.scales;
     a.w = (const uint8_t *)w->data; a.ws = (const uint8_t *)w->data + lw.scales;
-    a.m = rows; a.n = n; a.k = (unsigned)lw.stride; a.scale_stride = (unsigned)lw.scale_stride;
+    a.m = rows; a.n = n; a.k = (unsigned)lw.stride; a.groups = (unsigned)lw.groups;
     return a;
 }
 
@@ -221,7 +222,7 @@ int h3_require_fp8_block(h3_gpu *g, const h3_gpu_tensor *t, uint32_t tile, uint3
 
 Fp8BlockRows h3_fp8_block_rows(h3_gpu *g, const h3_gpu_tensor *t) {
     const Fp8BlockLayout l = layout_of(t);
-    return {(uint8_t *)t->data, (uint8_t *)t->data + l.scales, (unsigned)l.stride, (unsigned)l.scale_stride, g->fault + 2};
+    return {(uint8_t *)t->data, (uint8_t *)t->data + l.scales, (unsigned)l.stride, (unsigned)l.groups, g->fault + 2};
 }
 
 int h3_launch_swiglu_fp8_block(h3_gpu *g, Fp8BlockRows out, const void *fused, bool f32, uint32_t rows, uint32_t width) {
@@ -231,12 +232,12 @@ int h3_launch_swiglu_fp8_block(h3_gpu *g, Fp8BlockRows out, const void *fused, b
 
 // ------------------------------------------------------------------ tensors
 extern "C" int h3_hip_fp8_block_layout(uint32_t rows, uint32_t columns, uint32_t tile, size_t *stride, size_t *scales,
-                                       size_t *scale_stride, size_t *bytes) {
+                                       size_t *groups, size_t *bytes) {
     if (!valid_shape(rows, columns, tile)) return 0;
     const Fp8BlockLayout l = fp8_block_layout(rows, columns, tile);
     if (stride) *stride = l.stride;
     if (scales) *scales = l.scales;
-    if (scale_stride) *scale_stride = l.scale_stride;
+    if (groups) *groups = l.groups;
     if (bytes) *bytes = l.bytes;
     return 1;
 }
@@ -280,10 +281,15 @@ extern "C" h3_gpu_tensor *h3_hip_fp8_block_from_packed(h3_gpu *g, const uint8_t 
         h3_gpu_tensor *t = h3_hip_fp8_block_new(g, rows, columns, tile);
         if (!t) return nullptr;
         const Fp8BlockLayout l = fp8_block_layout(rows, columns, tile);
+        std::unique_ptr<uint8_t[]> placed(new (std::nothrow) uint8_t[l.bytes - l.scales]());
+        if (!placed) { h3_gpu_tensor_free(t); h3_set_error(g, "FP8 block matrix: out of host memory"); return nullptr; }
+        for (uint32_t r = 0; r < scale_rows; r++)
+            for (uint32_t b = 0; b < blocks; b++)
+                placed[fp8_block_scale_at(r, b, (unsigned)l.groups)] = scales[r * blocks + b];
         if (!h3_hip_check(g, hipMemcpy2D(t->data, l.stride, codes, columns, columns, rows, hipMemcpyHostToDevice),
                           "FP8 block codes upload") ||
-            !h3_hip_check(g, hipMemcpy2D((char *)t->data + l.scales, l.scale_stride, scales, blocks, blocks, scale_rows,
-                                         hipMemcpyHostToDevice), "FP8 block scales upload")) {
+            !h3_hip_check(g, hipMemcpy((char *)t->data + l.scales, placed.get(), l.bytes - l.scales, hipMemcpyHostToDevice),
+                          "FP8 block scales upload")) {
             h3_gpu_tensor_free(t);
             return nullptr;
         }
@@ -338,7 +344,7 @@ extern "C" int h3_hip_fp8_block_unpack(h3_gpu *g, h3_gpu_tensor *out, const h3_g
     auto kernel = columns % 8 == 0 ? fp8_block_unpack<true> : fp8_block_unpack<false>;
     if (!h3_tensor_acquire(g, in)) return 0;
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, g->compute, (const uint8_t *)in->data,
-                       (const uint8_t *)in->data + l.scales, (unsigned)l.stride, (unsigned)l.scale_stride, in->block_tile,
+                       (const uint8_t *)in->data + l.scales, (unsigned)l.stride, (unsigned)l.groups, in->block_tile,
                        (uint16_t *)out->data, rows, columns);
     return h3_launch_status(g, "FP8 block unpacking") && h3_tensor_release(g, in);
 }
@@ -406,7 +412,7 @@ int h3_fp8_block_mlp(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, con
         return 0;
     // The packed activation, and the FP32 product where SwiGLU is not its projection's epilogue.
     // The context keeps no more than MLP_WORKSPACE for them: calls of more rows run in parts.
-    const bool fused = h3_gemm_fp8_block_fuses(g, rows);
+    const bool fused = h3_gemm_fp8_block_fuses(g, rows, k, hidden);
     const size_t row_bytes = fp8_block_layout(1, hidden, 1).bytes + (fused ? 0 : (size_t)hidden * 8);
     const uint32_t most = (uint32_t)std::min<size_t>(std::max<size_t>(MLP_WORKSPACE / row_bytes / 256, 1) * 256, rows);
     const size_t act = (fp8_block_layout(most, hidden, 1).bytes + 511) & ~(size_t)255;
@@ -415,8 +421,9 @@ int h3_fp8_block_mlp(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, con
     if (!packed_input(g, in, rows, k, act + (fused ? 0 : (size_t)most * hidden * 8), "MLP input", &x, &rest)) return 0;
     for (uint32_t first = 0; first < rows; first += most) {
         const uint32_t m = std::min(most, rows - first);
-        const Fp8BlockRows part = {x.codes + (size_t)first * x.stride, x.scales + (size_t)first * x.scale_stride, x.stride,
-                                   x.scale_stride, x.fault};
+        // first is a multiple of 256: whole runs of 32 scale rows.
+        const Fp8BlockRows part = {x.codes + (size_t)first * x.stride, x.scales + fp8_block_scale_at(first, 0, x.groups),
+                                   x.stride, x.groups, x.fault};
         const Fp8BlockRows h = workspace_rows(g, rest, m, hidden);
         Fp8BlockGemmArgs a = gemm_args(part, w1, m, 2 * hidden);
         a.swiglu = fused;

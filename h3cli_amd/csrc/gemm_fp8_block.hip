@@ -26,30 +26,53 @@ __device__ inline __amdgpu_buffer_rsrc_t uniform_resource(const void *p, unsigne
                                              (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
+// Epilogues: BF16 rows of a multiple of eight columns, without and with a bias; SwiGLU, packed;
+// and any columns, BF16 (with or without a bias) or the FP32 sums. Kernels are instantiated
+// for each: the epilogue is straight-line code that runs once per tile, and one that branches
+// between them is 100 KB of it for 256 x 256 tiles (18225 rows, 5376 -> 28672: 1.3% slower).
+enum { EPI_PLAIN = 0, EPI_BIAS = 1, EPI_SWIGLU = 2, EPI_ANY = 3 };
+int epilogue_of(const Fp8BlockGemmArgs &a) {
+    return a.swiglu ? EPI_SWIGLU : a.y32 || a.n % 8 ? EPI_ANY : a.bias ? EPI_BIAS : EPI_PLAIN;
+}
+
+// Four values wherever they lie: global loads and stores need no alignment.
+struct __attribute__((packed, aligned(2))) u16x4_any { uint16_t v[4]; };
+struct __attribute__((packed, aligned(2))) u16x2_any { uint16_t v[2]; };
+
 // Four columns of an output row.
+template <int EPI>
 __device__ inline void store4(const Fp8BlockGemmArgs &a, unsigned row, unsigned col, f32x4 v) {
     if (row >= a.m || col >= a.n) return;
     const size_t at = (size_t)row * a.n + col;
-    const bool whole = a.n % 4 == 0;
-    if (a.y32) {
-        if (whole) *reinterpret_cast<f32x4 *>(a.y32 + at) = v;
-        else
+    if constexpr (EPI == EPI_ANY) {
+        if (a.y32) {       // the MLP's: a multiple of four columns
+            *reinterpret_cast<f32x4 *>(a.y32 + at) = v;
+            return;
+        }
+        const bool whole = col + 4 <= a.n;
+        u16x4_any b = {};
+        if (a.bias) {
+            if (whole) b = *reinterpret_cast<const u16x4_any *>(a.bias + col);
+            else
+                for (unsigned e = 0; col + e < a.n; e++) b.v[e] = a.bias[col + e];
+        }
+        u16x4_any o;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (col + e < a.n) a.y32[at + e] = v[e];
+        for (int e = 0; e < 4; e++) o.v[e] = f32_to_bf16(v[e] + bf16_to_f32(b.v[e]));
+        if (whole) *reinterpret_cast<u16x4_any *>(a.y + at) = o;
+        else
+            for (unsigned e = 0; col + e < a.n; e++) a.y[at + e] = o.v[e];
         return;
     }
-    if (a.bias)
+    if constexpr (EPI == EPI_BIAS) {
+        const u16x4 b = *reinterpret_cast<const u16x4 *>(a.bias + col);
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] += bf16_to_f32(a.bias[min(col + e, a.n - 1)]);
+        for (int e = 0; e < 4; e++) v[e] += bf16_to_f32(b[e]);
+    }
     u16x4 o;
 #pragma unroll
     for (int e = 0; e < 4; e++) o[e] = f32_to_bf16(v[e]);
-    if (whole) *reinterpret_cast<u16x4 *>(a.y + at) = o;
-    else
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (col + e < a.n) a.y[at + e] = o[e];
+    *reinterpret_cast<u16x4 *>(a.y + at) = o;
 }
 
 // Row of W that row r of a tile holds, counted from the tile's first row. SwiGLU: 32 gate
@@ -57,31 +80,156 @@ __device__ inline void store4(const Fp8BlockGemmArgs &a, unsigned row, unsigned 
 // hold both; a tile then makes 128 columns, one block of the packed result.
 __device__ inline unsigned swiglu_row(unsigned r) { return r / 64 * 32 + r % 32; }
 
-template <int WAVES> struct RowMax { unsigned value[WAVES][64]; };
+// ---------------------------------------------------------------- few rows
+// Reading W once is all the work there is, so the split is made for memory: a workgroup takes
+// 16 NB columns of 16 RB rows (rows: one workgroup's wherever W is large), and its waves take
+// the K steps in turn, so that together they read consecutive bytes of every weight row,
+// straight into registers; their sums meet in LDS, added in wave order. x and the scales come
+// from L2, which all workgroups share, as the operands of v_mfma_scale_f32_16x16x128_f8f6f4.
+//
+// HBM-bound: 1 row, 5376 -> 32256 (173 MB): 32 us, 5.4 TB/s, 4 us of them a launch's; 16 rows
+// 36, as x's reads weigh more. One row of the tile kernels: 37.
+template <int RB, int NB, int WAVES> constexpr int stream_lds() { return WAVES * NB * RB * 64 * 16; }
 
-// ---------------------------------------------------------------- tiles of 128 rows
-// Eight waves of 64 x 64 outputs (C^T = W . X^T), operands from memory to LDS without
-// registers, three stages of 128 bytes of K. The scales of 32 steps come to LDS together.
-constexpr int MID_M = 128, MID_N = 256, MID_T = 512, MID_STAGES = 3;
-constexpr unsigned MID_X = MID_M * TK, MID_W = MID_N * TK, MID_STAGE = MID_X + MID_W;
+template <int EPI, int RB, int NB, int WAVES, int U>
+__global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs a, unsigned groups) {
+    static_assert(U == 2 || U == 3, "steps of a call");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+    const unsigned r = lane % 16, q = lane / 16, pid = xcd_remap(blockIdx.x, gridDim.x);
+    const unsigned n0 = pid / groups * 16 * NB, m0 = pid % groups * 16 * RB, steps = a.k / TK;
+    // Rows past M and columns past N repeat the last one; not stored. An operand's 32 bytes of a
+    // step are two 16-byte pieces that lie beside those of the row's other lanes (which K value
+    // of the step a byte is does not matter where W and x agree).
+    const uint8_t *xp[RB], *wp[NB], *xsp[RB];
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+        const unsigned row = min(m0 + i * 16 + r, a.m - 1);
+        xp[i] = a.x + (size_t)row * a.k + 16 * q;
+        xsp[i] = a.xs + fp8_block_scale_at(row, 0, a.groups);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++) wp[i] = a.w + (size_t)min(n0 + i * 16 + r, a.n - 1) * a.k + 16 * q;
+    const uint8_t *wsp = a.ws + fp8_block_scale_at(n0 / FP8_BLOCK, 0, a.groups);
+    f32x4 acc[NB][RB];
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < RB; j++) acc[i][j] = f32x4{};
+
+    auto run = [&](unsigned s, auto count) {
+        constexpr int C = decltype(count)::value;
+        u32x4 w[C][NB][2], x[C][RB][2];
+        int ws[C], xs[C][RB];
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const unsigned step = s + c * WAVES, at = step / 4 * 128 + step % 4;
+            const size_t k = (size_t)step * TK;
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) w[c][i][h] = *reinterpret_cast<const u32x4 *>(wp[i] + k + 64 * h);
+            ws[c] = wsp[at];
+#pragma unroll
+            for (int j = 0; j < RB; j++) {
+                xs[c][j] = xsp[j][at];
+#pragma unroll
+                for (int h = 0; h < 2; h++) x[c][j][h] = *reinterpret_cast<const u32x4 *>(xp[j] + k + 64 * h);
+            }
+        }
+        auto whole = [](const u32x4 *v) {
+            return i32x8{(int)v[0][0], (int)v[0][1], (int)v[0][2], (int)v[0][3], (int)v[1][0], (int)v[1][1], (int)v[1][2], (int)v[1][3]};
+        };
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int j = 0; j < RB; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(whole(w[c][i]), whole(x[c][j]), acc[i][j], 0, 0,
+                                                                                 0, ws[c], 0, xs[c][j]);
+    };
+    unsigned s = wave;
+    for (; s + (U - 1) * WAVES < steps; s += U * WAVES) run(s, std::integral_constant<int, U>{});
+    // The rest in one go too: the loads of a call are in flight together.
+    const unsigned rest = s < steps ? (steps - s + WAVES - 1) / WAVES : 0;
+    if constexpr (U > 2)
+        if (rest == 2) run(s, std::integral_constant<int, 2>{});
+    if (rest == 1) run(s, std::integral_constant<int, 1>{});
+
+    // [wave][block][lane] of four sums.
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds);
+    constexpr unsigned ITEMS = NB * RB * 64;
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < RB; j++) part[wave * ITEMS + (i * RB + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+#pragma unroll
+    for (unsigned at = 0; at < ITEMS; at += 64 * WAVES) {
+        const unsigned item = at + tid;
+        if (ITEMS % (64 * WAVES) && item >= ITEMS) break;
+        f32x4 v = part[item];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) v += part[w * ITEMS + item];
+        store4<EPI>(a, m0 + item / 64 % RB * 16 + item % 16, n0 + item / 64 / RB * 16 + item % 64 / 16 * 4, v);
+    }
+}
+
+template <int EPI, int RB, int NB, int WAVES, int U>
+int launch_stream_as(h3_gpu *g, const Fp8BlockGemmArgs &a) {
+    constexpr int shared = stream_lds<RB, NB, WAVES>();
+    static_assert(shared <= 65536, "LDS without an attribute");
+    const unsigned groups = (a.m + 16 * RB - 1) / (16 * RB), columns = (a.n + 16 * NB - 1) / (16 * NB);
+    h3_note_kernel(g, "fp8_block_stream", 16 * RB);
+    hipLaunchKernelGGL((fp8_block_stream<EPI, RB, NB, WAVES, U>), dim3(columns * groups), dim3(64 * WAVES), shared, g->compute,
+                       a, groups);
+    return h3_launch_status(g, "FP8 block GEMM");
+}
+// Row blocks and column blocks of a workgroup.
+template <int EPI> int launch_stream(h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
+    return rb == 1 ? nb == 2 ? launch_stream_as<EPI, 1, 2, 8, 3>(g, a) : launch_stream_as<EPI, 1, 4, 8, 2>(g, a)
+           : rb == 2 ? nb == 2 ? launch_stream_as<EPI, 2, 2, 4, 3>(g, a) : launch_stream_as<EPI, 2, 4, 4, 3>(g, a)
+                     : launch_stream_as<EPI, 3, 2, 4, 2>(g, a);
+}
+
+// ---------------------------------------------------------------- tiles of 64 rows
+// Eight waves (two per SIMD) of 32 x 64 outputs (C^T = W . X^T). All operands go from
+// memory to LDS without registers, three stages of 128 bytes of K. A stage's second half of
+// fragments is read before a step's barrier, and the loads of the step after next but one go
+// into it right behind the barrier: every load has two steps' time. The scales of 32 steps come
+// to LDS together.
+constexpr int MID_M = 64, MID_N = 256, MID_T = 512, MID_STAGES = 3;
 constexpr unsigned SCALE_STEPS = 32;          // steps whose scales are loaded together
-constexpr unsigned MID_SCALES = MID_M * SCALE_STEPS + 1024, MID_LDS = MID_STAGES * MID_STAGE + 2 * MID_SCALES;
+constexpr unsigned MID_X = MID_M * TK, MID_STAGE = (MID_M + MID_N) * TK, MID_RUNS = MID_M / 32;
+constexpr unsigned MID_SCALES = MID_RUNS * 1024 + 256, MID_LDS = MID_STAGES * MID_STAGE + 2 * MID_SCALES;
 constexpr int MID_GROUP = 4;
 
+// Waits for all but N of this wave's vector-memory loads and for its LDS accesses, then for
+// the other waves. In asm because hipcc's own barrier waits for every load to LDS, those of
+// later steps included.
 template <int N> __device__ inline void step_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// The epilogue of a wave's 64 x 64 sums: row block j (32 rows), column blocks 0 and 1.
+__device__ inline void mid_tile(const Fp8BlockGemmArgs &a, unsigned pid, unsigned &m0, unsigned &n0) {
+    unsigned tm, tn;
+    band_tile((a.m + MID_M - 1) / MID_M, (a.n + MID_N - 1) / MID_N, MID_GROUP, pid, tm, tn);
+    m0 = __builtin_amdgcn_readfirstlane(tm * MID_M);
+    n0 = __builtin_amdgcn_readfirstlane(tn * MID_N);
+}
+
+// The epilogue of a wave's row block (32 rows from row0) and two column blocks from col0.
 // SwiGLU: the four waves of a row meet in `most` for the block's largest magnitude.
-__device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned m0, unsigned n0, unsigned wm, unsigned wn,
-                                    unsigned lane, unsigned j, f32x16 c0, f32x16 c1, unsigned (*most)[4][32]) {
-    const unsigned n32 = lane % 32, hf = lane / 32, row = m0 + wm * 64 + j * 32 + n32;
-    if (!a.swiglu) {
+template <int EPI>
+__device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, unsigned n0, unsigned wm, unsigned wn,
+                                    unsigned lane, const f32x16 &c0, const f32x16 &c1, unsigned (*most)[4][32]) {
+    const unsigned n32 = lane % 32, hf = lane / 32, row = row0 + n32;
+    if constexpr (EPI != EPI_SWIGLU) {
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-            store4(a, row, n0 + wn * 64 + g * 8 + hf * 4, f32x4{c0[4 * g], c0[4 * g + 1], c0[4 * g + 2], c0[4 * g + 3]});
-            store4(a, row, n0 + wn * 64 + 32 + g * 8 + hf * 4, f32x4{c1[4 * g], c1[4 * g + 1], c1[4 * g + 2], c1[4 * g + 3]});
+            store4<EPI>(a, row, n0 + wn * 64 + g * 8 + hf * 4, f32x4{c0[4 * g], c0[4 * g + 1], c0[4 * g + 2], c0[4 * g + 3]});
+            store4<EPI>(a, row, n0 + wn * 64 + 32 + g * 8 + hf * 4, f32x4{c1[4 * g], c1[4 * g + 1], c1[4 * g + 2], c1[4 * g + 3]});
         }
         return;
     }
@@ -104,11 +252,13 @@ __device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned m0, unsi
     uint8_t *dst = a.out.codes + (size_t)row * a.out.stride + n0 / 2 + wn * 32 + hf * 4;
 #pragma unroll
     for (int g = 0; g < 4; g++) *reinterpret_cast<unsigned *>(dst + g * 8) = fp8_block_encode4(v + 4 * g, inverse);
-    if (wn == 0 && hf == 0) a.out.scales[(size_t)row * a.out.scale_stride + n0 / 256] = (uint8_t)scale;
+    if (wn == 0 && hf == 0) a.out.scales[fp8_block_scale_at(row, n0 / 256, a.out.groups)] = (uint8_t)scale;
 }
 
+template <int EPI>
 __global__ __attribute__((amdgpu_flat_work_group_size(MID_T, MID_T), amdgpu_waves_per_eu(2, 2)))
 void fp8_block_mid(Fp8BlockGemmArgs a) {
+    constexpr bool SWIGLU = EPI == EPI_SWIGLU;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ unsigned most[2][4][32];
     const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
@@ -117,146 +267,143 @@ void fp8_block_mid(Fp8BlockGemmArgs a) {
     const TileShare t = tile_share(a.tile, ksteps);
     ksteps = __builtin_amdgcn_readfirstlane(ksteps);
     const unsigned first = __builtin_amdgcn_readfirstlane(t.first), k0 = first * TK;
-    unsigned tm, tn;
-    band_tile((a.m + MID_M - 1) / MID_M, (a.n + MID_N - 1) / MID_N, MID_GROUP, t.pid, tm, tn);
-    const unsigned m0 = __builtin_amdgcn_readfirstlane(tm * MID_M), n0 = __builtin_amdgcn_readfirstlane(tn * MID_N);
+    unsigned m0, n0;
+    mid_tile(a, t.pid, m0, n0);
 
     // Rows past M or N are past the resources' size and load zeros. SwiGLU: a wave loads
     // eight rows at a time, all gate or all up rows.
-    const unsigned half = a.swiglu && wave / 4 % 2, w_first = a.swiglu ? n0 / 2 + (half ? a.n / 2 : 0) : n0;
-    const unsigned xrows = min(a.m - m0, (unsigned)MID_M), wrows = a.swiglu ? 128u : min(a.n - n0, (unsigned)MID_N);
+    const unsigned half = SWIGLU && wave / 4 % 2, w_first = SWIGLU ? n0 / 2 + (half ? a.n / 2 : 0) : n0;
+    const unsigned xrows = min(a.m - m0, (unsigned)MID_M), wrows = SWIGLU ? 128u : min(a.n - n0, (unsigned)MID_N);
     const __amdgpu_buffer_rsrc_t xr = uniform_resource(a.x + (size_t)m0 * a.k + k0, xrows * a.k - k0);
     const __amdgpu_buffer_rsrc_t wr = uniform_resource(a.w + (size_t)w_first * a.k + k0, wrows * a.k - k0);
     const unsigned lrow = 8 * wave + lane / 8, part = swz(lrow, lane % 8) * 16;
-    unsigned xoff[2], woff[4];
+    const unsigned xoff = lrow * a.k + part;
+    unsigned woff[4];
 #pragma unroll
-    for (int b = 0; b < 2; b++) xoff[b] = (lrow + 64 * b) * a.k + part;
-#pragma unroll
-    for (int b = 0; b < 4; b++) woff[b] = (a.swiglu ? swiglu_row(lrow + 64 * b) : lrow + 64 * b) * a.k + part;
-    // Scales: 16-byte parts of 32 steps from the aligned one below the first; waves 0 to 3 the
-    // rows of X, wave 4 the two blocks of W in lanes 0 to 3.
-    const unsigned skip = first % 16, sbase = first - skip;
-    const unsigned xs_bytes = xrows * a.scale_stride - sbase;
-    const __amdgpu_buffer_rsrc_t xsr = uniform_resource(a.xs + (size_t)m0 * a.scale_stride + sbase, xs_bytes);
+    for (int b = 0; b < 4; b++) woff[b] = (SWIGLU ? swiglu_row(lrow + 64 * b) : lrow + 64 * b) * a.k + part;
+    // Scales of 32 steps from the group of four that holds the first: the first waves 32 rows of
+    // X each, [group][row][four], the next one the two blocks of W in lanes 0 to 15, [group].
+    const unsigned skip = first % 4, g0 = first / 4, runs = min((a.m + 31) / 32 - m0 / 32, MID_RUNS);
+    const __amdgpu_buffer_rsrc_t xsr =
+        uniform_resource(a.xs + ((size_t)(m0 / 32) * a.groups + g0) * 128, (runs * a.groups - g0) * 128);
     const unsigned wblocks = (a.n + 127) / 128;
-    const __amdgpu_buffer_rsrc_t wsr = uniform_resource(a.ws + sbase, wblocks * a.scale_stride - sbase);
-    const unsigned sb0 = a.swiglu ? n0 / 256 : n0 / 128, sb1 = a.swiglu ? n0 / 256 + a.n / 256 : min(n0 / 128 + 1, wblocks - 1);
-    const unsigned soff = wave < 4 ? (wave * 32 + lane / 2) * a.scale_stride + lane % 2 * 16
-                          : lane < 4 ? (lane / 2 ? sb1 : sb0) * a.scale_stride + lane % 2 * 16 : BUFFER_OOB;
+    const __amdgpu_buffer_rsrc_t wsr = uniform_resource(a.ws + (size_t)g0 * 128, ((wblocks + 31) / 32 * a.groups - g0) * 128);
+    const unsigned sb0 = SWIGLU ? n0 / 256 : n0 / 128, sb1 = SWIGLU ? n0 / 256 + a.n / 256 : min(n0 / 128 + 1, wblocks - 1);
     uint8_t *const scs = lds + MID_STAGES * MID_STAGE;
-    auto load_scales = [&](unsigned group) {
-        if (wave > 4) return;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            wave < 4 ? xsr : wsr, (__attribute__((address_space(3))) void *)(scs + (group & 1) * MID_SCALES + wave * 1024),
-            16, soff == BUFFER_OOB ? soff : soff + group * SCALE_STEPS, 0, 0, 0);
+    auto load_scales = [&](unsigned part) {
+        uint8_t *dst = scs + (part & 1) * MID_SCALES;
+        if (wave < MID_RUNS) {
+            // Behind a run's groups comes the next run, behind the last the resource's end: zeros.
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xsr, (__attribute__((address_space(3))) void *)(dst + wave * 1024), 16,
+                                                     (wave * a.groups + part * (SCALE_STEPS / 4)) * 128 + lane * 16, 0, 0, 0);
+        } else if (wave == MID_RUNS) {
+            const unsigned block = lane / 8 % 2 ? sb1 : sb0, group = part * (SCALE_STEPS / 4) + lane % 8;
+            const unsigned at = (block / 32 * a.groups + group) * 128 + block % 32 * 4;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (__attribute__((address_space(3))) void *)(dst + MID_RUNS * 1024), 4,
+                                                     lane < 16 && g0 + group < a.groups ? at : BUFFER_OOB, 0, 0, 0);
+        }
     };
 
-    f32x16 acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) acc[i][j] = f32x16{};
+    f32x16 acc[2] = {};
 
     // Loads of step kt into stage st; steps past the end reload the last one into a stage
     // that nobody reads again.
     auto load = [&](unsigned kt, unsigned st) {
         kt = __builtin_amdgcn_readfirstlane(min(kt, ksteps - 1));
         uint8_t *dst = lds + st * MID_STAGE + wave * 1024;
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void *)(dst + b * 8192), 16,
-                                                     xoff[b], kt * TK, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void *)dst, 16, xoff, kt * TK, 0, 0);
 #pragma unroll
         for (int b = 0; b < 4; b++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void *)(dst + MID_X + b * 8192),
-                                                     16, woff[b], kt * TK, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void *)(dst + MID_X + b * 8192), 16,
+                                                     woff[b], kt * TK, 0, 0);
     };
+    constexpr int LOADS = 5;                  // of a wave and step
     auto fragment = [&](const uint8_t *tile, unsigned r, int ks) {
         const u32x4 lo = *reinterpret_cast<const u32x4 *>(tile + r * TK + swz(r, 4 * ks + 2 * hf) * 16);
         const u32x4 hi = *reinterpret_cast<const u32x4 *>(tile + r * TK + swz(r, 4 * ks + 2 * hf + 1) * 16);
         return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
     };
-    auto frags = [&](unsigned st, int ks, i32x8 *wf, i32x8 *xf) {
+    auto frags = [&](unsigned st, int ks, i32x8 *wf, i32x8 &xf) {
         const uint8_t *xs = lds + st * MID_STAGE, *ws = xs + MID_X;
 #pragma unroll
         for (int i = 0; i < 2; i++) wf[i] = fragment(ws, wn * 64 + i * 32 + n32, ks);
-#pragma unroll
-        for (int j = 0; j < 2; j++) xf[j] = fragment(xs, wm * 64 + j * 32 + n32, ks);
+        xf = fragment(xs, wm * 32 + n32, ks);
     };
-    int ws[2], xs[2];
-    auto scales = [&](unsigned kt) {
+    auto scales = [&](unsigned kt, int *ws, int &xs) {
         const unsigned at = kt + skip;
-        const uint8_t *s = scs + at / SCALE_STEPS % 2 * MID_SCALES + at % SCALE_STEPS;
+        const uint8_t *s = scs + at / SCALE_STEPS % 2 * MID_SCALES;
+        const unsigned group = at % SCALE_STEPS / 4, byte = at % 4;
+        xs = s[wm * 1024 + group * 128 + n32 * 4 + byte];
 #pragma unroll
-        for (int j = 0; j < 2; j++) xs[j] = s[(wm * 64 + j * 32 + n32) * SCALE_STEPS];
+        for (int i = 0; i < 2; i++) ws[i] = s[MID_RUNS * 1024 + (SWIGLU ? i : wn / 2) * 32 + group * 4 + byte];
+    };
+    auto products = [&](const i32x8 *wf, const i32x8 &xf, const int *ws, int xs) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) ws[i] = s[4096 + (a.swiglu ? i : wn / 2) * SCALE_STEPS];
+        for (int i = 0; i < 2; i++)
+            acc[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[i], xf, acc[i], 0, 0, 0, ws[i], 0, xs);
     };
 
     load_scales(0);
     load_scales(1);
 #pragma unroll
-    for (int s = 0; s < MID_STAGES - 1; s++) load(s, s);
-    step_barrier<0>();
-    i32x8 wf[2][2], xf[2][2];
+    for (int s = 0; s < MID_STAGES; s++) load(s, s);
+    step_barrier<(MID_STAGES - 1) * LOADS>();
+    i32x8 wf[2][2], xf[2];
+    int ws[2][2], xs[2];
     frags(0, 0, wf[0], xf[0]);
-    scales(0);
+    scales(0, ws[0], xs[0]);
     unsigned cur = 0;
-    for (unsigned kt = 0; kt < ksteps; kt++) {
-        const unsigned next = cur + 1 == MID_STAGES ? 0 : cur + 1, last = cur == 0 ? MID_STAGES - 1 : cur - 1;
-        if (kt && (kt + skip) % SCALE_STEPS == 0) load_scales((kt + skip) / SCALE_STEPS + 1);
-        load(kt + MID_STAGES - 1, last);
+    auto step = [&](unsigned kt, int p) {
+        const unsigned next = cur + 1 == MID_STAGES ? 0 : cur + 1;
         frags(cur, 1, wf[1], xf[1]);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[0][i], xf[0][j], acc[i][j], 0, 0, 0, ws[i], 0, xs[j]);
-        step_barrier<(MID_STAGES - 2) * 6>();
-        frags(next, 0, wf[0], xf[0]);
-        const int ws1[2] = {ws[0], ws[1]}, xs1[2] = {xs[0], xs[1]};
-        scales(kt + 1);
+        products(wf[0], xf[0], ws[p], xs[p]);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[1][i], xf[1][j], acc[i][j], 0, 0, 0, ws1[i], 0, xs1[j]);
+        step_barrier<(MID_STAGES - 2) * LOADS>();
+        if (kt && (kt + skip) % SCALE_STEPS == 0) load_scales((kt + skip) / SCALE_STEPS + 1);
+        load(kt + MID_STAGES, cur);
+        frags(next, 0, wf[0], xf[0]);
+        scales(kt + 1, ws[p ^ 1], xs[p ^ 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        products(wf[1], xf[1], ws[p], xs[p]);
+        __builtin_amdgcn_sched_barrier(0);
         cur = next;
+    };
+    unsigned kt = 0;
+    for (; kt + 1 < ksteps; kt += 2) {
+        step(kt, 0);
+        step(kt + 1, 1);
     }
+    if (kt < ksteps) step(kt, 0);
     wait_vm_loads();   // LDS must not be written after the workgroup has ended
 
+    const unsigned row0 = m0 + wm * 32;
     if (t.partial) {
         f32x4 *dst = reinterpret_cast<f32x4 *>(a.tile.part) +
                      ((size_t)t.tile * a.tile.split + t.share) * (MID_M * MID_N / 4) + tid;
+        if (row0 >= a.m) return;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            if (m0 + wm * 64 + j * 32 >= a.m) break;
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-                    dst[((j * 2 + i) * 4 + g) * MID_T] = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
-                                                               acc[i][j][4 * g + 3]};
-        }
+            for (int g = 0; g < 4; g++)
+                dst[(i * 4 + g) * MID_T] = f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
         return;
     }
-#pragma unroll
-    for (int j = 0; j < 2; j++) mid_epilogue(a, m0, n0, wm, wn, lane, j, acc[0][j], acc[1][j], most);
+    mid_epilogue<EPI>(a, row0, n0, wm, wn, lane, acc[0], acc[1], most);
 }
 
-// The split tiles' shares added in order, and the epilogue. One workgroup per (tile, row block).
+// The split tiles' shares added in order, and the epilogue. One workgroup per tile.
+template <int EPI>
 __global__ __launch_bounds__(MID_T) void fp8_block_mid_reduce(Fp8BlockGemmArgs a) {
     __shared__ unsigned most[2][4][32];
-    const unsigned tile = blockIdx.x / 2, j = blockIdx.x % 2, tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    unsigned tm, tn;
-    band_tile((a.m + MID_M - 1) / MID_M, (a.n + MID_N - 1) / MID_N, MID_GROUP, split_tile(a.tile, tile), tm, tn);
-    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tile.part) + (size_t)tile * a.tile.split * (MID_M * MID_N / 4) +
-                       j * 8 * MID_T + tid;
-    const bool rows = tm * MID_M + wave / 4 * 64 + j * 32 < a.m;   // else no share was written
+    const unsigned tile = blockIdx.x, tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    unsigned m0, n0;
+    mid_tile(a, split_tile(a.tile, tile), m0, n0);
+    const unsigned row0 = m0 + wave / 4 * 32;
+    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tile.part) + (size_t)tile * a.tile.split * (MID_M * MID_N / 4) + tid;
     f32x16 c[2] = {};
-    for (unsigned s = 0; rows && s < a.tile.split; s++, src += MID_M * MID_N / 4)
+    // A row block past M: no share was written.
+    for (unsigned s = 0; row0 < a.m && s < a.tile.split; s++, src += MID_M * MID_N / 4)
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -265,14 +412,476 @@ __global__ __launch_bounds__(MID_T) void fp8_block_mid_reduce(Fp8BlockGemmArgs a
 #pragma unroll
                 for (int e = 0; e < 4; e++) c[i][4 * g + e] += v[e];
             }
-    mid_epilogue(a, tm * MID_M, tn * MID_N, wave / 4, wave % 4, lane, j, c[0], c[1], most);
+    mid_epilogue<EPI>(a, row0, n0, wave / 4, wave % 4, lane, c[0], c[1], most);
 }
 
-int launch_mid(h3_gpu *g, Fp8BlockGemmArgs a, unsigned split) {
+// ---------------------------------------------------------------- tiles of 256 rows
+// 256 x 256 outputs per workgroup, four waves of 128 x 128 (one per SIMD), each 4 x 4
+// accumulator blocks of 32 x 32 in AGPRs, so that one fragment read from LDS feeds four
+// MFMAs. The K loop is one inline-asm block, because its value is the order of the
+// instructions; with one wave per SIMD nothing else hides a stall:
+//  * a K tile is one block of 128 bytes, two substeps of sixteen MFMAs; the eight 32-byte
+//    fragments of the next substep are read in the first eight MFMA slots of the current
+//    one, two ds_read_b128 each, into the other register set;
+//  * the sixteen global -> LDS loads of a K tile (1 KB each) are issued two tiles ahead,
+//    one per MFMA of the second substep, into the stage this tile has finished reading;
+//  * one barrier per tile, between the substeps;
+//  * the scales of four tiles are the bytes of one dword per fragment row, loaded into the
+//    other one of two register sets a group of four tiles ahead; the MFMAs of tile B of a
+//    group take byte B (op_sel), so the body is two groups.
+// LDS (128 KB): X stages at 0 and 32 KB, W stages at 64 and 96 KB; rows of 128 codes with
+// XOR-swizzled 16-byte chunks. Fixed registers: fragment set S in v[64 + 64 S ..], W block
+// I at + 8 I, X block J at + 32 + 8 J; scale set Z in v[192 + 6 Z ..], X block J at + J, W at
+// + 4 (even blocks) and + 5 (odd ones: with SwiGLU those are up rows).
+//
+// Tiles of 128 rows are the same with waves of 64 x 128 and half as many products a tile, too
+// few to cover the memory's latency with one tile of lead: three stages, X at 0, 16 and 32 KB,
+// W at 48, 80 and 112 KB, and loads three tiles ahead. Fragment set S in v[64 + 48 S ..], X
+// block J at + 32 + 8 J; scale set Z in v[160 + 4 Z ..], X block J at + J, W at + 2 and + 3. The
+// body is 24 tiles: three stages, four bytes, two sets.
+constexpr int PIPE_N = 256, PIPE_T = 256;
+template <int TM> constexpr unsigned pipe_lds() { return TM == 256 ? 4 * 256 * TK : 3 * (128 + 256) * TK; }
+constexpr int PIPE_GROUP = 4;
+constexpr unsigned QUAD = 4;                  // K tiles whose scales are loaded together
+
+#define FB_LX(ST, T) "s_add_u32 m0, %[mb], 32768*" #ST "+4096*" #T "\n"                                             \
+    "buffer_load_dwordx4 %[x" #T "], %[sx], %[kc] offen lds\n"
+#define FB_LW(ST, T, R) "s_add_u32 m0, %[mb], 65536+32768*" #ST "+4096*" #T "\n"                                    \
+    "buffer_load_dwordx4 %[y" #T "], %[sw" #R "], %[kc] offen lds\n"
+#define FB_LOADS(ST) FB_LX(ST, 0), FB_LW(ST, 0, 0), FB_LX(ST, 1), FB_LW(ST, 1, 1), FB_LX(ST, 2), FB_LW(ST, 2, 0),    \
+    FB_LX(ST, 3), FB_LW(ST, 3, 1), FB_LX(ST, 4), FB_LW(ST, 4, 0), FB_LX(ST, 5), FB_LW(ST, 5, 1), FB_LX(ST, 6),         \
+    FB_LW(ST, 6, 0), FB_LX(ST, 7), FB_LW(ST, 7, 1)
+#define FB_NONE "", "", "", "", "", "", "", "", "", "", "", "", "", "", "", ""
+// The scales of the group at byte kg of a run of rows into set Z.
+#define FB_SCALES(Z)                                                                                                \
+    "buffer_load_dword v[192+6*" #Z "], %[e0], %[tx], %[kg] offen\n"                                                 \
+    "buffer_load_dword v[192+6*" #Z "+1], %[e1], %[tx], %[kg] offen\n"                                               \
+    "buffer_load_dword v[192+6*" #Z "+2], %[e2], %[tx], %[kg] offen\n"                                               \
+    "buffer_load_dword v[192+6*" #Z "+3], %[e3], %[tx], %[kg] offen\n"                                               \
+    "buffer_load_dword v[192+6*" #Z "+4], %[e4], %[tw], %[kg] offen\n"                                               \
+    "buffer_load_dword v[192+6*" #Z "+5], %[e5], %[tw], %[kg] offen\n"                                               \
+    "s_add_u32 %[kg], %[kg], 128\n"                                                                                 \
+    "s_min_u32 %[kg], %[kg], %[kgmax]\n"
+#define FB_SEL_0 " op_sel:[0,0,0] op_sel_hi:[0,0,0]\n"
+#define FB_SEL_1 " op_sel:[1,1,0] op_sel_hi:[0,0,0]\n"
+#define FB_SEL_2 " op_sel:[0,0,0] op_sel_hi:[1,1,0]\n"
+#define FB_SEL_3 " op_sel:[1,1,0] op_sel_hi:[1,1,0]\n"
+#define FB_MFMA(S, Z, B, I, J, P)                                                                                   \
+    "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #I #J "], v[64+64*" #S "+8*" #I ":64+64*" #S "+8*" #I "+7], "             \
+    "v[64+64*" #S "+32+8*" #J ":64+64*" #S "+32+8*" #J "+7], %[c" #I #J "], v[192+6*" #Z "+4+" #P "], "              \
+    "v[192+6*" #Z "+" #J "]" FB_SEL_##B
+// Fragment F of substep KS, stage ST, into set T: its two 16-byte halves.
+#define FB_RW(T, F, KS, ST)                                                                                         \
+    "ds_read_b128 v[64+64*" #T "+8*" #F ":64+64*" #T "+8*" #F "+3], %[w" #KS "0] offset:32768*" #ST "+4096*" #F "\n"     \
+    "ds_read_b128 v[64+64*" #T "+8*" #F "+4:64+64*" #T "+8*" #F "+7], %[w" #KS "1] offset:32768*" #ST "+4096*" #F "\n"
+#define FB_RX(T, F, KS, ST)                                                                                         \
+    "ds_read_b128 v[64+64*" #T "+32+8*" #F ":64+64*" #T "+32+8*" #F "+3], %[r" #KS "0] offset:32768*" #ST "+4096*" #F "\n" \
+    "ds_read_b128 v[64+64*" #T "+32+8*" #F "+4:64+64*" #T "+32+8*" #F "+7], %[r" #KS "1] offset:32768*" #ST "+4096*" #F "\n"
+// A substep of set S with scale set Z, byte B, that reads substep KS of stage ST into set T;
+// L0..L15 behind its MFMAs.
+#define FB_SUB(S, Z, B, T, KS, ST, L0, L1, L2, L3, L4, L5, L6, L7, L8, L9, L10, L11, L12, L13, L14, L15)              \
+    FB_MFMA(S, Z, B, 0, 0, 0) FB_RW(T, 0, KS, ST) L0 FB_MFMA(S, Z, B, 0, 1, 0) FB_RX(T, 0, KS, ST) L1                \
+    FB_MFMA(S, Z, B, 0, 2, 0) FB_RX(T, 1, KS, ST) L2 FB_MFMA(S, Z, B, 0, 3, 0) FB_RX(T, 2, KS, ST) L3                \
+    FB_MFMA(S, Z, B, 1, 0, 1) FB_RX(T, 3, KS, ST) L4 FB_MFMA(S, Z, B, 1, 1, 1) FB_RW(T, 1, KS, ST) L5                \
+    FB_MFMA(S, Z, B, 1, 2, 1) FB_RW(T, 2, KS, ST) L6 FB_MFMA(S, Z, B, 1, 3, 1) FB_RW(T, 3, KS, ST) L7                \
+    FB_MFMA(S, Z, B, 2, 0, 0) L8 FB_MFMA(S, Z, B, 2, 1, 0) L9 FB_MFMA(S, Z, B, 2, 2, 0) L10                          \
+    FB_MFMA(S, Z, B, 2, 3, 0) L11 FB_MFMA(S, Z, B, 3, 0, 1) L12 FB_MFMA(S, Z, B, 3, 1, 1) L13                        \
+    FB_MFMA(S, Z, B, 3, 2, 1) L14 FB_MFMA(S, Z, B, 3, 3, 1) L15
+#define FB_SUB_EXP(...) FB_SUB(__VA_ARGS__)
+// K tile B of a group in stage ST, next tile's stage OT; NEXT: loads of the next group's scales.
+#define FB_TILE(ST, OT, Z, B, NEXT)                                                                                 \
+    FB_SUB_EXP(0, Z, B, 1, 1, ST, FB_NONE)                                                                           \
+    "s_waitcnt vmcnt(0) lgkmcnt(0)\n"                                                                               \
+    "s_barrier\n"                                                                                                   \
+    "s_min_u32 %[kc], %[kn], %[kmax]\n"                                                                             \
+    "s_add_u32 %[kn], %[kn], 128\n" NEXT                                                                            \
+    FB_SUB_EXP(1, Z, B, 0, 0, OT, FB_LOADS(ST))                                                                      \
+    "s_waitcnt lgkmcnt(0)\n"                                                                                        \
+    "s_sub_u32 %[steps], %[steps], 1\n"                                                                             \
+    "s_cmp_eq_u32 %[steps], 0\n"                                                                                    \
+    "s_cbranch_scc1 fb_end_%=\n"
+#define FB_QUAD(Z, OZ) FB_TILE(0, 1, Z, 0, FB_SCALES(OZ)) FB_TILE(1, 0, Z, 1, "") FB_TILE(0, 1, Z, 2, "") FB_TILE(1, 0, Z, 3, "")
+#define FB_FIRST(ST, KC) "s_mov_b32 %[kc], " KC "\n" FB_LX(ST, 0) FB_LW(ST, 0, 0) FB_LX(ST, 1) FB_LW(ST, 1, 1)           \
+    FB_LX(ST, 2) FB_LW(ST, 2, 0) FB_LX(ST, 3) FB_LW(ST, 3, 1) FB_LX(ST, 4) FB_LW(ST, 4, 0) FB_LX(ST, 5) FB_LW(ST, 5, 1) \
+    FB_LX(ST, 6) FB_LW(ST, 6, 0) FB_LX(ST, 7) FB_LW(ST, 7, 1)
+// Tiles of 128 rows.
+#define FH_LX(ST, T) "s_add_u32 m0, %[mb], 16384*" #ST "+4096*" #T "\n"                                             \
+    "buffer_load_dwordx4 %[x" #T "], %[sx], %[kc] offen lds\n"
+#define FH_LW(ST, T, R) "s_add_u32 m0, %[mb], 49152+32768*" #ST "+4096*" #T "\n"                                    \
+    "buffer_load_dwordx4 %[y" #T "], %[sw" #R "], %[kc] offen lds\n"
+#define FH_SCALES(Z)                                                                                                \
+    "buffer_load_dword v[160+4*" #Z "], %[e0], %[tx], %[kg] offen\n"                                                 \
+    "buffer_load_dword v[160+4*" #Z "+1], %[e1], %[tx], %[kg] offen\n"                                               \
+    "buffer_load_dword v[160+4*" #Z "+2], %[e4], %[tw], %[kg] offen\n"                                               \
+    "buffer_load_dword v[160+4*" #Z "+3], %[e5], %[tw], %[kg] offen\n"                                               \
+    "s_add_u32 %[kg], %[kg], 128\n"                                                                                 \
+    "s_min_u32 %[kg], %[kg], %[kgmax]\n"
+#define FH_MFMA(S, Z, B, I, J, P)                                                                                   \
+    "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #I #J "], v[64+48*" #S "+8*" #I ":64+48*" #S "+8*" #I "+7], "             \
+    "v[64+48*" #S "+32+8*" #J ":64+48*" #S "+32+8*" #J "+7], %[c" #I #J "], v[160+4*" #Z "+2+" #P "], "              \
+    "v[160+4*" #Z "+" #J "]" FB_SEL_##B
+// W's stage ST is within a ds_read's offset of base 0 (stages 0 and 1) or of its own (2).
+#define FH_WAT_0(KS, H) "%[w" #KS #H "] offset:"
+#define FH_WAT_1(KS, H) "%[w" #KS #H "] offset:32768+"
+#define FH_WAT_2(KS, H) "%[u" #KS #H "] offset:"
+#define FH_RW(T, F, KS, ST)                                                                                         \
+    "ds_read_b128 v[64+48*" #T "+8*" #F ":64+48*" #T "+8*" #F "+3], " FH_WAT_##ST(KS, 0) "4096*" #F "\n"              \
+    "ds_read_b128 v[64+48*" #T "+8*" #F "+4:64+48*" #T "+8*" #F "+7], " FH_WAT_##ST(KS, 1) "4096*" #F "\n"
+#define FH_RX(T, F, KS, ST)                                                                                         \
+    "ds_read_b128 v[64+48*" #T "+32+8*" #F ":64+48*" #T "+32+8*" #F "+3], %[r" #KS "0] offset:16384*" #ST "+4096*" #F "\n" \
+    "ds_read_b128 v[64+48*" #T "+32+8*" #F "+4:64+48*" #T "+32+8*" #F "+7], %[r" #KS "1] offset:16384*" #ST "+4096*" #F "\n"
+#define FH_SUB(S, Z, B, T, KS, ST, L0, L1, L2, L3, L4, L5, L6, L7)                                                    \
+    FH_MFMA(S, Z, B, 0, 0, 0) FH_RW(T, 0, KS, ST) L0 FH_MFMA(S, Z, B, 0, 1, 0) FH_RX(T, 0, KS, ST) L1                \
+    FH_MFMA(S, Z, B, 1, 0, 1) FH_RX(T, 1, KS, ST) L2 FH_MFMA(S, Z, B, 1, 1, 1) FH_RW(T, 1, KS, ST) L3                \
+    FH_MFMA(S, Z, B, 2, 0, 0) FH_RW(T, 2, KS, ST) L4 FH_MFMA(S, Z, B, 2, 1, 0) FH_RW(T, 3, KS, ST) L5                \
+    FH_MFMA(S, Z, B, 3, 0, 1) L6 FH_MFMA(S, Z, B, 3, 1, 1) L7
+#define FH_SUB_EXP(...) FH_SUB(__VA_ARGS__)
+#define FH_NONE "", "", "", "", "", "", "", ""
+#define FH_LOADS(ST) FH_LX(ST, 0), FH_LW(ST, 0, 0), FH_LX(ST, 1), FH_LW(ST, 1, 1), FH_LX(ST, 2) FH_LW(ST, 2, 0),      \
+    FH_LX(ST, 3) FH_LW(ST, 3, 1), FH_LW(ST, 4, 0) FH_LW(ST, 5, 1), FH_LW(ST, 6, 0) FH_LW(ST, 7, 1)
+// The loads of the tile after next (12, the youngest) stay in flight at the barrier.
+#define FH_TILE(ST, OT, Z, B, NEXT)                                                                                 \
+    FH_SUB_EXP(0, Z, B, 1, 1, ST, FH_NONE)                                                                           \
+    "s_waitcnt vmcnt(12) lgkmcnt(0)\n"                                                                              \
+    "s_barrier\n"                                                                                                   \
+    "s_min_u32 %[kc], %[kn], %[kmax]\n"                                                                             \
+    "s_add_u32 %[kn], %[kn], 128\n" NEXT                                                                            \
+    FH_SUB_EXP(1, Z, B, 0, 0, OT, FH_LOADS(ST))                                                                      \
+    "s_waitcnt lgkmcnt(0)\n"                                                                                        \
+    "s_sub_u32 %[steps], %[steps], 1\n"                                                                             \
+    "s_cmp_eq_u32 %[steps], 0\n"                                                                                    \
+    "s_cbranch_scc1 fh_end_%=\n"
+// Four tiles from stage S0 on.
+#define FH_QUAD(S0, S1, S2, Z, OZ) FH_TILE(S0, S1, Z, 0, FH_SCALES(OZ)) FH_TILE(S1, S2, Z, 1, "")                     \
+    FH_TILE(S2, S0, Z, 2, "") FH_TILE(S0, S1, Z, 3, "")
+#define FH_FIRST(ST, KC) "s_mov_b32 %[kc], " KC "\n" FH_LX(ST, 0) FH_LW(ST, 0, 0) FH_LX(ST, 1) FH_LW(ST, 1, 1)           \
+    FH_LX(ST, 2) FH_LW(ST, 2, 0) FH_LX(ST, 3) FH_LW(ST, 3, 1) FH_LW(ST, 4, 0) FH_LW(ST, 5, 1) FH_LW(ST, 6, 0) FH_LW(ST, 7, 1)
+#define FH_ACC2(I) [c##I##0] "+a"(c[I][0]), [c##I##1] "+a"(c[I][1])
+#define FB_ACC4(I) [c##I##0] "+a"(c[I][0]), [c##I##1] "+a"(c[I][1]), [c##I##2] "+a"(c[I][2]), [c##I##3] "+a"(c[I][3])
+#define FB_CL10(x) "v" #x "0", "v" #x "1", "v" #x "2", "v" #x "3", "v" #x "4", "v" #x "5", "v" #x "6", "v" #x "7",     \
+    "v" #x "8", "v" #x "9"
+
+template <int TM>
+__device__ inline void pipe_tile(const Fp8BlockGemmArgs &a, unsigned pid, unsigned &m0, unsigned &n0) {
+    unsigned tm, tn;
+    band_tile((a.m + TM - 1) / TM, (a.n + PIPE_N - 1) / PIPE_N, PIPE_GROUP, pid, tm, tn);
+    m0 = __builtin_amdgcn_readfirstlane(tm * TM);
+    n0 = __builtin_amdgcn_readfirstlane(tn * PIPE_N);
+}
+
+// The workgroup's share of the K tiles: whole groups of four, so that the scales' dwords stay
+// aligned. On return t.first counts tiles and ksteps is their number.
+__device__ inline TileShare pipe_share(const Fp8BlockGemmArgs &a, unsigned &ksteps) {
+    unsigned quads = (ksteps + QUAD - 1) / QUAD;
+    TileShare t = tile_share(a.tile, quads);
+    t.first *= QUAD;
+    ksteps = min(quads * QUAD, ksteps - t.first);
+    return t;
+}
+
+// 32 columns of an output row from col, registers as the MFMA leaves them: group g of lane
+// half hf holds columns 8 g + 4 hf + 0..3. Groups g and g + 1 go out together as 16-byte
+// stores: v_permlane32_swap gives the low half both halves of group g, the high half those
+// of group g + 1.
+template <int EPI>
+__device__ inline void pipe_store(const Fp8BlockGemmArgs &a, unsigned row, unsigned col, unsigned hf, const f32x16 &c) {
+    uint16_t *dst = a.y + (size_t)row * a.n;
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+        unsigned w[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            f32x4 v = {c[4 * (g + h)], c[4 * (g + h) + 1], c[4 * (g + h) + 2], c[4 * (g + h) + 3]};
+            if constexpr (EPI == EPI_BIAS) {
+                const u16x4 b = *reinterpret_cast<const u16x4 *>(a.bias + min(col + 8 * (g + h) + 4 * hf, a.n - 4));
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] += bf16_to_f32(b[e]);
+            }
+            u16x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = f32_to_bf16(v[e]);
+            w[h][0] = o[0] | ((unsigned)o[1] << 16);
+            w[h][1] = o[2] | ((unsigned)o[3] << 16);
+        }
+        const auto s0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+        const auto s1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+        const unsigned at = col + 8 * (g + hf);
+        if (row < a.m && at < a.n) *reinterpret_cast<u32x4 *>(dst + at) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+    }
+}
+
+// 32 rows x 128 columns of a wave through LDS, so that rows of any alignment go out whole: two
+// columns a lane.
+constexpr unsigned ANY_ROW = 132;             // FP32 values of a row in LDS, padded against bank conflicts
+constexpr unsigned ANY_LDS = 4 * 32 * ANY_ROW * 4;
+__device__ inline void pipe_any(const Fp8BlockGemmArgs &a, unsigned row0, unsigned col, unsigned lane, const f32x16 &c0,
+                                const f32x16 &c1, const f32x16 &c2, const f32x16 &c3, float *rows) {
+    const unsigned n32 = lane % 32, hf = lane / 32;
+    const f32x16 *c[4] = {&c0, &c1, &c2, &c3};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<f32x4 *>(rows + n32 * ANY_ROW + 32 * i + 8 * g + 4 * hf) =
+                f32x4{(*c[i])[4 * g], (*c[i])[4 * g + 1], (*c[i])[4 * g + 2], (*c[i])[4 * g + 3]};
+    // Only this wave's lanes read what they wrote: no barrier, but the stores come first.
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const unsigned at = col + 2 * lane;
+    float bias[2] = {};
+    if (a.bias)
+        for (unsigned e = 0; e < 2; e++) bias[e] = at + e < a.n ? bf16_to_f32(a.bias[at + e]) : 0.f;
+    const unsigned count = at < a.n ? min(a.m > row0 ? a.m - row0 : 0u, 32u) : 0u;
+    for (unsigned r = 0; r < count; r++) {
+        const f32x2 v = *reinterpret_cast<const f32x2 *>(rows + r * ANY_ROW + 2 * lane);
+        const size_t to = (size_t)(row0 + r) * a.n + at;
+        if (a.y32) {
+            *reinterpret_cast<f32x2 *>(a.y32 + to) = v;
+            continue;
+        }
+        const u16x2_any o = {{f32_to_bf16(v[0] + bias[0]), f32_to_bf16(v[1] + bias[1])}};
+        if (at + 1 < a.n) *reinterpret_cast<u16x2_any *>(a.y + to) = o;
+        else a.y[to] = o.v[0];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The epilogue of a wave's 32 rows from row0 x 128 columns, blocks c0 to c3. SwiGLU: the
+// two waves of a row meet in scratch (LDS) for the largest magnitude of its 128 columns.
+template <int EPI>
+__device__ inline void pipe_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, unsigned n0, unsigned wm, unsigned wn,
+                                     unsigned lane, const f32x16 &c0, const f32x16 &c1, const f32x16 &c2,
+                                     const f32x16 &c3, void *scratch) {
+    const unsigned n32 = lane % 32, hf = lane / 32, row = row0 + n32, col = n0 + wn * 128;
+    auto most = (unsigned(*)[2][32])scratch;
+    if constexpr (EPI == EPI_ANY) {
+        pipe_any(a, row0, col, lane, c0, c1, c2, c3, (float *)scratch + (wm * 2 + wn) * 32 * ANY_ROW);
+        return;
+    }
+    if constexpr (EPI != EPI_SWIGLU) {
+        pipe_store<EPI>(a, row, col, hf, c0);
+        pipe_store<EPI>(a, row, col + 32, hf, c1);
+        pipe_store<EPI>(a, row, col + 64, hf, c2);
+        pipe_store<EPI>(a, row, col + 96, hf, c3);
+        return;
+    }
+    float v[32];
+    unsigned amax = 0;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        v[e] = swiglu_exact(c0[e], c1[e]);
+        v[16 + e] = swiglu_exact(c2[e], c3[e]);
+        amax = max(amax, max(finite_magnitude(v[e], bad), finite_magnitude(v[16 + e], bad)));
+    }
+    if (bad && row < a.m) *a.out.fault = 1u;
+    amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
+    if (hf == 0) most[wm][wn][n32] = amax;
+    __syncthreads();
+    const unsigned scale = fp8_block_scale(max(most[wm][0][n32], most[wm][1][n32]));
+    __syncthreads();
+    const float inverse = fp8_block_inverse(scale);
+    // Groups g and g + 1 go out together, eight codes a lane.
+    uint8_t *dst = a.out.codes + (size_t)row * a.out.stride + n0 / 2 + wn * 64 + hf * 8;
+#pragma unroll
+    for (int g = 0; g < 8; g += 2) {
+        const auto s = __builtin_amdgcn_permlane32_swap(fp8_block_encode4(v + 4 * g, inverse),
+                                                        fp8_block_encode4(v + 4 * g + 4, inverse), false, false);
+        if (row < a.m) *reinterpret_cast<uint2 *>(dst + g * 8) = make_uint2(s[0], s[1]);
+    }
+    if (row < a.m && wn == 0 && hf == 0) a.out.scales[fp8_block_scale_at(row, n0 / 256, a.out.groups)] = (uint8_t)scale;
+}
+
+// SPLIT: the tiles of the last, incomplete wave are shared over K.
+template <int EPI, bool SPLIT, int TM>
+__global__ __attribute__((amdgpu_flat_work_group_size(PIPE_T, PIPE_T), amdgpu_waves_per_eu(1, 1)))
+void fp8_block_pipe(Fp8BlockGemmArgs a) {
+    constexpr bool SWIGLU = EPI == EPI_SWIGLU;
+    constexpr int NJ = TM / 64;               // row blocks of a wave
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const unsigned tid = threadIdx.x, lane = tid % 64, n32 = lane % 32, hf = lane / 32;
+    const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64), wm = wave / 2, wn = wave % 2;
+    unsigned ksteps = a.k / TK;
+    TileShare t{};
+    if constexpr (SPLIT) t = pipe_share(a, ksteps);
+    else t.pid = xcd_remap(blockIdx.x, gridDim.x);
+    const unsigned k0 = t.first * TK;
+    unsigned m0, n0;
+    pipe_tile<TM>(a, t.pid, m0, n0);
+    // Rows past M or N are past the resources' size and load zeros. SwiGLU: loads of even
+    // number hold gate rows, of odd number up rows.
+    const unsigned xrows = min(a.m - m0, (unsigned)TM), wrows = SWIGLU ? 128u : min(a.n - n0, (unsigned)PIPE_N);
+    const unsigned w0 = SWIGLU ? n0 / 2 : n0, w1 = SWIGLU ? n0 / 2 + a.n / 2 : n0;
+    auto resource = [](const uint8_t *p, unsigned bytes) {
+        const uint64_t v = (uint64_t)p;
+        return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)v), (int)__builtin_amdgcn_readfirstlane((unsigned)(v >> 32)),
+                     (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+    };
+    const i32x4 sx = resource(a.x + (size_t)m0 * a.k + k0, xrows * a.k - k0);
+    const i32x4 sw0 = resource(a.w + (size_t)w0 * a.k + k0, wrows * a.k - k0);
+    const i32x4 sw1 = resource(a.w + (size_t)w1 * a.k + k0, wrows * a.k - k0);
+    const unsigned blocks = (a.n + FP8_BLOCK - 1) / FP8_BLOCK;
+    const unsigned g0 = t.first / QUAD;
+    const i32x4 tx = resource(a.xs + ((size_t)(m0 / 32) * a.groups + g0) * 128, (min((a.m + 31) / 32 - m0 / 32, TM / 32u) * a.groups - g0) * 128);
+    const i32x4 tw = resource(a.ws + (size_t)g0 * 128, ((blocks + 31) / 32 * a.groups - g0) * 128);
+    const unsigned lrow = 8 * wave + lane / 8;
+    unsigned ox[8], ow[8], oe[6];
+#pragma unroll
+    for (int b = 0; b < 8; b++) {
+        ox[b] = (lrow + 32 * b) * a.k + swz(lrow, lane % 8) * 16;
+        ow[b] = SWIGLU ? (lrow + 32 * (b / 2)) * a.k + swz(lrow, lane % 8) * 16 : ox[b];
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; j++) oe[j] = (wm * NJ + j) * a.groups * 128 + n32 * 4;
+    // A wave's 128 columns are one block of W; with SwiGLU the tile's gate rows are one, its up
+    // rows another. A block past the end (a half-empty last tile) has no codes.
+    const unsigned first_block = SWIGLU ? n0 / 256 : min(n0 / 128 + wn, blocks - 1);
+    oe[4] = (unsigned)fp8_block_scale_at(first_block, 0, a.groups);
+    oe[5] = SWIGLU ? (unsigned)fp8_block_scale_at(first_block + a.n / 256, 0, a.groups) : oe[4];
+    const unsigned mb = __builtin_amdgcn_readfirstlane(wave * 1024);
+    const unsigned kmax = __builtin_amdgcn_readfirstlane((ksteps - 1) * TK);
+    const unsigned kgmax = __builtin_amdgcn_readfirstlane((ksteps - 1) / QUAD * 128);
+    const unsigned kone = min(kmax, TK), ktwo = min(kmax, 2 * TK);
+    unsigned kn = (TM == 256 ? 2 : 3) * TK, kc = 0, kg = 0, steps = __builtin_amdgcn_readfirstlane(ksteps);
+    // Fragment bases in stage 0: row n32 of the wave's half, bytes 32 hf .. + 31 of substep
+    // s, that is chunks 4 s + 2 hf and the next one.
+    unsigned pw[2][2], px[2][2];
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const unsigned part = n32 * TK + swz(n32, 4 * s + 2 * hf + h) * 16;
+            pw[s][h] = (TM == 256 ? 512 : 384) * TK + wn * 128 * TK + part;
+            px[s][h] = wm * (TM / 2) * TK + part;
+        }
+    f32x16 c[4][NJ];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++) c[i][j] = f32x16{};
+    // Prologue: the first group's scales into set 0, tiles 0 and 1 into stages 0 and 1, substep
+    // 0 of tile 0 into fragment set 0. The loop body is two groups of four tiles, left after
+    // the last tile; loads past the end reload the last tile into a stage nobody reads again,
+    // or the last group's scales.
+    if constexpr (TM == 256)
+    asm volatile(
+        FB_SCALES(0)
+        FB_FIRST(0, "0") FB_FIRST(1, "%[kone]")
+        "s_waitcnt vmcnt(0)\n"
+        "s_barrier\n"
+        FB_RW(0, 0, 0, 0) FB_RW(0, 1, 0, 0) FB_RW(0, 2, 0, 0) FB_RW(0, 3, 0, 0)
+        FB_RX(0, 0, 0, 0) FB_RX(0, 1, 0, 0) FB_RX(0, 2, 0, 0) FB_RX(0, 3, 0, 0)
+        "s_waitcnt lgkmcnt(0)\n"
+        "fb_loop_%=:\n"
+        FB_QUAD(0, 1)
+        FB_QUAD(1, 0)
+        "s_branch fb_loop_%=\n"
+        "fb_end_%=:\n"
+        "s_waitcnt vmcnt(0) lgkmcnt(0)\n"
+        // The last MFMAs' results are complete before the epilogue reads the accumulators
+        // (hipcc does not see the MFMAs inside this block).
+        "s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n"
+        : FB_ACC4(0), FB_ACC4(1), FB_ACC4(2), FB_ACC4(3), [kc] "+s"(kc), [kn] "+s"(kn), [kg] "+s"(kg), [steps] "+s"(steps)
+        : [sx] "s"(sx), [sw0] "s"(sw0), [sw1] "s"(sw1), [tx] "s"(tx), [tw] "s"(tw), [x0] "v"(ox[0]), [x1] "v"(ox[1]),
+          [x2] "v"(ox[2]), [x3] "v"(ox[3]), [x4] "v"(ox[4]), [x5] "v"(ox[5]), [x6] "v"(ox[6]), [x7] "v"(ox[7]),
+          [y0] "v"(ow[0]), [y1] "v"(ow[1]), [y2] "v"(ow[2]), [y3] "v"(ow[3]), [y4] "v"(ow[4]), [y5] "v"(ow[5]),
+          [y6] "v"(ow[6]), [y7] "v"(ow[7]), [e0] "v"(oe[0]), [e1] "v"(oe[1]), [e2] "v"(oe[2]), [e3] "v"(oe[3]),
+          [e4] "v"(oe[4]), [e5] "v"(oe[5]), [mb] "s"(mb), [kmax] "s"(kmax), [kgmax] "s"(kgmax), [kone] "s"(kone),
+          [w00] "v"(pw[0][0]), [w01] "v"(pw[0][1]), [w10] "v"(pw[1][0]), [w11] "v"(pw[1][1]), [r00] "v"(px[0][0]),
+          [r01] "v"(px[0][1]), [r10] "v"(px[1][0]), [r11] "v"(px[1][1])
+        : "v64", "v65", "v66", "v67", "v68", "v69", FB_CL10(7), FB_CL10(8), FB_CL10(9), FB_CL10(10), FB_CL10(11),
+          FB_CL10(12), FB_CL10(13), FB_CL10(14), FB_CL10(15), FB_CL10(16), FB_CL10(17), FB_CL10(18), FB_CL10(19),
+          "v200", "v201", "v202", "v203", "m0", "scc", "memory");
+    else {
+    const unsigned pu[2][2] = {{pw[0][0] + 65536, pw[0][1] + 65536}, {pw[1][0] + 65536, pw[1][1] + 65536}};
+    asm volatile(
+        FH_SCALES(0)
+        FH_FIRST(0, "0") FH_FIRST(1, "%[kone]") FH_FIRST(2, "%[ktwo]")
+        "s_waitcnt vmcnt(24)\n"
+        "s_barrier\n"
+        FH_RW(0, 0, 0, 0) FH_RW(0, 1, 0, 0) FH_RW(0, 2, 0, 0) FH_RW(0, 3, 0, 0) FH_RX(0, 0, 0, 0) FH_RX(0, 1, 0, 0)
+        "s_waitcnt lgkmcnt(0)\n"
+        "fh_loop_%=:\n"
+        FH_QUAD(0, 1, 2, 0, 1) FH_QUAD(1, 2, 0, 1, 0) FH_QUAD(2, 0, 1, 0, 1)
+        FH_QUAD(0, 1, 2, 1, 0) FH_QUAD(1, 2, 0, 0, 1) FH_QUAD(2, 0, 1, 1, 0)
+        "s_branch fh_loop_%=\n"
+        "fh_end_%=:\n"
+        "s_waitcnt vmcnt(0) lgkmcnt(0)\n"
+        "s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n"
+        : FH_ACC2(0), FH_ACC2(1), FH_ACC2(2), FH_ACC2(3), [kc] "+s"(kc), [kn] "+s"(kn), [kg] "+s"(kg), [steps] "+s"(steps)
+        : [sx] "s"(sx), [sw0] "s"(sw0), [sw1] "s"(sw1), [tx] "s"(tx), [tw] "s"(tw), [x0] "v"(ox[0]), [x1] "v"(ox[1]),
+          [x2] "v"(ox[2]), [x3] "v"(ox[3]), [y0] "v"(ow[0]), [y1] "v"(ow[1]), [y2] "v"(ow[2]), [y3] "v"(ow[3]),
+          [y4] "v"(ow[4]), [y5] "v"(ow[5]), [y6] "v"(ow[6]), [y7] "v"(ow[7]), [e0] "v"(oe[0]), [e1] "v"(oe[1]),
+          [e4] "v"(oe[4]), [e5] "v"(oe[5]), [mb] "s"(mb), [kmax] "s"(kmax), [kgmax] "s"(kgmax), [kone] "s"(kone),
+          [ktwo] "s"(ktwo), [w00] "v"(pw[0][0]), [w01] "v"(pw[0][1]), [w10] "v"(pw[1][0]), [w11] "v"(pw[1][1]),
+          [u00] "v"(pu[0][0]), [u01] "v"(pu[0][1]), [u10] "v"(pu[1][0]), [u11] "v"(pu[1][1]), [r00] "v"(px[0][0]),
+          [r01] "v"(px[0][1]), [r10] "v"(px[1][0]), [r11] "v"(px[1][1])
+        : "v64", "v65", "v66", "v67", "v68", "v69", FB_CL10(7), FB_CL10(8), FB_CL10(9), FB_CL10(10), FB_CL10(11),
+          FB_CL10(12), FB_CL10(13), FB_CL10(14), FB_CL10(15), "v160", "v161", "v162", "v163", "v164", "v165", "v166",
+          "v167", "m0", "scc", "memory");
+    }
+
+    // Block (i, j): lane holds output row m0 + TM / 2 wm + 32 j + n32.
+    if (SPLIT && t.partial) {
+        f32x4 *dst = reinterpret_cast<f32x4 *>(a.tile.part) +
+                     ((size_t)t.tile * a.tile.split + t.share) * (TM * PIPE_N / 4) + tid;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            if (m0 + wm * (TM / 2) + j * 32 >= a.m) break;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                hold(c[i][j]);
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    dst[((j * 4 + i) * 4 + g) * 256] =
+                        f32x4{c[i][j][4 * g], c[i][j][4 * g + 1], c[i][j][4 * g + 2], c[i][j][4 * g + 3]};
+            }
+        }
+        return;
+    }
+    // Behind the last tile no wave reads its fragments any more once all have arrived here.
+    if constexpr (SWIGLU || EPI == EPI_ANY) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) hold(c[i][j]);
+        pipe_epilogue<EPI>(a, m0 + wm * (TM / 2) + j * 32, n0, wm, wn, lane, c[0][j], c[1][j], c[2][j], c[3][j], lds);
+    }
+}
+
+// The split tiles' shares added in order, and the epilogue. One workgroup per (tile, row block).
+template <int EPI, int TM>
+__global__ __launch_bounds__(PIPE_T) void fp8_block_pipe_reduce(Fp8BlockGemmArgs a) {
+    constexpr unsigned NJ = TM / 64;
+    __shared__ __attribute__((aligned(16))) uint8_t scratch[EPI == EPI_ANY ? ANY_LDS : 512];
+    const unsigned tile = blockIdx.x / NJ, j = blockIdx.x % NJ, tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    unsigned m0, n0;
+    pipe_tile<TM>(a, split_tile(a.tile, tile), m0, n0);
+    const unsigned row0 = m0 + wave / 2 * (TM / 2) + j * 32;
+    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tile.part) + (size_t)tile * a.tile.split * (TM * PIPE_N / 4) +
+                       j * 16 * 256 + tid;
+    f32x16 c[4] = {};
+    // A row block past M: no share was written.
+    for (unsigned s = 0; row0 < a.m && s < a.tile.split; s++, src += TM * PIPE_N / 4)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const f32x4 v = src[(i * 4 + g) * 256];
+#pragma unroll
+                for (int e = 0; e < 4; e++) c[i][4 * g + e] += v[e];
+            }
+    pipe_epilogue<EPI>(a, row0, n0, wave / 2, wave % 2, lane, c[0], c[1], c[2], c[3], scratch);
+}
+
+template <int EPI> int launch_mid(h3_gpu *g, Fp8BlockGemmArgs a, unsigned split) {
     static bool configured = false;
     if (!configured) {
-        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)fp8_block_mid, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                 MID_LDS), "FP8 block GEMM shared memory"))
+        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)fp8_block_mid<EPI>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, MID_LDS),
+                          "FP8 block GEMM shared memory"))
             return 0;
         configured = true;
     }
@@ -281,17 +890,108 @@ int launch_mid(h3_gpu *g, Fp8BlockGemmArgs a, unsigned split) {
     const unsigned rest = tiles - a.tile.full;
     h3_note_kernel(g, "fp8_block_mid", MID_M, a.tile.split);
     hipEvent_t timing = h3_kernel_timing_begin(g);
-    hipLaunchKernelGGL(fp8_block_mid, dim3(a.tile.full + rest * a.tile.split), dim3(MID_T), MID_LDS, g->compute, a);
+    hipLaunchKernelGGL((fp8_block_mid<EPI>), dim3(a.tile.full + rest * a.tile.split), dim3(MID_T), MID_LDS,
+                       g->compute, a);
     if (rest && h3_launch_status(g, "FP8 block GEMM"))
-        hipLaunchKernelGGL(fp8_block_mid_reduce, dim3(rest * 2), dim3(MID_T), 0, g->compute, a);
+        hipLaunchKernelGGL((fp8_block_mid_reduce<EPI>), dim3(rest), dim3(MID_T), 0, g->compute, a);
     h3_kernel_timing_end(g, timing);
     return h3_launch_status(g, "FP8 block GEMM");
 }
 
+template <int EPI, int TM> int launch_pipe(h3_gpu *g, Fp8BlockGemmArgs a, unsigned split) {
+    constexpr unsigned shared = pipe_lds<TM>();
+    static bool configured = false;
+    if (!configured) {
+        for (const void *kernel : {(const void *)fp8_block_pipe<EPI, false, TM>, (const void *)fp8_block_pipe<EPI, true, TM>})
+            if (!h3_hip_check(g, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, shared),
+                              "FP8 block GEMM shared memory"))
+                return 0;
+        configured = true;
+    }
+    const unsigned tiles = (a.m + TM - 1) / TM * ((a.n + PIPE_N - 1) / PIPE_N), quads = (a.k / TK + QUAD - 1) / QUAD;
+    a.tile = split_last_wave(g, tiles, split, quads, TM * PIPE_N);
+    const unsigned rest = tiles - a.tile.full;
+    h3_note_kernel(g, "fp8_block_pipe", TM, a.tile.split);
+    hipEvent_t timing = h3_kernel_timing_begin(g);
+    if (!rest) {
+        hipLaunchKernelGGL((fp8_block_pipe<EPI, false, TM>), dim3(tiles), dim3(PIPE_T), shared, g->compute, a);
+    } else {
+        hipLaunchKernelGGL((fp8_block_pipe<EPI, true, TM>), dim3(a.tile.full + rest * a.tile.split), dim3(PIPE_T), shared,
+                           g->compute, a);
+        if (h3_launch_status(g, "FP8 block GEMM"))
+            hipLaunchKernelGGL((fp8_block_pipe_reduce<EPI, TM>), dim3(rest * (TM / 64)), dim3(PIPE_T), 0, g->compute, a);
+    }
+    h3_kernel_timing_end(g, timing);
+    return h3_launch_status(g, "FP8 block GEMM");
+}
+
+// ---------------------------------------------------------------- choice
+// The kernel whose modelled time is least. Tiles by gemm_last_wave: 64 rows (a unit is a K step
+// of 128), 128 and 256 rows (four of them), rates fitted to the measured times of all three in
+// one to nine shares at 112 projections of 17 to 8000 rows (K 256 to 14336, N 777 to 28672);
+// the choice is 1% slower than the best of them in the mean. Few rows: a workgroup's rounds on
+// the busiest CU by its K steps, a step 0.13 to 0.43 us as it has more rows and columns.
+// Measured, in us, the runner-up in brackets: 1 row, 7168 -> 5376: 9.3 (tiles of 64 rows in 6
+// shares 17); 32 rows, 5376 -> 21504: tiles of 64 in 3 shares 28 (few rows 36); 301 rows, 5376
+// -> 21504: 128 rows 44 (256 rows 63); 1024 rows, 7168 -> 5376: 128 rows 39 (256 in two shares
+// 50); 1500 rows, 5376 -> 21504: 256 rows 146 (128 rows 158).
+struct Choice {
+    float us;
+    unsigned rows, split;     // tile rows (64, 128, 256) and shares; or
+    unsigned rb, nb;          // few rows: row and column blocks (rb 0: tiles)
+};
+Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
+    static constexpr GemmRates RATES[3] = {{.66f, .39f, .067f, .15f, 2.8f, .095f, .67f},
+                                           {3.4f, 2.1f, 1.1f, .15f, 3.7f, .055f, 2.9f},
+                                           {5.9f, 3.6f, 2.45f, .15f, 5.5f, .035f, 2.4f}};
+    static constexpr float LAUNCH[3] = {4.2f, 2.4f, 1.9f};
+    const unsigned steps = a.k / TK;
+    Choice best{3.4e38f, 0, 1, 0, 0};
+    for (unsigned i = 0; i < 3; i++) {
+        const unsigned rows = 64u << i, units = i ? (steps + QUAD - 1) / QUAD : steps;
+        const uint64_t tiles = ((uint64_t)a.m + rows - 1) / rows * ((a.n + 255) / 256);
+        if (tiles > 0x7fffffffu) continue;
+        const GemmPlan p = gemm_last_wave(g, (unsigned)tiles, units, RATES[i], rows / 256.f);
+        const float us = (p.us + LAUNCH[i]) * (p.split > 1 ? 1.02f : 1.f);
+        if (us < best.us) best = {us, rows, p.split, 0, 0};
+    }
+    if (!stream || a.m > 256) return best;
+    // us of a step: [row blocks - 1][column blocks 2, 4].
+    static constexpr float STEP[3][2] = {{.16f, .32f}, {.22f, .39f}, {.28f, 0.f}};
+    for (unsigned rb = 1; rb <= 3; rb++)
+        for (unsigned nb = 2; nb <= (rb < 3 ? 4u : 2u); nb += 2) {
+            const unsigned groups = ((a.m + 16 * rb - 1) / (16 * rb)) * ((a.n + 16 * nb - 1) / (16 * nb));
+            const float us = 3.8f + (float)((groups + g->cus - 1) / g->cus * steps) * STEP[rb - 1][nb / 4];
+            if (us < best.us) best = {us, 0, 1, rb, nb};
+        }
+    return best;
+}
+
+template <int EPI> int run(h3_gpu *g, const Fp8BlockGemmArgs &a) {
+    const Choice c = choose(g, a, EPI != EPI_SWIGLU);
+    if constexpr (EPI != EPI_SWIGLU)
+        if (c.rb) return launch_stream<EPI>(g, a, c.rb, c.nb);
+    return c.rows == 256   ? launch_pipe<EPI, 256>(g, a, c.split)
+           : c.rows == 128 ? launch_pipe<EPI, 128>(g, a, c.split)
+                           : launch_mid<EPI>(g, a, c.split);
+}
+
 }  // namespace
 
-bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m) { return m > 0 && g; }
+// Without it the product goes through memory in FP32 and another launch packs it.
+bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m, uint32_t k, uint32_t hidden) {
+    Fp8BlockGemmArgs a{};
+    a.m = m; a.n = 2 * hidden; a.k = (k + TK - 1) / TK * TK;
+    return choose(g, a, false).us <= choose(g, a, true).us + 4.f + (float)m * hidden * 4e-6f;
+}
 
 int h3_gemm_fp8_block(h3_gpu *g, const Fp8BlockGemmArgs &a) {
-    return launch_mid(g, a, 1);
+    if (((uint64_t)a.m + 63) / 64 * ((a.n + 255) / 256) > 0x7fffffffu)
+        return h3_set_error(g, "FP8 block projection: %u rows by %u columns are too many for one call", a.m, a.n);
+    switch (epilogue_of(a)) {
+    case EPI_PLAIN: return run<EPI_PLAIN>(g, a);
+    case EPI_BIAS: return run<EPI_BIAS>(g, a);
+    case EPI_SWIGLU: return run<EPI_SWIGLU>(g, a);
+    default: return run<EPI_ANY>(g, a);
+    }
 }

@@ -166,12 +166,13 @@ h3_gpu_tensor *h3_hip_quant_weight_from_bf16(h3_gpu *gpu, const h3_gpu_tensor *w
  * Work with rows <= the tensor's rows leaves the rows behind as they were.
  *
  * h3_hip_fp8_block_layout: where a matrix has its parts, in bytes: codes of
- * row r from r * stride on (zeros behind `columns`), scales of row r (tile 1)
- * or of rows 128 r to 128 r + 127 from scales + r * scale_stride on; bytes in
- * all. h3_hip_tensor_copy_to_host, h3_hip_tensor_stream_host and
+ * row r from r * stride on (zeros behind `columns`); the scale of block b of
+ * scale row s (row s, or rows 128 s to 128 s + 127 of a weight) at scales +
+ * (s / 32 * groups + b / 4) * 128 + s % 32 * 4 + b % 4; bytes in all.
+ * h3_hip_tensor_copy_to_host, h3_hip_tensor_stream_host and
  * h3_hip_tensor_device_pointer give that memory. 0 on an invalid shape. */
 int h3_hip_fp8_block_layout(uint32_t rows, uint32_t columns, uint32_t tile, size_t *stride,
-                            size_t *scales, size_t *scale_stride, size_t *bytes);
+                            size_t *scales, size_t *groups, size_t *bytes);
 /* A matrix of zeros. */
 h3_gpu_tensor *h3_hip_fp8_block_new(h3_gpu *gpu, uint32_t rows, uint32_t columns, uint32_t tile);
 /* From host memory: codes [rows, columns], scales [ceil(rows / tile)]

@@ -65,9 +65,9 @@ class Packed:
         if not handle:
             raise H3Error(g.error())
         self.g, self.rows, self.columns, self.tile = g, rows, columns, tile
-        stride, scales, scale_stride, size = (C.c_size_t() for _ in range(4))
-        assert g.lib.h3_hip_fp8_block_layout(rows, columns, tile, stride, scales, scale_stride, size)
-        self.stride, self.scales, self.scale_stride, self.bytes = (v.value for v in (stride, scales, scale_stride, size))
+        stride, scales, groups, size = (C.c_size_t() for _ in range(4))
+        assert g.lib.h3_hip_fp8_block_layout(rows, columns, tile, stride, scales, groups, size)
+        self.stride, self.scales, self.groups, self.bytes = (v.value for v in (stride, scales, groups, size))
         self.tensor = g._track(handle, rows * columns, _lib.I8)
         self.handle = handle
 
@@ -81,7 +81,8 @@ class Packed:
         raw = self.raw()
         n = -(-self.rows // self.tile)
         codes = raw[:self.rows * self.stride].reshape(self.rows, self.stride)
-        scales = raw[self.scales:].reshape(n, self.scale_stride)[:, :-(-self.columns // 128)]
+        scales = raw[self.scales:].reshape(-1, self.groups, 32, 4).transpose(0, 2, 1, 3).reshape(-1, self.groups * 4)
+        scales = scales[:n, :-(-self.columns // 128)]
         return codes, scales
 
     def values(self):

@@ -5,9 +5,6 @@ import pytest
 
 from h3cli_amd import _lib
 
-LEAST_SCALES = 16
-
-
 def layout(*args):
     v = [C.c_size_t() for _ in range(4)]
     return tuple(x.value for x in v) if _lib.load().h3_hip_fp8_block_layout(*args, *v) else None
@@ -16,12 +13,12 @@ def layout(*args):
 @pytest.mark.parametrize("rows,columns,tile", [(1, 1, 1), (1, 128, 1), (7, 129, 1), (128, 5376, 128), (129, 1000, 128),
                                                (100000, 14336, 1), (1 << 20, 8192, 1), (3, (1 << 24) - 128, 128)])
 def test_layout(rows, columns, tile):
-    stride, scales, scale_stride, size = layout(rows, columns, tile)
+    stride, scales, groups, size = layout(rows, columns, tile)
     blocks = -(-columns // 128)
     assert stride == 128 * blocks
     assert scales % 256 == 0 and rows * stride <= scales < rows * stride + 256
-    assert scale_stride % LEAST_SCALES == 0 and blocks <= scale_stride < blocks + LEAST_SCALES
-    assert size == scales + -(-rows // tile) * scale_stride
+    assert groups == -(-blocks // 4)
+    assert size == scales + -(--(-rows // tile) // 32) * groups * 128
 
 
 def test_layout_refuses():
