@@ -128,13 +128,13 @@ __global__ __launch_bounds__(256) void adaln_kernel(AdaLNArgs a) {
                 for (int e = 0; e < 8; e++) {
                     y[e] = bf16_to_f32(raw[i][e]) * inv * bf16_to_f32(wr[e]);
                     if constexpr (!PLAIN) y[e] = fmaf(y[e], 1.0f + bf16_to_f32(sc[e]), bf16_to_f32(sh[e]));
-                    amax = max(amax, finite_magnitude(y[e], bad));
                 }
+                amax = fp8_block_magnitude<8>(y, bad);
             }
             const unsigned scale = fp8_block_scale(lanes_max<16>(amax));
-            const float inverse = fp8_block_inverse(scale);
+            const float value = fp8_block_value(scale);
             *reinterpret_cast<uint2 *>(a.packed.codes + (size_t)row * a.packed.stride + c * 8) =
-                make_uint2(fp8_block_encode4(y, inverse), fp8_block_encode4(y + 4, inverse));
+                make_uint2(fp8_block_encode4(y, value), fp8_block_encode4(y + 4, value));
             if (c % 16 == 0) a.packed.scales[fp8_block_scale_at(row, c / 16, a.packed.groups)] = (uint8_t)scale;
         }
         if (bad) *a.packed.fault = 1u;

@@ -52,15 +52,25 @@ struct Fp8BlockRows {
 };
 
 #if defined(__HIPCC__)
-// Magnitude bits of a finite value; a non-finite one counts as zero and sets bad. (The opaque
-// step keeps the compiler, which assumes that no value is NaN, from folding the test.)
-__device__ inline unsigned finite_magnitude(float v, bool &bad) {
-    unsigned u = __builtin_bit_cast(unsigned, v);
-    asm("" : "+v"(u));
-    u &= 0x7fffffffu;
-    const bool wrong = u >= 0x7f800000u;
-    bad |= wrong;
-    return wrong ? 0u : u;
+// Largest magnitude of N values as its bits, whose order is that of the values. Values that are
+// not finite set bad and count as zero; they are looked for in the maximum only, above all of
+// which they are. (The opaque step keeps the compiler, which assumes that no value is NaN, from
+// folding the test.)
+template <int N> __device__ inline unsigned fp8_block_magnitude(const float *v, bool &bad) {
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++) m = max(m, __builtin_bit_cast(unsigned, v[e]) & 0x7fffffffu);
+    asm("" : "+v"(m));
+    if (m >= 0x7f800000u) {
+        bad = true;
+        m = 0;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const unsigned u = __builtin_bit_cast(unsigned, v[e]) & 0x7fffffffu;
+            m = max(m, u >= 0x7f800000u ? 0u : u);
+        }
+    }
+    return m;
 }
 // Scale byte of a block whose largest magnitude has these bits: the least e >= -64 with
 // amax <= 448 * 2^e. 448 = 1.75 * 2^8, so e = exponent - 8, one more if the mantissa is
@@ -69,12 +79,15 @@ __device__ inline unsigned fp8_block_scale(unsigned amax) {
     const int e = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
     return (unsigned)max(e, FP8_BLOCK_LEAST + 127);
 }
-// 2^-e of a scale byte (63 to 247), for the encoding.
-__device__ inline float fp8_block_inverse(unsigned scale) { return __builtin_bit_cast(float, (254u - scale) << 23); }
-// Four codes of v * inverse: round to nearest even; |v * inverse| <= 448.
-__device__ inline unsigned fp8_block_encode4(const float *v, float inverse) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inverse, v[1] * inverse, 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inverse, v[3] * inverse, w, true);
+// The scale's value, for the encoding.
+__device__ inline float fp8_block_value(unsigned scale) { return __builtin_bit_cast(float, scale << 23); }
+// Four codes of v / 2^e: round to nearest even; |v| <= 448 * 2^e.
+__device__ inline unsigned fp8_block_encode4(const float *v, float value) {
+    typedef short i16x2 __attribute__((ext_vector_type(2)));
+    i16x2 w = {};
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[0], v[1], value, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[2], v[3], value, true);
+    return __builtin_bit_cast(unsigned, w);
 }
 // Largest of `lanes` neighbouring lanes (a power of two up to 64).
 template <int LANES> __device__ inline unsigned lanes_max(unsigned v) {
@@ -84,20 +97,17 @@ template <int LANES> __device__ inline unsigned lanes_max(unsigned v) {
 }
 // silu(gate) * up = gate / (1 + exp(-gate)) * up in FP32, each step within about a unit in
 // the last place, because a code flips where the value crosses a midpoint: exp(-gate) as 2^hi
-// (1 + lo ln 2) with the product's rounding error in lo, and the reciprocal with a Newton
-// step, on (1 + exp) / 16, whose reciprocal is normal up to exp's overflow, where the result
-// is zero.
+// (1 + lo ln 2) with the product's rounding error in lo, and the reciprocal with a Newton step.
+// Below gate = -87, where the reciprocal leaves FP32's normal range, the result is zero: it
+// is under 1.5e-36 |up| (not a number where the gate is infinite).
 __device__ inline float swiglu_exact(float gate, float up) {
     constexpr float L = 1.4426950408889634f, L_LOW = 1.9259629911266175e-8f, LN2 = 0.6931471805599453f;
-    const float x = __builtin_amdgcn_fmed3f(gate, -128.f, 128.f);      // exp(-x) is 0 beside 1, or infinite, outside
+    const float x = __builtin_amdgcn_fmed3f(gate, -87.f, 128.f);       // exp(-128) is nothing beside 1
     const float hi = -x * L, lo = -fmaf(x, L, hi) - x * L_LOW;
-    float e = __builtin_amdgcn_exp2f(hi);
-    e = e < 3e38f ? fmaf(e, lo * LN2, e) : 3e38f;
-    const float d = fmaf(e, 0.0625f, 0.0625f);
+    const float e = __builtin_amdgcn_exp2f(hi), d = 1.f + fmaf(e, lo * LN2, e);
     float r = __builtin_amdgcn_rcpf(d);
-    r = fmaf(fmaf(-d, r, 1.f), r, r);
-    r = e < 3e38f ? r : 0.f;
-    return gate * 0.0625f * r * up;
+    r = gate < -87.f ? 0.f : fmaf(fmaf(-d, r, 1.f), r, r);
+    return gate * r * up;
 }
 #endif
 

@@ -49,16 +49,9 @@ __device__ inline void load16(const T *row, unsigned col, unsigned columns, floa
 
 // The 16 codes of a lane whose block has this scale.
 __device__ inline u32x4 encode16(const float *v, unsigned scale) {
-    const float inverse = fp8_block_inverse(scale);
-    return u32x4{fp8_block_encode4(v, inverse), fp8_block_encode4(v + 4, inverse), fp8_block_encode4(v + 8, inverse),
-                 fp8_block_encode4(v + 12, inverse)};
-}
-
-__device__ inline unsigned magnitude16(const float *v, bool &bad) {
-    unsigned m = 0;
-#pragma unroll
-    for (unsigned e = 0; e < LANE; e++) m = max(m, finite_magnitude(v[e], bad));
-    return m;
+    const float value = fp8_block_value(scale);
+    return u32x4{fp8_block_encode4(v, value), fp8_block_encode4(v + 4, value), fp8_block_encode4(v + 8, value),
+                 fp8_block_encode4(v + 12, value)};
 }
 
 // PACK: values of rows [rows, columns]. SWIGLU: silu(gate) * up of rows that hold `columns`
@@ -80,7 +73,7 @@ __global__ __launch_bounds__(256) void fp8_block_pack(const T *in, Fp8BlockRows 
         for (unsigned e = 0; e < LANE; e++) v[e] = swiglu_exact(v[e], up[e]);
     }
     bool bad = false;
-    const unsigned scale = fp8_block_scale(lanes_max<LANES>(magnitude16(v, bad)));
+    const unsigned scale = fp8_block_scale(lanes_max<LANES>(fp8_block_magnitude<LANE>(v, bad)));
     if (bad) *out.fault = 1u;
     *reinterpret_cast<u32x4 *>(out.codes + (size_t)row * out.stride + col) = encode16(v, scale);
     if (id % LANES == 0) out.scales[fp8_block_scale_at(row, block, out.groups)] = (uint8_t)scale;
@@ -99,7 +92,7 @@ __global__ __launch_bounds__(256) void fp8_block_pack_weight(const uint16_t *in,
     float v[LANE];
     for (unsigned at = r; at < FP8_BLOCK && r0 + at < rows; at += 32) {
         load16<VEC>(in + (size_t)(r0 + at) * columns, col, columns, v);
-        amax = max(amax, magnitude16(v, bad));
+        amax = max(amax, fp8_block_magnitude<LANE>(v, bad));
     }
     if (bad) *out.fault = 1u;
     amax = lanes_max<64>(amax);

@@ -234,13 +234,10 @@ __device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, un
         return;
     }
     float v[16];
-    unsigned amax = 0;
     bool bad = false;
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-        v[e] = swiglu_exact(c0[e], c1[e]);
-        amax = max(amax, finite_magnitude(v[e], bad));
-    }
+    for (int e = 0; e < 16; e++) v[e] = swiglu_exact(c0[e], c1[e]);
+    unsigned amax = fp8_block_magnitude<16>(v, bad);
     if (bad && row < a.m) *a.out.fault = 1u;
     amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
     if (hf == 0) most[wm][wn][n32] = amax;
@@ -248,10 +245,10 @@ __device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, un
     const unsigned scale = fp8_block_scale(max(max(most[wm][0][n32], most[wm][1][n32]), max(most[wm][2][n32], most[wm][3][n32])));
     __syncthreads();
     if (row >= a.m) return;
-    const float inverse = fp8_block_inverse(scale);
+    const float value = fp8_block_value(scale);
     uint8_t *dst = a.out.codes + (size_t)row * a.out.stride + n0 / 2 + wn * 32 + hf * 4;
 #pragma unroll
-    for (int g = 0; g < 4; g++) *reinterpret_cast<unsigned *>(dst + g * 8) = fp8_block_encode4(v + 4 * g, inverse);
+    for (int g = 0; g < 4; g++) *reinterpret_cast<unsigned *>(dst + g * 8) = fp8_block_encode4(v + 4 * g, value);
     if (wn == 0 && hf == 0) a.out.scales[fp8_block_scale_at(row, n0 / 256, a.out.groups)] = (uint8_t)scale;
 }
 
@@ -668,27 +665,26 @@ __device__ inline void pipe_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, u
         return;
     }
     float v[32];
-    unsigned amax = 0;
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
         v[e] = swiglu_exact(c0[e], c1[e]);
         v[16 + e] = swiglu_exact(c2[e], c3[e]);
-        amax = max(amax, max(finite_magnitude(v[e], bad), finite_magnitude(v[16 + e], bad)));
     }
+    unsigned amax = fp8_block_magnitude<32>(v, bad);
     if (bad && row < a.m) *a.out.fault = 1u;
     amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
     if (hf == 0) most[wm][wn][n32] = amax;
     __syncthreads();
     const unsigned scale = fp8_block_scale(max(most[wm][0][n32], most[wm][1][n32]));
     __syncthreads();
-    const float inverse = fp8_block_inverse(scale);
+    const float value = fp8_block_value(scale);
     // Groups g and g + 1 go out together, eight codes a lane.
     uint8_t *dst = a.out.codes + (size_t)row * a.out.stride + n0 / 2 + wn * 64 + hf * 8;
 #pragma unroll
     for (int g = 0; g < 8; g += 2) {
-        const auto s = __builtin_amdgcn_permlane32_swap(fp8_block_encode4(v + 4 * g, inverse),
-                                                        fp8_block_encode4(v + 4 * g + 4, inverse), false, false);
+        const auto s = __builtin_amdgcn_permlane32_swap(fp8_block_encode4(v + 4 * g, value),
+                                                        fp8_block_encode4(v + 4 * g + 4, value), false, false);
         if (row < a.m) *reinterpret_cast<uint2 *>(dst + g * 8) = make_uint2(s[0], s[1]);
     }
     if (row < a.m && wn == 0 && hf == 0) a.out.scales[fp8_block_scale_at(row, n0 / 256, a.out.groups)] = (uint8_t)scale;
