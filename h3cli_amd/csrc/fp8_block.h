@@ -118,12 +118,18 @@ struct Fp8BlockGemmArgs {
     Fp8BlockRows out;           // silu(gate) * up packed [m, n / 2]: w holds gate rows, then up rows
     const uint16_t *bias;       // [n], y only
     const uint8_t *x, *w;       // codes, rows of k bytes (a multiple of 128)
+    const uint16_t *xb;         // BF16 rows of `columns` values instead of x and xs, only where
+    unsigned columns;           // h3_gemm_fp8_block_packs; a value that is not finite sets fault
+    unsigned *fault;
     const uint8_t *xs, *ws;     // scales; a scale row of w per 128 rows
     unsigned m, n, k, groups;
     bool swiglu;                // n / 2 a multiple of 128
     TileSplit tile;             // set by the kernels' launchers
 };
 int h3_gemm_fp8_block(h3_gpu *g, const Fp8BlockGemmArgs &a);
+// Whether the projection would better pack a BF16 input itself than read a packed one (the
+// same result bit for bit).
+bool h3_gemm_fp8_block_packs(const h3_gpu *g, const Fp8BlockGemmArgs &a);
 // Whether the SwiGLU variant is faster as one launch than as y32 and h3_launch_swiglu_fp8_block.
 bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m, uint32_t k, uint32_t hidden);
 // Packs silu(gate) * up of FP32 or BF16 rows [rows, 2 * width].

@@ -182,10 +182,9 @@ Fp8BlockRows workspace_rows(h3_gpu *g, void *data, uint32_t rows, uint32_t colum
     return {(uint8_t *)data, (uint8_t *)data + l.scales, (unsigned)l.stride, (unsigned)l.groups, g->fault + 2};
 }
 
-Fp8BlockGemmArgs gemm_args(const Fp8BlockRows &x, const h3_gpu_tensor *w, uint32_t rows, uint32_t n) {
+Fp8BlockGemmArgs gemm_args(const h3_gpu_tensor *w, uint32_t rows, uint32_t n) {
     const Fp8BlockLayout lw = layout_of(w);
     Fp8BlockGemmArgs a{};
-    a.x = x.codes; a.xs = x.scales;
     a.w = (const uint8_t *)w->data; a.ws = (const uint8_t *)w->data + lw.scales;
     a.m = rows; a.n = n; a.k = (unsigned)lw.stride; a.groups = (unsigned)lw.groups;
     return a;
@@ -352,26 +351,35 @@ extern "C" int h3_hip_swiglu_fp8_block(h3_gpu *g, h3_gpu_tensor *out, const h3_g
 }
 
 // ------------------------------------------------------------------ projections
-// The packed rows of a projection's input: as they are, or a BF16 input packed into `workspace`
-// bytes of the context's buffer from `at` on. Refused while the stream is being captured: a
-// graph would keep the buffer's address, which later calls use and, growing it, free.
-static int packed_input(h3_gpu *g, const h3_gpu_tensor *in, uint32_t rows, uint32_t k, size_t extra, const char *what,
-                        Fp8BlockRows *x, char **rest) {
-    const bool pack = in && !in->block_tile;
-    const size_t own = pack ? (fp8_block_layout(rows, k, 1).bytes + 511) & ~(size_t)255 : 0;
-    if (pack ? !h3_require(g, in, H3_GPU_BF16, (size_t)rows * k, what) : !h3_require_fp8_block(g, in, 1, rows, k, what))
+// The input of a projection (a.m rows of k columns; a's output and weight are set): packed rows
+// as they are, a BF16 input packed by the projection itself or here, into the context's
+// workspace, whose `extra` bytes behind it *rest is. Refused while the stream is being captured:
+// a graph would keep the workspace's address, which later calls use and, growing it, free.
+static int projection_input(h3_gpu *g, const h3_gpu_tensor *in, uint32_t k, size_t extra, const char *what,
+                            Fp8BlockGemmArgs &a, char **rest) {
+    if (in && in->block_tile) {
+        if (!h3_require_fp8_block(g, in, 1, a.m, k, what)) return 0;
+    } else if (!h3_require(g, in, H3_GPU_BF16, (size_t)a.m * k, what)) {
         return 0;
-    if (own + extra) {
-        if (h3_capturing(g)) return h3_set_error(g, "%s: needs a workspace, but the compute stream is being captured", what);
-        if (!h3_buffer_reserve(g, &g->block_workspace, own + extra, what)) return 0;
     }
+    const bool pack = !in->block_tile;
+    if ((pack || extra) && h3_capturing(g))
+        return h3_set_error(g, "%s: needs a workspace, but the compute stream is being captured", what);
+    const bool inside = pack && h3_gemm_fp8_block_packs(g, a);
+    const size_t own = pack && !inside ? (fp8_block_layout(a.m, k, 1).bytes + 511) & ~(size_t)255 : 0;
+    if (own + extra && !h3_buffer_reserve(g, &g->block_workspace, own + extra, what)) return 0;
     *rest = (char *)g->block_workspace.ptr + own;
-    if (!pack) {
-        *x = h3_fp8_block_rows(g, in);
-        return h3_tensor_acquire(g, in);
+    if (!h3_tensor_acquire(g, in)) return 0;
+    if (inside) {
+        a.xb = (const uint16_t *)in->data;
+        a.columns = k;
+        a.fault = g->fault + 2;
+        return 1;
     }
-    *x = workspace_rows(g, g->block_workspace.ptr, rows, k);
-    return launch_pack<false>(g, (const uint16_t *)in->data, *x, rows, k, "FP8 block packing");
+    const Fp8BlockRows x = pack ? workspace_rows(g, g->block_workspace.ptr, a.m, k) : h3_fp8_block_rows(g, in);
+    a.x = x.codes;
+    a.xs = x.scales;
+    return !pack || launch_pack<false>(g, (const uint16_t *)in->data, x, a.m, k, "FP8 block packing");
 }
 
 int h3_fp8_block_linear(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *w,
@@ -383,13 +391,11 @@ int h3_fp8_block_linear(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, 
         (bias && !h3_require(g, bias, H3_GPU_BF16, n, "linear bias")))
         return 0;
     if (overlap(out, in) || overlap(out, bias)) return h3_set_error(g, "linear: output aliases input");
-    Fp8BlockRows x;
-    char *rest;
-    if (!packed_input(g, in, rows, k, 0, "linear input", &x, &rest)) return 0;
-    Fp8BlockGemmArgs a = gemm_args(x, w, rows, n);
+    Fp8BlockGemmArgs a = gemm_args(w, rows, n);
     a.y = (uint16_t *)out->data;
     a.bias = bias ? (const uint16_t *)bias->data : nullptr;
-    return run_gemm(g, w, a) && (!in->block_tile || h3_tensor_release(g, in));
+    char *rest;
+    return projection_input(g, in, k, 0, "linear input", a, &rest) && run_gemm(g, w, a) && h3_tensor_release(g, in);
 }
 
 int h3_fp8_block_mlp(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *w1,
@@ -409,25 +415,32 @@ int h3_fp8_block_mlp(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, con
     const size_t row_bytes = fp8_block_layout(1, hidden, 1).bytes + (fused ? 0 : (size_t)hidden * 8);
     const uint32_t most = (uint32_t)std::min<size_t>(std::max<size_t>(MLP_WORKSPACE / row_bytes / 256, 1) * 256, rows);
     const size_t act = (fp8_block_layout(most, hidden, 1).bytes + 511) & ~(size_t)255;
-    Fp8BlockRows x;
+    Fp8BlockGemmArgs all = gemm_args(w1, rows, 2 * hidden);
+    all.swiglu = fused;
     char *rest;
-    if (!packed_input(g, in, rows, k, act + (fused ? 0 : (size_t)most * hidden * 8), "MLP input", &x, &rest)) return 0;
+    if (!projection_input(g, in, k, act + (fused ? 0 : (size_t)most * hidden * 8), "MLP input", all, &rest)) return 0;
     for (uint32_t first = 0; first < rows; first += most) {
         const uint32_t m = std::min(most, rows - first);
-        // first is a multiple of 256: whole runs of 32 scale rows.
-        const Fp8BlockRows part = {x.codes + (size_t)first * x.stride, x.scales + fp8_block_scale_at(first, 0, x.groups),
-                                   x.stride, x.groups, x.fault};
         const Fp8BlockRows h = workspace_rows(g, rest, m, hidden);
-        Fp8BlockGemmArgs a = gemm_args(part, w1, m, 2 * hidden);
-        a.swiglu = fused;
+        // first is a multiple of 256: whole runs of 32 scale rows.
+        Fp8BlockGemmArgs a = all;
+        a.m = m;
+        if (a.xb) {
+            a.xb += (size_t)first * k;
+        } else {
+            a.x += (size_t)first * a.k;
+            a.xs += fp8_block_scale_at(first, 0, a.groups);
+        }
         if (fused) a.out = h;
         else a.y32 = (float *)(rest + act);
         if (!run_gemm(g, w1, a) || (!fused && !h3_launch_swiglu_fp8_block(g, h, a.y32, true, m, hidden))) return 0;
-        Fp8BlockGemmArgs b = gemm_args(h, w2, m, n);
+        Fp8BlockGemmArgs b = gemm_args(w2, m, n);
+        b.x = h.codes;
+        b.xs = h.scales;
         b.y = (uint16_t *)out->data + (size_t)first * n;
         if (!run_gemm(g, w2, b)) return 0;
     }
-    return !in->block_tile || h3_tensor_release(g, in);
+    return h3_tensor_release(g, in);
 }
 
 extern "C" int h3_hip_linear_fp8_block(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *w,

@@ -9,6 +9,7 @@
 #include "fp8_block.h"
 #include "internal.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -38,6 +39,7 @@ int epilogue_of(const Fp8BlockGemmArgs &a) {
 // Four values wherever they lie: global loads and stores need no alignment.
 struct __attribute__((packed, aligned(2))) u16x4_any { uint16_t v[4]; };
 struct __attribute__((packed, aligned(2))) u16x2_any { uint16_t v[2]; };
+struct __attribute__((packed, aligned(2))) u32x4_any { u32x4 v; };
 
 // Four columns of an output row.
 template <int EPI>
@@ -86,12 +88,14 @@ __device__ inline unsigned swiglu_row(unsigned r) { return r / 64 * 32 + r % 32;
 // the K steps in turn, so that together they read consecutive bytes of every weight row,
 // straight into registers; their sums meet in LDS, added in wave order. x and the scales come
 // from L2, which all workgroups share, as the operands of v_mfma_scale_f32_16x16x128_f8f6f4.
+// PACK: x is BF16 and every workgroup packs it for itself, where that is less than the launch it
+// saves (1 row, 256 -> 5376: 4.3 us, 8.0 with a launch of its own).
 //
 // HBM-bound: 1 row, 5376 -> 32256 (173 MB): 32 us, 5.4 TB/s, 4 us of them a launch's; 16 rows
 // 36, as x's reads weigh more. One row of the tile kernels: 37.
 template <int RB, int NB, int WAVES> constexpr int stream_lds() { return WAVES * NB * RB * 64 * 16; }
 
-template <int EPI, int RB, int NB, int WAVES, int U>
+template <int EPI, bool PACK, int RB, int NB, int WAVES, int U>
 __global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs a, unsigned groups) {
     static_assert(U == 2 || U == 3, "steps of a call");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -101,12 +105,19 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs 
     // Rows past M and columns past N repeat the last one; not stored. An operand's 32 bytes of a
     // step are two 16-byte pieces that lie beside those of the row's other lanes (which K value
     // of the step a byte is does not matter where W and x agree).
-    const uint8_t *xp[RB], *wp[NB], *xsp[RB];
+    using X = std::conditional_t<PACK, uint16_t, uint8_t>;
+    constexpr int XV = 2 * sizeof(X);         // 16-byte loads of an operand of x
+    const X *xp[RB];
+    const uint8_t *wp[NB], *xsp[RB];
 #pragma unroll
     for (int i = 0; i < RB; i++) {
         const unsigned row = min(m0 + i * 16 + r, a.m - 1);
-        xp[i] = a.x + (size_t)row * a.k + 16 * q;
-        xsp[i] = a.xs + fp8_block_scale_at(row, 0, a.groups);
+        if constexpr (PACK) {
+            xp[i] = a.xb + (size_t)row * a.columns + 16 * q;
+        } else {
+            xp[i] = a.x + (size_t)row * a.k + 16 * q;
+            xsp[i] = a.xs + fp8_block_scale_at(row, 0, a.groups);
+        }
     }
 #pragma unroll
     for (int i = 0; i < NB; i++) wp[i] = a.w + (size_t)min(n0 + i * 16 + r, a.n - 1) * a.k + 16 * q;
@@ -117,9 +128,34 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs 
 #pragma unroll
         for (int j = 0; j < RB; j++) acc[i][j] = f32x4{};
 
+    // BF16 values of a step, as fp8_block_pack packs them: a row's four lanes hold a block.
+    auto pack = [&](unsigned step, u32x4 *x) {
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+            const unsigned word = x[e / 8][e % 8 / 2];
+            v[e] = __builtin_bit_cast(float, e % 2 ? word & 0xffff0000u : word << 16);
+        }
+        if ((step + 1) * TK > a.columns)      // the last block is cut off
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+                if (step * TK + 64 * (e / 16) + 16 * q + e % 16 >= a.columns) v[e] = 0.f;
+        bool bad = false;
+        unsigned amax = fp8_block_magnitude<32>(v, bad);
+        if (bad) *a.fault = 1u;
+        amax = max(amax, (unsigned)__shfl_xor((int)amax, 16, 64));
+        amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
+        const unsigned scale = fp8_block_scale(amax);
+        const float value = fp8_block_value(scale);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) x[h][w] = fp8_block_encode4(v + 16 * h + 4 * w, value);
+        return (int)scale;
+    };
     auto run = [&](unsigned s, auto count) {
         constexpr int C = decltype(count)::value;
-        u32x4 w[C][NB][2], x[C][RB][2];
+        u32x4 w[C][NB][2], x[C][RB][XV];
         int ws[C], xs[C][RB];
 #pragma unroll
         for (int c = 0; c < C; c++) {
@@ -132,22 +168,27 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs 
             ws[c] = wsp[at];
 #pragma unroll
             for (int j = 0; j < RB; j++) {
-                xs[c][j] = xsp[j][at];
+                if constexpr (!PACK) xs[c][j] = xsp[j][at];
 #pragma unroll
-                for (int h = 0; h < 2; h++) x[c][j][h] = *reinterpret_cast<const u32x4 *>(xp[j] + k + 64 * h);
+                for (int h = 0; h < XV; h++)
+                    x[c][j][h] = reinterpret_cast<const u32x4_any *>(xp[j] + k + 64 * (h * 2 / XV) + 8 * (h % (XV / 2)))->v;
             }
         }
         auto whole = [](const u32x4 *v) {
             return i32x8{(int)v[0][0], (int)v[0][1], (int)v[0][2], (int)v[0][3], (int)v[1][0], (int)v[1][1], (int)v[1][2], (int)v[1][3]};
         };
 #pragma unroll
-        for (int c = 0; c < C; c++)
+        for (int c = 0; c < C; c++) {
+            if constexpr (PACK)
+#pragma unroll
+                for (int j = 0; j < RB; j++) xs[c][j] = pack(s + c * WAVES, x[c][j]);
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
                 for (int j = 0; j < RB; j++)
                     acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(whole(w[c][i]), whole(x[c][j]), acc[i][j], 0, 0,
                                                                                  0, ws[c], 0, xs[c][j]);
+        }
     };
     unsigned s = wave;
     for (; s + (U - 1) * WAVES < steps; s += U * WAVES) run(s, std::integral_constant<int, U>{});
@@ -176,21 +217,21 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs 
     }
 }
 
-template <int EPI, int RB, int NB, int WAVES, int U>
+template <int EPI, bool PACK, int RB, int NB, int WAVES, int U>
 int launch_stream_as(h3_gpu *g, const Fp8BlockGemmArgs &a) {
     constexpr int shared = stream_lds<RB, NB, WAVES>();
     static_assert(shared <= 65536, "LDS without an attribute");
     const unsigned groups = (a.m + 16 * RB - 1) / (16 * RB), columns = (a.n + 16 * NB - 1) / (16 * NB);
-    h3_note_kernel(g, "fp8_block_stream", 16 * RB);
-    hipLaunchKernelGGL((fp8_block_stream<EPI, RB, NB, WAVES, U>), dim3(columns * groups), dim3(64 * WAVES), shared, g->compute,
-                       a, groups);
+    h3_note_kernel(g, PACK ? "fp8_block_stream packing" : "fp8_block_stream", 16 * RB);
+    hipLaunchKernelGGL((fp8_block_stream<EPI, PACK, RB, NB, WAVES, U>), dim3(columns * groups), dim3(64 * WAVES), shared,
+                       g->compute, a, groups);
     return h3_launch_status(g, "FP8 block GEMM");
 }
 // Row blocks and column blocks of a workgroup.
-template <int EPI> int launch_stream(h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
-    return rb == 1 ? nb == 2 ? launch_stream_as<EPI, 1, 2, 8, 3>(g, a) : launch_stream_as<EPI, 1, 4, 8, 2>(g, a)
-           : rb == 2 ? nb == 2 ? launch_stream_as<EPI, 2, 2, 4, 3>(g, a) : launch_stream_as<EPI, 2, 4, 4, 3>(g, a)
-                     : launch_stream_as<EPI, 3, 2, 4, 2>(g, a);
+template <int EPI, bool PACK> int launch_stream(h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
+    return rb == 1 ? nb == 2 ? launch_stream_as<EPI, PACK, 1, 2, 8, 3>(g, a) : launch_stream_as<EPI, PACK, 1, 4, 8, 2>(g, a)
+           : rb == 2 ? nb == 2 ? launch_stream_as<EPI, PACK, 2, 2, 4, 3>(g, a) : launch_stream_as<EPI, PACK, 2, 4, 4, 3>(g, a)
+                     : launch_stream_as<EPI, PACK, 3, 2, 4, 2>(g, a);
 }
 
 // ---------------------------------------------------------------- tiles of 64 rows
@@ -923,24 +964,30 @@ template <int EPI, int TM> int launch_pipe(h3_gpu *g, Fp8BlockGemmArgs a, unsign
 
 // ---------------------------------------------------------------- choice
 // The kernel whose modelled time is least. Tiles by gemm_last_wave: 64 rows (a unit is a K step
-// of 128), 128 and 256 rows (four of them), rates fitted to the measured times of all three in
-// one to nine shares at 112 projections of 17 to 8000 rows (K 256 to 14336, N 777 to 28672);
-// the choice is 1% slower than the best of them in the mean. Few rows: a workgroup's rounds on
-// the busiest CU by its K steps, a step 0.13 to 0.43 us as it has more rows and columns.
-// Measured, in us, the runner-up in brackets: 1 row, 7168 -> 5376: 9.3 (tiles of 64 rows in 6
-// shares 17); 32 rows, 5376 -> 21504: tiles of 64 in 3 shares 28 (few rows 36); 301 rows, 5376
-// -> 21504: 128 rows 44 (256 rows 63); 1024 rows, 7168 -> 5376: 128 rows 39 (256 in two shares
-// 50); 1500 rows, 5376 -> 21504: 256 rows 146 (128 rows 158).
+// of 128), 128 and 256 rows (four of them). Few rows: the workgroups of the busiest CU by their
+// K steps. Rates fitted to the measured times of all of them, the tiles in one to nine shares,
+// at 231 projections of 1 to 8000 rows (K 256 to 14336, N 300 to 32256; weights that rotate
+// through more than the last cache holds); the choice is 1.2% slower than the best of them in the
+// mean. Measured, in us, the runner-up in brackets: 1 row, 7168 -> 5376: 9.3 (tiles of 64 rows
+// in 6 shares 17); 32 rows, 5376 -> 21504: tiles of 64 in 3 shares 28 (few rows 36); 301 rows,
+// 5376 -> 21504: 128 rows 44 (256 rows 63); 1024 rows, 7168 -> 5376: 128 rows 39 (256 in two
+// shares 50); 1500 rows, 5376 -> 21504: 256 rows 146 (128 rows 158).
 struct Choice {
     float us;
     unsigned rows, split;     // tile rows (64, 128, 256) and shares; or
     unsigned rb, nb;          // few rows: row and column blocks (rb 0: tiles)
 };
+// Few rows: us of a step, [row blocks - 1][column blocks 2, 4], and the busiest CU's workgroups.
+constexpr float STREAM_LAUNCH = 2.4f, STREAM_STEP[3][2] = {{.157f, .298f}, {.224f, .344f}, {.313f, 0.f}};
+float stream_rounds(const h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
+    const uint64_t groups = ((uint64_t)a.m + 16 * rb - 1) / (16 * rb) * (((uint64_t)a.n + 16 * nb - 1) / (16 * nb));
+    return (float)((groups + g->cus - 1) / g->cus);
+}
 Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
-    static constexpr GemmRates RATES[3] = {{.66f, .39f, .067f, .15f, 2.8f, .095f, .67f},
-                                           {3.4f, 2.1f, 1.1f, .15f, 3.7f, .055f, 2.9f},
-                                           {5.9f, 3.6f, 2.45f, .15f, 5.5f, .035f, 2.4f}};
-    static constexpr float LAUNCH[3] = {4.2f, 2.4f, 1.9f};
+    static constexpr GemmRates RATES[3] = {{.68f, .518f, .355f, .6f, 3.8f, .088f, .77f},
+                                           {3.65f, 2.f, 1.36f, .15f, 3.95f, .085f, 2.3f},
+                                           {6.3f, 3.63f, 3.2f, .15f, 6.9f, .034f, 2.8f}};
+    static constexpr float LAUNCH[3] = {3.f, 3.35f, 0.f};
     const unsigned steps = a.k / TK;
     Choice best{3.4e38f, 0, 1, 0, 0};
     for (unsigned i = 0; i < 3; i++) {
@@ -951,28 +998,38 @@ Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
         const float us = (p.us + LAUNCH[i]) * (p.split > 1 ? 1.02f : 1.f);
         if (us < best.us) best = {us, rows, p.split, 0, 0};
     }
-    if (!stream || a.m > 256) return best;
-    // us of a step: [row blocks - 1][column blocks 2, 4].
-    static constexpr float STEP[3][2] = {{.16f, .32f}, {.22f, .39f}, {.28f, 0.f}};
+    if (!stream) return best;
     for (unsigned rb = 1; rb <= 3; rb++)
         for (unsigned nb = 2; nb <= (rb < 3 ? 4u : 2u); nb += 2) {
-            const unsigned groups = ((a.m + 16 * rb - 1) / (16 * rb)) * ((a.n + 16 * nb - 1) / (16 * nb));
-            const float us = 3.8f + (float)((groups + g->cus - 1) / g->cus * steps) * STEP[rb - 1][nb / 4];
-            if (us < best.us) best = {us, 0, 1, rb, nb};
+            const float rounds = stream_rounds(g, a, rb, nb);
+            const float us = STREAM_LAUNCH + rounds * steps * STREAM_STEP[rb - 1][nb / 4];
+            if (us < best.us && rounds < 1e6f) best = {us, 0, 1, rb, nb};
         }
     return best;
+}
+
+// Whether a projection of few rows packs its BF16 input itself: a launch is 2.5 us, packing a
+// step and row block 0.07 us beside the loads of a CU's one workgroup, 0.3 us where several
+// share its VALU.
+bool packs(const h3_gpu *g, const Fp8BlockGemmArgs &a, const Choice &c) {
+    if (!c.rb) return false;
+    const float rounds = stream_rounds(g, a, c.rb, c.nb);
+    return rounds * (a.k / TK) * c.rb * (rounds > 1.f ? .3f : .07f) < 2.5f;
 }
 
 template <int EPI> int run(h3_gpu *g, const Fp8BlockGemmArgs &a) {
     const Choice c = choose(g, a, EPI != EPI_SWIGLU);
     if constexpr (EPI != EPI_SWIGLU)
-        if (c.rb) return launch_stream<EPI>(g, a, c.rb, c.nb);
+        if (c.rb) return a.xb ? launch_stream<EPI, true>(g, a, c.rb, c.nb) : launch_stream<EPI, false>(g, a, c.rb, c.nb);
+    if (a.xb) return h3_set_error(g, "FP8 block projection: %u rows of BF16 are to be packed first", a.m);
     return c.rows == 256   ? launch_pipe<EPI, 256>(g, a, c.split)
            : c.rows == 128 ? launch_pipe<EPI, 128>(g, a, c.split)
                            : launch_mid<EPI>(g, a, c.split);
 }
 
 }  // namespace
+
+bool h3_gemm_fp8_block_packs(const h3_gpu *g, const Fp8BlockGemmArgs &a) { return packs(g, a, choose(g, a, !a.swiglu)); }
 
 // Without it the product goes through memory in FP32 and another launch packs it.
 bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m, uint32_t k, uint32_t hidden) {
