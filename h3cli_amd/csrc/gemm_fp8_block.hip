@@ -19,12 +19,11 @@ constexpr unsigned TK = FP8_BLOCK;            // K bytes of a step: one block of
 
 __device__ inline unsigned swz(unsigned row, unsigned ch) { return ch ^ ((row >> 1) & 7); }
 
-__device__ inline __amdgpu_buffer_rsrc_t uniform_resource(const void *p, unsigned bytes) {
+// A buffer resource in scalar registers. Raw: loads past `bytes` give zeros.
+__device__ inline i32x4 asm_resource(const uint8_t *p, unsigned bytes) {
     const uint64_t v = (uint64_t)p;
-    // readfirstlane returns int: through uint32_t, so that the low word's sign stays out of the high one.
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc((void *)(lo | (uint64_t)hi << 32), (short)0,
-                                             (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+    return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)v), (int)__builtin_amdgcn_readfirstlane((unsigned)(v >> 32)),
+                 (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000};
 }
 
 // Epilogues: BF16 rows of a multiple of eight columns, without and with a bias; SwiGLU, packed;
@@ -56,14 +55,17 @@ __device__ inline void store4(const Fp8BlockGemmArgs &a, unsigned row, unsigned 
         if (a.bias) {
             if (whole) b = *reinterpret_cast<const u16x4_any *>(a.bias + col);
             else
-                for (unsigned e = 0; col + e < a.n; e++) b.v[e] = a.bias[col + e];
+#pragma unroll
+                for (unsigned e = 0; e < 3; e++) b.v[e] = a.bias[min(col + e, a.n - 1)];
         }
         u16x4_any o;
 #pragma unroll
         for (int e = 0; e < 4; e++) o.v[e] = f32_to_bf16(v[e] + bf16_to_f32(b.v[e]));
         if (whole) *reinterpret_cast<u16x4_any *>(a.y + at) = o;
         else
-            for (unsigned e = 0; col + e < a.n; e++) a.y[at + e] = o.v[e];
+#pragma unroll
+            for (unsigned e = 0; e < 3; e++)
+                if (col + e < a.n) a.y[at + e] = o.v[e];
         return;
     }
     if constexpr (EPI == EPI_BIAS) {
@@ -76,11 +78,6 @@ __device__ inline void store4(const Fp8BlockGemmArgs &a, unsigned row, unsigned 
     for (int e = 0; e < 4; e++) o[e] = f32_to_bf16(v[e]);
     *reinterpret_cast<u16x4 *>(a.y + at) = o;
 }
-
-// Row of W that row r of a tile holds, counted from the tile's first row. SwiGLU: 32 gate
-// rows and the 32 up rows of the same columns alternate, so that a lane's accumulator blocks
-// hold both; a tile then makes 128 columns, one block of the packed result.
-__device__ inline unsigned swiglu_row(unsigned r) { return r / 64 * 32 + r % 32; }
 
 // ---------------------------------------------------------------- few rows
 // Reading W once is all the work there is, so the split is made for memory: a workgroup takes
@@ -232,225 +229,6 @@ template <int EPI, bool PACK> int launch_stream(h3_gpu *g, const Fp8BlockGemmArg
     return rb == 1 ? nb == 2 ? launch_stream_as<EPI, PACK, 1, 2, 8, 3>(g, a) : launch_stream_as<EPI, PACK, 1, 4, 8, 2>(g, a)
            : rb == 2 ? nb == 2 ? launch_stream_as<EPI, PACK, 2, 2, 4, 3>(g, a) : launch_stream_as<EPI, PACK, 2, 4, 4, 3>(g, a)
                      : launch_stream_as<EPI, PACK, 3, 2, 4, 2>(g, a);
-}
-
-// ---------------------------------------------------------------- tiles of 64 rows
-// Eight waves (two per SIMD) of 32 x 64 outputs (C^T = W . X^T). All operands go from
-// memory to LDS without registers, three stages of 128 bytes of K. A stage's second half of
-// fragments is read before a step's barrier, and the loads of the step after next but one go
-// into it right behind the barrier: every load has two steps' time. The scales of 32 steps come
-// to LDS together.
-constexpr int MID_M = 64, MID_N = 256, MID_T = 512, MID_STAGES = 3;
-constexpr unsigned SCALE_STEPS = 32;          // steps whose scales are loaded together
-constexpr unsigned MID_X = MID_M * TK, MID_STAGE = (MID_M + MID_N) * TK, MID_RUNS = MID_M / 32;
-constexpr unsigned MID_SCALES = MID_RUNS * 1024 + 256, MID_LDS = MID_STAGES * MID_STAGE + 2 * MID_SCALES;
-constexpr int MID_GROUP = 4;
-
-// Waits for all but N of this wave's vector-memory loads and for its LDS accesses, then for
-// the other waves. In asm because hipcc's own barrier waits for every load to LDS, those of
-// later steps included.
-template <int N> __device__ inline void step_barrier() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
-__device__ inline void mid_tile(const Fp8BlockGemmArgs &a, unsigned pid, unsigned &m0, unsigned &n0) {
-    unsigned tm, tn;
-    band_tile((a.m + MID_M - 1) / MID_M, (a.n + MID_N - 1) / MID_N, MID_GROUP, pid, tm, tn);
-    m0 = __builtin_amdgcn_readfirstlane(tm * MID_M);
-    n0 = __builtin_amdgcn_readfirstlane(tn * MID_N);
-}
-
-// The epilogue of a wave's row block (32 rows from row0) and two column blocks from col0.
-// SwiGLU: the four waves of a row meet in `most` for the block's largest magnitude.
-template <int EPI>
-__device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, unsigned n0, unsigned wm, unsigned wn,
-                                    unsigned lane, const f32x16 &c0, const f32x16 &c1, unsigned (*most)[4][32]) {
-    const unsigned n32 = lane % 32, hf = lane / 32, row = row0 + n32;
-    if constexpr (EPI != EPI_SWIGLU) {
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            store4<EPI>(a, row, n0 + wn * 64 + g * 8 + hf * 4, f32x4{c0[4 * g], c0[4 * g + 1], c0[4 * g + 2], c0[4 * g + 3]});
-            store4<EPI>(a, row, n0 + wn * 64 + 32 + g * 8 + hf * 4, f32x4{c1[4 * g], c1[4 * g + 1], c1[4 * g + 2], c1[4 * g + 3]});
-        }
-        return;
-    }
-    float v[16];
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 16; e++) v[e] = swiglu_exact(c0[e], c1[e]);
-    unsigned amax = fp8_block_magnitude<16>(v, bad);
-    if (bad && row < a.m) *a.out.fault = 1u;
-    amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
-    if (hf == 0) most[wm][wn][n32] = amax;
-    __syncthreads();
-    const unsigned scale = fp8_block_scale(max(max(most[wm][0][n32], most[wm][1][n32]), max(most[wm][2][n32], most[wm][3][n32])));
-    __syncthreads();
-    if (row >= a.m) return;
-    const float value = fp8_block_value(scale);
-    uint8_t *dst = a.out.codes + (size_t)row * a.out.stride + n0 / 2 + wn * 32 + hf * 4;
-#pragma unroll
-    for (int g = 0; g < 4; g++) *reinterpret_cast<unsigned *>(dst + g * 8) = fp8_block_encode4(v + 4 * g, value);
-    if (wn == 0 && hf == 0) a.out.scales[fp8_block_scale_at(row, n0 / 256, a.out.groups)] = (uint8_t)scale;
-}
-
-template <int EPI>
-__global__ __attribute__((amdgpu_flat_work_group_size(MID_T, MID_T), amdgpu_waves_per_eu(2, 2)))
-void fp8_block_mid(Fp8BlockGemmArgs a) {
-    constexpr bool SWIGLU = EPI == EPI_SWIGLU;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    __shared__ unsigned most[2][4][32];
-    const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
-    const unsigned n32 = lane % 32, hf = lane / 32, wm = wave / 4, wn = wave % 4;
-    unsigned ksteps = a.k / TK;
-    const TileShare t = tile_share(a.tile, ksteps);
-    ksteps = __builtin_amdgcn_readfirstlane(ksteps);
-    const unsigned first = __builtin_amdgcn_readfirstlane(t.first), k0 = first * TK;
-    unsigned m0, n0;
-    mid_tile(a, t.pid, m0, n0);
-
-    // Rows past M or N are past the resources' size and load zeros. SwiGLU: a wave loads
-    // eight rows at a time, all gate or all up rows.
-    const unsigned half = SWIGLU && wave / 4 % 2, w_first = SWIGLU ? n0 / 2 + (half ? a.n / 2 : 0) : n0;
-    const unsigned xrows = min(a.m - m0, (unsigned)MID_M), wrows = SWIGLU ? 128u : min(a.n - n0, (unsigned)MID_N);
-    const __amdgpu_buffer_rsrc_t xr = uniform_resource(a.x + (size_t)m0 * a.k + k0, xrows * a.k - k0);
-    const __amdgpu_buffer_rsrc_t wr = uniform_resource(a.w + (size_t)w_first * a.k + k0, wrows * a.k - k0);
-    const unsigned lrow = 8 * wave + lane / 8, part = swz(lrow, lane % 8) * 16;
-    const unsigned xoff = lrow * a.k + part;
-    unsigned woff[4];
-#pragma unroll
-    for (int b = 0; b < 4; b++) woff[b] = (SWIGLU ? swiglu_row(lrow + 64 * b) : lrow + 64 * b) * a.k + part;
-    // Scales of 32 steps from the group of four that holds the first: the first waves 32 rows of
-    // X each, [group][row][four], the next one the two blocks of W in lanes 0 to 15, [group].
-    const unsigned skip = first % 4, g0 = first / 4, runs = min((a.m + 31) / 32 - m0 / 32, MID_RUNS);
-    const __amdgpu_buffer_rsrc_t xsr =
-        uniform_resource(a.xs + ((size_t)(m0 / 32) * a.groups + g0) * 128, (runs * a.groups - g0) * 128);
-    const unsigned wblocks = (a.n + 127) / 128;
-    const __amdgpu_buffer_rsrc_t wsr = uniform_resource(a.ws + (size_t)g0 * 128, ((wblocks + 31) / 32 * a.groups - g0) * 128);
-    const unsigned sb0 = SWIGLU ? n0 / 256 : n0 / 128, sb1 = SWIGLU ? n0 / 256 + a.n / 256 : min(n0 / 128 + 1, wblocks - 1);
-    uint8_t *const scs = lds + MID_STAGES * MID_STAGE;
-    auto load_scales = [&](unsigned part) {
-        uint8_t *dst = scs + (part & 1) * MID_SCALES;
-        if (wave < MID_RUNS) {
-            // Behind a run's groups comes the next run, behind the last the resource's end: zeros.
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xsr, (__attribute__((address_space(3))) void *)(dst + wave * 1024), 16,
-                                                     (wave * a.groups + part * (SCALE_STEPS / 4)) * 128 + lane * 16, 0, 0, 0);
-        } else if (wave == MID_RUNS) {
-            const unsigned block = lane / 8 % 2 ? sb1 : sb0, group = part * (SCALE_STEPS / 4) + lane % 8;
-            const unsigned at = (block / 32 * a.groups + group) * 128 + block % 32 * 4;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (__attribute__((address_space(3))) void *)(dst + MID_RUNS * 1024), 4,
-                                                     lane < 16 && g0 + group < a.groups ? at : BUFFER_OOB, 0, 0, 0);
-        }
-    };
-
-    f32x16 acc[2] = {};
-
-    // Loads of step kt into stage st; steps past the end reload the last one into a stage
-    // that nobody reads again.
-    auto load = [&](unsigned kt, unsigned st) {
-        kt = __builtin_amdgcn_readfirstlane(min(kt, ksteps - 1));
-        uint8_t *dst = lds + st * MID_STAGE + wave * 1024;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void *)dst, 16, xoff, kt * TK, 0, 0);
-#pragma unroll
-        for (int b = 0; b < 4; b++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void *)(dst + MID_X + b * 8192), 16,
-                                                     woff[b], kt * TK, 0, 0);
-    };
-    constexpr int LOADS = 5;                  // of a wave and step
-    auto fragment = [&](const uint8_t *tile, unsigned r, int ks) {
-        const u32x4 lo = *reinterpret_cast<const u32x4 *>(tile + r * TK + swz(r, 4 * ks + 2 * hf) * 16);
-        const u32x4 hi = *reinterpret_cast<const u32x4 *>(tile + r * TK + swz(r, 4 * ks + 2 * hf + 1) * 16);
-        return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-    };
-    auto frags = [&](unsigned st, int ks, i32x8 *wf, i32x8 &xf) {
-        const uint8_t *xs = lds + st * MID_STAGE, *ws = xs + MID_X;
-#pragma unroll
-        for (int i = 0; i < 2; i++) wf[i] = fragment(ws, wn * 64 + i * 32 + n32, ks);
-        xf = fragment(xs, wm * 32 + n32, ks);
-    };
-    auto scales = [&](unsigned kt, int *ws, int &xs) {
-        const unsigned at = kt + skip;
-        const uint8_t *s = scs + at / SCALE_STEPS % 2 * MID_SCALES;
-        const unsigned group = at % SCALE_STEPS / 4, byte = at % 4;
-        xs = s[wm * 1024 + group * 128 + n32 * 4 + byte];
-#pragma unroll
-        for (int i = 0; i < 2; i++) ws[i] = s[MID_RUNS * 1024 + (SWIGLU ? i : wn / 2) * 32 + group * 4 + byte];
-    };
-    auto products = [&](const i32x8 *wf, const i32x8 &xf, const int *ws, int xs) {
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[i], xf, acc[i], 0, 0, 0, ws[i], 0, xs);
-    };
-
-    load_scales(0);
-    load_scales(1);
-#pragma unroll
-    for (int s = 0; s < MID_STAGES; s++) load(s, s);
-    step_barrier<(MID_STAGES - 1) * LOADS>();
-    i32x8 wf[2][2], xf[2];
-    int ws[2][2], xs[2];
-    frags(0, 0, wf[0], xf[0]);
-    scales(0, ws[0], xs[0]);
-    unsigned cur = 0;
-    auto step = [&](unsigned kt, int p) {
-        const unsigned next = cur + 1 == MID_STAGES ? 0 : cur + 1;
-        frags(cur, 1, wf[1], xf[1]);
-        __builtin_amdgcn_sched_barrier(0);
-        products(wf[0], xf[0], ws[p], xs[p]);
-        __builtin_amdgcn_sched_barrier(0);
-        step_barrier<(MID_STAGES - 2) * LOADS>();
-        if (kt && (kt + skip) % SCALE_STEPS == 0) load_scales((kt + skip) / SCALE_STEPS + 1);
-        load(kt + MID_STAGES, cur);
-        frags(next, 0, wf[0], xf[0]);
-        scales(kt + 1, ws[p ^ 1], xs[p ^ 1]);
-        __builtin_amdgcn_sched_barrier(0);
-        products(wf[1], xf[1], ws[p], xs[p]);
-        __builtin_amdgcn_sched_barrier(0);
-        cur = next;
-    };
-    unsigned kt = 0;
-    for (; kt + 1 < ksteps; kt += 2) {
-        step(kt, 0);
-        step(kt + 1, 1);
-    }
-    if (kt < ksteps) step(kt, 0);
-    wait_vm_loads();   // LDS must not be written after the workgroup has ended
-
-    const unsigned row0 = m0 + wm * 32;
-    if (t.partial) {
-        f32x4 *dst = reinterpret_cast<f32x4 *>(a.tile.part) +
-                     ((size_t)t.tile * a.tile.split + t.share) * (MID_M * MID_N / 4) + tid;
-        if (row0 >= a.m) return;
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int g = 0; g < 4; g++)
-                dst[(i * 4 + g) * MID_T] = f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
-        return;
-    }
-    mid_epilogue<EPI>(a, row0, n0, wm, wn, lane, acc[0], acc[1], most);
-}
-
-// The split tiles' shares added in order, and the epilogue. One workgroup per tile.
-template <int EPI>
-__global__ __launch_bounds__(MID_T) void fp8_block_mid_reduce(Fp8BlockGemmArgs a) {
-    __shared__ unsigned most[2][4][32];
-    const unsigned tile = blockIdx.x, tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    unsigned m0, n0;
-    mid_tile(a, split_tile(a.tile, tile), m0, n0);
-    const unsigned row0 = m0 + wave / 4 * 32;
-    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tile.part) + (size_t)tile * a.tile.split * (MID_M * MID_N / 4) + tid;
-    f32x16 c[2] = {};
-    // A row block past M: no share was written.
-    for (unsigned s = 0; row0 < a.m && s < a.tile.split; s++, src += MID_M * MID_N / 4)
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const f32x4 v = src[(i * 4 + g) * MID_T];
-#pragma unroll
-                for (int e = 0; e < 4; e++) c[i][4 * g + e] += v[e];
-            }
-    mid_epilogue<EPI>(a, row0, n0, wave / 4, wave % 4, lane, c[0], c[1], most);
 }
 
 // ---------------------------------------------------------------- tiles of 256 rows
@@ -747,22 +525,19 @@ void fp8_block_pipe(Fp8BlockGemmArgs a) {
     const unsigned k0 = t.first * TK;
     unsigned m0, n0;
     pipe_tile<TM>(a, t.pid, m0, n0);
-    // Rows past M or N are past the resources' size and load zeros. SwiGLU: loads of even
-    // number hold gate rows, of odd number up rows.
+    // Rows past M or N are past the resources' size and load zeros. SwiGLU: 32 gate rows and the
+    // 32 up rows of the same columns alternate (loads of even and of odd number), so that a
+    // lane's accumulator blocks hold both; a tile then makes 128 columns, one block of the
+    // packed result.
     const unsigned xrows = min(a.m - m0, (unsigned)TM), wrows = SWIGLU ? 128u : min(a.n - n0, (unsigned)PIPE_N);
     const unsigned w0 = SWIGLU ? n0 / 2 : n0, w1 = SWIGLU ? n0 / 2 + a.n / 2 : n0;
-    auto resource = [](const uint8_t *p, unsigned bytes) {
-        const uint64_t v = (uint64_t)p;
-        return i32x4{(int)__builtin_amdgcn_readfirstlane((unsigned)v), (int)__builtin_amdgcn_readfirstlane((unsigned)(v >> 32)),
-                     (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000};
-    };
-    const i32x4 sx = resource(a.x + (size_t)m0 * a.k + k0, xrows * a.k - k0);
-    const i32x4 sw0 = resource(a.w + (size_t)w0 * a.k + k0, wrows * a.k - k0);
-    const i32x4 sw1 = resource(a.w + (size_t)w1 * a.k + k0, wrows * a.k - k0);
+    const i32x4 sx = asm_resource(a.x + (size_t)m0 * a.k + k0, xrows * a.k - k0);
+    const i32x4 sw0 = asm_resource(a.w + (size_t)w0 * a.k + k0, wrows * a.k - k0);
+    const i32x4 sw1 = asm_resource(a.w + (size_t)w1 * a.k + k0, wrows * a.k - k0);
     const unsigned blocks = (a.n + FP8_BLOCK - 1) / FP8_BLOCK;
     const unsigned g0 = t.first / QUAD;
-    const i32x4 tx = resource(a.xs + ((size_t)(m0 / 32) * a.groups + g0) * 128, (min((a.m + 31) / 32 - m0 / 32, TM / 32u) * a.groups - g0) * 128);
-    const i32x4 tw = resource(a.ws + (size_t)g0 * 128, ((blocks + 31) / 32 * a.groups - g0) * 128);
+    const i32x4 tx = asm_resource(a.xs + ((size_t)(m0 / 32) * a.groups + g0) * 128, (min((a.m + 31) / 32 - m0 / 32, TM / 32u) * a.groups - g0) * 128);
+    const i32x4 tw = asm_resource(a.ws + (size_t)g0 * 128, ((blocks + 31) / 32 * a.groups - g0) * 128);
     const unsigned lrow = 8 * wave + lane / 8;
     unsigned ox[8], ow[8], oe[6];
 #pragma unroll
@@ -913,24 +688,258 @@ __global__ __launch_bounds__(PIPE_T) void fp8_block_pipe_reduce(Fp8BlockGemmArgs
     pipe_epilogue<EPI>(a, row0, n0, wave / 2, wave % 2, lane, c[0], c[1], c[2], c[3], scratch);
 }
 
+// ---------------------------------------------------------------- tiles of 64 rows
+// 64 x 256 outputs per workgroup, four waves of 64 x 64 and half as many products a tile again:
+// four stages, X at 0, 8, 16 and 24 KB, W at 32, 64, 96 and 128 KB (all of a CU's LDS), loads
+// four tiles ahead. Fragment set S in v[64 + 32 S ..], W block I at + 8 I, X block J at + 16 +
+// 8 J; scale set Z in v[128 + 4 Z ..], X block J at + J, W at + 2 and + 3. Tile B of a group of
+// four is in stage B. Bound by LDS, whose reads and writes take 1.6 times as long as the
+// products, and by the memory's latency.
+constexpr int MID_M = 64, MID_N = 256, MID_T = 256;
+constexpr unsigned MID_LDS = 4 * (MID_M + MID_N) * TK;
+constexpr int MID_GROUP = 4;
+
+#define FQ_LX(ST, T) "s_add_u32 m0, %[mb], 8192*" #ST "+4096*" #T "\n"                                              \
+    "buffer_load_dwordx4 %[x" #T "], %[sx], %[kc] offen lds\n"
+#define FQ_LW(ST, T, R) "s_add_u32 m0, %[mb], 32768+32768*" #ST "+4096*" #T "\n"                                    \
+    "buffer_load_dwordx4 %[y" #T "], %[sw" #R "], %[kc] offen lds\n"
+#define FQ_SCALES(Z)                                                                                                \
+    "buffer_load_dword v[128+4*" #Z "], %[e0], %[tx], %[kg] offen\n"                                                 \
+    "buffer_load_dword v[128+4*" #Z "+1], %[e1], %[tx], %[kg] offen\n"                                               \
+    "buffer_load_dword v[128+4*" #Z "+2], %[e2], %[tw], %[kg] offen\n"                                               \
+    "buffer_load_dword v[128+4*" #Z "+3], %[e3], %[tw], %[kg] offen\n"                                               \
+    "s_add_u32 %[kg], %[kg], 128\n"                                                                                 \
+    "s_min_u32 %[kg], %[kg], %[kgmax]\n"
+#define FQ_MFMA(S, Z, B, I, J)                                                                                      \
+    "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #I #J "], v[64+32*" #S "+8*" #I ":64+32*" #S "+8*" #I "+7], "             \
+    "v[64+32*" #S "+16+8*" #J ":64+32*" #S "+16+8*" #J "+7], %[c" #I #J "], v[128+4*" #Z "+2+" #I "], "              \
+    "v[128+4*" #Z "+" #J "]" FB_SEL_##B
+#define FQ_WAT_0(KS, H) "%[w" #KS #H "] offset:"
+#define FQ_WAT_1(KS, H) "%[w" #KS #H "] offset:32768+"
+#define FQ_WAT_2(KS, H) "%[u" #KS #H "] offset:"
+#define FQ_WAT_3(KS, H) "%[u" #KS #H "] offset:32768+"
+#define FQ_RW(T, F, KS, ST)                                                                                         \
+    "ds_read_b128 v[64+32*" #T "+8*" #F ":64+32*" #T "+8*" #F "+3], " FQ_WAT_##ST(KS, 0) "4096*" #F "\n"              \
+    "ds_read_b128 v[64+32*" #T "+8*" #F "+4:64+32*" #T "+8*" #F "+7], " FQ_WAT_##ST(KS, 1) "4096*" #F "\n"
+#define FQ_RX(T, F, KS, ST)                                                                                         \
+    "ds_read_b128 v[64+32*" #T "+16+8*" #F ":64+32*" #T "+16+8*" #F "+3], %[r" #KS "0] offset:8192*" #ST "+4096*" #F "\n" \
+    "ds_read_b128 v[64+32*" #T "+16+8*" #F "+4:64+32*" #T "+16+8*" #F "+7], %[r" #KS "1] offset:8192*" #ST "+4096*" #F "\n"
+#define FQ_SUB(S, Z, B, T, KS, ST, L0, L1, L2, L3)                                                                  \
+    FQ_MFMA(S, Z, B, 0, 0) FQ_RW(T, 0, KS, ST) FQ_RX(T, 0, KS, ST) L0                                                \
+    FQ_MFMA(S, Z, B, 0, 1) FQ_RX(T, 1, KS, ST) FQ_RW(T, 1, KS, ST) L1                                                \
+    FQ_MFMA(S, Z, B, 1, 0) L2 FQ_MFMA(S, Z, B, 1, 1) L3
+#define FQ_SUB_EXP(...) FQ_SUB(__VA_ARGS__)
+#define FQ_NONE "", "", "", ""
+#define FQ_LOADS(ST) FQ_LX(ST, 0) FQ_LW(ST, 0, 0), FQ_LX(ST, 1) FQ_LW(ST, 1, 1),                                      \
+    FQ_LW(ST, 2, 0) FQ_LW(ST, 3, 1) FQ_LW(ST, 4, 0), FQ_LW(ST, 5, 1) FQ_LW(ST, 6, 0) FQ_LW(ST, 7, 1)
+// The loads of the two tiles after the next (20, the youngest) stay in flight at the barrier.
+#define FQ_TILE(ST, OT, Z, NEXT)                                                                                    \
+    FQ_SUB_EXP(0, Z, ST, 1, 1, ST, FQ_NONE)                                                                          \
+    "s_waitcnt vmcnt(20) lgkmcnt(0)\n"                                                                              \
+    "s_barrier\n"                                                                                                   \
+    "s_min_u32 %[kc], %[kn], %[kmax]\n"                                                                             \
+    "s_add_u32 %[kn], %[kn], 128\n" NEXT                                                                            \
+    FQ_SUB_EXP(1, Z, ST, 0, 0, OT, FQ_LOADS(ST))                                                                     \
+    "s_waitcnt lgkmcnt(0)\n"                                                                                        \
+    "s_sub_u32 %[steps], %[steps], 1\n"                                                                             \
+    "s_cmp_eq_u32 %[steps], 0\n"                                                                                    \
+    "s_cbranch_scc1 fq_end_%=\n"
+#define FQ_QUAD(Z, OZ) FQ_TILE(0, 1, Z, FQ_SCALES(OZ)) FQ_TILE(1, 2, Z, "") FQ_TILE(2, 3, Z, "") FQ_TILE(3, 0, Z, "")
+#define FQ_FIRST(ST, KC) "s_mov_b32 %[kc], " KC "\n" FQ_LX(ST, 0) FQ_LW(ST, 0, 0) FQ_LX(ST, 1) FQ_LW(ST, 1, 1)           \
+    FQ_LW(ST, 2, 0) FQ_LW(ST, 3, 1) FQ_LW(ST, 4, 0) FQ_LW(ST, 5, 1) FQ_LW(ST, 6, 0) FQ_LW(ST, 7, 1)
+
+__device__ inline void mid_tile(const Fp8BlockGemmArgs &a, unsigned pid, unsigned &m0, unsigned &n0) {
+    unsigned tm, tn;
+    band_tile((a.m + MID_M - 1) / MID_M, (a.n + MID_N - 1) / MID_N, MID_GROUP, pid, tm, tn);
+    m0 = __builtin_amdgcn_readfirstlane(tm * MID_M);
+    n0 = __builtin_amdgcn_readfirstlane(tn * MID_N);
+}
+
+// The epilogue of a wave's row block (32 rows from row0) and two column blocks from col0.
+// SwiGLU: the four waves of a row meet in `most` for the block's largest magnitude.
+template <int EPI>
+__device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, unsigned n0, unsigned wn, unsigned lane,
+                                    const f32x16 &c0, const f32x16 &c1, unsigned (*most)[32]) {
+    const unsigned n32 = lane % 32, hf = lane / 32, row = row0 + n32;
+    if constexpr (EPI != EPI_SWIGLU) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            store4<EPI>(a, row, n0 + wn * 64 + g * 8 + hf * 4, f32x4{c0[4 * g], c0[4 * g + 1], c0[4 * g + 2], c0[4 * g + 3]});
+            store4<EPI>(a, row, n0 + wn * 64 + 32 + g * 8 + hf * 4, f32x4{c1[4 * g], c1[4 * g + 1], c1[4 * g + 2], c1[4 * g + 3]});
+        }
+        return;
+    }
+    float v[16];
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 16; e++) v[e] = swiglu_exact(c0[e], c1[e]);
+    unsigned amax = fp8_block_magnitude<16>(v, bad);
+    if (bad && row < a.m) *a.out.fault = 1u;
+    amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
+    if (hf == 0) most[wn][n32] = amax;
+    __syncthreads();
+    const unsigned scale = fp8_block_scale(max(max(most[0][n32], most[1][n32]), max(most[2][n32], most[3][n32])));
+    __syncthreads();
+    if (row >= a.m) return;
+    const float value = fp8_block_value(scale);
+    uint8_t *dst = a.out.codes + (size_t)row * a.out.stride + n0 / 2 + wn * 32 + hf * 4;
+#pragma unroll
+    for (int g = 0; g < 4; g++) *reinterpret_cast<unsigned *>(dst + g * 8) = fp8_block_encode4(v + 4 * g, value);
+    if (wn == 0 && hf == 0) a.out.scales[fp8_block_scale_at(row, n0 / 256, a.out.groups)] = (uint8_t)scale;
+}
+
+template <int EPI, bool SPLIT>
+__global__ __attribute__((amdgpu_flat_work_group_size(MID_T, MID_T), amdgpu_waves_per_eu(1, 1)))
+void fp8_block_mid(Fp8BlockGemmArgs a) {
+    constexpr bool SWIGLU = EPI == EPI_SWIGLU;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const unsigned tid = threadIdx.x, lane = tid % 64, n32 = lane % 32, hf = lane / 32;
+    const unsigned wn = __builtin_amdgcn_readfirstlane(tid / 64);
+    unsigned ksteps = a.k / TK;
+    TileShare t{};
+    if constexpr (SPLIT) t = pipe_share(a, ksteps);
+    else t.pid = xcd_remap(blockIdx.x, gridDim.x);
+    const unsigned k0 = t.first * TK;
+    unsigned m0, n0;
+    mid_tile(a, t.pid, m0, n0);
+    // As in fp8_block_pipe.
+    const unsigned xrows = min(a.m - m0, (unsigned)MID_M), wrows = SWIGLU ? 128u : min(a.n - n0, (unsigned)MID_N);
+    const unsigned w0 = SWIGLU ? n0 / 2 : n0, w1 = SWIGLU ? n0 / 2 + a.n / 2 : n0;
+    const i32x4 sx = asm_resource(a.x + (size_t)m0 * a.k + k0, xrows * a.k - k0);
+    const i32x4 sw0 = asm_resource(a.w + (size_t)w0 * a.k + k0, wrows * a.k - k0);
+    const i32x4 sw1 = asm_resource(a.w + (size_t)w1 * a.k + k0, wrows * a.k - k0);
+    const unsigned blocks = (a.n + FP8_BLOCK - 1) / FP8_BLOCK, g0 = t.first / QUAD;
+    const i32x4 tx = asm_resource(a.xs + ((size_t)(m0 / 32) * a.groups + g0) * 128,
+                                  (min((a.m + 31) / 32 - m0 / 32, MID_M / 32u) * a.groups - g0) * 128);
+    const i32x4 tw = asm_resource(a.ws + (size_t)g0 * 128, ((blocks + 31) / 32 * a.groups - g0) * 128);
+    const unsigned lrow = 8 * wn + lane / 8, part = swz(lrow, lane % 8) * 16;
+    unsigned ow[8];
+#pragma unroll
+    for (int b = 0; b < 8; b++) ow[b] = (lrow + 32 * (SWIGLU ? b / 2 : b)) * a.k + part;
+    const unsigned ox0 = lrow * a.k + part, ox1 = ox0 + 32 * a.k;
+    const unsigned oe0 = n32 * 4, oe1 = a.groups * 128 + n32 * 4;
+    // A wave's 64 columns are in one block of W; SwiGLU: 32 gate and 32 up columns.
+    const unsigned first_block = SWIGLU ? n0 / 256 : min(n0 / 128 + wn / 2, blocks - 1);
+    const unsigned oe2 = (unsigned)fp8_block_scale_at(first_block, 0, a.groups);
+    const unsigned oe3 = SWIGLU ? (unsigned)fp8_block_scale_at(first_block + a.n / 256, 0, a.groups) : oe2;
+    const unsigned mb = __builtin_amdgcn_readfirstlane(wn * 1024);
+    const unsigned kmax = __builtin_amdgcn_readfirstlane((ksteps - 1) * TK);
+    const unsigned kgmax = __builtin_amdgcn_readfirstlane((ksteps - 1) / QUAD * 128);
+    const unsigned kone = min(kmax, TK), ktwo = min(kmax, 2 * TK), kthree = min(kmax, 3 * TK);
+    unsigned kn = 4 * TK, kc = 0, kg = 0, steps = __builtin_amdgcn_readfirstlane(ksteps);
+    unsigned pw[2][2], pu[2][2], px[2][2];
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            px[s][h] = n32 * TK + swz(n32, 4 * s + 2 * hf + h) * 16;
+            pw[s][h] = 32768 + wn * 64 * TK + px[s][h];
+            pu[s][h] = pw[s][h] + 65536;
+        }
+    f32x16 c[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) c[i][j] = f32x16{};
+    asm volatile(
+        FQ_SCALES(0)
+        FQ_FIRST(0, "0") FQ_FIRST(1, "%[kone]") FQ_FIRST(2, "%[ktwo]") FQ_FIRST(3, "%[kthree]")
+        "s_waitcnt vmcnt(30)\n"
+        "s_barrier\n"
+        FQ_RW(0, 0, 0, 0) FQ_RW(0, 1, 0, 0) FQ_RX(0, 0, 0, 0) FQ_RX(0, 1, 0, 0)
+        "s_waitcnt lgkmcnt(0)\n"
+        "fq_loop_%=:\n"
+        FQ_QUAD(0, 1)
+        FQ_QUAD(1, 0)
+        "s_branch fq_loop_%=\n"
+        "fq_end_%=:\n"
+        "s_waitcnt vmcnt(0) lgkmcnt(0)\n"
+        "s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n s_nop 7\n"
+        : [c00] "+a"(c[0][0]), [c01] "+a"(c[0][1]), [c10] "+a"(c[1][0]), [c11] "+a"(c[1][1]), [kc] "+s"(kc), [kn] "+s"(kn),
+          [kg] "+s"(kg), [steps] "+s"(steps)
+        : [sx] "s"(sx), [sw0] "s"(sw0), [sw1] "s"(sw1), [tx] "s"(tx), [tw] "s"(tw), [x0] "v"(ox0), [x1] "v"(ox1),
+          [y0] "v"(ow[0]), [y1] "v"(ow[1]), [y2] "v"(ow[2]), [y3] "v"(ow[3]), [y4] "v"(ow[4]), [y5] "v"(ow[5]),
+          [y6] "v"(ow[6]), [y7] "v"(ow[7]), [e0] "v"(oe0), [e1] "v"(oe1), [e2] "v"(oe2), [e3] "v"(oe3), [mb] "s"(mb),
+          [kmax] "s"(kmax), [kgmax] "s"(kgmax), [kone] "s"(kone), [ktwo] "s"(ktwo), [kthree] "s"(kthree),
+          [w00] "v"(pw[0][0]), [w01] "v"(pw[0][1]), [w10] "v"(pw[1][0]), [w11] "v"(pw[1][1]), [u00] "v"(pu[0][0]),
+          [u01] "v"(pu[0][1]), [u10] "v"(pu[1][0]), [u11] "v"(pu[1][1]), [r00] "v"(px[0][0]), [r01] "v"(px[0][1]),
+          [r10] "v"(px[1][0]), [r11] "v"(px[1][1])
+        : "v64", "v65", "v66", "v67", "v68", "v69", FB_CL10(7), FB_CL10(8), FB_CL10(9), FB_CL10(10), FB_CL10(11),
+          FB_CL10(12), "v130", "v131", "v132", "v133", "v134", "v135", "m0", "scc", "memory");
+
+    // Block (i, j): lane holds output row m0 + 32 j + n32.
+    if (SPLIT && t.partial) {
+        f32x4 *dst = reinterpret_cast<f32x4 *>(a.tile.part) +
+                     ((size_t)t.tile * a.tile.split + t.share) * (MID_M * MID_N / 4) + tid;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if (m0 + j * 32 >= a.m) break;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                hold(c[i][j]);
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    dst[((j * 2 + i) * 4 + g) * MID_T] =
+                        f32x4{c[i][j][4 * g], c[i][j][4 * g + 1], c[i][j][4 * g + 2], c[i][j][4 * g + 3]};
+            }
+        }
+        return;
+    }
+    if constexpr (SWIGLU) __syncthreads();     // all have read their last fragments
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        hold(c[0][j]);
+        hold(c[1][j]);
+        mid_epilogue<EPI>(a, m0 + j * 32, n0, wn, lane, c[0][j], c[1][j], (unsigned(*)[32])lds);
+    }
+}
+
+// The split tiles' shares added in order, and the epilogue. One workgroup per (tile, row block).
+template <int EPI>
+__global__ __launch_bounds__(MID_T) void fp8_block_mid_reduce(Fp8BlockGemmArgs a) {
+    __shared__ unsigned most[4][32];
+    const unsigned tile = blockIdx.x / 2, j = blockIdx.x % 2, tid = threadIdx.x;
+    unsigned m0, n0;
+    mid_tile(a, split_tile(a.tile, tile), m0, n0);
+    const unsigned row0 = m0 + j * 32;
+    if (row0 >= a.m) return;       // no share was written
+    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tile.part) + (size_t)tile * a.tile.split * (MID_M * MID_N / 4) +
+                       j * 8 * MID_T + tid;
+    f32x16 c[2] = {};
+#pragma unroll 2
+    for (unsigned s = 0; s < a.tile.split; s++, src += MID_M * MID_N / 4)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const f32x4 v = src[(i * 4 + g) * MID_T];
+#pragma unroll
+                for (int e = 0; e < 4; e++) c[i][4 * g + e] += v[e];
+            }
+    mid_epilogue<EPI>(a, row0, n0, tid / 64, tid % 64, c[0], c[1], most);
+}
+
 template <int EPI> int launch_mid(h3_gpu *g, Fp8BlockGemmArgs a, unsigned split) {
     static bool configured = false;
     if (!configured) {
-        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)fp8_block_mid<EPI>,
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, MID_LDS),
-                          "FP8 block GEMM shared memory"))
-            return 0;
+        for (const void *kernel : {(const void *)fp8_block_mid<EPI, false>, (const void *)fp8_block_mid<EPI, true>})
+            if (!h3_hip_check(g, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MID_LDS),
+                              "FP8 block GEMM shared memory"))
+                return 0;
         configured = true;
     }
-    const unsigned tiles = (a.m + MID_M - 1) / MID_M * ((a.n + MID_N - 1) / MID_N);
-    a.tile = split_last_wave(g, tiles, split, a.k / TK, MID_M * MID_N);
+    const unsigned tiles = (a.m + MID_M - 1) / MID_M * ((a.n + MID_N - 1) / MID_N), quads = (a.k / TK + QUAD - 1) / QUAD;
+    a.tile = split_last_wave(g, tiles, split, quads, MID_M * MID_N);
     const unsigned rest = tiles - a.tile.full;
     h3_note_kernel(g, "fp8_block_mid", MID_M, a.tile.split);
     hipEvent_t timing = h3_kernel_timing_begin(g);
-    hipLaunchKernelGGL((fp8_block_mid<EPI>), dim3(a.tile.full + rest * a.tile.split), dim3(MID_T), MID_LDS,
-                       g->compute, a);
-    if (rest && h3_launch_status(g, "FP8 block GEMM"))
-        hipLaunchKernelGGL((fp8_block_mid_reduce<EPI>), dim3(rest), dim3(MID_T), 0, g->compute, a);
+    if (!rest) {
+        hipLaunchKernelGGL((fp8_block_mid<EPI, false>), dim3(tiles), dim3(MID_T), MID_LDS, g->compute, a);
+    } else {
+        hipLaunchKernelGGL((fp8_block_mid<EPI, true>), dim3(a.tile.full + rest * a.tile.split), dim3(MID_T), MID_LDS, g->compute, a);
+        if (h3_launch_status(g, "FP8 block GEMM"))
+            hipLaunchKernelGGL(fp8_block_mid_reduce<EPI>, dim3(rest * 2), dim3(MID_T), 0, g->compute, a);
+    }
     h3_kernel_timing_end(g, timing);
     return h3_launch_status(g, "FP8 block GEMM");
 }
@@ -963,35 +972,35 @@ template <int EPI, int TM> int launch_pipe(h3_gpu *g, Fp8BlockGemmArgs a, unsign
 }
 
 // ---------------------------------------------------------------- choice
-// The kernel whose modelled time is least. Tiles by gemm_last_wave: 64 rows (a unit is a K step
-// of 128), 128 and 256 rows (four of them). Few rows: the workgroups of the busiest CU by their
-// K steps. Rates fitted to the measured times of all of them, the tiles in one to nine shares,
-// at 231 projections of 1 to 8000 rows (K 256 to 14336, N 300 to 32256; weights that rotate
-// through more than the last cache holds); the choice is 1.2% slower than the best of them in the
-// mean. Measured, in us, the runner-up in brackets: 1 row, 7168 -> 5376: 9.3 (tiles of 64 rows
-// in 6 shares 17); 32 rows, 5376 -> 21504: tiles of 64 in 3 shares 28 (few rows 36); 301 rows,
-// 5376 -> 21504: 128 rows 44 (256 rows 63); 1024 rows, 7168 -> 5376: 128 rows 39 (256 in two
-// shares 50); 1500 rows, 5376 -> 21504: 256 rows 146 (128 rows 158).
+// The kernel whose modelled time is least. Tiles by gemm_last_wave in units of four K steps of
+// 128. Few rows: the workgroups of the busiest CU by their K steps. Rates fitted to the measured
+// times of all of them, the tiles in one to nine shares, at 231 projections of 1 to 8000 rows
+// (K 256 to 14336, N 300 to 32256; weights that rotate through more than the last cache holds);
+// the choice is 1.1% slower than the best of them in the mean. Measured, in us, the runner-up in
+// brackets: 1 row, 7168 -> 5376: 10.0 (tiles of 64 rows in 4 shares 15.9); 32 rows, 5376 ->
+// 21504: tiles of 64 in 2 shares 29.4 (few rows 36.1); 640 rows, 13824 -> 5120: tiles of 64 59.7
+// (128 rows 67.0); 1024 rows, 7168 -> 5376: 128 rows 42.9 (256 in two shares 51.7); 1500 rows,
+// 5376 -> 21504: 256 rows 151.6 (128 rows 161.5).
 struct Choice {
     float us;
     unsigned rows, split;     // tile rows (64, 128, 256) and shares; or
     unsigned rb, nb;          // few rows: row and column blocks (rb 0: tiles)
 };
 // Few rows: us of a step, [row blocks - 1][column blocks 2, 4], and the busiest CU's workgroups.
-constexpr float STREAM_LAUNCH = 2.4f, STREAM_STEP[3][2] = {{.157f, .298f}, {.224f, .344f}, {.313f, 0.f}};
+constexpr float STREAM_LAUNCH = 3.1f, STREAM_STEP[3][2] = {{.157f, .279f}, {.195f, .387f}, {.308f, 0.f}};
 float stream_rounds(const h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
     const uint64_t groups = ((uint64_t)a.m + 16 * rb - 1) / (16 * rb) * (((uint64_t)a.n + 16 * nb - 1) / (16 * nb));
     return (float)((groups + g->cus - 1) / g->cus);
 }
 Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
-    static constexpr GemmRates RATES[3] = {{.68f, .518f, .355f, .6f, 3.8f, .088f, .77f},
-                                           {3.65f, 2.f, 1.36f, .15f, 3.95f, .085f, 2.3f},
-                                           {6.3f, 3.63f, 3.2f, .15f, 6.9f, .034f, 2.8f}};
-    static constexpr float LAUNCH[3] = {3.f, 3.35f, 0.f};
+    static constexpr GemmRates RATES[3] = {{2.38f, 1.49f, 1.18f, .15f, 3.45f, .0738f, .678f},
+                                           {3.68f, 1.87f, 1.56f, .15f, 3.84f, .0769f, 1.83f},
+                                           {6.49f, 3.63f, 3.31f, .15f, 6.69f, .0311f, 1.93f}};
+    static constexpr float LAUNCH[3] = {2.48f, 3.21f, 0.f};
     const unsigned steps = a.k / TK;
     Choice best{3.4e38f, 0, 1, 0, 0};
     for (unsigned i = 0; i < 3; i++) {
-        const unsigned rows = 64u << i, units = i ? (steps + QUAD - 1) / QUAD : steps;
+        const unsigned rows = 64u << i, units = (steps + QUAD - 1) / QUAD;
         const uint64_t tiles = ((uint64_t)a.m + rows - 1) / rows * ((a.n + 255) / 256);
         if (tiles > 0x7fffffffu) continue;
         const GemmPlan p = gemm_last_wave(g, (unsigned)tiles, units, RATES[i], rows / 256.f);
