@@ -25,6 +25,8 @@ constexpr uint32_t FP8_BLOCK = 128;
 constexpr int FP8_BLOCK_LEAST = -64;
 // 256 rows of codes have 32-bit offsets.
 constexpr uint32_t FP8_BLOCK_COLUMNS = (1u << 24) - FP8_BLOCK;
+// Most rows of one projection launch: its tile numbers are computed in 32 bits.
+constexpr uint32_t FP8_BLOCK_ROWS = 1u << 22;
 
 struct Fp8BlockLayout {
     size_t stride, scales, groups, bytes;

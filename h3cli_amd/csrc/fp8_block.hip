@@ -197,6 +197,19 @@ int run_gemm(h3_gpu *g, const h3_gpu_tensor *w, const Fp8BlockGemmArgs &a) {
     return h3_tensor_release(g, w);
 }
 
+// Rows [first, first + m) of a projection; first a multiple of 256: whole runs of 32 scale rows.
+Fp8BlockGemmArgs rows_of(Fp8BlockGemmArgs a, uint32_t first, uint32_t m) {
+    a.m = m;
+    if (a.xb) {
+        a.xb += (size_t)first * a.columns;
+    } else {
+        a.x += (size_t)first * a.k;
+        a.xs += fp8_block_scale_at(first, 0, a.groups);
+    }
+    if (a.y) a.y += (size_t)first * a.n;
+    return a;
+}
+
 bool overlap(const h3_gpu_tensor *a, const h3_gpu_tensor *b) { return a && b && a->data == b->data; }
 
 }  // namespace
@@ -395,7 +408,10 @@ int h3_fp8_block_linear(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, 
     a.y = (uint16_t *)out->data;
     a.bias = bias ? (const uint16_t *)bias->data : nullptr;
     char *rest;
-    return projection_input(g, in, k, 0, "linear input", a, &rest) && run_gemm(g, w, a) && h3_tensor_release(g, in);
+    if (!projection_input(g, in, k, 0, "linear input", a, &rest)) return 0;
+    for (uint32_t first = 0; first < rows; first += std::min(rows - first, FP8_BLOCK_ROWS))
+        if (!run_gemm(g, w, rows_of(a, first, std::min(rows - first, FP8_BLOCK_ROWS)))) return 0;
+    return h3_tensor_release(g, in);
 }
 
 int h3_fp8_block_mlp(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *w1,
@@ -413,24 +429,19 @@ int h3_fp8_block_mlp(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, con
     // The context keeps no more than MLP_WORKSPACE for them: calls of more rows run in parts.
     const bool fused = h3_gemm_fp8_block_fuses(g, rows, k, hidden);
     const size_t row_bytes = fp8_block_layout(1, hidden, 1).bytes + (fused ? 0 : (size_t)hidden * 8);
-    const uint32_t most = (uint32_t)std::min<size_t>(std::max<size_t>(MLP_WORKSPACE / row_bytes / 256, 1) * 256, rows);
+    const uint32_t most = (uint32_t)std::min<size_t>(std::max<size_t>(MLP_WORKSPACE / row_bytes / 256, 1) * 256,
+                                                     std::min(rows, FP8_BLOCK_ROWS));
     const size_t act = (fp8_block_layout(most, hidden, 1).bytes + 511) & ~(size_t)255;
     Fp8BlockGemmArgs all = gemm_args(w1, rows, 2 * hidden);
     all.swiglu = fused;
     char *rest;
     if (!projection_input(g, in, k, act + (fused ? 0 : (size_t)most * hidden * 8), "MLP input", all, &rest)) return 0;
-    for (uint32_t first = 0; first < rows; first += most) {
-        const uint32_t m = std::min(most, rows - first);
+    // The output may be the input: a BF16 input is packed as a whole first, or by a projection of
+    // so few rows that there is one part.
+    for (uint32_t first = 0, m; first < rows; first += m) {
+        m = std::min(most, rows - first);
         const Fp8BlockRows h = workspace_rows(g, rest, m, hidden);
-        // first is a multiple of 256: whole runs of 32 scale rows.
-        Fp8BlockGemmArgs a = all;
-        a.m = m;
-        if (a.xb) {
-            a.xb += (size_t)first * k;
-        } else {
-            a.x += (size_t)first * a.k;
-            a.xs += fp8_block_scale_at(first, 0, a.groups);
-        }
+        Fp8BlockGemmArgs a = rows_of(all, first, m);
         if (fused) a.out = h;
         else a.y32 = (float *)(rest + act);
         if (!run_gemm(g, w1, a) || (!fused && !h3_launch_swiglu_fp8_block(g, h, a.y32, true, m, hidden))) return 0;

@@ -125,7 +125,9 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs 
 #pragma unroll
         for (int j = 0; j < RB; j++) acc[i][j] = f32x4{};
 
-    // BF16 values of a step, as fp8_block_pack packs them: a row's four lanes hold a block.
+    // BF16 values of a step, as fp8_block_pack packs them: a row's four lanes hold a block. (A
+    // last block that is cut off is loaded whole: up to 254 bytes behind the last row, which a
+    // tensor's allocation has.)
     auto pack = [&](unsigned step, u32x4 *x) {
         float v[32];
 #pragma unroll
@@ -1048,7 +1050,7 @@ bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m, uint32_t k, uint32_t h
 }
 
 int h3_gemm_fp8_block(h3_gpu *g, const Fp8BlockGemmArgs &a) {
-    if (((uint64_t)a.m + 63) / 64 * ((a.n + 255) / 256) > 0x7fffffffu)
+    if (a.m > FP8_BLOCK_ROWS || ((uint64_t)a.m + 63) / 64 * ((a.n + 255) / 256) > 0x7fffffffu)
         return h3_set_error(g, "FP8 block projection: %u rows by %u columns are too many for one call", a.m, a.n);
     switch (epilogue_of(a)) {
     case EPI_PLAIN: return run<EPI_PLAIN>(g, a);
