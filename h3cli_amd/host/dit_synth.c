@@ -46,6 +46,7 @@ struct h3_hip_dit_synth {
     /* activations and tables */
     h3_gpu_tensor **qn, **kn;      /* per block Q/K RMSNorm weights [128] (qk_norm) */
     h3_gpu_tensor *latent, *latent_bf16, *x, *xn, *qkv, *q, *k, *v, *attn, *o, *h, *act, *f, *vel;
+    h3_gpu_tensor *xq;                 /* projection_quant 3: the norms' output, packed in place of xn */
     h3_sol_block *layout_blocks;   /* attention_mode 4: the bound 64-row layout */
     h3_gpu_tensor *cos_t, *sin_t, *row_map;
     uint64_t kept, total;
@@ -236,6 +237,14 @@ static h3_gpu_tensor *quant_random(h3_gpu *g, uint32_t n, uint32_t k, uint64_t s
     return t;
 }
 
+/* Block-scaled FP8 weight (projection_quant 3) of N(0, 1/k) BF16 values. */
+static h3_gpu_tensor *block_random(h3_gpu *g, uint32_t n, uint32_t k, uint64_t seed) {
+    h3_gpu_tensor *b = normal_tensor(g, (size_t)n * k, seed, 1.0f / sqrtf((float)k), 0.f);
+    h3_gpu_tensor *t = b ? h3_hip_fp8_block_weight_from_bf16(g, b, n, k) : NULL;
+    h3_gpu_tensor_free(b);
+    return t;
+}
+
 static int weights(h3_hip_dit_synth *m, char *error, size_t size) {
     h3_gpu *g = m->gpu;
     const h3_hip_dit_synth_config *c = &m->c;
@@ -244,9 +253,11 @@ static int weights(h3_hip_dit_synth *m, char *error, size_t size) {
         uint32_t n, k;
         proj_shape(c, j, &n, &k);
         m->host_bytes[j] = (size_t)n * k + (size_t)n * 4;
+        if (c->projection_quant == 3) h3_hip_fp8_block_layout(n, k, 128, NULL, NULL, NULL, &m->host_bytes[j]);
         if (streamed)
             for (int s = 0; s < 2; s++)
-                if (!(m->slot[s][j] = h3_hip_q8_new(g, n, k, k))) return fail(error, size, "slot: %s", h3_gpu_error(g));
+                if (!(m->slot[s][j] = c->projection_quant == 3 ? h3_hip_fp8_block_new(g, n, k, 128) : h3_hip_q8_new(g, n, k, k)))
+                    return fail(error, size, "slot: %s", h3_gpu_error(g));
     }
     size_t block_bytes = 0;
     for (int j = 0; j < PROJ; j++) block_bytes += m->host_bytes[j];
@@ -258,8 +269,10 @@ static int weights(h3_hip_dit_synth *m, char *error, size_t size) {
         for (int j = 0; j < PROJ; j++) {
             uint32_t n, k;
             proj_shape(c, j, &n, &k);
-            h3_gpu_tensor *t = c->projection_quant ? quant_random(g, n, k, c->seed * 7919ull + b * 8 + j)
-                                                   : q8_random(g, n, k, c->seed * 7919ull + b * 8 + j);
+            const uint64_t seed = c->seed * 7919ull + b * 8 + j;
+            h3_gpu_tensor *t = c->projection_quant == 3 ? block_random(g, n, k, seed)
+                               : c->projection_quant    ? quant_random(g, n, k, seed)
+                                                        : q8_random(g, n, k, seed);
             if (!t) return fail(error, size, "block %u weight %d: %s", b, j, h3_gpu_error(g));
             if (resident) m->proj[(size_t)b * PROJ + j] = t;
             else {
@@ -294,12 +307,13 @@ h3_hip_dit_synth *h3_hip_dit_synth_create(h3_gpu *g, const h3_hip_dit_synth_conf
         c->latent % 256 || !c->frames || !c->height || !c->width ||
         (c->rope_half != 64 && (!c->rope_half || c->rope_half > 64 || c->rope_half % 3)) ||
         (c->attention_mode != 0 && c->attention_mode != 1 && c->attention_mode != 4) ||
-        (c->projection_quant < 0 || c->projection_quant > 2) || c->trace_block > c->blocks) {
+        (c->projection_quant < 0 || c->projection_quant > 3) || c->trace_block > c->blocks) {
         fail(error, size, "synthetic DiT: hidden/mlp/latent multiples of 256, rope_half 64 or a multiple of 3 "
-                          "below it, attention mode 0/1/4, projection_quant 0/1/2, trace_block <= blocks");
+                          "below it, attention mode 0/1/4, projection_quant 0 to 3, trace_block <= blocks");
         return NULL;
     }
-    if (c->projection_quant && c->streamed_first < c->blocks) {
+    const int packed = c->projection_quant == 1 || c->projection_quant == 2, blocked = c->projection_quant == 3;
+    if (packed && c->streamed_first < c->blocks) {
         fail(error, size, "synthetic DiT: quantized projections need every block resident");
         return NULL;
     }
@@ -324,7 +338,7 @@ h3_hip_dit_synth *h3_hip_dit_synth_create(h3_gpu *g, const h3_hip_dit_synth_conf
         fail(error, size, "attention configure: %s", h3_gpu_error(g));
         goto bad;
     }
-    if (c->projection_quant) {
+    if (packed) {
         /* Synthetic weights are packed in place; checkpoints go through the
          * artifact cache. No H3 admission bytes: every block is resident. */
         const char *tmp = getenv("TMPDIR");
@@ -351,15 +365,18 @@ h3_hip_dit_synth *h3_hip_dit_synth_create(h3_gpu *g, const h3_hip_dit_synth_conf
         m->q = bf16_buffer(g, R * I); m->k = bf16_buffer(g, R * I); m->v = bf16_buffer(g, R * I);
         m->attn = bf16_buffer(g, R * I); m->o = bf16_buffer(g, R * H);
         /* The SwiGLU MLP is one call with a workspace of its own; its stages are
-         * separate only for packed weights and, beside it, for the trace. */
-        const int stages = c->projection_quant || !c->swiglu || c->trace_block;
-        const int act = c->projection_quant || (c->swiglu && c->trace_block);
+         * separate only for packed weights and, beside it, for the trace. Weights in FP8
+         * blocks take the norms' output in blocks too. */
+        const int stages = packed || !c->swiglu || c->trace_block;
+        const int act = packed || (blocked && !c->swiglu) || (c->swiglu && c->trace_block);
+        m->xq = blocked ? h3_hip_fp8_block_new(g, m->rows, c->hidden, 1) : NULL;
         m->h = stages ? bf16_buffer(g, R * c->mlp * (c->swiglu ? 2 : 1)) : NULL;
         m->f = bf16_buffer(g, R * H);
         m->act = act ? bf16_buffer(g, R * c->mlp) : NULL;
         m->vel = bf16_buffer(g, R * c->latent);
         if (!m->row_map || !m->latent || !m->latent_bf16 || !m->x || !m->xn || !m->qkv || !m->q || !m->k || !m->v ||
-            !m->attn || !m->o || (stages && !m->h) || !m->f || !m->vel || (act && !m->act)) {
+            !m->attn || !m->o || (stages && !m->h) || !m->f || !m->vel || (act && !m->act) ||
+            (blocked && !m->xq)) {
             fail(error, size, "activations: %s", h3_gpu_error(g));
             h3_gpu_cancel(g);
             goto bad;
@@ -430,7 +447,7 @@ void h3_hip_dit_synth_free(h3_hip_dit_synth *m) {
         if (m->kn) h3_gpu_tensor_free(m->kn[b]);
     }
     h3_gpu_tensor *all[] = {m->patch, m->head, m->head_norm, m->head_mod, m->latent, m->latent_bf16, m->x, m->xn,
-                            m->qkv, m->q, m->k, m->v, m->attn, m->o, m->h, m->act, m->f, m->vel, m->cos_t, m->sin_t,
+                            m->qkv, m->q, m->k, m->v, m->attn, m->o, m->h, m->act, m->f, m->xq, m->vel, m->cos_t, m->sin_t,
                             m->row_map};
     for (size_t i = 0; i < sizeof(all) / sizeof(*all); i++) h3_gpu_tensor_free(all[i]);
     for (int i = 0; i < TRACE_COUNT; i++) h3_gpu_tensor_free(m->trace[i]);
@@ -463,6 +480,7 @@ int h3_hip_dit_synth_step(h3_hip_dit_synth *m, int step, float dt) {
     const h3_hip_dit_synth_config *c = &m->c;
     const uint32_t R = m->rows, H = c->hidden, L = c->latent, I = c->heads * 128;
     const float scale = 1.0f / sqrtf(128.0f);
+    const int blocked = c->projection_quant == 3;
     if (!h3_gpu_begin(g)) return 0;
     int ok = h3_gpu_dit_attention_noise(g, step, 0.5f, 0.5f) && prefetch(m, c->streamed_first) &&
              h3_gpu_cast_f32_to_bf16(g, m->latent_bf16, m->latent, R * L) &&
@@ -474,23 +492,38 @@ int h3_hip_dit_synth_step(h3_hip_dit_synth *m, int step, float dt) {
         const h3_gpu_tensor *qn = c->qk_norm ? m->qn[b] : NULL, *kn = c->qk_norm ? m->kn[b] : NULL;
         const int tr = c->trace_block == b + 1;
         ok = (!tr || keep(m, T_X0, m->x)) &&
-             h3_gpu_adaln_bf16(g, m->xn, m->x, m->norm1[b], m->mod[b], m->row_map, R, H, SLOTS, 0, 1, c->eps);
-        if (c->grouped_qkv)
+             (blocked ? h3_hip_adaln_fp8_block(g, m->xq, m->x, m->norm1[b], m->mod[b], m->row_map, R, H, SLOTS, 0, 1, c->eps) &&
+                            (!tr || h3_hip_fp8_block_unpack(g, m->xn, m->xq, R, H))
+                      : h3_gpu_adaln_bf16(g, m->xn, m->x, m->norm1[b], m->mod[b], m->row_map, R, H, SLOTS, 0, 1, c->eps));
+        if (c->grouped_qkv && !blocked)
             ok = ok && h3_gpu_grouped_qkv_linear_rope_bf16(g, m->q, m->k, m->v, m->qkv, m->xn, w[0], qn, kn, m->cos_t,
                                                            m->sin_t, R, H, c->heads, 128, c->rope_half, c->eps);
         else
-            ok = ok && h3_gpu_linear_bf16(g, m->qkv, m->xn, w[0], NULL, R, H, 3 * I) &&
-                 h3_gpu_qkv_rope_bf16(g, m->q, m->k, m->v, m->qkv, qn, kn, m->cos_t, m->sin_t, R, c->heads, 128,
-                                      c->rope_half, c->eps);
+            ok = ok &&
+                 (blocked ? h3_hip_linear_fp8_block(g, m->qkv, m->xq, w[0], NULL, R, H, 3 * I)
+                          : h3_gpu_linear_bf16(g, m->qkv, m->xn, w[0], NULL, R, H, 3 * I)) &&
+                 (c->grouped_qkv ? h3_gpu_grouped_qkv_rope_bf16 : h3_gpu_qkv_rope_bf16)(
+                     g, m->q, m->k, m->v, m->qkv, qn, kn, m->cos_t, m->sin_t, R, c->heads, 128, c->rope_half, c->eps);
         ok = ok && (!tr || (keep(m, T_XN1, m->xn) && keep(m, T_QKV, m->qkv) && keep(m, T_Q, m->q) &&
                             keep(m, T_K, m->k) && keep(m, T_V, m->v)));
         ok = ok && h3_gpu_dit_sdpa_bf16(g, m->attn, m->q, m->k, m->v, R, c->heads, 128, scale, 0, b, step) &&
              h3_gpu_linear_bf16(g, m->o, m->attn, w[1], NULL, R, I, H) &&
              (!tr || (keep(m, T_ATTN, m->attn) && keep(m, T_O, m->o))) &&
-             h3_gpu_gate_adaln_bf16(g, m->x, m->xn, m->x, m->o, m->norm2[b], m->mod[b], m->mod[b], m->row_map, R, H,
-                                    SLOTS, 2, 3, 4, c->eps) &&
+             (blocked ? h3_hip_gate_adaln_fp8_block(g, m->x, m->xq, m->x, m->o, m->norm2[b], m->mod[b], m->mod[b], m->row_map,
+                                                    R, H, SLOTS, 2, 3, 4, c->eps) &&
+                            (!tr || h3_hip_fp8_block_unpack(g, m->xn, m->xq, R, H))
+                      : h3_gpu_gate_adaln_bf16(g, m->x, m->xn, m->x, m->o, m->norm2[b], m->mod[b], m->mod[b], m->row_map, R, H,
+                                               SLOTS, 2, 3, 4, c->eps)) &&
              (!tr || (keep(m, T_X1, m->x) && keep(m, T_XN2, m->xn)));
-        if (c->swiglu && !c->projection_quant) {
+        if (blocked && c->swiglu) {
+            ok = ok && (!tr || (h3_hip_linear_fp8_block(g, m->h, m->xq, w[2], NULL, R, H, 2 * c->mlp) &&
+                                h3_gpu_swiglu_bf16(g, m->act, m->h, R, c->mlp))) &&
+                 h3_hip_mlp_fp8_block(g, m->f, m->xq, w[2], w[3], R, H, c->mlp, H);
+        } else if (blocked) {
+            ok = ok && h3_hip_linear_fp8_block(g, m->h, m->xq, w[2], NULL, R, H, c->mlp) &&
+                 h3_gpu_gelu_bf16(g, m->act, m->h, (uint32_t)(R * c->mlp), 1) &&
+                 h3_gpu_linear_bf16(g, m->f, m->act, w[3], NULL, R, c->mlp, H);
+        } else if (c->swiglu && !c->projection_quant) {
             /* The traced block runs the same MLP; its product and activation, which that
              * call does not write, are computed beside it. */
             ok = ok && (!tr || (h3_gpu_linear_bf16(g, m->h, m->xn, w[2], NULL, R, H, 2 * c->mlp) &&
@@ -546,6 +579,14 @@ static void block_shape(const h3_hip_dit_synth_config *c, int i, uint32_t *rows,
     *cols = 0;
 }
 
+/* A BF16 weight of a file, packed in FP8 blocks. */
+static h3_gpu_tensor *block_load(h3_gpu *g, const char *path, uint64_t offset, uint32_t n, uint32_t k) {
+    h3_gpu_tensor *b = h3_gpu_tensor_load_bf16(g, path, offset, (size_t)n * k);
+    h3_gpu_tensor *t = b ? h3_hip_fp8_block_weight_from_bf16(g, b, n, k) : NULL;
+    h3_gpu_tensor_free(b);
+    return t;
+}
+
 int h3_hip_dit_synth_load(h3_hip_dit_synth *m, const char *path, char *error, size_t size) {
     if (!m || !path) return fail(error, size, "missing model or path");
     const h3_hip_dit_synth_config *c = &m->c;
@@ -576,6 +617,7 @@ int h3_hip_dit_synth_load(h3_hip_dit_synth *m, const char *path, char *error, si
             snprintf(name, sizeof(name), "blocks.%u.%s", b, BLOCK_NAMES[i]);
             const h3_st_tensor *t = h3_st_find(&header, name);
             h3_gpu_tensor *loaded = !cols ? h3_gpu_tensor_load_bf16(g, path, t->file_offset, rows)
+                                    : c->projection_quant == 3 ? block_load(g, path, t->file_offset, rows, cols)
                                     : c->projection_quant ? h3_gpu_quant_load(g, path, t->file_offset, rows, cols)
                                                           : h3_gpu_q8_load(g, path, t->file_offset, rows, cols);
             if (!loaded) { ok = fail(error, size, "%s: %s", name, h3_gpu_error(g)); break; }

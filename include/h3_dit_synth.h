@@ -35,7 +35,8 @@ typedef struct {
     int grouped_qkv;            /* 1: QKV rows grouped per head [heads, 3, 128] (H3 checkpoint layout) */
     float subblock_sparsity;    /* attention_mode 4: the request's sparsity (0.75) */
     int projection_quant;       /* 0: W8A16 q8 projections; 1: FP8 W8A8, 2: NVFP4 W4A4
-                                   (h3_gpu_quant_configure mode 1/2, every block resident) */
+                                   (h3_gpu_quant_configure mode 1/2, every block resident); 3:
+                                   block-scaled FP8 (h3_hip_ext.h), norms with packed output */
     uint32_t trace_block;       /* 0: off; b + 1: each step keeps device copies of block b's stage
                                    tensors, read back as "trace.<stage>" (h3_hip_dit_synth_tensor) */
 } h3_hip_dit_synth_config;
@@ -71,7 +72,7 @@ typedef struct h3_hip_dit_synth h3_hip_dit_synth;
  * the block mask): seeded W8A16 projection weights (int8 U[-127,127], per-output
  * channel fp32 scales U[1e-3,1e-2]) or, with projection_quant 1 or 2, FP8 or
  * NVFP4 weights packed from N(0, 1/k) BF16 values (the context's quantization is configured,
- * artifacts under $TMPDIR/h3cli-amd-quant), AdaLN norms and modulation from a 256-d
+ * artifacts under $TMPDIR/h3cli-amd-quant), with 3 such values packed in FP8 blocks, AdaLN norms and modulation from a 256-d
  * sinusoidal timestep embedding, 3D RoPE tables, a seeded latent. Blocks from
  * streamed_first on live in pinned host memory and are copied into two device
  * slots on the copy stream one block ahead of use. */
@@ -92,7 +93,7 @@ int h3_hip_dit_synth_step(h3_hip_dit_synth *model, int step, float dt);
  * (SwiGLU) or mlp, hidden], "mlp.fc2.weight" [hidden, mlp]; all BF16. The four
  * projections are packed to W8A16 on the device with the reference q8 recipe
  * (group 64), or with projection_quant 1 / 2 to FP8 / NVFP4 through
- * h3_gpu_quant_load and its artifact cache. Every block must be resident (streamed_first >= blocks); no
+ * h3_gpu_quant_load and its artifact cache, with 3 to FP8 blocks. Every block must be resident (streamed_first >= blocks); no
  * command may be active. Errors name the first missing or mismatched tensor. */
 int h3_hip_dit_synth_load(h3_hip_dit_synth *model, const char *path, char *error, size_t error_size);
 
@@ -103,9 +104,10 @@ int h3_hip_dit_synth_load(h3_hip_dit_synth *model, const char *path, char *error
  * "rope_sin" [rows, rope_half], "row_map" (U32 [rows]: 0 video, 1 audio), a
  * block's modulation "blocks.<b>.modulation" [2, 6, hidden], a resident
  * block's weights under the checkpoint names above
- * ("blocks.0.attn.qkv_proj.weight": a W8A16 tensor; norms BF16), and with
+ * ("blocks.0.attn.qkv_proj.weight": a W8A16 tensor, or as projection_quant
+ * says; norms BF16), and with
  * trace_block the traced block's stages "trace.x0" (block input), "xn1"
- * (AdaLN), "qkv", "q", "k", "v", "attn", "o" (out projection), "x1" (gated
+ * (AdaLN; with projection_quant 3 the values of its blocks, as "xn2"), "qkv", "q", "k", "v", "attn", "o" (out projection), "x1" (gated
  * residual), "xn2" (second AdaLN), "h" (fc1, GELU applied when fused),
  * "act" (SwiGLU or separate GELU; with SwiGLU the step's MLP is one call and
  * these two are computed beside it), "f" (fc2) and "x2" (block output), and
