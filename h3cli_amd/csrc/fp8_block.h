@@ -111,6 +111,12 @@ __device__ inline float swiglu_exact(float gate, float up) {
     r = gate < -87.f ? 0.f : fmaf(fmaf(-d, r, 1.f), r, r);
     return gate * r * up;
 }
+// The same for a projection's sums, whose own error (1.5e-5, the matrix core's additions) is
+// far above what the two differ by, |gate| 2^-24: half the instructions, which nothing hides in
+// an epilogue. A gate whose exponential overflows gives zero.
+__device__ inline float swiglu_of_sums(float gate, float up) {
+    return gate * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(gate * -1.4426950408889634f)) * up;
+}
 #endif
 
 // y = bf16(x . w^T + bias) and its variants (h3_gemm_fp8_block).

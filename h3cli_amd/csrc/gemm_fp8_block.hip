@@ -409,7 +409,7 @@ __device__ inline void wave_stores_first() {
 // lane half hf holds columns 8 g + 4 hf + 0..3. v_permlane32_swap gives the low half both halves
 // of group g, the high half those of group g + 1: 16 bytes a lane.
 template <int EPI>
-__device__ inline void pipe_round(const Fp8BlockGemmArgs &a, unsigned col, unsigned hf, const f32x16 &c, uint8_t *to) {
+__device__ inline void round_row(const Fp8BlockGemmArgs &a, unsigned col, unsigned hf, const f32x16 &c, uint8_t *to) {
 #pragma unroll
     for (int g = 0; g < 4; g += 2) {
         unsigned w[2][2];
@@ -433,28 +433,31 @@ __device__ inline void pipe_round(const Fp8BlockGemmArgs &a, unsigned col, unsig
     }
 }
 
-// 32 rows x 128 columns of a wave, n a multiple of 8, through LDS into whole cache lines, past the
-// L2's resident lines. All workgroups of a wave of tiles store at once, 33 MB; stored from the
-// registers, 32 bytes of 32 rows an instruction, that takes 12 of a tile's 75 us (18225 rows, 5376
-// -> 28672: 2385 us, 1975 without any stores); so 2157. (The lines alone: 2370; past the L2 alone:
-// 2440.)
-constexpr unsigned ROW_LDS = 128 * 2 + 16;    // bytes of a row in LDS, padded against bank conflicts
-template <int EPI>
-__device__ inline void pipe_rows(const Fp8BlockGemmArgs &a, unsigned row0, unsigned col, unsigned lane, const f32x16 &c0,
-                                 const f32x16 &c1, const f32x16 &c2, const f32x16 &c3, uint8_t *rows) {
-    const unsigned hf = lane / 32, row = row0 + lane / 16, at = col + lane % 16 * 8;
-    uint8_t *to = rows + lane % 32 * ROW_LDS;
-    pipe_round<EPI>(a, col, hf, c0, to);
-    pipe_round<EPI>(a, col + 32, hf, c1, to + 64);
-    pipe_round<EPI>(a, col + 64, hf, c2, to + 128);
-    pipe_round<EPI>(a, col + 96, hf, c3, to + 192);
+// 32 rows x 32 NB columns of a wave, n a multiple of 8, through LDS into whole cache lines.
+//
+// PAST: past the L2's resident lines. All workgroups of a wave of 256-row tiles store at once, 33
+// MB; stored from the registers, 32 bytes of 32 rows an instruction, that takes 12 of a tile's 75
+// us (18225 rows, 5376 -> 28672: 2385 us, 1975 without any stores); so 2132. (The lines alone:
+// 2370; past the L2 alone: 2440.)
+template <int NB> constexpr unsigned ROW_LDS = NB * 64 + 16;    // bytes of a row in LDS, padded against bank conflicts
+template <int EPI, bool PAST, int NB>
+__device__ inline void store_rows(const Fp8BlockGemmArgs &a, unsigned row0, unsigned col, unsigned lane,
+                                  const f32x16 *const (&c)[NB], uint8_t *rows) {
+    constexpr unsigned LANES = NB * 4, STEP = 64 / LANES;       // lanes of a row, rows of an instruction
+    const unsigned hf = lane / 32, row = row0 + lane / LANES, at = col + lane % LANES * 8;
+    uint8_t *to = rows + lane % 32 * ROW_LDS<NB>;
+#pragma unroll
+    for (int i = 0; i < NB; i++) round_row<EPI>(a, col + 32 * i, hf, *c[i], to + 64 * i);
     wave_stores_first();
-    const uint8_t *from = rows + lane / 16 * ROW_LDS + lane % 16 * 16;
+    const uint8_t *from = rows + lane / LANES * ROW_LDS<NB> + lane % LANES * 16;
     uint16_t *dst = a.y + (size_t)row * a.n + at;
 #pragma unroll
-    for (unsigned r = 0; r < 32; r += 4) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(from + r * ROW_LDS);
-        if (row + r < a.m && at < a.n) __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(dst + (size_t)r * a.n));
+    for (unsigned r = 0; r < 32; r += STEP) {
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(from + r * ROW_LDS<NB>);
+        if (row + r >= a.m || at >= a.n) continue;
+        u32x4 *line = reinterpret_cast<u32x4 *>(dst + (size_t)r * a.n);
+        if constexpr (PAST) __builtin_nontemporal_store(v, line);
+        else *line = v;
     }
     wave_stores_first();
 }
@@ -493,6 +496,7 @@ __device__ inline void pipe_any(const Fp8BlockGemmArgs &a, unsigned row0, unsign
     wave_stores_first();
 }
 
+constexpr unsigned CODE_ROW = 128 + 16, CODE_ROWS = 512;      // a row of codes in LDS, and where they begin
 // The epilogue of a wave's 32 rows from row0 x 128 columns, blocks c0 to c3. SwiGLU: the
 // two waves of a row meet in scratch (LDS) for the largest magnitude of its 128 columns.
 template <int EPI>
@@ -506,15 +510,15 @@ __device__ inline void pipe_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, u
         return;
     }
     if constexpr (EPI != EPI_SWIGLU) {
-        pipe_rows<EPI>(a, row0, col, lane, c0, c1, c2, c3, (uint8_t *)scratch + (wm * 2 + wn) * 32 * ROW_LDS);
+        store_rows<EPI, true, 4>(a, row0, col, lane, {&c0, &c1, &c2, &c3}, (uint8_t *)scratch + (wm * 2 + wn) * 32 * ROW_LDS<4>);
         return;
     }
     float v[32];
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        v[e] = swiglu_exact(c0[e], c1[e]);
-        v[16 + e] = swiglu_exact(c2[e], c3[e]);
+        v[e] = swiglu_of_sums(c0[e], c1[e]);
+        v[16 + e] = swiglu_of_sums(c2[e], c3[e]);
     }
     unsigned amax = fp8_block_magnitude<32>(v, bad);
     if (bad && row < a.m) *a.out.fault = 1u;
@@ -524,13 +528,22 @@ __device__ inline void pipe_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, u
     const unsigned scale = fp8_block_scale(max(most[wm][0][n32], most[wm][1][n32]));
     __syncthreads();
     const float value = fp8_block_value(scale);
-    // Groups g and g + 1 go out together, eight codes a lane.
-    uint8_t *dst = a.out.codes + (size_t)row * a.out.stride + n0 / 2 + wn * 64 + hf * 8;
+    // The codes in whole cache lines, as in store_rows (8193 rows, 5376 -> 14336 -> 5376: 0.5%). The
+    // next row block writes there behind its own barriers.
+    uint8_t *rows = (uint8_t *)scratch + CODE_ROWS + wm * 32 * CODE_ROW;
 #pragma unroll
     for (int g = 0; g < 8; g += 2) {
         const auto s = __builtin_amdgcn_permlane32_swap(fp8_block_encode4(v + 4 * g, value),
                                                         fp8_block_encode4(v + 4 * g + 4, value), false, false);
-        if (row < a.m) *reinterpret_cast<uint2 *>(dst + g * 8) = make_uint2(s[0], s[1]);
+        *reinterpret_cast<uint2 *>(rows + n32 * CODE_ROW + wn * 64 + hf * 8 + g * 8) = make_uint2(s[0], s[1]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (unsigned r = wn * 16 + lane / 8, h = 0; h < 2; h++, r += 8) {
+        const u32x4 o = *reinterpret_cast<const u32x4 *>(rows + r * CODE_ROW + lane % 8 * 16);
+        if (row0 + r < a.m)
+            __builtin_nontemporal_store(o, reinterpret_cast<u32x4 *>(a.out.codes + (size_t)(row0 + r) * a.out.stride + n0 / 2 +
+                                                                     lane % 8 * 16));
     }
     if (row < a.m && wn == 0 && hf == 0) a.out.scales[fp8_block_scale_at(row, n0 / 256, a.out.groups)] = (uint8_t)scale;
 }
@@ -693,7 +706,7 @@ void fp8_block_pipe(Fp8BlockGemmArgs a) {
 template <int EPI, int TM>
 __global__ __launch_bounds__(PIPE_T) void fp8_block_pipe_reduce(Fp8BlockGemmArgs a) {
     constexpr unsigned NJ = TM / 64;
-    __shared__ __attribute__((aligned(16))) uint8_t scratch[EPI == EPI_ANY ? ANY_LDS : EPI == EPI_SWIGLU ? 512 : 4 * 32 * ROW_LDS];
+    __shared__ __attribute__((aligned(16))) uint8_t scratch[EPI == EPI_ANY ? ANY_LDS : EPI == EPI_SWIGLU ? CODE_ROWS + 2 * 32 * CODE_ROW : 4 * 32 * ROW_LDS<4>];
     const unsigned tile = blockIdx.x / NJ, j = blockIdx.x % NJ, tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
     unsigned m0, n0;
     pipe_tile<TM>(a, split_tile(a.tile, tile), m0, n0);
@@ -782,12 +795,17 @@ __device__ inline void mid_tile(const Fp8BlockGemmArgs &a, unsigned pid, unsigne
 }
 
 // The epilogue of a wave's row block (32 rows from row0) and two column blocks from col0.
-// SwiGLU: the four waves of a row meet in `most` for the block's largest magnitude.
+// SwiGLU: the four waves of a row meet in scratch (LDS) for the block's largest magnitude.
 template <int EPI>
 __device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, unsigned n0, unsigned wn, unsigned lane,
-                                    const f32x16 &c0, const f32x16 &c1, unsigned (*most)[32]) {
+                                    const f32x16 &c0, const f32x16 &c1, void *scratch) {
     const unsigned n32 = lane % 32, hf = lane / 32, row = row0 + n32;
-    if constexpr (EPI != EPI_SWIGLU) {
+    auto most = (unsigned(*)[32])scratch;
+    if constexpr (EPI == EPI_PLAIN || EPI == EPI_BIAS) {
+        store_rows<EPI, false, 2>(a, row0, n0 + wn * 64, lane, {&c0, &c1}, (uint8_t *)scratch + wn * 32 * ROW_LDS<2>);
+        return;
+    }
+    if constexpr (EPI == EPI_ANY) {
 #pragma unroll
         for (int g = 0; g < 4; g++) {
             store4<EPI>(a, row, n0 + wn * 64 + g * 8 + hf * 4, f32x4{c0[4 * g], c0[4 * g + 1], c0[4 * g + 2], c0[4 * g + 3]});
@@ -798,7 +816,7 @@ __device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, un
     float v[16];
     bool bad = false;
 #pragma unroll
-    for (int e = 0; e < 16; e++) v[e] = swiglu_exact(c0[e], c1[e]);
+    for (int e = 0; e < 16; e++) v[e] = swiglu_of_sums(c0[e], c1[e]);
     unsigned amax = fp8_block_magnitude<16>(v, bad);
     if (bad && row < a.m) *a.out.fault = 1u;
     amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
@@ -911,19 +929,19 @@ void fp8_block_mid(Fp8BlockGemmArgs a) {
         }
         return;
     }
-    if constexpr (SWIGLU) __syncthreads();     // all have read their last fragments
+    if constexpr (EPI != EPI_ANY) __syncthreads();     // all have read their last fragments
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         hold(c[0][j]);
         hold(c[1][j]);
-        mid_epilogue<EPI>(a, m0 + j * 32, n0, wn, lane, c[0][j], c[1][j], (unsigned(*)[32])lds);
+        mid_epilogue<EPI>(a, m0 + j * 32, n0, wn, lane, c[0][j], c[1][j], lds);
     }
 }
 
 // The split tiles' shares added in order, and the epilogue. One workgroup per (tile, row block).
 template <int EPI>
 __global__ __launch_bounds__(MID_T) void fp8_block_mid_reduce(Fp8BlockGemmArgs a) {
-    __shared__ unsigned most[4][32];
+    __shared__ __attribute__((aligned(16))) uint8_t scratch[EPI == EPI_SWIGLU ? 512 : EPI == EPI_ANY ? 16 : 4 * 32 * ROW_LDS<2>];
     const unsigned tile = blockIdx.x / 2, j = blockIdx.x % 2, tid = threadIdx.x;
     unsigned m0, n0;
     mid_tile(a, split_tile(a.tile, tile), m0, n0);
@@ -942,7 +960,7 @@ __global__ __launch_bounds__(MID_T) void fp8_block_mid_reduce(Fp8BlockGemmArgs a
 #pragma unroll
                 for (int e = 0; e < 4; e++) c[i][4 * g + e] += v[e];
             }
-    mid_epilogue<EPI>(a, row0, n0, tid / 64, tid % 64, c[0], c[1], most);
+    mid_epilogue<EPI>(a, row0, n0, tid / 64, tid % 64, c[0], c[1], scratch);
 }
 
 template <int EPI> int launch_mid(h3_gpu *g, Fp8BlockGemmArgs a, unsigned split) {
@@ -1003,26 +1021,28 @@ template <int EPI, int TM> int launch_pipe(h3_gpu *g, Fp8BlockGemmArgs a, unsign
 // times of all of them, the tiles in one to nine shares, at 231 projections of 1 to 8000 rows
 // (K 256 to 14336, N 300 to 32256; weights that rotate through more than the last cache holds);
 // the choice is 1.1% slower than the best of them in the mean. Measured, in us, the runner-up in
-// brackets: 1 row, 7168 -> 5376: 10.0 (tiles of 64 rows in 4 shares 15.9); 32 rows, 5376 ->
-// 21504: tiles of 64 in 2 shares 29.4 (few rows 36.1); 640 rows, 13824 -> 5120: tiles of 64 59.7
-// (128 rows 67.0); 1024 rows, 7168 -> 5376: 128 rows 42.9 (256 in two shares 51.7); 1500 rows,
-// 5376 -> 21504: 256 rows 151.6 (128 rows 161.5).
+// brackets: 1 row, 7168 -> 5376: 9.7 (tiles of 64 rows in 4 shares 15.7); 32 rows, 5376 -> 21504:
+// tiles of 64 in 2 shares 28.8 (128 rows in 2 shares 30.5); 640 rows, 13824 -> 5120: 128 rows in 2
+// shares 50.5 (64 rows 57.6); 1024 rows, 7168 -> 5376: 128 rows 38.7 (256 in 2 shares 49.4); 1500
+// rows, 5376 -> 21504: 256 rows 146.4 (128 rows 153.8).
 struct Choice {
     float us;
     unsigned rows, split;     // tile rows (64, 128, 256) and shares; or
     unsigned rb, nb;          // few rows: row and column blocks (rb 0: tiles)
 };
-// Few rows: us of a step, [row blocks - 1][column blocks 2, 4], and the busiest CU's workgroups.
-constexpr float STREAM_LAUNCH = 3.1f, STREAM_STEP[3][2] = {{.157f, .279f}, {.195f, .387f}, {.308f, 0.f}};
+// Few rows: us of a step, [row blocks - 1][column blocks 2, 4], and the busiest CU's workgroups;
+// no less than the weight's reads (5.3 TB/s).
+constexpr float STREAM_LAUNCH = 3.96f, STREAM_BYTE = 1.9e-7f;
+constexpr float STREAM_STEP[3][2] = {{.169f, .279f}, {.188f, .342f}, {.293f, 0.f}};
 float stream_rounds(const h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
     const uint64_t groups = ((uint64_t)a.m + 16 * rb - 1) / (16 * rb) * (((uint64_t)a.n + 16 * nb - 1) / (16 * nb));
     return (float)((groups + g->cus - 1) / g->cus);
 }
 Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
-    static constexpr GemmRates RATES[3] = {{2.38f, 1.49f, 1.18f, .15f, 3.45f, .0738f, .678f},
-                                           {3.68f, 1.87f, 1.56f, .15f, 3.84f, .0769f, 1.83f},
-                                           {6.49f, 3.63f, 3.31f, .15f, 6.69f, .0311f, 1.93f}};
-    static constexpr float LAUNCH[3] = {2.48f, 3.21f, 0.f};
+    static constexpr GemmRates RATES[3] = {{2.44f, 1.74f, .722f, .15f, 1.81f, .083f, .98f},
+                                           {3.63f, 1.99f, 1.82f, .3f, 3.61f, .0532f, 1.02f},
+                                           {6.35f, 3.62f, 3.8f, .3f, 7.63f, .0346f, 1.f}};
+    static constexpr float LAUNCH[3] = {2.77f, 3.54f, 0.f};
     const unsigned steps = a.k / TK;
     Choice best{3.4e38f, 0, 1, 0, 0};
     for (unsigned i = 0; i < 3; i++) {
@@ -1037,7 +1057,7 @@ Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
     for (unsigned rb = 1; rb <= 3; rb++)
         for (unsigned nb = 2; nb <= (rb < 3 ? 4u : 2u); nb += 2) {
             const float rounds = stream_rounds(g, a, rb, nb);
-            const float us = STREAM_LAUNCH + rounds * steps * STREAM_STEP[rb - 1][nb / 4];
+            const float us = STREAM_LAUNCH + std::max(rounds * steps * STREAM_STEP[rb - 1][nb / 4], (float)a.n * a.k * STREAM_BYTE);
             if (us < best.us && rounds < 1e6f) best = {us, 0, 1, rb, nb};
         }
     return best;

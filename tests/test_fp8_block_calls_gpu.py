@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from h3cli_amd import synth
-from h3cli_amd.runtime import Gpu
+from h3cli_amd.runtime import Gpu, H3Error
 from tests.helpers import bf16
 from tests.test_capture_gpu import Graph
 from tests.test_fp8_block_gpu import (HALF_BF16, MFMA, Packed, activation, linear, new, quantized, values, weight,
@@ -198,3 +198,22 @@ def test_two_graphs():
             rows_within(g, t, w, got.reshape(rows, n), rows, k, n, "graph")
         for graph in graphs:
             graph.close()
+
+
+@pytest.mark.parametrize("rows", [16, 300, 1500])
+def test_mlp_overflow_fails_the_submit(rows):
+    """Sums beyond FP32's range: the activation is not finite."""
+    k, hidden = 256, 14336
+    with Gpu() as g:
+        def ones(n, columns, tile, scale):
+            codes = np.full((n, columns), 0x38, np.uint8)
+            scales = np.full((-(-n // tile), -(-columns // 128)), scale, np.uint8)
+            return Packed(g, g.lib.h3_hip_fp8_block_from_packed(g.handle, codes.ctypes.data, scales.ctypes.data, n, columns, tile),
+                          n, columns, tile)
+        w1, w2, out = ones(2 * hidden, k, 128, 254), ones(k, hidden, 128, 100), g.empty(rows * k)
+        x = ones(rows, k, 1, 254)
+        g.begin()
+        g.check(g.lib.h3_hip_mlp_fp8_block(g.handle, out.handle, x.handle, w1.handle, w2.handle, rows, k, hidden, k), "mlp")
+        with pytest.raises(H3Error, match="nonfinite"):
+            g.submit()
+        g.cancel()
