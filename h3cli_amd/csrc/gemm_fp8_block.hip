@@ -1020,7 +1020,7 @@ template <int EPI, int TM> int launch_pipe(h3_gpu *g, Fp8BlockGemmArgs a, unsign
 // 128. Few rows: the workgroups of the busiest CU by their K steps. Rates fitted to the measured
 // times of all of them, the tiles in one to nine shares, at 231 projections of 1 to 8000 rows
 // (K 256 to 14336, N 300 to 32256; weights that rotate through more than the last cache holds);
-// the choice is 1.1% slower than the best of them in the mean. Measured, in us, the runner-up in
+// the choice is 0.8% slower than the best of them in the mean. Measured, in us, the runner-up in
 // brackets: 1 row, 7168 -> 5376: 9.7 (tiles of 64 rows in 4 shares 15.7); 32 rows, 5376 -> 21504:
 // tiles of 64 in 2 shares 28.8 (128 rows in 2 shares 30.5); 640 rows, 13824 -> 5120: 128 rows in 2
 // shares 50.5 (64 rows 57.6); 1024 rows, 7168 -> 5376: 128 rows 38.7 (256 in 2 shares 49.4); 1500
@@ -1030,19 +1030,21 @@ struct Choice {
     unsigned rows, split;     // tile rows (64, 128, 256) and shares; or
     unsigned rb, nb;          // few rows: row and column blocks (rb 0: tiles)
 };
-// Few rows: us of a step, [row blocks - 1][column blocks 2, 4], and the busiest CU's workgroups;
-// no less than the weight's reads (5.3 TB/s).
-constexpr float STREAM_LAUNCH = 3.96f, STREAM_BYTE = 1.9e-7f;
+// Few rows: us of a step, [row blocks - 1][column blocks 2, 4], and the busiest CU's workgroups.
+// None is faster than the weight's reads: 5.3 TB/s for few rows, where those of x count too, 4.9
+// for tiles.
+constexpr float STREAM_LAUNCH = 3.96f, STREAM_BYTE = 1.9e-7f, TILE_BYTE = 2.05e-7f;
 constexpr float STREAM_STEP[3][2] = {{.169f, .279f}, {.188f, .342f}, {.293f, 0.f}};
 float stream_rounds(const h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
     const uint64_t groups = ((uint64_t)a.m + 16 * rb - 1) / (16 * rb) * (((uint64_t)a.n + 16 * nb - 1) / (16 * nb));
     return (float)((groups + g->cus - 1) / g->cus);
 }
 Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
-    static constexpr GemmRates RATES[3] = {{2.44f, 1.74f, .722f, .15f, 1.81f, .083f, .98f},
-                                           {3.63f, 1.99f, 1.82f, .3f, 3.61f, .0532f, 1.02f},
-                                           {6.35f, 3.62f, 3.8f, .3f, 7.63f, .0346f, 1.f}};
+    static constexpr GemmRates RATES[3] = {{2.44f, 1.74f, .682f, .15f, 1.67f, .0881f, 1.12f},
+                                           {4.02f, 1.99f, 1.82f, .3f, 3.61f, .0557f, 1.02f},
+                                           {7.38f, 3.62f, 4.18f, .3f, 8.77f, .0346f, 1.f}};
     static constexpr float LAUNCH[3] = {2.77f, 3.54f, 0.f};
+    const float reads = (float)a.n * a.k;
     const unsigned steps = a.k / TK;
     Choice best{3.4e38f, 0, 1, 0, 0};
     for (unsigned i = 0; i < 3; i++) {
@@ -1050,14 +1052,14 @@ Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
         const uint64_t tiles = ((uint64_t)a.m + rows - 1) / rows * ((a.n + 255) / 256);
         if (tiles > 0x7fffffffu) continue;
         const GemmPlan p = gemm_last_wave(g, (unsigned)tiles, units, RATES[i], rows / 256.f);
-        const float us = (p.us + LAUNCH[i]) * (p.split > 1 ? 1.02f : 1.f);
+        const float us = (std::max(p.us, reads * TILE_BYTE) + LAUNCH[i]) * (p.split > 1 ? 1.02f : 1.f);
         if (us < best.us) best = {us, rows, p.split, 0, 0};
     }
     if (!stream) return best;
     for (unsigned rb = 1; rb <= 3; rb++)
         for (unsigned nb = 2; nb <= (rb < 3 ? 4u : 2u); nb += 2) {
             const float rounds = stream_rounds(g, a, rb, nb);
-            const float us = STREAM_LAUNCH + std::max(rounds * steps * STREAM_STEP[rb - 1][nb / 4], (float)a.n * a.k * STREAM_BYTE);
+            const float us = STREAM_LAUNCH + std::max(rounds * steps * STREAM_STEP[rb - 1][nb / 4], reads * STREAM_BYTE * (.9f + .1f * rb));
             if (us < best.us && rounds < 1e6f) best = {us, 0, 1, rb, nb};
         }
     return best;

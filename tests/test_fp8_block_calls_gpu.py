@@ -44,7 +44,7 @@ def test_every_kernel():
     and in shares of K."""
     seen = set()
     for rows, k, n in [(1, 256, 5376), (9, 5376, 5376), (17, 1000, 777), (17, 7168, 5376), (48, 1000, 777), (70, 128, 4096),
-                       (8193, 2048, 4096), (300, 1000, 5000), (300, 7168, 5376), (300, 5376, 21504), (300, 13824, 5120),
+                       (8193, 2048, 4096), (1000, 14336, 8000), (300, 1000, 5000), (300, 7168, 5376), (300, 5376, 21504), (300, 13824, 5120),
                        (2300, 13824, 5120), (640, 5376, 28672), (1500, 5376, 21504)]:
         print(f"[fp8 block] {rows}x{k}x{n}", flush=True)
         with Gpu() as g:
