@@ -65,28 +65,48 @@ __global__ __launch_bounds__(256) void adaln_kernel(AdaLNArgs a) {
     const unsigned chunks = a.width / 8;
     const size_t base = (size_t)row * a.width;
     const size_t mbase = PLAIN ? 0 : (size_t)a.row_map[row] * a.slots * a.width;
-    u16x8 raw[CH];
+    // EARLY: all that a row needs is loaded at once (16 rows of 5376, sum and RMSNorm: 4.7 us -> 4.2).
+    constexpr bool EARLY = PACK && W == 4;
+    u16x8 raw[CH], early[EARLY ? CH : 1][5];
     float sumsq = 0.f;
 #pragma unroll
     for (int i = 0; i < CH; i++) {
         const unsigned c = lane + STRIDE * i;
         if (c >= chunks) break;
         raw[i] = *reinterpret_cast<const u16x8 *>(a.x + base + c * 8);
+        if constexpr (EARLY) {
+            if constexpr (GATE || MODE == ADD_RMS_NORM) early[i][0] = *reinterpret_cast<const u16x8 *>(a.branch + base + c * 8);
+            if constexpr (GATE)
+                early[i][1] = *reinterpret_cast<const u16x8 *>(a.gate_mod + mbase + (size_t)a.gate_slot * a.width + c * 8);
+            early[i][2] = *reinterpret_cast<const u16x8 *>(a.weight + c * 8);
+            if constexpr (!PLAIN) {
+                early[i][3] = *reinterpret_cast<const u16x8 *>(a.mod + mbase + (size_t)a.shift_slot * a.width + c * 8);
+                early[i][4] = *reinterpret_cast<const u16x8 *>(a.mod + mbase + (size_t)a.scale_slot * a.width + c * 8);
+            }
+        }
     }
 #pragma unroll
     for (int i = 0; i < CH; i++) {
         const unsigned c = lane + STRIDE * i;
         if (c >= chunks) break;
         if constexpr (GATE) {
-            u16x8 br = *reinterpret_cast<const u16x8 *>(a.branch + base + c * 8);
-            u16x8 gr = *reinterpret_cast<const u16x8 *>(a.gate_mod + mbase + (size_t)a.gate_slot * a.width + c * 8);
+            u16x8 br, gr;
+            if constexpr (EARLY) {
+                br = early[i][0];
+                gr = early[i][1];
+            } else {
+                br = *reinterpret_cast<const u16x8 *>(a.branch + base + c * 8);
+                gr = *reinterpret_cast<const u16x8 *>(a.gate_mod + mbase + (size_t)a.gate_slot * a.width + c * 8);
+            }
 #pragma unroll
             for (int e = 0; e < 8; e++)
                 raw[i][e] = f32_to_bf16(fmaf(bf16_to_f32(br[e]), bf16_to_f32(gr[e]), bf16_to_f32(raw[i][e])));
             *reinterpret_cast<u16x8 *>(a.gated + base + c * 8) = raw[i];
         }
         if constexpr (MODE == ADD_RMS_NORM) {
-            u16x8 br = *reinterpret_cast<const u16x8 *>(a.branch + base + c * 8);
+            u16x8 br;
+            if constexpr (EARLY) br = early[i][0];
+            else br = *reinterpret_cast<const u16x8 *>(a.branch + base + c * 8);
 #pragma unroll
             for (int e = 0; e < 8; e++) raw[i][e] = f32_to_bf16(bf16_to_f32(raw[i][e]) + bf16_to_f32(br[e]));
             *reinterpret_cast<u16x8 *>(a.gated + base + c * 8) = raw[i];
@@ -118,9 +138,13 @@ __global__ __launch_bounds__(256) void adaln_kernel(AdaLNArgs a) {
             float y[8] = {};
             unsigned amax = 0;
             if (c < chunks) {
-                const u16x8 wr = *reinterpret_cast<const u16x8 *>(a.weight + c * 8);
-                u16x8 sh = {}, sc = {};
-                if constexpr (!PLAIN) {
+                u16x8 wr, sh = {}, sc = {};
+                if constexpr (EARLY) wr = early[i][2];
+                else wr = *reinterpret_cast<const u16x8 *>(a.weight + c * 8);
+                if constexpr (EARLY && !PLAIN) {
+                    sh = early[i][3];
+                    sc = early[i][4];
+                } else if constexpr (!PLAIN) {
                     sh = *reinterpret_cast<const u16x8 *>(a.mod + mbase + (size_t)a.shift_slot * a.width + c * 8);
                     sc = *reinterpret_cast<const u16x8 *>(a.mod + mbase + (size_t)a.scale_slot * a.width + c * 8);
                 }
