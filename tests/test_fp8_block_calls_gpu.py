@@ -11,8 +11,8 @@ from h3cli_amd import synth
 from h3cli_amd.runtime import Gpu, H3Error
 from tests.helpers import bf16
 from tests.test_capture_gpu import Graph
-from tests.test_fp8_block_gpu import (HALF_BF16, MFMA, Packed, activation, linear, new, quantized, values, weight,
-                                        within)
+from tests.test_fp8_block_gpu import (HALF_BF16, MFMA, Packed, activation, linear, new, packed_bound, quantized, values,
+                                        weight, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -217,3 +217,20 @@ def test_mlp_overflow_fails_the_submit(rows):
         with pytest.raises(H3Error, match="nonfinite"):
             g.submit()
         g.cancel()
+
+
+def test_norm_of_large_and_small_rows():
+    """Rows whose squares leave FP32's range on either side."""
+    width, eps = 256, 1e-5
+    with Gpu() as g:
+        lib, h = g.lib, g.handle
+        x = np.random.default_rng(1).standard_normal((4, width)) * np.array([[1e25], [1e-25], [1.0], [3e37]])
+        bits = synth.f32_to_bf16(x.astype(np.float32))
+        norm = synth.f32_to_bf16(np.ones(width, np.float32))
+        t, w, packed = g.from_bf16(bits), g.from_bf16(norm), new(g, 4, width)
+        g.begin()
+        g.check(lib.h3_hip_add_rms_norm_fp8_block(h, None, packed.handle, t.handle, None, w.handle, 4, width, eps), "norm")
+        g.submit()
+        x = bf16(bits).reshape(4, width).astype(np.float64)
+        y = x / np.sqrt((x * x).mean(axis=1, keepdims=True) + float(np.float32(eps)))
+        within(packed.values(), y, packed_bound(packed, y, 2.0 ** -23 * np.abs(y)), "norm")
