@@ -216,6 +216,12 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs 
     }
 }
 
+// Workgroups of the busiest CU.
+float stream_rounds(const h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
+    const uint64_t groups = ((uint64_t)a.m + 16 * rb - 1) / (16 * rb) * (((uint64_t)a.n + 16 * nb - 1) / (16 * nb));
+    return (float)((groups + g->cus - 1) / g->cus);
+}
+
 template <int EPI, bool PACK, int RB, int NB, int WAVES, int U>
 int launch_stream_as(h3_gpu *g, const Fp8BlockGemmArgs &a) {
     constexpr int shared = stream_lds<RB, NB, WAVES>();
@@ -226,11 +232,15 @@ int launch_stream_as(h3_gpu *g, const Fp8BlockGemmArgs &a) {
                        g->compute, a, groups);
     return h3_launch_status(g, "FP8 block GEMM");
 }
-// Row blocks and column blocks of a workgroup.
+// Row blocks and column blocks of a workgroup. With 64 columns of 16 rows and more than a workgroup
+// per CU, four waves of fewer registers, so that more of those run at a time (1 row, 5376 -> 32256:
+// 32.2 us, eight waves 34.5; 16128 columns, a workgroup per CU: 16.5, 15.1).
 template <int EPI, bool PACK> int launch_stream(h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
-    return rb == 1 ? nb == 2 ? launch_stream_as<EPI, PACK, 1, 2, 8, 3>(g, a) : launch_stream_as<EPI, PACK, 1, 4, 8, 2>(g, a)
-           : rb == 2 ? nb == 2 ? launch_stream_as<EPI, PACK, 2, 2, 4, 3>(g, a) : launch_stream_as<EPI, PACK, 2, 4, 4, 3>(g, a)
-                     : launch_stream_as<EPI, PACK, 3, 2, 4, 2>(g, a);
+    if (rb == 1 && nb == 2) return launch_stream_as<EPI, PACK, 1, 2, 8, 3>(g, a);
+    if (rb == 1) return stream_rounds(g, a, 1, 4) > 1.f ? launch_stream_as<EPI, PACK, 1, 4, 4, 2>(g, a)
+                                                        : launch_stream_as<EPI, PACK, 1, 4, 8, 2>(g, a);
+    if (rb == 2) return nb == 2 ? launch_stream_as<EPI, PACK, 2, 2, 4, 3>(g, a) : launch_stream_as<EPI, PACK, 2, 4, 4, 3>(g, a);
+    return launch_stream_as<EPI, PACK, 3, 2, 4, 2>(g, a);
 }
 
 // ---------------------------------------------------------------- tiles of 256 rows
@@ -1018,9 +1028,9 @@ template <int EPI, int TM> int launch_pipe(h3_gpu *g, Fp8BlockGemmArgs a, unsign
 // ---------------------------------------------------------------- choice
 // The kernel whose modelled time is least. Tiles by gemm_last_wave in units of four K steps of
 // 128. Few rows: the workgroups of the busiest CU by their K steps. Rates fitted to the measured
-// times of all of them, the tiles in one to nine shares, at 231 projections of 1 to 8000 rows
+// times of all of them, the tiles in one to nine shares, at 259 projections of 1 to 8000 rows
 // (K 256 to 14336, N 300 to 32256; weights that rotate through more than the last cache holds);
-// the choice is 0.8% slower than the best of them in the mean. Measured, in us, the runner-up in
+// the choice is 0.9% slower than the best of them in the mean. Measured, in us, the runner-up in
 // brackets: 1 row, 7168 -> 5376: 9.7 (tiles of 64 rows in 4 shares 15.7); 32 rows, 5376 -> 21504:
 // tiles of 64 in 2 shares 28.8 (128 rows in 2 shares 30.5); 640 rows, 13824 -> 5120: 128 rows in 2
 // shares 50.5 (64 rows 57.6); 1024 rows, 7168 -> 5376: 128 rows 38.7 (256 in 2 shares 49.4); 1500
@@ -1030,17 +1040,13 @@ struct Choice {
     unsigned rows, split;     // tile rows (64, 128, 256) and shares; or
     unsigned rb, nb;          // few rows: row and column blocks (rb 0: tiles)
 };
-// Few rows: us of a step, [row blocks - 1][column blocks 2, 4], and the busiest CU's workgroups.
-// None is faster than the weight's reads: 5.3 TB/s for few rows, where those of x count too, 4.9
-// for tiles.
-constexpr float STREAM_LAUNCH = 3.96f, STREAM_BYTE = 1.9e-7f, TILE_BYTE = 2.05e-7f;
-constexpr float STREAM_STEP[3][2] = {{.169f, .279f}, {.188f, .342f}, {.293f, 0.f}};
-float stream_rounds(const h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
-    const uint64_t groups = ((uint64_t)a.m + 16 * rb - 1) / (16 * rb) * (((uint64_t)a.n + 16 * nb - 1) / (16 * nb));
-    return (float)((groups + g->cus - 1) / g->cus);
-}
+// Few rows: us of a step, [row blocks - 1][column blocks 2, 4], and the busiest CU's workgroups;
+// of a byte of x that such a CU reads (from L2). None is faster than the weight's reads: 6.6 TB/s
+// for few rows, beside their launch, 5.1 for tiles.
+constexpr float STREAM_LAUNCH = 3.26f, STREAM_BYTE = 1.52e-7f, STREAM_X = 2.05e-5f, TILE_BYTE = 1.95e-7f;
+constexpr float STREAM_STEP[3][2] = {{.14f, .26f}, {.17f, .32f}, {.27f, 0.f}};
 Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
-    static constexpr GemmRates RATES[3] = {{2.44f, 1.74f, .682f, .15f, 1.67f, .0881f, 1.12f},
+    static constexpr GemmRates RATES[3] = {{2.44f, 1.82f, .654f, .15f, 1.67f, .0881f, 1.12f},
                                            {4.02f, 1.99f, 1.82f, .3f, 3.61f, .0557f, 1.02f},
                                            {7.38f, 3.62f, 4.18f, .3f, 8.77f, .0346f, 1.f}};
     static constexpr float LAUNCH[3] = {2.77f, 3.54f, 0.f};
@@ -1059,7 +1065,8 @@ Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
     for (unsigned rb = 1; rb <= 3; rb++)
         for (unsigned nb = 2; nb <= (rb < 3 ? 4u : 2u); nb += 2) {
             const float rounds = stream_rounds(g, a, rb, nb);
-            const float us = STREAM_LAUNCH + std::max(rounds * steps * STREAM_STEP[rb - 1][nb / 4], reads * STREAM_BYTE * (.9f + .1f * rb));
+            const float us = STREAM_LAUNCH + std::max(rounds * steps * STREAM_STEP[rb - 1][nb / 4], reads * STREAM_BYTE) +
+                             rounds * std::min(a.m, 16 * rb) * a.k * STREAM_X;
             if (us < best.us && rounds < 1e6f) best = {us, 0, 1, rb, nb};
         }
     return best;
