@@ -187,7 +187,8 @@ int h3_gpu_sdpa_bf16_head_major_output(h3_gpu *gpu, h3_gpu_tensor *out,
 
 /* ---- DiT block operators ---------------------------------------------- */
 /* gpu.h:501. y[rows,output_dim] = x[rows,input_dim] . W[output_dim,input_dim]^T (+bias),
- * FP32 accumulate, BF16 out. A q8 weight dispatches the W8A16 GEMM. */
+ * FP32 accumulate, BF16 out. A q8 weight dispatches the W8A16 GEMM, one in FP8
+ * blocks (h3_hip_ext.h) the projection that packs its input. */
 int h3_gpu_linear_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
                        const h3_gpu_tensor *weight, const h3_gpu_tensor *bias,
                        uint32_t rows, uint32_t input_dim, uint32_t output_dim);

@@ -11,8 +11,8 @@ from h3cli_amd import synth
 from h3cli_amd.runtime import Gpu, H3Error
 from tests.helpers import bf16
 from tests.test_capture_gpu import Graph
-from tests.test_fp8_block_gpu import (HALF_BF16, MFMA, Packed, activation, linear, new, packed_bound, quantized, values,
-                                        weight, within)
+from tests.test_fp8_block_gpu import (HALF_BF16, MFMA, Packed, activation, linear, mlp_reference, new, packed_bound,
+                                        quantized, values, weight, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -96,6 +96,24 @@ def test_mlp_in_place(rows):
             g.check(g.lib.h3_gpu_mlp_bf16(g.handle, into.handle, t.handle, w1.handle, w2.handle, rows, k, hidden, k), "mlp")
             g.submit()
         assert np.array_equal(out.read(), t.read())
+
+
+def test_mlp_in_parts():
+    """More rows than the activation's workspace of 1 GiB holds, the output in the input's place."""
+    rows, k, hidden = 80000, 128, 14336
+    with Gpu() as g:
+        w1 = weight(g, synth.normal_bf16(1, 2 * hidden * k, scale=1 / math.sqrt(k)), 2 * hidden, k)
+        w2 = weight(g, synth.normal_bf16(2, k * hidden, scale=1 / math.sqrt(hidden)), k, hidden)
+        t = normal(g, rows * k, 3, 1.0)
+        x = t.read().reshape(rows, k)
+        g.begin()
+        g.check(g.lib.h3_gpu_mlp_bf16(g.handle, t.handle, t.handle, w1.handle, w2.handle, rows, k, hidden, k), "mlp")
+        g.submit()
+        got = t.read().reshape(rows, k)
+        at = np.r_[0:6, 30000:30006, 59898:59910, 70000:70006, rows - 6:rows]
+        want, bound = mlp_reference(quantized(bf16(x[at]).astype(np.float64), 1)[0], w1.values(), w2.values(), hidden)
+        within(bf16(got[at]), want, bound)
+        assert np.linalg.norm(bf16(got[at]) - want) <= 1e-2 * np.linalg.norm(want)
 
 
 def test_norm_sums_in_place():
@@ -234,3 +252,28 @@ def test_norm_of_large_and_small_rows():
         x = bf16(bits).reshape(4, width).astype(np.float64)
         y = x / np.sqrt((x * x).mean(axis=1, keepdims=True) + float(np.float32(eps)))
         within(packed.values(), y, packed_bound(packed, y, 2.0 ** -23 * np.abs(y)), "norm")
+
+
+@pytest.mark.parametrize("rows", [5, 257])
+def test_longest_rows(rows):
+    """The most columns a matrix may have: offsets near and above 32 bits. All codes are zero but
+    for a few columns, whose small integers give exact sums."""
+    k, n = (1 << 24) - 128, 130
+    code = {0: 0, 1: 0x38, 2: 0x40, 3: 0x44, 4: 0x48}
+    columns = [0, 127, 128, (1 << 23) + 5, (1 << 24) - 300, k - 1]
+    rng = np.random.default_rng(rows)
+    with Gpu() as g:
+        print(f"[fp8 block] {rows}x{k}x{n}", flush=True)
+
+        def sparse(count, tile):
+            p, v = new(g, count, k, tile), rng.integers(0, 5, (count, len(columns)))
+            raw = np.zeros(p.bytes, np.uint8)
+            raw[:count * p.stride].reshape(count, p.stride)[:, columns] = np.vectorize(code.get)(v)
+            raw[p.scales:] = 127
+            assert g.lib.h3_hip_tensor_stream_host(p.handle, raw.ctypes.data, raw.size), g.error()
+            return p, v
+
+        (x, xv), (w, wv) = sparse(rows, 1), sparse(n, 128)
+        got, kernel = linear(g, g.empty(rows * n), x, w, None, rows, k, n)
+        print(f"[fp8 block] {kernel}", flush=True)
+        assert np.array_equal(bf16(got), (xv @ wv.T).astype(np.float32)), kernel
