@@ -1,0 +1,84 @@
+"""Block-scaled FP8 at the ends of what the types hold: weights and rows of any size in the norms,
+gates whose sigmoid leaves FP32's range, faults and refusals that meet. Bounds as in
+test_fp8_block_gpu.py."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from h3cli_amd import synth
+from h3cli_amd.runtime import Gpu, H3Error
+from tests.helpers import bf16
+from tests.test_fp8_block_gpu import (HALF_BF16, MFMA, Packed, activation, blocks, e4m3, exponents, linear, new, quantized,
+                                        values, weight, within)
+
+pytestmark = pytest.mark.gpu
+
+
+def codes_within(p, y, error):
+    """Each code is that of y, or of a value that is `error` times it away, and so is each scale."""
+    _, scales = p.read()
+    e = scales.astype(np.int64) - 127
+    top = np.abs(blocks(y, 1)).max(axis=(1, 3))
+    assert np.all(exponents(top * (1 - error)) <= e) and np.all(e <= exponents(top * (1 + error)))
+    s = np.repeat(np.ldexp(1.0, e), 128, axis=1)[:, :y.shape[1]]
+    got, size = p.values() / s, np.abs(y) / s
+    assert np.all((got == 0) | (np.sign(got) == np.sign(y)))
+    low, high = e4m3(np.minimum(size * (1 - error), 448)), e4m3(np.minimum(size * (1 + error), 448))
+    off = np.maximum(low - np.abs(got), np.abs(got) - high)
+    assert np.all(off <= 0), (int((off > 0).sum()), np.unravel_index(np.argmax(off), off.shape), float(off.max()))
+
+
+@pytest.mark.parametrize("eps", [1e-5, 0.0])
+def test_norm_weights_of_any_size(eps):
+    """Row values times weights beyond FP32's range on either side, where the normalized result is not."""
+    width = 264
+    with Gpu() as g:
+        rng = np.random.default_rng(1)
+        size = np.array([[3e37], [1e30], [1.0]] + ([[1e-30], [1e-38]] if eps == 0 else [[1e-3], [1e-9]]))
+        bits = synth.f32_to_bf16((rng.standard_normal((5, width)) * size).astype(np.float32))
+        scale = np.where(np.arange(width) < 128, 40.0, np.where(np.arange(width) < 256, 1e-12, 1e37))
+        norm = synth.f32_to_bf16((scale * rng.uniform(1, 2, width)).astype(np.float32))
+        t, w, packed = g.from_bf16(bits), g.from_bf16(norm), new(g, 5, width)
+        g.begin()
+        g.check(g.lib.h3_hip_add_rms_norm_fp8_block(g.handle, None, packed.handle, t.handle, None, w.handle, 5, width, eps),
+                "norm")
+        g.submit()
+        x = bf16(bits).reshape(5, width).astype(np.float64)
+        y = x / np.sqrt((x * x).mean(axis=1, keepdims=True) + float(np.float32(eps))) * bf16(norm)
+        codes_within(packed, y, 2.0 ** -23)
+
+
+@pytest.mark.parametrize("rows,width", [(5, 5376), (700, 2048), (2050, 4096)])
+@pytest.mark.parametrize("kind", ["rms", "add", "adaln", "gate"])
+def test_norms_in_64_bits(rows, width, kind):
+    """The codes are those of the values but for one FP32 rounding (2^-24; 2^-23 here). Of a million
+    values some are near enough to a midpoint that a sum in FP32 would show."""
+    print(f"[fp8 block] {kind} {rows}x{width}", flush=True)
+    rng = np.random.default_rng(rows + width)
+    eps, slots = 1e-5, 6
+    res, branch, norm = values(rows, width, 1, 1.0), values(rows, width, 2, 1.0), values(1, width, 3, 0.5)
+    mod = synth.f32_to_bf16((0.3 * rng.standard_normal((3, slots, width))).astype(np.float32))
+    row_map = rng.integers(0, 3, rows).astype(np.uint32)
+    with Gpu() as g:
+        tr, tb, tw, tm, tmap = (g.from_bf16(res), g.from_bf16(branch), g.from_bf16(norm), g.from_bf16(mod), g.from_u32(row_map))
+        total, packed, lib, h = g.empty(rows * width), new(g, rows, width), g.lib, g.handle
+        g.begin()
+        if kind in ("rms", "add"):
+            s, b = (total.handle, tb.handle) if kind == "add" else (None, None)
+            ok = lib.h3_hip_add_rms_norm_fp8_block(h, s, packed.handle, tr.handle, b, tw.handle, rows, width, eps)
+        elif kind == "adaln":
+            ok = lib.h3_hip_adaln_fp8_block(h, packed.handle, tr.handle, tw.handle, tm.handle, tmap.handle, rows, width,
+                                            slots, 3, 4, eps)
+        else:
+            ok = lib.h3_hip_gate_adaln_fp8_block(h, total.handle, packed.handle, tr.handle, tb.handle, tw.handle, tm.handle,
+                                                 tm.handle, tmap.handle, rows, width, slots, 2, 3, 4, eps)
+        g.check(ok, kind)
+        g.submit()
+        x = bf16(total.read() if kind in ("add", "gate") else res.reshape(-1)).reshape(rows, width).astype(np.float64)
+        y = x / np.sqrt((x * x).mean(axis=1, keepdims=True) + float(np.float32(eps))) * bf16(norm).reshape(1, width)
+        if kind in ("adaln", "gate"):
+            mv = bf16(mod).reshape(3, slots, width).astype(np.float64)[row_map]
+            y = y * (1 + mv[:, 4]) + mv[:, 3]
+        codes_within(packed, y, 2.0 ** -23)
