@@ -310,16 +310,20 @@ extern "C" h3_gpu_tensor *h3_hip_fp8_block_weight_from_bf16(h3_gpu *g, const h3_
     if (!h3_require(g, w, H3_GPU_BF16, (size_t)rows * columns, "FP8 block weight source")) return nullptr;
     h3_gpu_tensor *t = h3_hip_fp8_block_new(g, rows, columns, FP8_BLOCK);
     if (!t) return nullptr;
-    // A weight that is not finite is an error here, not at the next submit.
+    // A weight that is not finite is an error here, not at the next submit; a fault that waits for
+    // that submit is put aside meanwhile.
+    const unsigned none = 0;
     unsigned before = 0, flag = 0, *fault = g->fault + 2;
-    const int ok = h3_tensor_acquire(g, w) && h3_hip_check(g, hipStreamSynchronize(g->compute), "FP8 block weight") &&
-                   h3_hip_check(g, hipMemcpy(&before, fault, 4, hipMemcpyDeviceToHost), "FP8 block weight") &&
-                   launch_pack_weight(g, (const uint16_t *)w->data, h3_fp8_block_rows(g, t), rows, columns) &&
-                   h3_tensor_release(g, w) && h3_hip_check(g, hipStreamSynchronize(g->compute), "FP8 block weight") &&
-                   h3_hip_check(g, hipMemcpy(&flag, fault, 4, hipMemcpyDeviceToHost), "FP8 block weight");
-    if (ok && (!flag || before)) return t;
-    if (ok && h3_hip_check(g, hipMemcpy(fault, &before, 4, hipMemcpyHostToDevice), "FP8 block weight"))
-        h3_set_error(g, "FP8 block weight: nonfinite value");
+    int ok = h3_tensor_acquire(g, w) && h3_hip_check(g, hipStreamSynchronize(g->compute), "FP8 block weight") &&
+             h3_hip_check(g, hipMemcpy(&before, fault, 4, hipMemcpyDeviceToHost), "FP8 block weight") &&
+             (!before || h3_hip_check(g, hipMemcpy(fault, &none, 4, hipMemcpyHostToDevice), "FP8 block weight")) &&
+             launch_pack_weight(g, (const uint16_t *)w->data, h3_fp8_block_rows(g, t), rows, columns) &&
+             h3_tensor_release(g, w) && h3_hip_check(g, hipStreamSynchronize(g->compute), "FP8 block weight") &&
+             h3_hip_check(g, hipMemcpy(&flag, fault, 4, hipMemcpyDeviceToHost), "FP8 block weight");
+    if (flag != before)
+        ok = h3_hip_check(g, hipMemcpy(fault, &before, 4, hipMemcpyHostToDevice), "FP8 block weight") && ok;
+    if (ok && !flag) return t;
+    if (ok) h3_set_error(g, "FP8 block weight: nonfinite value");
     h3_gpu_tensor_free(t);
     return nullptr;
 }

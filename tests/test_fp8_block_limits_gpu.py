@@ -82,3 +82,25 @@ def test_norms_in_64_bits(rows, width, kind):
             mv = bf16(mod).reshape(3, slots, width).astype(np.float64)[row_map]
             y = y * (1 + mv[:, 4]) + mv[:, 3]
         codes_within(packed, y, 2.0 ** -23)
+
+
+def test_weight_behind_a_pending_fault():
+    """A fault that waits for the next submit hides no weight that is not finite, and stays; nor does
+    it refuse a finite one."""
+    rows, width = 4, 256
+    with Gpu() as g:
+        lib, h = g.lib, g.handle
+        good = values(rows, width, 1)
+        flat = good.reshape(-1).copy()
+        flat[300] = 0x7fc0
+        t, finite, packed = g.from_bf16(flat), g.from_bf16(good), new(g, rows, width)
+        g.begin()
+        g.check(lib.h3_hip_fp8_block_pack(h, packed.handle, t.handle, rows, width), "pack")
+        assert not lib.h3_hip_fp8_block_weight_from_bf16(h, t.handle, rows, width) and "nonfinite" in g.error()
+        w = Packed(g, lib.h3_hip_fp8_block_weight_from_bf16(h, finite.handle, rows, width), rows, width, 128)
+        assert np.array_equal(w.values(), quantized(bf16(good).reshape(rows, width).astype(np.float64), 128)[0])
+        with pytest.raises(H3Error, match="nonfinite"):
+            g.submit()
+        g.cancel()
+        g.begin()
+        g.submit()
