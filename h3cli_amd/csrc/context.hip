@@ -674,7 +674,11 @@ int h3_buffer_reserve(h3_gpu *g, h3_device_buffer *b, size_t bytes, const char *
     if (b->bytes >= bytes) return 1;
     if (b->ptr && !h3_hip_check(g, hipStreamSynchronize(g->compute), what)) return 0;
     h3_buffer_free(b);
-    if (!h3_hip_check(g, hipMalloc(&b->ptr, bytes), what)) { b->ptr = nullptr; return 0; }
+    if (!h3_hip_check(g, hipMalloc(&b->ptr, bytes), what)) {
+        (void)hipGetLastError();     // reported here, not by the next launch
+        b->ptr = nullptr;
+        return 0;
+    }
     b->bytes = bytes;
     return 1;
 }

@@ -104,3 +104,21 @@ def test_weight_behind_a_pending_fault():
         g.cancel()
         g.begin()
         g.submit()
+
+
+def test_short_memory_leaves_no_error_behind():
+    """A projection whose packed input is larger than the device's memory: refused, and the next call
+    and its submit are fine."""
+    rows = 3 << 30
+    with Gpu() as g:
+        lib, h = g.lib, g.handle
+        w = weight(g, values(1, 1, 1), 1, 1)
+        x, out = g.empty(rows), g.empty(rows)
+        g.begin()
+        assert not lib.h3_gpu_linear_bf16(h, out.handle, x.handle, w.handle, None, rows, 1, 1) and "memory" in g.error()
+        g.check(lib.h3_hip_fill_normal_bf16(h, x.handle, 1, C.c_float(1.0), 300), "fill")
+        g.check(lib.h3_gpu_linear_bf16(h, out.handle, x.handle, w.handle, None, 300, 1, 1), "linear")
+        g.submit()
+        xv, _ = quantized(bf16(x.read(300)).reshape(300, 1).astype(np.float64), 1)
+        want = xv * w.values()
+        within(bf16(out.read(300)).reshape(300, 1), want, (HALF_BF16 + 2 * MFMA) * np.abs(want))
