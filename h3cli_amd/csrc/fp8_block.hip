@@ -65,12 +65,13 @@ __global__ __launch_bounds__(256) void fp8_block_pack(const T *in, Fp8BlockRows 
     const unsigned col = block * FP8_BLOCK + (unsigned)(id % LANES) * LANE;
     const T *src = in + (size_t)row * columns * (SWIGLU ? 2 : 1);
     float v[LANE];
-    load16<VEC>(src, col, columns, v);
-    if constexpr (SWIGLU) {
-        float up[LANE];
+    if constexpr (!SWIGLU) {
+        load16<VEC>(src, col, columns, v);
+    } else {
+        float gate[LANE], up[LANE];
+        load16<VEC>(src, col, columns, gate);
         load16<VEC>(src + columns, col, columns, up);
-#pragma unroll
-        for (unsigned e = 0; e < LANE; e++) v[e] = swiglu_exact(v[e], up[e]);
+        swiglu<LANE, false>(gate, up, v);
     }
     bool bad = false;
     const unsigned scale = fp8_block_scale(lanes_max<LANES>(fp8_block_magnitude<LANE>(v, bad)));

@@ -525,11 +525,15 @@ __device__ inline void pipe_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, u
     }
     float v[32];
     bool bad = false;
+    float gate[32], up[32];
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        v[e] = swiglu_of_sums(c0[e], c1[e]);
-        v[16 + e] = swiglu_of_sums(c2[e], c3[e]);
+        gate[e] = c0[e];
+        up[e] = c1[e];
+        gate[16 + e] = c2[e];
+        up[16 + e] = c3[e];
     }
+    swiglu<32, true>(gate, up, v);
     unsigned amax = fp8_block_magnitude<32>(v, bad);
     if (bad && row < a.m) *a.out.fault = 1u;
     amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
@@ -825,8 +829,13 @@ __device__ inline void mid_epilogue(const Fp8BlockGemmArgs &a, unsigned row0, un
     }
     float v[16];
     bool bad = false;
+    float gate[16], up[16];
 #pragma unroll
-    for (int e = 0; e < 16; e++) v[e] = swiglu_of_sums(c0[e], c1[e]);
+    for (int e = 0; e < 16; e++) {
+        gate[e] = c0[e];
+        up[e] = c1[e];
+    }
+    swiglu<16, true>(gate, up, v);
     unsigned amax = fp8_block_magnitude<16>(v, bad);
     if (bad && row < a.m) *a.out.fault = 1u;
     amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));

@@ -122,3 +122,58 @@ def test_short_memory_leaves_no_error_behind():
         xv, _ = quantized(bf16(x.read(300)).reshape(300, 1).astype(np.float64), 1)
         want = xv * w.values()
         within(bf16(out.read(300)).reshape(300, 1), want, (HALF_BF16 + 2 * MFMA) * np.abs(want))
+
+
+def silu(gate):
+    return gate * np.exp(-np.logaddexp(0, -gate))
+
+
+def test_swiglu_of_gates_below_the_end_of_exp():
+    """Gates whose sigmoid is below FP32's normal range, beside ups with which the product is not
+    nothing: a block for each, since the largest value of a block hides the others."""
+    gates = [-60.0, -60.5, -80.0, -86.5, -87.0, -87.5, -88.0, -88.5, -89.0, -95.0, -100.0, -104.0, -120.0, -140.0, -152.0,
+             -153.0, -153.5, -154.0, -160.0, -1e4, -3e38]
+    width = 128
+    up = np.concatenate([np.exp2(np.linspace(0, 127.9, len(gates) - 6)), np.full(6, 3e38)])
+    x = np.zeros((len(gates), 2 * width))
+    x[:, :width] = np.array(gates)[:, None]
+    x[:, width:] = up[:, None] * np.linspace(1 / 64, 1, width) * np.where(np.arange(width) % 3, 1, -1)
+    for scale in (1.0, 2.0 ** -20, 3e38):
+        bits = synth.f32_to_bf16(np.clip(x * np.where(np.arange(2 * width) < width, 1, scale), -3.3e38, 3.3e38).astype(np.float32))
+        v = bf16(bits).reshape(x.shape).astype(np.float64)
+        with Gpu() as g:
+            t, packed = g.from_bf16(bits), new(g, len(gates), width)
+            g.begin()
+            g.check(g.lib.h3_hip_swiglu_fp8_block(g.handle, packed.handle, t.handle, len(gates), width), "swiglu")
+            g.submit()
+            y = silu(v[:, :width]) * v[:, width:]
+            codes_within(packed, y, 2.0 ** -21)
+
+
+@pytest.mark.parametrize("m,kernel", [(5, None), (1500, "fp8_block_mid rows=64"), (4097, "fp8_block_pipe rows=128"),
+                                      (8193, "fp8_block_pipe rows=256")])
+def test_mlp_of_gates_below_the_end_of_exp(m, kernel):
+    """The same in the MLP, its activation packed by fc1's epilogue (5 rows: from FP32 sums): one
+    input value, a block of the activation for each gate, an fc2 that copies a value of each. fc1's
+    kernel is that of the plain projection of its shape."""
+    gates, ups = [-60.0, -88.0, -96.0, -104.0, -120.0], [40, 100, 100, 120, 126]
+    k, hidden, n = 256 if kernel else 640, 128 * len(gates), 8
+    print(f"[fp8 block] mlp gates {m} rows", flush=True)
+    x, w1, w2 = np.zeros((m, k)), np.zeros((2 * hidden, k)), np.zeros((n, hidden))
+    x[:, 0] = 1
+    w1[:hidden, 0], w1[hidden:, 0] = np.repeat(gates, 128), np.repeat(np.exp2(ups), 128)
+    w2[np.arange(len(gates)), 128 * np.arange(len(gates)) + 7] = 1
+    with Gpu() as g:
+        tx, t1, t2 = (synth.f32_to_bf16(v.astype(np.float32).reshape(-1)) for v in (x, w1, w2))
+        px, p1, p2 = activation(g, tx, m, k), weight(g, t1, 2 * hidden, k), weight(g, t2, n, hidden)
+        assert np.array_equal(p1.values(), w1)
+        if kernel:
+            assert linear(g, g.empty(m * 2 * hidden), px, p1, None, m, k, 2 * hidden)[1] == kernel
+        out = g.empty(m * n)
+        g.begin()
+        g.check(g.lib.h3_hip_mlp_fp8_block(g.handle, out.handle, px.handle, p1.handle, p2.handle, m, k, hidden, n), "mlp")
+        g.submit()
+        want = np.zeros(n)
+        want[:len(gates)] = silu(np.array(gates)) * np.exp2(ups)
+        # A value is off by half a step of E4M3; its gate's product with 1 / ln 2 by 2^-24 of it.
+        within(bf16(out.read()).reshape(m, n), np.broadcast_to(want, (m, n)), (2.0 ** -4 + 2.0 ** -15) * np.abs(want))
