@@ -216,10 +216,12 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_block_stream(Fp8BlockGemmArgs 
     }
 }
 
+uint64_t stream_groups(const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
+    return ((uint64_t)a.m + 16 * rb - 1) / (16 * rb) * (((uint64_t)a.n + 16 * nb - 1) / (16 * nb));
+}
 // Workgroups of the busiest CU.
 float stream_rounds(const h3_gpu *g, const Fp8BlockGemmArgs &a, unsigned rb, unsigned nb) {
-    const uint64_t groups = ((uint64_t)a.m + 16 * rb - 1) / (16 * rb) * (((uint64_t)a.n + 16 * nb - 1) / (16 * nb));
-    return (float)((groups + g->cus - 1) / g->cus);
+    return (float)((stream_groups(a, rb, nb) + g->cus - 1) / g->cus);
 }
 
 template <int EPI, bool PACK, int RB, int NB, int WAVES, int U>
@@ -1044,6 +1046,8 @@ template <int EPI, int TM> int launch_pipe(h3_gpu *g, Fp8BlockGemmArgs a, unsign
 // tiles of 64 in 2 shares 28.8 (128 rows in 2 shares 30.5); 640 rows, 13824 -> 5120: 128 rows in 2
 // shares 50.5 (64 rows 57.6); 1024 rows, 7168 -> 5376: 128 rows 38.7 (256 in 2 shares 49.4); 1500
 // rows, 5376 -> 21504: 256 rows 146.4 (128 rows 153.8).
+// A launch has fewer than 2^32 threads: kernels whose grid would have more are no candidates.
+constexpr uint64_t MAX_THREADS = 0xffffffffu;
 struct Choice {
     float us;
     unsigned rows, split;     // tile rows (64, 128, 256) and shares; or
@@ -1064,8 +1068,8 @@ Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
     Choice best{3.4e38f, 0, 1, 0, 0};
     for (unsigned i = 0; i < 3; i++) {
         const unsigned rows = 64u << i, units = (steps + QUAD - 1) / QUAD;
-        const uint64_t tiles = ((uint64_t)a.m + rows - 1) / rows * ((a.n + 255) / 256);
-        if (tiles > 0x7fffffffu) continue;
+        const uint64_t tiles = ((uint64_t)a.m + rows - 1) / rows * (((uint64_t)a.n + 255) / 256);
+        if ((tiles + 2 * g->cus) * 256 > MAX_THREADS) continue;     // and the shares of a last wave
         const GemmPlan p = gemm_last_wave(g, (unsigned)tiles, units, RATES[i], rows / 256.f);
         const float us = (std::max(p.us, reads * TILE_BYTE) + LAUNCH[i]) * (p.split > 1 ? 1.02f : 1.f);
         if (us < best.us) best = {us, rows, p.split, 0, 0};
@@ -1074,9 +1078,10 @@ Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
     for (unsigned rb = 1; rb <= 3; rb++)
         for (unsigned nb = 2; nb <= (rb < 3 ? 4u : 2u); nb += 2) {
             const float rounds = stream_rounds(g, a, rb, nb);
+            if (stream_groups(a, rb, nb) * (rb == 1 && nb == 2 ? 512 : 256) > MAX_THREADS) continue;
             const float us = STREAM_LAUNCH + std::max(rounds * steps * STREAM_STEP[rb - 1][nb / 4], reads * STREAM_BYTE) +
                              rounds * std::min(a.m, 16 * rb) * a.k * STREAM_X;
-            if (us < best.us && rounds < 1e6f) best = {us, 0, 1, rb, nb};
+            if (us < best.us) best = {us, 0, 1, rb, nb};
         }
     return best;
 }
@@ -1092,6 +1097,8 @@ bool packs(const h3_gpu *g, const Fp8BlockGemmArgs &a, const Choice &c) {
 
 template <int EPI> int run(h3_gpu *g, const Fp8BlockGemmArgs &a) {
     const Choice c = choose(g, a, EPI != EPI_SWIGLU);
+    if (a.m > FP8_BLOCK_ROWS || (!c.rb && !c.rows))
+        return h3_set_error(g, "FP8 block projection: %u rows by %u columns are too many for one call", a.m, a.n);
     if constexpr (EPI != EPI_SWIGLU)
         if (c.rb) return a.xb ? launch_stream<EPI, true>(g, a, c.rb, c.nb) : launch_stream<EPI, false>(g, a, c.rb, c.nb);
     if (a.xb) return h3_set_error(g, "FP8 block projection: %u rows of BF16 are to be packed first", a.m);
@@ -1112,8 +1119,6 @@ bool h3_gemm_fp8_block_fuses(const h3_gpu *g, uint32_t m, uint32_t k, uint32_t h
 }
 
 int h3_gemm_fp8_block(h3_gpu *g, const Fp8BlockGemmArgs &a) {
-    if (a.m > FP8_BLOCK_ROWS || ((uint64_t)a.m + 63) / 64 * ((a.n + 255) / 256) > 0x7fffffffu)
-        return h3_set_error(g, "FP8 block projection: %u rows by %u columns are too many for one call", a.m, a.n);
     switch (epilogue_of(a)) {
     case EPI_PLAIN: return run<EPI_PLAIN>(g, a);
     case EPI_BIAS: return run<EPI_BIAS>(g, a);

@@ -177,3 +177,34 @@ def test_mlp_of_gates_below_the_end_of_exp(m, kernel):
         want[:len(gates)] = silu(np.array(gates)) * np.exp2(ups)
         # A value is off by half a step of E4M3; its gate's product with 1 / ln 2 by 2^-24 of it.
         within(bf16(out.read()).reshape(m, n), np.broadcast_to(want, (m, n)), (2.0 ** -4 + 2.0 ** -15) * np.abs(want))
+
+
+def copied(g, t, at, width):
+    """Rows of a tensor that is too large to read."""
+    part = g.empty(len(at) * width)
+    g.begin()
+    for i, row in enumerate(at):
+        g.check(g.lib.h3_gpu_copy_bf16(g.handle, part.handle, i * width, t.handle, int(row) * width, width), "copy")
+    g.submit()
+    return bf16(part.read()).reshape(len(at), width).astype(np.float64)
+
+
+@pytest.mark.parametrize("rows,k,n", [(1 << 22, 128, 8192), (1 << 20, 128, 33000)])
+def test_more_threads_than_a_launch_takes(rows, k, n):
+    """Projections of one K block, for which the few-row kernels are modelled fastest, but whose
+    workgroups would be 2^24 of 256 threads: 64 GiB of results, by another kernel."""
+    print(f"[fp8 block] {rows}x{k}x{n}", flush=True)
+    with Gpu() as g:
+        t, out, packed = g.empty(rows * k), g.empty(rows * n), new(g, rows, k)
+        w = weight(g, values(n, k, 2, 1.0), n, k)
+        g.begin()
+        g.check(g.lib.h3_hip_fill_normal_bf16(g.handle, t.handle, 1, C.c_float(1.0), rows * k), "fill")
+        g.check(g.lib.h3_hip_fp8_block_pack(g.handle, packed.handle, t.handle, rows, k), "pack")
+        g.check(g.lib.h3_hip_linear_fp8_block(g.handle, out.handle, packed.handle, w.handle, None, rows, k, n), "linear")
+        kernel = g.last_kernel()
+        g.submit()
+        print(f"[fp8 block] {kernel}", flush=True)
+        at = np.unique(np.r_[0, 1, np.linspace(0, rows - 1, 30).astype(int), rows - 2, rows - 1])
+        xv, wv = quantized(copied(g, t, at, k), 1)[0], w.values()
+        want = xv @ wv.T
+        within(copied(g, out, at, n), want, HALF_BF16 * np.abs(want) + 2 * MFMA * (np.abs(xv) @ np.abs(wv).T), kernel)
