@@ -515,6 +515,8 @@ extern "C" int h3_gpu_gate_adaln_bf16(h3_gpu *g, h3_gpu_tensor *gated, h3_gpu_te
 static int packed_norm_shape(h3_gpu *g, const h3_gpu_tensor *out, uint32_t rows, uint32_t width, const char *what) {
     if (!rows || !width || width % 8 || width > 64 * MAX_CHUNKS * 8)
         return h3_set_error(g, "%s: width must be a multiple of 8 up to 8192", what);
+    // A wave a row, four to a workgroup, and fewer than 2^32 threads a launch.
+    if (rows > (1u << 26) - 4) return h3_set_error(g, "%s: %u rows are too many for one call", what, rows);
     return h3_require_fp8_block(g, out, 1, rows, width, what);
 }
 

@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 from h3cli_amd import synth
+from h3cli_amd._lib import U32
 from h3cli_amd.runtime import Gpu, H3Error
 from tests.helpers import bf16
 from tests.test_fp8_block_gpu import (HALF_BF16, MFMA, Packed, activation, blocks, e4m3, exponents, linear, new, quantized,
@@ -208,3 +209,31 @@ def test_more_threads_than_a_launch_takes(rows, k, n):
         xv, wv = quantized(copied(g, t, at, k), 1)[0], w.values()
         want = xv @ wv.T
         within(copied(g, out, at, n), want, HALF_BF16 * np.abs(want) + 2 * MFMA * (np.abs(xv) @ np.abs(wv).T), kernel)
+
+
+def test_norms_of_too_many_rows():
+    """Rows whose waves are more threads than a launch takes are refused, and the command goes on."""
+    rows, width = 1 << 26, 8
+    with Gpu() as g:
+        lib, h = g.lib, g.handle
+        t, norm, mod = g.empty(rows * width), g.from_bf16(values(1, width, 1)), g.from_bf16(values(6, width, 2))
+        total, row_map, packed = g.empty(rows * width), g.empty(rows, U32), new(g, rows, width)
+        g.begin()
+        for call in (lambda r: lib.h3_hip_add_rms_norm_fp8_block(h, None, packed.handle, t.handle, None, norm.handle, r, width, 1e-5),
+                     lambda r: lib.h3_hip_adaln_fp8_block(h, packed.handle, t.handle, norm.handle, mod.handle, row_map.handle, r,
+                                                          width, 6, 0, 1, 1e-5),
+                     lambda r: lib.h3_hip_gate_adaln_fp8_block(h, total.handle, packed.handle, t.handle, t.handle, norm.handle,
+                                                               mod.handle, mod.handle, row_map.handle, r, width, 6, 2, 3, 4, 1e-5)):
+            for r in (rows, rows - 3):      # 2^24 workgroups of 256
+                assert not call(r) and "too many" in g.error()
+        n = rows - 4
+        g.check(lib.h3_hip_fill_normal_bf16(h, t.handle, 1, C.c_float(1.0), n * width), "fill")
+        g.check(lib.h3_hip_add_rms_norm_fp8_block(h, None, packed.handle, t.handle, None, norm.handle, n, width, 1e-5), "norm")
+        g.check(lib.h3_hip_fp8_block_unpack(h, total.handle, packed.handle, rows, width), "unpack")
+        g.submit()
+        at = np.r_[0:8, n // 2:n // 2 + 8, n - 8:n]
+        x = copied(g, t, at, width)
+        y = x / np.sqrt((x * x).mean(axis=1, keepdims=True) + float(np.float32(1e-5))) * bf16(norm.read())
+        top = np.abs(y).max(axis=1, keepdims=True)
+        within(copied(g, total, at, width), y, np.maximum(2.0 ** -4 * np.abs(y), 2.0 ** -10 * top / 224) * (1 + 2.0 ** -20))
+        assert not copied(g, total, np.array([n]), width).any()
