@@ -154,10 +154,10 @@ template <bool SWIGLU, class T>
 int launch_pack(h3_gpu *g, const T *in, const Fp8BlockRows &out, uint32_t rows, uint32_t columns, const char *what) {
     const unsigned grid = grid_of((size_t)rows * (out.stride / LANE));
     if (!grid) return h3_set_error(g, "%s: %u rows of %u columns are too many for one call", what, rows, columns);
-    if (columns % 8 == 0)
-        hipLaunchKernelGGL((fp8_block_pack<SWIGLU, true, T>), dim3(grid), dim3(256), 0, g->compute, in, out, rows, columns);
-    else
-        hipLaunchKernelGGL((fp8_block_pack<SWIGLU, false, T>), dim3(grid), dim3(256), 0, g->compute, in, out, rows, columns);
+    auto kernel = fp8_block_pack<SWIGLU, true, T>;
+    if constexpr (sizeof(T) == 2)           // FP32 rows are the MLP's, a multiple of 128
+        if (columns % 8) kernel = fp8_block_pack<SWIGLU, false, T>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, g->compute, in, out, rows, columns);
     return h3_launch_status(g, what);
 }
 

@@ -27,12 +27,12 @@ __device__ inline i32x4 asm_resource(const uint8_t *p, unsigned bytes) {
 }
 
 // Epilogues: BF16 rows of a multiple of eight columns, without and with a bias; SwiGLU, packed;
-// and any columns, BF16 (with or without a bias) or the FP32 sums. Kernels are instantiated
-// for each: the epilogue is straight-line code that runs once per tile, and one that branches
-// between them is 100 KB of it for 256 x 256 tiles (18225 rows, 5376 -> 28672: 1.3% slower).
-enum { EPI_PLAIN = 0, EPI_BIAS = 1, EPI_SWIGLU = 2, EPI_ANY = 3 };
+// any columns, BF16 (with or without a bias); and the FP32 sums (few rows only). Kernels are
+// instantiated for each: the epilogue is straight-line code that runs once per tile, and one that
+// branches between them is 100 KB of it for 256 x 256 tiles (18225 rows, 5376 -> 28672: 1.3% slower).
+enum { EPI_PLAIN = 0, EPI_BIAS = 1, EPI_SWIGLU = 2, EPI_ANY = 3, EPI_SUMS = 4 };
 int epilogue_of(const Fp8BlockGemmArgs &a) {
-    return a.swiglu ? EPI_SWIGLU : a.y32 || a.n % 8 ? EPI_ANY : a.bias ? EPI_BIAS : EPI_PLAIN;
+    return a.swiglu ? EPI_SWIGLU : a.y32 ? EPI_SUMS : a.n % 8 ? EPI_ANY : a.bias ? EPI_BIAS : EPI_PLAIN;
 }
 
 // Four values wherever they lie: global loads and stores need no alignment.
@@ -45,11 +45,11 @@ template <int EPI>
 __device__ inline void store4(const Fp8BlockGemmArgs &a, unsigned row, unsigned col, f32x4 v) {
     if (row >= a.m || col >= a.n) return;
     const size_t at = (size_t)row * a.n + col;
+    if constexpr (EPI == EPI_SUMS) {       // the MLP's: a multiple of four columns
+        *reinterpret_cast<f32x4 *>(a.y32 + at) = v;
+        return;
+    }
     if constexpr (EPI == EPI_ANY) {
-        if (a.y32) {       // the MLP's: a multiple of four columns
-            *reinterpret_cast<f32x4 *>(a.y32 + at) = v;
-            return;
-        }
         const bool whole = col + 4 <= a.n;
         u16x4_any b = {};
         if (a.bias) {
@@ -497,10 +497,6 @@ __device__ inline void pipe_any(const Fp8BlockGemmArgs &a, unsigned row0, unsign
     for (unsigned r = 0; r < count; r++) {
         const f32x2 v = *reinterpret_cast<const f32x2 *>(rows + r * ANY_ROW + 2 * lane);
         const size_t to = (size_t)(row0 + r) * a.n + at;
-        if (a.y32) {
-            *reinterpret_cast<f32x2 *>(a.y32 + to) = v;
-            continue;
-        }
         const u16x2_any o = {{f32_to_bf16(v[0] + bias[0]), f32_to_bf16(v[1] + bias[1])}};
         if (at + 1 < a.n) *reinterpret_cast<u16x2_any *>(a.y + to) = o;
         else a.y[to] = o.v[0];
@@ -1058,7 +1054,7 @@ struct Choice {
 // for few rows, beside their launch, 5.1 for tiles.
 constexpr float STREAM_LAUNCH = 3.26f, STREAM_BYTE = 1.52e-7f, STREAM_X = 2.05e-5f, TILE_BYTE = 1.95e-7f;
 constexpr float STREAM_STEP[3][2] = {{.14f, .26f}, {.17f, .32f}, {.27f, 0.f}};
-Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
+Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool few, bool tiled = true) {
     static constexpr GemmRates RATES[3] = {{2.44f, 1.82f, .654f, .15f, 1.67f, .0881f, 1.12f},
                                            {4.02f, 1.99f, 1.82f, .3f, 3.61f, .0557f, 1.02f},
                                            {7.38f, 3.62f, 4.18f, .3f, 8.77f, .0346f, 1.f}};
@@ -1066,7 +1062,7 @@ Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
     const float reads = (float)a.n * a.k;
     const unsigned steps = a.k / TK;
     Choice best{3.4e38f, 0, 1, 0, 0};
-    for (unsigned i = 0; i < 3; i++) {
+    for (unsigned i = 0; tiled && i < 3; i++) {
         const unsigned rows = 64u << i, units = (steps + QUAD - 1) / QUAD;
         const uint64_t tiles = ((uint64_t)a.m + rows - 1) / rows * (((uint64_t)a.n + 255) / 256);
         if ((tiles + 2 * g->cus) * 256 > MAX_THREADS) continue;     // and the shares of a last wave
@@ -1074,7 +1070,7 @@ Choice choose(const h3_gpu *g, const Fp8BlockGemmArgs &a, bool stream) {
         const float us = (std::max(p.us, reads * TILE_BYTE) + LAUNCH[i]) * (p.split > 1 ? 1.02f : 1.f);
         if (us < best.us) best = {us, rows, p.split, 0, 0};
     }
-    if (!stream) return best;
+    if (!few) return best;
     for (unsigned rb = 1; rb <= 3; rb++)
         for (unsigned nb = 2; nb <= (rb < 3 ? 4u : 2u); nb += 2) {
             const float rounds = stream_rounds(g, a, rb, nb);
@@ -1096,15 +1092,20 @@ bool packs(const h3_gpu *g, const Fp8BlockGemmArgs &a, const Choice &c) {
 }
 
 template <int EPI> int run(h3_gpu *g, const Fp8BlockGemmArgs &a) {
-    const Choice c = choose(g, a, EPI != EPI_SWIGLU);
+    // SwiGLU is an epilogue of tiles only; the sums are asked for where few rows' kernels are faster.
+    constexpr bool few = EPI != EPI_SWIGLU, tiles = EPI != EPI_SUMS;
+    const Choice c = choose(g, a, few, tiles);
     if (a.m > FP8_BLOCK_ROWS || (!c.rb && !c.rows))
         return h3_set_error(g, "FP8 block projection: %u rows by %u columns are too many for one call", a.m, a.n);
-    if constexpr (EPI != EPI_SWIGLU)
+    if constexpr (few)
         if (c.rb) return a.xb ? launch_stream<EPI, true>(g, a, c.rb, c.nb) : launch_stream<EPI, false>(g, a, c.rb, c.nb);
-    if (a.xb) return h3_set_error(g, "FP8 block projection: %u rows of BF16 are to be packed first", a.m);
-    return c.rows == 256   ? launch_pipe<EPI, 256>(g, a, c.split)
-           : c.rows == 128 ? launch_pipe<EPI, 128>(g, a, c.split)
-                           : launch_mid<EPI>(g, a, c.split);
+    if constexpr (tiles) {
+        if (a.xb) return h3_set_error(g, "FP8 block projection: %u rows of BF16 are to be packed first", a.m);
+        return c.rows == 256   ? launch_pipe<EPI, 256>(g, a, c.split)
+               : c.rows == 128 ? launch_pipe<EPI, 128>(g, a, c.split)
+                               : launch_mid<EPI>(g, a, c.split);
+    }
+    return 0;
 }
 
 }  // namespace
@@ -1123,6 +1124,7 @@ int h3_gemm_fp8_block(h3_gpu *g, const Fp8BlockGemmArgs &a) {
     case EPI_PLAIN: return run<EPI_PLAIN>(g, a);
     case EPI_BIAS: return run<EPI_BIAS>(g, a);
     case EPI_SWIGLU: return run<EPI_SWIGLU>(g, a);
+    case EPI_SUMS: return run<EPI_SUMS>(g, a);
     default: return run<EPI_ANY>(g, a);
     }
 }
