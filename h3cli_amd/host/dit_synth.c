@@ -317,6 +317,13 @@ h3_hip_dit_synth *h3_hip_dit_synth_create(h3_gpu *g, const h3_hip_dit_synth_conf
         fail(error, size, "synthetic DiT: quantized projections need every block resident");
         return NULL;
     }
+    const uint64_t rows = (uint64_t)c->frames * c->height * c->width + c->audio_rows;
+    if ((packed || blocked) && !c->swiglu && rows * c->mlp > UINT32_MAX) {
+        /* One GELU over the MLP's hidden values, whose number that operator takes in 32 bits. */
+        fail(error, size, "synthetic DiT: %llu rows of %u hidden values are too many for the GELU MLP of quantized projections",
+             (unsigned long long)rows, c->mlp);
+        return NULL;
+    }
     h3_hip_dit_synth *m = calloc(1, sizeof(*m));
     if (!m) { fail(error, size, "out of host memory"); return NULL; }
     m->gpu = g;

@@ -9,7 +9,7 @@ import pytest
 
 from h3cli_amd import synth
 from h3cli_amd._lib import U32
-from h3cli_amd.runtime import Gpu, H3Error
+from h3cli_amd.runtime import DitSynth, Gpu, H3Error
 from tests.helpers import bf16
 from tests.test_fp8_block_gpu import (HALF_BF16, MFMA, Packed, activation, blocks, e4m3, exponents, linear, new, quantized,
                                         values, weight, within)
@@ -237,3 +237,11 @@ def test_norms_of_too_many_rows():
         top = np.abs(y).max(axis=1, keepdims=True)
         within(copied(g, total, at, width), y, np.maximum(2.0 ** -4 * np.abs(y), 2.0 ** -10 * top / 224) * (1 + 2.0 ** -20))
         assert not copied(g, total, np.array([n]), width).any()
+
+
+@pytest.mark.parametrize("quant", [1, 3])
+def test_dit_of_too_many_hidden_values(quant):
+    """The GELU MLP of quantized projections takes fewer than 2^32 hidden values; more were cut off."""
+    with pytest.raises(H3Error, match="too many for the GELU MLP"):
+        DitSynth(geometry="h3", blocks=1, hidden=256, heads=1, mlp=1 << 16, frames=256, height=16, width=16, audio_rows=0,
+                 latent=256, streamed_first=1, swiglu=0, projection_quant=quant)
