@@ -22,7 +22,9 @@ constexpr unsigned LANE = 16;                     // values per lane
 constexpr unsigned LANES = FP8_BLOCK / LANE;      // lanes per block
 
 // 16 values of a row from `col` on, zeros from `columns` on. VEC: rows of a multiple of eight
-// values, so that 16-byte loads are aligned and a half is inside or outside as a whole.
+// values, so that 16-byte loads are aligned and a half is inside or outside as a whole. Without it
+// values are loaded one by one, at a quarter of the rate (SwiGLU of 4000 rows with unpacking: 13824
+// wide 83.5 us, 13823 wide 362).
 template <bool VEC, class T>
 __device__ inline void load16(const T *row, unsigned col, unsigned columns, float *v) {
     constexpr unsigned PER = 16 / sizeof(T);
@@ -107,7 +109,7 @@ __global__ __launch_bounds__(256) void fp8_block_pack_weight(const uint16_t *in,
     if (threadIdx.x == 0) out.scales[fp8_block_scale_at(r0 / FP8_BLOCK, block, out.groups)] = (uint8_t)scale;
 }
 
-// BF16 values code * 2^e, exact but for values below BF16's range. 16 values per lane.
+// BF16 values code * 2^e, exact but for values outside BF16's normal range. 16 values per lane.
 template <bool VEC>
 __global__ __launch_bounds__(256) void fp8_block_unpack(const uint8_t *codes, const uint8_t *scales, unsigned stride,
                                                         unsigned groups, unsigned tile, uint16_t *out,
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(256) void fp8_block_unpack(const uint8_t *codes, co
     const unsigned row = (unsigned)(id / lanes), col = (unsigned)(id % lanes) * LANE;
     if (col >= columns) return;
     const u32x4 q = *reinterpret_cast<const u32x4 *>(codes + (size_t)row * stride + col);
-    // The two halves of the power of two: their product with a code has one rounding.
+    // Codes times a power of two: exact, and BF16 rounds only what is outside its normal range.
     const int e = (int)scales[fp8_block_scale_at(row / tile, col / FP8_BLOCK, groups)] - 127;
     uint16_t v[LANE];
 #pragma unroll

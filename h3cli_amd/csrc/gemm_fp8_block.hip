@@ -450,7 +450,7 @@ __device__ inline void round_row(const Fp8BlockGemmArgs &a, unsigned col, unsign
 // PAST: past the L2's resident lines. All workgroups of a wave of 256-row tiles store at once, 33
 // MB; stored from the registers, 32 bytes of 32 rows an instruction, that takes 12 of a tile's 75
 // us (18225 rows, 5376 -> 28672: 2385 us, 1975 without any stores); so 2132. (The lines alone:
-// 2370; past the L2 alone: 2440.)
+// 2370; past the L2 alone: 2440. One card; others, or runs of other lengths, 1967 to 2184.)
 template <int NB> constexpr unsigned ROW_LDS = NB * 64 + 16;    // bytes of a row in LDS, padded against bank conflicts
 template <int EPI, bool PAST, int NB>
 __device__ inline void store_rows(const Fp8BlockGemmArgs &a, unsigned row0, unsigned col, unsigned lane,

@@ -164,6 +164,8 @@ h3_gpu_tensor *h3_hip_quant_weight_from_bf16(h3_gpu *gpu, const h3_gpu_tensor *w
  * fails the next submit, like one in an FP8 projection's input. The packed
  * type is a tensor of its own: the operators below take it, others refuse it.
  * Work with rows <= the tensor's rows leaves the rows behind as they were.
+ * Rows of a multiple of 8 values are packed, unpacked and activated several
+ * times as fast as others.
  *
  * h3_hip_fp8_block_layout: where a matrix has its parts, in bytes: codes of
  * row r from r * stride on (zeros behind `columns`); the scale of block b of
@@ -191,7 +193,8 @@ int h3_hip_fp8_block_unpack(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_ten
                             uint32_t rows, uint32_t columns);
 /* y[rows, output_dim] = bf16(x . W^T (+ bias)), x an activation and W a weight,
  * FP32 sums. h3_gpu_linear_bf16 takes such a weight too and packs its BF16
- * input per call, in a workspace of the context (refused under capture). */
+ * input per call, as a rule in a workspace of the context (refused under
+ * capture at any size). */
 int h3_hip_linear_fp8_block(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
                             const h3_gpu_tensor *weight, const h3_gpu_tensor *bias,
                             uint32_t rows, uint32_t input_dim, uint32_t output_dim);
