@@ -2,6 +2,7 @@
 shares of K, and the rule that a graph keeps no partial sums. Bounds as in test_fp8_block_gpu.py."""
 import ctypes as C
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -149,3 +150,36 @@ def test_graphs_keep_no_partial_sums():
             rows_within(g, t, w, got.reshape(m, n), m, k, n, "graph")
         for graph in graphs:
             graph.close()
+
+
+def test_two_contexts_at_once():
+    """Two contexts, a thread each: shares of K, packing and the MLP's workspace are each its own."""
+    m, k, hidden = 300, 5376, 2560
+
+    def model(seed):
+        g = Gpu()
+        t = normal(g, m * k, seed, 1.0)
+        w1 = weight_of(g, normal(g, 2 * hidden * k, seed + 1, 1 / math.sqrt(k)), 2 * hidden, k)
+        w2 = weight_of(g, normal(g, k * hidden, seed + 2, 1 / math.sqrt(hidden)), k, hidden)
+        return g, t, w1, w2, g.empty(m * k), g.empty(m * 2 * hidden)
+
+    def run(model, times):
+        g, t, w1, w2, out, product = model
+        got = []
+        for _ in range(times):
+            g.begin()
+            g.check(g.lib.h3_gpu_linear_bf16(g.handle, product.handle, t.handle, w1.handle, None, m, k, 2 * hidden), "linear")
+            g.check(g.lib.h3_gpu_mlp_bf16(g.handle, out.handle, t.handle, w1.handle, w2.handle, m, k, hidden, k), "mlp")
+            g.submit()
+            got.append((product.read(), out.read()))
+        return got
+
+    models = [model(seed) for seed in (1, 11)]
+    try:
+        want = [run(x, 1)[0] for x in models]
+        with ThreadPoolExecutor(2) as pool:
+            for (product, out), got in zip(want, pool.map(lambda x: run(x, 10), models)):
+                assert all(np.array_equal(product, p) and np.array_equal(out, o) for p, o in got)
+    finally:
+        for x in models:
+            x[0].close()
