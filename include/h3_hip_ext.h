@@ -206,7 +206,9 @@ int h3_hip_mlp_fp8_block(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor
                          uint32_t rows, uint32_t input_dim, uint32_t hidden_dim, uint32_t output_dim);
 /* h3_gpu_swiglu_bf16, h3_gpu_adaln_bf16, h3_gpu_gate_adaln_bf16 and
  * h3_gpu_rms_norm_bf16 with an activation for their (normalized) output,
- * packed from the FP32 values. */
+ * packed from the FP32 values. Norms take up to 2^26 - 4 rows a call; packing
+ * (a projection's BF16 input too), unpacking and SwiGLU fewer than 2^35 values,
+ * blocks that are cut off counted whole. More are refused. */
 int h3_hip_swiglu_fp8_block(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
                             uint32_t rows, uint32_t width);
 int h3_hip_adaln_fp8_block(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
