@@ -169,6 +169,20 @@ _SIGNATURES.update({
     "h3_hip_adaln_fp8_block": (_i, [_p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _f]),
     "h3_hip_gate_adaln_fp8_block": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _u32, _f]),
     "h3_hip_add_rms_norm_fp8_block": (_i, [_p, _p, _p, _p, _p, _p, _u32, _u32, _f]),
+    # several requests in one step
+    "h3_hip_sequences_new": (_p, [_p, _p, _p, _u32, _u32, _u32]),
+    "h3_hip_sequences_free": (None, [_p]),
+    "h3_hip_sdpa_sequences_bf16": (_i, [_p, _p, _p, _p, _p, _p, _f]),
+    "h3_hip_rope_axes_new": (_p, [_p, _p, _p, _u32, _u32, _i]),
+    "h3_hip_rope_axes_free": (None, [_p]),
+    "h3_hip_qkv_rope_axes_bf16": (_i, [_p] * 9 + [_u32, _u32, _u32, _u32, _i, _f]),
+    "h3_hip_adapters_new": (_p, [_p, _p, _u32, _u32, _u32]),
+    "h3_hip_adapters_set": (_i, [_p, _p, _u32, _p, _p, _f]),
+    "h3_hip_adapters_free": (None, [_p]),
+    "h3_hip_adapter_rows_new": (_p, [_p, _p, _u32, _u32, _u32]),
+    "h3_hip_adapter_rows_free": (None, [_p]),
+    "h3_hip_adapters_add_bf16": (_i, [_p] * 6 + [_u32, _u32, _u32]),
+    "h3_hip_linear_adapters_bf16": (_i, [_p] * 7 + [_u32, _u32, _u32]),
     # the rest of the reference surface implemented here (include/h3_gpu_surface.h)
     "h3_gpu_adaln_bf16_offset": (_i, [_p, _p, _p, _sz, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _f]),
     "h3_gpu_rms_norm_bf16": (_i, [_p, _p, _p, _p, _u32, _u32, _f]),

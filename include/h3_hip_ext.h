@@ -228,6 +228,78 @@ int h3_hip_add_rms_norm_fp8_block(h3_gpu *gpu, h3_gpu_tensor *sum, h3_gpu_tensor
                                   const h3_gpu_tensor *norm_weight, uint32_t rows, uint32_t width,
                                   float epsilon);
 
+/* ---- several requests in one step --------------------------------------
+ * The rows of several requests lie behind one another in one tensor (two of a
+ * guidance pair, clips of different sizes) and share the model's weights.
+ * Projections, norms and gates take such rows as they are; these operators know
+ * whose they are. Plans hold what the operators read on the device, and the
+ * workspace of their calls: they allocate nothing and may be captured into a
+ * graph. A plan serves any number of calls in turn, not two at once (calls of
+ * two streams, say), and is freed before its context.
+ *
+ * Sequence i of `count` has the query rows [q_offsets[i], q_offsets[i + 1]) and
+ * the key rows [k_offsets[i], k_offsets[i + 1]) (NULL: as the queries); either
+ * may be empty. heads is a multiple of kv_heads: query head h reads key head
+ * h / (heads / kv_heads). */
+typedef struct h3_hip_sequences h3_hip_sequences;
+h3_hip_sequences *h3_hip_sequences_new(h3_gpu *gpu, const uint32_t *q_offsets, const uint32_t *k_offsets,
+                                       uint32_t count, uint32_t heads, uint32_t kv_heads);
+void h3_hip_sequences_free(h3_hip_sequences *sequences);
+/* softmax(scale * Q K^T) V within each sequence: q and out [rows, heads, 128], k and v
+ * [rows, kv_heads, 128] BF16, the scale rounded to BF16, as h3_gpu_sdpa_bf16 of each
+ * sequence alone. A query of a sequence without keys gets zeros; rows of no
+ * sequence stay as they were. */
+int h3_hip_sdpa_sequences_bf16(h3_gpu *gpu, h3_gpu_tensor *out, const h3_gpu_tensor *q, const h3_gpu_tensor *k,
+                               const h3_gpu_tensor *v, const h3_hip_sequences *sequences, float scale);
+
+/* Rotation by positions of several axes: pair j turns by position[axis[j]] *
+ * frequencies[j] radians. interleaved 0: pair j are the channels j and j + pairs,
+ * as h3_gpu_qkv_rope_bf16 has them; 1: the channels 2 j and 2 j + 1. Up to 128 pairs
+ * and 16 axes. */
+typedef struct h3_hip_rope_axes h3_hip_rope_axes;
+h3_hip_rope_axes *h3_hip_rope_axes_new(h3_gpu *gpu, const double *frequencies, const uint32_t *axis, uint32_t pairs,
+                                       uint32_t axes, int interleaved);
+void h3_hip_rope_axes_free(h3_hip_rope_axes *rope);
+/* h3_gpu_qkv_rope_bf16 with each row's positions (F32 [rows, axes]) for its tables and
+ * with kv_heads key heads. qkv rows are [heads + 2 * kv_heads, dim], queries first, then
+ * keys, then values; grouped 1: for each key head its query heads, its key and its
+ * value, [kv_heads, heads / kv_heads + 2, dim]. The angles' phase is exact to 2^-23 of
+ * a turn for positions of any size. dim <= 256; rows of a multiple of 8 channels
+ * and pairs are several times as fast as others. */
+int h3_hip_qkv_rope_axes_bf16(h3_gpu *gpu, h3_gpu_tensor *query, h3_gpu_tensor *key, h3_gpu_tensor *value,
+                              const h3_gpu_tensor *qkv, const h3_gpu_tensor *q_norm, const h3_gpu_tensor *k_norm,
+                              const h3_hip_rope_axes *rope, const h3_gpu_tensor *positions, uint32_t rows,
+                              uint32_t heads, uint32_t kv_heads, uint32_t dim, int grouped, float epsilon);
+
+/* Low-rank adapters of a projection W [output_dim, input_dim]: adapter i adds
+ * scale_i * (x . A_i^T) . B_i^T to the rows that take it, A_i [ranks[i],
+ * input_dim] and B_i [output_dim, ranks[i]] BF16, ranks 1 to 256. A new adapter
+ * is zero; h3_hip_adapters_set copies A and B of one (in the stream's order, any
+ * time within a command). W itself may be of any type: it is neither read nor
+ * packed anew. */
+typedef struct h3_hip_adapters h3_hip_adapters;
+h3_hip_adapters *h3_hip_adapters_new(h3_gpu *gpu, const uint32_t *ranks, uint32_t count, uint32_t input_dim,
+                                     uint32_t output_dim);
+int h3_hip_adapters_set(h3_gpu *gpu, h3_hip_adapters *adapters, uint32_t index, const h3_gpu_tensor *a,
+                        const h3_gpu_tensor *b, float scale);
+void h3_hip_adapters_free(h3_hip_adapters *adapters);
+/* Which of `count` adapters each row takes (an index from count on: none), for
+ * adapters of ranks up to max_rank. One plan serves all projections. */
+typedef struct h3_hip_adapter_rows h3_hip_adapter_rows;
+h3_hip_adapter_rows *h3_hip_adapter_rows_new(h3_gpu *gpu, const uint32_t *row_map, uint32_t rows, uint32_t count,
+                                             uint32_t max_rank);
+void h3_hip_adapter_rows_free(h3_hip_adapter_rows *rows);
+/* output = bf16(base + the adapters' parts), FP32 sums; rows without adapter are
+ * base's. output may be base. */
+int h3_hip_adapters_add_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *base, const h3_gpu_tensor *input,
+                             const h3_hip_adapters *adapters, const h3_hip_adapter_rows *adapter_rows, uint32_t rows,
+                             uint32_t input_dim, uint32_t output_dim);
+/* h3_gpu_linear_bf16 and the adapters' parts, which are added to its BF16 output. */
+int h3_hip_linear_adapters_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                                const h3_gpu_tensor *weight, const h3_gpu_tensor *bias,
+                                const h3_hip_adapters *adapters, const h3_hip_adapter_rows *adapter_rows,
+                                uint32_t rows, uint32_t input_dim, uint32_t output_dim);
+
 /* Sage quantization of sequence-major BF16 Q, K, V [seq, heads, 128] into the
  * layouts the quantized attention kernel consumes (all head-major, rows padded
  * to a multiple of 64, padded rows zero):

@@ -1,0 +1,500 @@
+"""Operators of a step that serves several requests at once: attention of packed sequences,
+rotation by positions of several axes with the norms of Q and K, low-rank adapters beside a
+projection. Each against its formula in 64 bits.
+
+Bounds. HALF is BF16's largest rounding error relative to the value, F32 that of FP32; a sum
+of n products in FP32 is off by at most n * F32 times the sum of the products' magnitudes."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from h3cli_amd import synth
+from h3cli_amd._lib import F32 as F32_TENSOR
+from h3cli_amd.runtime import Gpu, H3Error
+from tests.helpers import bf16
+from tests.test_capture_gpu import Graph
+
+pytestmark = pytest.mark.gpu
+
+HALF, F32 = 2.0 ** -8, 2.0 ** -24
+SCALE = 0.08837890625   # 1 / sqrt(128) in BF16
+EPS = 1e-5
+
+
+def u32(values):
+    return (C.c_uint32 * len(values))(*(int(v) for v in values))
+
+
+def normal(count, seed, scale=1.0):
+    return synth.normal_bf16(seed, max(int(count), 1), scale=scale)[:int(count)]
+
+
+def within(got, want, bound, what=""):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    off = np.abs(got - want) - bound
+    assert np.all(np.isfinite(got)) and np.all(off <= 0), (what, float(np.max(off)), int(np.argmax(off)))
+
+
+class Plan:
+    def __init__(self, g, handle, free):
+        g.check(handle, "plan")
+        self.g, self.handle, self.free_handle = g, handle, free
+
+    def __enter__(self):
+        return self.handle
+
+    def __exit__(self, *exc):
+        self.free_handle(self.handle)
+
+
+# ------------------------------------------------------------------ attention of sequences
+def sequences(g, q_offsets, k_offsets, heads, kv_heads):
+    h = g.lib.h3_hip_sequences_new(g.handle, u32(q_offsets), None if k_offsets is None else u32(k_offsets),
+                                   len(q_offsets) - 1, heads, kv_heads)
+    return Plan(g, h, g.lib.h3_hip_sequences_free)
+
+
+def attention_reference(q, k, v, scale):
+    """softmax(scale q k^T) v of one head in 64 bits, and the bound of the operator's error."""
+    s = scale * (q @ k.T)
+    size = scale * (np.abs(q) @ np.abs(k).T)
+    p = np.exp(s - s.max(axis=1, keepdims=True))
+    p /= p.sum(axis=1, keepdims=True)
+    out, weight = p @ v, p @ np.abs(v)
+    # A score is off by 128 products' sum, its scaling and the exponential's argument and result; a
+    # probability relatively by as much, in the numerator and in the sum; P is rounded to BF16.
+    score = (130 * F32 * size + 8 * F32 * (1 + np.abs(s))).max(axis=1, keepdims=True) + 8 * F32
+    return out, HALF * np.abs(out) + (HALF + 2 * score + 2 * (len(k) + 64) * F32) * weight * (1 + HALF)
+
+
+def check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=1, spread=1.0, scale=SCALE, rows=None):
+    """One call against the reference; rows of no sequence hold NaN in the inputs and must stay in the output."""
+    at = k_offsets if k_offsets is not None else q_offsets
+    rows = rows or (q_offsets[-1] + 3, at[-1] + 5)
+    share = heads // kv_heads
+    q, k, v = (normal(rows[i > 0] * n * 128, seed + i, scale=spread if i < 2 else 1.0).reshape(rows[i > 0], n, 128).copy()
+               for i, n in ((0, heads), (1, kv_heads), (2, kv_heads)))
+    for t, ends in ((q, q_offsets), (k, at), (v, at)):
+        t[:ends[0]] = 0x7fc0
+        t[ends[-1]:] = 0x7f80
+    mark = normal(q.size, seed + 9).reshape(q.shape)
+    tq, tk, tv, out = (g.from_bf16(t) for t in (q, k, v, mark))
+    with sequences(g, q_offsets, k_offsets, heads, kv_heads) as plan:
+        g.begin()
+        g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, out.handle, tq.handle, tk.handle, tv.handle, plan, C.c_float(scale)),
+                "attention")
+        kernel = g.last_kernel()
+        g.submit()
+        got = out.read().reshape(q.shape)
+        g.begin()
+        g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, out.handle, tq.handle, tk.handle, tv.handle, plan, C.c_float(scale)),
+                "attention")
+        g.submit()
+        assert np.array_equal(out.read().reshape(q.shape), got)
+    assert np.array_equal(got[:q_offsets[0]], mark[:q_offsets[0]]) and np.array_equal(got[q_offsets[-1]:], mark[q_offsets[-1]:])
+    fq, fk, fv = (bf16(t).astype(np.float64) for t in (q, k, v))
+    for i in range(len(q_offsets) - 1):
+        qs, ks = slice(q_offsets[i], q_offsets[i + 1]), slice(at[i], at[i + 1])
+        if at[i] == at[i + 1]:
+            assert not np.any(got[qs] & 0x7fff)
+            continue
+        for h in range(heads):
+            want, bound = attention_reference(fq[qs, h], fk[ks, h // share], fv[ks, h // share], scale)
+            within(bf16(got[qs, h]), want, bound, (kernel, i, h))
+    for t in (tq, tk, tv, out):
+        g.free(t)
+    return kernel
+
+
+@pytest.mark.parametrize("q_offsets,k_offsets,heads,kv_heads", [
+    ([0, 1], None, 1, 1),
+    ([0, 1, 8, 72], None, 8, 8),
+    ([2, 65, 65, 194, 195], None, 3, 3),                    # rows before the first, an empty sequence
+    ([0, 31, 64, 97], [0, 63, 127, 192], 2, 1),             # tiles of 64 keys, less one and one more
+    ([0, 1, 2, 5, 6], [0, 700, 701, 701, 1300], 10, 2),     # single rows, one of a sequence without keys
+    ([0, 5, 5, 9], [7, 7, 20, 333], 6, 3),                  # queries without keys, keys without queries
+    ([0, 33], [0, 129], 7, 1),                              # all query heads share a key head
+    ([0, 300, 1100, 1130], None, 4, 4),
+    ([0, 200], [0, 900], 40, 8),
+])
+def test_attention_of_sequences(q_offsets, k_offsets, heads, kv_heads):
+    print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads}", flush=True)
+    with Gpu() as g:
+        check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=len(q_offsets) * 17 + heads)
+
+
+@pytest.mark.parametrize("spread,scale", [(6.0, SCALE), (0.01, SCALE), (1.0, 3.0), (1.0, 2.0 ** -20)])
+def test_attention_of_sequences_peaks_and_flat_rows(spread, scale):
+    with Gpu() as g:
+        check_attention(g, [0, 70, 135], [0, 300, 650], 2, 2, seed=5, spread=spread, scale=scale)
+
+
+def test_attention_of_sequences_reports_values_that_are_not_finite():
+    """In a query, key or value of any sequence; the others' results stay whole."""
+    for which in range(3):
+        with Gpu() as g:
+            ts = [normal(100 * 256, 3 + i).reshape(100, 2, 128).copy() for i in range(3)]
+            clean = [g.from_bf16(t) for t in ts]
+            ts[which][77, 1, 5] = 0x7f80 if which else 0x7fc0
+            dirty = [g.from_bf16(t) for t in ts]
+            out, other = g.empty(100 * 256), g.empty(100 * 256)
+            with sequences(g, [0, 40, 100], None, 2, 2) as plan:
+                args = (plan, C.c_float(SCALE))
+                g.begin()
+                g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, out.handle, *(t.handle for t in clean), *args))
+                g.submit()
+                g.begin()
+                g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, other.handle, *(t.handle for t in dirty), *args))
+                with pytest.raises(H3Error, match="nonfinite attention"):
+                    g.submit()
+                g.cancel()
+                a, b = out.read().reshape(100, 2, 128), other.read().reshape(100, 2, 128)
+                assert np.array_equal(a[:40], b[:40]) and np.array_equal(a[40:, 0], b[40:, 0])
+
+
+# ------------------------------------------------------------------ rotation by axes
+def rope_axes(g, frequencies, axis, axes, interleaved):
+    h = g.lib.h3_hip_rope_axes_new(g.handle, (C.c_double * len(frequencies))(*frequencies), u32(axis), len(frequencies), axes,
+                                   interleaved)
+    return Plan(g, h, g.lib.h3_hip_rope_axes_free)
+
+
+def rope_reference(qkv, weights, frequencies, axis, positions, heads, kv_heads, grouped, interleaved):
+    """Query, key and value in 64 bits, each with the bound of the operator's error."""
+    rows, dim, pairs, share = qkv.shape[0], qkv.shape[2], len(frequencies), heads // kv_heads
+    if grouped:
+        x = qkv.reshape(rows, kv_heads, share + 2, dim)
+        parts = [x[:, :, :share].reshape(rows, heads, dim), x[:, :, share], x[:, :, share + 1]]
+    else:
+        parts = [qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]]
+    angle = positions.astype(np.float64)[:, axis] * np.asarray(frequencies)
+    c, s = np.cos(angle)[:, None], np.sin(angle)[:, None]
+    first = np.arange(pairs) * (2 if interleaved else 1)
+    second = first + (1 if interleaved else pairs)
+    out = []
+    for x, w in zip(parts, weights):
+        y = x / np.sqrt((x * x).mean(axis=2, keepdims=True) + EPS) * w if w is not None else x.copy()
+        a, b = y[..., first].copy(), y[..., second].copy()
+        size = np.abs(y)
+        y[..., first], y[..., second] = a * c - b * s, b * c + a * s
+        size[..., first] = size[..., second] = np.abs(a) + np.abs(b)
+        # The norm: a sum of dim squares, its root's reciprocal, three products; the rotation: the
+        # hardware's sine and cosine to 2^-18 at phases off by 2^-23 turns; one rounding to BF16.
+        out.append((y, HALF * np.abs(y) + size * (1 + HALF) * (2.0 ** -18 + 2 * math.pi * 2.0 ** -23 + (dim + 12) * F32)))
+    out.append((parts[2], np.zeros_like(parts[2])))
+    return out
+
+
+def check_rope(g, rows, heads, kv_heads, dim, pairs, axes=3, grouped=0, interleaved=0, norm=True, far=0.0, seed=1):
+    rng = np.random.RandomState(seed)
+    qkv = normal(rows * (heads + 2 * kv_heads) * dim, seed, scale=2.0).reshape(rows, -1, dim)
+    weights = [synth.f32_to_bf16((1 + 0.2 * rng.randn(dim)).astype(np.float32)) for _ in range(2)] if norm else [None, None]
+    frequencies, axis = 10000.0 ** -rng.rand(pairs), rng.randint(0, axes, pairs)
+    positions = (rng.randint(-40, 40, (rows, axes)) * 0.37 + far).astype(np.float32)
+    mark = [normal((rows + 2) * n * dim, seed + 3) for n in (heads, kv_heads, kv_heads)]
+    outs = [g.from_bf16(m) for m in mark]
+    held = [g.from_bf16(qkv), g.from_f32(positions)] + [g.from_bf16(w) for w in weights if w is not None]
+    with rope_axes(g, frequencies, axis, axes, interleaved) as plan:
+        g.begin()
+        g.check(g.lib.h3_hip_qkv_rope_axes_bf16(
+            g.handle, *(o.handle for o in outs), held[0].handle, held[2].handle if norm else None,
+            held[3].handle if norm else None, plan, held[1].handle, rows, heads, kv_heads, dim, grouped, C.c_float(EPS)), "rope")
+        g.submit()
+    want = rope_reference(bf16(qkv).astype(np.float64), [None if w is None else bf16(w).astype(np.float64) for w in weights],
+                          frequencies, axis, positions, heads, kv_heads, grouped, interleaved)
+    for o, m, (y, bound), n in zip(outs, mark, want, (heads, kv_heads, kv_heads)):
+        got = o.read().reshape(-1, n, dim)
+        assert np.array_equal(got[rows:].reshape(-1), m[rows * n * dim:])
+        within(bf16(got[:rows]), y, bound, (rows, heads, kv_heads, dim, pairs, grouped, interleaved))
+    for t in outs + held:
+        g.free(t)
+
+
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("grouped", [0, 1])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,pairs", [
+    (1, 1, 1, 128, 64), (1, 56, 56, 128, 48), (5, 6, 2, 90, 37), (33, 4, 1, 64, 32), (7, 5, 5, 128, 3), (3, 3, 3, 7, 3),
+    (19, 2, 2, 256, 128), (6, 8, 2, 256, 96), (5, 2, 1, 80, 24), (9, 3, 3, 24, 8), (300, 7, 7, 128, 48), (2, 4, 2, 255, 127),
+    (4, 1, 1, 2, 1), (11, 17, 17, 8, 4), (23, 6, 3, 16, 8), (3, 2, 2, 32, 12),
+])
+def test_rope_by_axes(rows, heads, kv_heads, dim, pairs, grouped, interleaved):
+    with Gpu() as g:
+        check_rope(g, rows, heads, kv_heads, dim, pairs, grouped=grouped, interleaved=interleaved, seed=rows + dim)
+        check_rope(g, rows, heads, kv_heads, dim, pairs, axes=1, grouped=grouped, interleaved=interleaved, norm=False, seed=rows)
+
+
+@pytest.mark.parametrize("far", [1e5, -1e5, 1.6e7, 3e9])
+def test_rope_by_axes_keeps_the_phase_of_far_positions(far):
+    with Gpu() as g:
+        check_rope(g, 12, 2, 2, 128, 48, axes=16, far=far)
+        check_rope(g, 12, 2, 2, 90, 45, interleaved=1, far=far)
+
+
+def test_rope_by_axes_passes_other_channels_as_they_are():
+    """Without norms, channels behind the pairs and all of V: infinities and NaN's bits among them."""
+    for dim, pairs in ((128, 32), (90, 21)):
+        with Gpu() as g:
+            qkv = normal(6 * 3 * dim, 4).reshape(6, 3, dim).copy()
+            qkv[2, :, 2 * pairs + 1], qkv[3, 2, 0], qkv[4, 2, 1] = 0x7f80, 0x7fc1, 0xff80
+            t, p = g.from_bf16(qkv), g.from_f32(np.ones((6, 1), np.float32))
+            outs = [g.empty(6 * dim) for _ in range(3)]
+            with rope_axes(g, [0.5] * pairs, [0] * pairs, 1, 0) as plan:
+                g.begin()
+                g.check(g.lib.h3_hip_qkv_rope_axes_bf16(g.handle, *(o.handle for o in outs), t.handle, None, None, plan, p.handle,
+                                                        6, 1, 1, dim, 0, C.c_float(EPS)), "rope")
+                g.submit()
+            q, k, v = (o.read().reshape(6, dim) for o in outs)
+            assert np.array_equal(v, qkv[:, 2])
+            assert np.array_equal(q[:, 2 * pairs:], qkv[:, 0, 2 * pairs:]) and np.array_equal(k[:, 2 * pairs:], qkv[:, 1, 2 * pairs:])
+
+
+# ------------------------------------------------------------------ adapters
+class Adapters:
+    def __init__(self, g, ranks, k, n, seed=1, scales=None):
+        self.g, self.ranks, self.k, self.n = g, ranks, k, n
+        self.handle = g.check(g.lib.h3_hip_adapters_new(g.handle, u32(ranks), len(ranks), k, n), "adapters")
+        self.a = [normal(r * k, seed + 2 * i, scale=1 / math.sqrt(k)).reshape(r, k) for i, r in enumerate(ranks)]
+        self.b = [normal(n * r, seed + 2 * i + 1, scale=1 / math.sqrt(r)).reshape(n, r) for i, r in enumerate(ranks)]
+        self.scales = scales or [0.5 + 0.75 * (i % 3) for i in range(len(ranks))]
+        for i in range(len(ranks)):
+            self.set(i)
+
+    def set(self, i, a=None, b=None, scale=None):
+        g = self.g
+        self.a[i], self.b[i] = self.a[i] if a is None else a, self.b[i] if b is None else b
+        self.scales[i] = self.scales[i] if scale is None else scale
+        ta, tb = g.from_bf16(self.a[i]), g.from_bf16(self.b[i])
+        g.begin()
+        g.check(g.lib.h3_hip_adapters_set(g.handle, self.handle, i, ta.handle, tb.handle, C.c_float(self.scales[i])), "set")
+        g.submit()
+        g.free(ta)
+        g.free(tb)
+
+    def close(self):
+        self.g.lib.h3_hip_adapters_free(self.handle)
+
+    def reference(self, x, at, base, base_error):
+        """base + the parts of the rows' adapters in 64 bits, and the bound of the operator's error."""
+        y, bound = base.copy(), base_error.copy()
+        for i, r in enumerate(self.ranks):
+            rows = np.flatnonzero(at == i)
+            a, b, scale = bf16(self.a[i]).astype(np.float64), bf16(self.b[i]).astype(np.float64), float(np.float32(self.scales[i]))
+            t, size = x[rows] @ a.T, np.abs(x[rows]) @ np.abs(a).T
+            y[rows] += scale * t @ b.T
+            # t: K products (in shares) and their scaling; two BF16 roundings in turn; 2 r products.
+            t_error = (self.k + 16) * F32 * size + HALF ** 2 * np.abs(t)
+            bound[rows] += abs(scale) * (t_error @ np.abs(b).T + (2 * r + 40) * F32 * (np.abs(t) + t_error) @ np.abs(b).T)
+        return y, bound + HALF * (np.abs(y) + bound) + F32 * np.abs(y)
+
+
+def adapter_rows(g, at, count, max_rank):
+    h = g.lib.h3_hip_adapter_rows_new(g.handle, u32(at), len(at), count, max_rank)
+    return Plan(g, h, g.lib.h3_hip_adapter_rows_free)
+
+
+def row_map(rows, count, seed, none=True, mixed=True):
+    rng = np.random.RandomState(seed)
+    at = np.sort(rng.randint(0, count + (1 if none else 0), rows))
+    return rng.permutation(at) if mixed else at
+
+
+def check_adapters(g, rows, k, n, ranks, at=None, seed=1, in_place=False, max_rank=None):
+    at = row_map(rows, len(ranks), seed) if at is None else np.asarray(at)
+    x, base = normal(rows * k, seed + 50).reshape(rows, k), normal(rows * n, seed + 51).reshape(rows, n)
+    w = Adapters(g, ranks, k, n, seed=seed)
+    mark = normal((rows + 2) * n, seed + 52)
+    if in_place:
+        mark[:rows * n] = base.reshape(-1)
+    tx, tb, out = g.from_bf16(x), g.from_bf16(base), g.from_bf16(mark)
+    with adapter_rows(g, at, len(ranks), max_rank or max(ranks)) as plan:
+        g.begin()
+        g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, out.handle, out.handle if in_place else tb.handle, tx.handle, w.handle,
+                                               plan, rows, k, n), "adapters")
+        g.submit()
+    got = out.read()
+    assert np.array_equal(got[rows * n:], mark[rows * n:])
+    got = got[:rows * n].reshape(rows, n)
+    none = at >= len(ranks)
+    assert np.array_equal(got[none], base[none])
+    fb = bf16(base).astype(np.float64)
+    want, bound = w.reference(bf16(x).astype(np.float64), at, fb, np.zeros_like(fb))
+    within(bf16(got[~none]), want[~none], bound[~none], (rows, k, n, ranks))
+    w.close()
+    for t in (tx, tb, out):
+        g.free(t)
+    return got
+
+
+@pytest.mark.parametrize("rows,k,n,ranks", [
+    (1, 64, 128, [16]), (1, 1, 1, [1]), (9, 256, 640, [16] * 8 + [64]), (31, 1001, 777, [1, 40, 7, 19]), (33, 72, 136, [33]),
+    (64, 128, 1000, [32, 31]), (300, 136, 264, [128, 4, 65]), (130, 520, 1032, [256, 200, 96]), (1000, 64, 64, [8, 8, 8]),
+    (5, 5376, 96, [16, 3]), (70, 2056, 516, [64]), (257, 500, 130, [17, 128]),
+])
+def test_adapters(rows, k, n, ranks):
+    print(f"[adapters] {rows}x{k}x{n} {ranks}", flush=True)
+    with Gpu() as g:
+        first = check_adapters(g, rows, k, n, ranks, seed=rows + n)
+        assert np.array_equal(check_adapters(g, rows, k, n, ranks, seed=rows + n, in_place=True, max_rank=256), first)
+
+
+def test_adapters_of_rows_in_runs_and_of_no_row():
+    with Gpu() as g:
+        check_adapters(g, 100, 64, 192, [16, 32, 8], at=np.repeat([0, 2, 3], [40, 33, 27]))
+        check_adapters(g, 100, 64, 192, [16, 32], at=[2] * 100)                    # none: base as it is
+        check_adapters(g, 3, 64, 192, [16, 32], at=[0xffffffff, 1, 7])             # any index past the last is none
+
+
+def test_adapters_are_replaced_and_start_as_zero():
+    rows, k, n = 40, 96, 200
+    with Gpu() as g:
+        x, base = normal(rows * k, 1).reshape(rows, k), normal(rows * n, 2).reshape(rows, n)
+        tx, tb, out = g.from_bf16(x), g.from_bf16(base), g.empty(rows * n)
+        w = Adapters(g, [8, 24], k, n)
+        fresh = g.check(g.lib.h3_hip_adapters_new(g.handle, u32([8, 24]), 2, k, n))
+        at = row_map(rows, 2, 3)
+        with adapter_rows(g, at, 2, 24) as plan:
+            def call(handle):
+                g.begin()
+                g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, out.handle, tb.handle, tx.handle, handle, plan, rows, k, n))
+                g.submit()
+                return out.read().reshape(rows, n)
+
+            assert np.array_equal(call(fresh), base)
+            first = call(w.handle)
+            w.set(1, a=normal(24 * k, 70, scale=0.1).reshape(24, k), scale=-1.25)
+            second = call(w.handle)
+            assert np.array_equal(first[at != 1], second[at != 1]) and not np.array_equal(first[at == 1], second[at == 1])
+            fb = bf16(base).astype(np.float64)
+            want, bound = w.reference(bf16(x).astype(np.float64), at, fb, np.zeros_like(fb))
+            within(bf16(second), want, bound)
+        g.lib.h3_hip_adapters_free(fresh)
+        w.close()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q8", "fp8_block"])
+@pytest.mark.parametrize("rows", [1, 70, 300])
+def test_linear_with_adapters_is_the_projection_and_the_adapters(kind, rows):
+    """Beside a projection of any type: the same bits as the two calls."""
+    k, n, ranks = 512, 1024, [16, 48]
+    with Gpu() as g:
+        x = normal(rows * k, 1)
+        tx, bias, out, base, sum_ = g.from_bf16(x), g.from_bf16(normal(n, 5)), g.empty(rows * n), g.empty(rows * n), g.empty(rows * n)
+        bits = normal(n * k, 2, scale=1 / math.sqrt(k))
+        if kind == "bf16":
+            w = g.from_bf16(bits).handle
+        elif kind == "q8":
+            codes = np.random.RandomState(1).randint(-127, 128, (n, k)).astype(np.int8)
+            scales = np.full((n, 1), 4e-4, np.float32)
+            w = g.check(g.lib.h3_hip_q8_from_packed(g.handle, codes.ctypes.data, scales.ctypes.data, n, k, k))
+        else:
+            w = g.check(g.lib.h3_hip_fp8_block_weight_from_bf16(g.handle, g.from_bf16(bits).handle, n, k))
+        at = row_map(rows, 2, 3)
+        ad = Adapters(g, ranks, k, n)
+        with adapter_rows(g, at, 2, 48) as plan:
+            g.begin()
+            g.check(g.lib.h3_hip_linear_adapters_bf16(g.handle, out.handle, tx.handle, w, bias.handle, ad.handle, plan, rows, k, n))
+            g.check(g.lib.h3_gpu_linear_bf16(g.handle, base.handle, tx.handle, w, bias.handle, rows, k, n))
+            g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, sum_.handle, base.handle, tx.handle, ad.handle, plan, rows, k, n))
+            g.submit()
+        got = out.read()
+        assert np.array_equal(got, sum_.read())
+        fb = bf16(base.read()).astype(np.float64).reshape(rows, n)
+        want, bound = ad.reference(bf16(x).astype(np.float64).reshape(rows, k), at, fb, np.zeros_like(fb))
+        within(bf16(got).reshape(rows, n), want, bound)
+        ad.close()
+        if kind != "bf16":
+            g.lib.h3_gpu_tensor_free(w)
+
+
+# ------------------------------------------------------------------ refusals
+def refused(g, ok, text):
+    assert not ok
+    assert text in g.error(), g.error()
+
+
+def test_refusals():
+    with Gpu() as g, Gpu() as other:
+        lib = g.lib
+        # Plans.
+        for ends, heads, kv in (([0, 4], 3, 2), ([0, 4], 0, 1), ([0, 4], 4, 0), ([4, 3], 1, 1), ([0, 4], 65536, 1)):
+            refused(g, lib.h3_hip_sequences_new(g.handle, u32(ends), None, 1, heads, kv), "sequences")
+        refused(g, lib.h3_hip_sequences_new(g.handle, u32([0, 4]), u32([5, 4]), 1, 1, 1), "fall")
+        refused(g, lib.h3_hip_sequences_new(g.handle, u32([0]), None, 0, 1, 1), "sequences")
+        refused(g, lib.h3_hip_sequences_new(g.handle, u32([0, 2 ** 32 - 1]), None, 1, 1, 1), "longer")
+        f = (C.c_double * 2)(1.0, 0.5)
+        for args in ((f, u32([0, 1]), 0, 2, 0), (f, u32([0, 1]), 129, 2, 0), (f, u32([0, 1]), 2, 0, 0), (f, u32([0, 1]), 2, 17, 0),
+                     (f, u32([0, 1]), 2, 2, 2), (None, u32([0, 1]), 2, 2, 0), (f, None, 2, 2, 0), (f, u32([0, 2]), 2, 2, 0),
+                     ((C.c_double * 2)(1.0, math.inf), u32([0, 1]), 2, 2, 0), ((C.c_double * 2)(math.nan, 1.0), u32([0, 1]), 2, 2, 0)):
+            refused(g, lib.h3_hip_rope_axes_new(g.handle, *args), "RoPE axes")
+        for ranks, k, n in (([], 8, 8), ([0], 8, 8), ([257], 8, 8), ([4], 0, 8), ([4], 8, 0), ([4], 2 ** 24 + 1, 8)):
+            refused(g, lib.h3_hip_adapters_new(g.handle, u32(ranks), len(ranks), k, n), "adapters")
+        for at, count, rank in (([], 1, 8), ([0], 0, 8), ([0], 1, 0), ([0], 1, 257)):
+            refused(g, lib.h3_hip_adapter_rows_new(g.handle, u32(at), len(at), count, rank), "adapter rows")
+
+        q, small, f32, foreign = g.empty(8 * 256), g.empty(100), g.empty(8 * 256, F32_TENSOR), other.empty(8 * 256)
+        k, v, out, qkv = g.empty(8 * 256), g.empty(8 * 256), g.empty(8 * 256), g.empty(8 * 3 * 256)
+        plan = lib.h3_hip_sequences_new(g.handle, u32([0, 3, 8]), None, 2, 2, 2)
+        theirs = lib.h3_hip_sequences_new(other.handle, u32([0, 3, 8]), None, 2, 2, 2)
+
+        def attend(o=out, a=q, b=k, c=v, p=plan, scale=1.0):
+            return lib.h3_hip_sdpa_sequences_bf16(g.handle, *(t.handle if t else None for t in (o, a, b, c)), p, C.c_float(scale))
+
+        refused(g, attend(), "no active")
+        g.begin()
+        for bad, text in ((dict(p=None), "plan"), (dict(p=theirs), "context"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
+                          (dict(o=q), "disjoint"), (dict(o=k), "disjoint"), (dict(o=None), "disjoint"), (dict(a=small), "need"),
+                          (dict(b=small), "need"), (dict(c=f32), "dtype"), (dict(o=foreign), "another context"), (dict(a=None), "missing")):
+            refused(g, attend(**bad), text)
+
+        rope = lib.h3_hip_rope_axes_new(g.handle, f, u32([0, 1]), 2, 2, 0)
+        pos, w = g.empty(16, F32_TENSOR), g.empty(128)
+
+        def turn(o=(q, k, v), x=qkv, qw=w, kw=w, r=rope, p=pos, rows=8, heads=2, kv=2, dim=128, grouped=0, eps=EPS):
+            return lib.h3_hip_qkv_rope_axes_bf16(g.handle, *(t.handle for t in o), x.handle, qw and qw.handle, kw and kw.handle, r,
+                                                 p.handle, rows, heads, kv, dim, grouped, C.c_float(eps))
+
+        for bad, text in ((dict(r=None), "axes"), (dict(rows=0), "rows"), (dict(heads=3), "heads"), (dict(kv=0), "heads"),
+                          (dict(dim=257), "dim"), (dict(dim=3), "pairs"), (dict(qw=None), "norm"), (dict(grouped=2), "grouped"),
+                          (dict(eps=-1.0), "eps"), (dict(eps=math.nan), "eps"), (dict(o=(q, q, v)), "disjoint"),
+                          (dict(o=(qkv, k, v)), "disjoint"), (dict(p=f32, x=small), "need"), (dict(p=w), "dtype"), (dict(rows=9), "need"),
+                          (dict(qw=small, kw=small), "need")):
+            refused(g, turn(**bad), text)
+
+        ad = lib.h3_hip_adapters_new(g.handle, u32([4, 40]), 2, 16, 32)
+        rows = lib.h3_hip_adapter_rows_new(g.handle, u32([0, 1, 2]), 3, 2, 40)
+        low = lib.h3_hip_adapter_rows_new(g.handle, u32([0, 1, 2]), 3, 2, 8)
+        x, base = g.empty(48), g.empty(96)
+        for index, a, b, scale, text in ((2, q, q, 1.0, "index"), (0, q, q, math.inf, "finite"), (1, small, q, 1.0, "need"),
+                                         (0, q, f32, 1.0, "dtype")):
+            refused(g, lib.h3_hip_adapters_set(g.handle, ad, index, a.handle, b.handle, C.c_float(scale)), text)
+
+        def adapt(o=out, b=base, i=x, a=ad, p=rows, m=3, k=16, n=32):
+            return lib.h3_hip_adapters_add_bf16(g.handle, o.handle, b.handle, i.handle, a, p, m, k, n)
+
+        for bad, text in ((dict(a=None), "missing"), (dict(p=None), "missing"), (dict(m=4), "need"), (dict(k=8), "need"),
+                          (dict(n=33), "need"), (dict(p=low), "rank"), (dict(o=x), "need"), (dict(i=small, o=small), "aliases"),
+                          (dict(b=f32), "dtype"), (dict(i=foreign), "another context")):
+            refused(g, adapt(**bad), text)
+        refused(g, lib.h3_hip_linear_adapters_bf16(g.handle, out.handle, x.handle, None, None, ad, rows, 3, 16, 32), "weight")
+        g.submit()
+        lib.h3_hip_sequences_free(plan)
+        lib.h3_hip_sequences_free(theirs)
+        lib.h3_hip_rope_axes_free(rope)
+        lib.h3_hip_adapters_free(ad)
+        lib.h3_hip_adapter_rows_free(rows)
+        lib.h3_hip_adapter_rows_free(low)
+
+
+def test_no_context():
+    from h3cli_amd import _lib
+    lib = _lib.load()
+    assert not lib.h3_hip_sequences_new(None, u32([0, 1]), None, 1, 1, 1)
+    assert not lib.h3_hip_sdpa_sequences_bf16(None, None, None, None, None, None, C.c_float(1))
+    assert not lib.h3_hip_rope_axes_new(None, None, None, 1, 1, 0)
+    assert not lib.h3_hip_adapters_new(None, u32([1]), 1, 1, 1)
+    assert not lib.h3_hip_adapter_rows_new(None, u32([0]), 1, 1, 1)
+    assert not lib.h3_hip_linear_adapters_bf16(None, None, None, None, None, None, None, 1, 1, 1)
+    for free in (lib.h3_hip_sequences_free, lib.h3_hip_rope_axes_free, lib.h3_hip_adapters_free, lib.h3_hip_adapter_rows_free):
+        free(None)
