@@ -172,6 +172,7 @@ _SIGNATURES.update({
     # several requests in one step
     "h3_hip_sequences_new": (_p, [_p, _p, _p, _u32, _u32, _u32]),
     "h3_hip_sequences_free": (None, [_p]),
+    "h3_hip_sequences_layout": (_i, [_p, _p, _u32, _u32, _u32, C.POINTER(_sz)]),
     "h3_hip_sdpa_sequences_bf16": (_i, [_p, _p, _p, _p, _p, _p, _f]),
     "h3_hip_rope_axes_new": (_p, [_p, _p, _p, _u32, _u32, _i]),
     "h3_hip_rope_axes_free": (None, [_p]),

@@ -85,7 +85,46 @@ struct Args {
     // K and V^T fit 32-bit buffer offsets (below 4 GiB each): the dense
     // kernels then load tiles with buffer loads.
     int buffered;
+    // Packed sequences (kernels with SEQ): their table, the blocks of rows, and the query
+    // heads, `share` of them a key head; seq, heads, padded, qrows and the pointers above are then
+    // set per workgroup (enter_sequence), heads to the key heads.
+    const h3_sequence *sequences;
+    const h3_sequence_item *items;
+    unsigned item_count, q_heads, share;
 };
+
+// A workgroup's key head, block of rows and retry bytes; SEQ: those of its item, with `a` set to the
+// item's sequence as if it were alone.
+template <bool SEQ> __device__ inline void enter_sequence(Args &a, unsigned BM, unsigned &head, unsigned &qb, size_t &retry_at) {
+    const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
+    if constexpr (SEQ) {
+        head = __builtin_amdgcn_readfirstlane(id / a.item_count);
+        const unsigned i = __builtin_amdgcn_readfirstlane(id % a.item_count);
+        const h3_sequence_item item = a.items[i];
+        qb = __builtin_amdgcn_readfirstlane(item.block);
+        const h3_sequence *s = a.sequences + __builtin_amdgcn_readfirstlane(item.sequence);
+        a.seq = __builtin_amdgcn_readfirstlane(s->lk);
+        a.qrows = __builtin_amdgcn_readfirstlane(s->lq) * a.share;
+        a.padded = (a.seq + BN - 1) / BN * BN;
+        const size_t q0 = (size_t)__builtin_amdgcn_readfirstlane(s->q0) * a.q_heads * D;
+        a.q += q0;
+        a.out += q0;
+        a.k += (size_t)__builtin_amdgcn_readfirstlane(s->k0) * a.heads * D;
+        a.vt += (size_t)__builtin_amdgcn_readfirstlane((unsigned)s->vt) |
+                (size_t)__builtin_amdgcn_readfirstlane((unsigned)(s->vt >> 32)) << 32;
+        retry_at = (size_t)head * a.item_count + i;
+    } else {
+        const unsigned nqb = ((a.qrows ? a.qrows : a.seq) + BM - 1) / BM;
+        head = __builtin_amdgcn_readfirstlane(id / nqb);
+        qb = __builtin_amdgcn_readfirstlane(id % nqb);
+        retry_at = (size_t)head * nqb + qb;
+    }
+}
+// Where row v of a key head has its query and, sequence-major, its output.
+template <bool SEQ> __device__ inline size_t query_at(const Args &a, unsigned head, unsigned v) {
+    if constexpr (SEQ) return ((size_t)(v / a.share) * a.q_heads + head * a.share + v % a.share) * D;
+    return ((size_t)v * a.heads + head) * D;
+}
 
 // Whether K [seq, heads, 128] and V^T [heads, 128, padded] both fit 32-bit
 // buffer offsets.
@@ -103,10 +142,10 @@ __host__ __device__ inline unsigned v_position(unsigned j) {
 
 // V [seq, heads, 128] -> Vt [heads, 128, padded]; one workgroup per (64-key tile,
 // head). The pass also screens this tile's K and V rows for Inf/NaN.
-__global__ __launch_bounds__(256) void transpose_v(const uint16_t *v, const uint16_t *k, uint16_t *vt, unsigned seq,
-                                                  unsigned heads, unsigned padded, unsigned *fault) {
+__device__ inline void transpose_tile(const uint16_t *v, const uint16_t *k, uint16_t *vt, unsigned seq, unsigned heads,
+                                      unsigned padded, unsigned blk, unsigned head, unsigned *fault) {
     __shared__ uint16_t tile[BN][D + 8];
-    const unsigned blk = blockIdx.x, head = blockIdx.y, t = threadIdx.x;
+    const unsigned t = threadIdx.x;
     const size_t stride = (size_t)heads * D;
     bool bad = false;
 #pragma unroll
@@ -133,6 +172,22 @@ __global__ __launch_bounds__(256) void transpose_v(const uint16_t *v, const uint
     uint16_t *dst = vt + ((size_t)head * D + d) * padded + blk * BN + half * 32;
 #pragma unroll
     for (int j = 0; j < 4; j++) *reinterpret_cast<u16x8 *>(dst + j * 8) = w[j];
+}
+
+__global__ __launch_bounds__(256) void transpose_v(const uint16_t *v, const uint16_t *k, uint16_t *vt, unsigned seq,
+                                                  unsigned heads, unsigned padded, unsigned *fault) {
+    transpose_tile(v, k, vt, seq, heads, padded, blockIdx.x, blockIdx.y, fault);
+}
+
+// The same for the 64-key blocks of packed sequences.
+__global__ __launch_bounds__(256) void transpose_sequences(const uint16_t *v, const uint16_t *k, uint16_t *vt,
+                                                          const h3_sequence *sequences, const h3_sequence_item *items,
+                                                          unsigned heads, unsigned *fault) {
+    const unsigned head = blockIdx.x % heads;
+    const h3_sequence_item item = items[blockIdx.x / heads];
+    const h3_sequence s = sequences[item.sequence];
+    const size_t k0 = (size_t)s.k0 * heads * D;
+    transpose_tile(v + k0, k + k0, vt + s.vt, s.lk, heads, (s.lk + BN - 1) / BN * BN, item.block, head, fault);
 }
 
 // WAVES wavefronts per workgroup, each owning NB x 32 queries; OCC waves share a
@@ -389,7 +444,7 @@ int launch(h3_gpu *g, const Args &a, unsigned groups) {
 // Wide tiles: each barrier interval covers KT consecutive 64-key sub-tiles, so
 // the per-interval fixed costs (the barrier, the load wait and the serial
 // max / ballot chain) are paid once per KT * 64 keys.
-template <int KT, bool SPARSE, bool MSUM, bool NOMAX, int WAVES = 8>
+template <int KT, bool SPARSE, bool MSUM, bool NOMAX, int WAVES = 8, bool SEQ = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * WAVES, 64 * WAVES), amdgpu_waves_per_eu(2, 2)))
 void attn_bf16_wide(Args a) {
     static_assert(!(NOMAX && MSUM), "the overflow test reads the VALU row sums");
@@ -403,12 +458,12 @@ void attn_bf16_wide(Args a) {
     // buffer offsets stay scalar.
     const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     const unsigned n = lane % 32, hf = lane / 32;
+    unsigned head, qb;
+    size_t retry_at;
+    enter_sequence<SEQ>(a, BM, head, qb, retry_at);
     const unsigned qrows = a.qrows ? a.qrows : a.seq;
-    const unsigned nqb = (qrows + BM - 1) / BM;
-    const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
-    const unsigned head = __builtin_amdgcn_readfirstlane(id / nqb), qb = __builtin_amdgcn_readfirstlane(id % nqb);
     const unsigned q0 = qb * BM;
-    uint8_t *const retry = a.retry ? a.retry + ((size_t)head * nqb + qb) * WAVES : nullptr;
+    uint8_t *const retry = a.retry ? a.retry + retry_at * WAVES : nullptr;
     // The recomputation launch runs only the workgroups the fast kernel flagged.
     if constexpr (!NOMAX) {
         if constexpr (WAVES == 8) {
@@ -418,7 +473,6 @@ void attn_bf16_wide(Args a) {
         }
     }
     const size_t stride = (size_t)a.heads * D;
-    const uint16_t *qh = a.q + (size_t)head * D;
     const uint16_t *kh = a.k + (size_t)head * D;
     const uint16_t *vth = a.vt + (size_t)head * D * a.padded;
     const float c = a.scale_log2;
@@ -438,7 +492,7 @@ void attn_bf16_wide(Args a) {
     {
         unsigned row = q0 + wave * 32 + n;
         row = row < qrows ? row : qrows - 1;
-        const uint16_t *p = qh + (size_t)row * stride + hf * 8;
+        const uint16_t *p = a.q + query_at<SEQ>(a, head, row) + hf * 8;
         bool bad = false;
 #pragma unroll
         for (int ks = 0; ks < 8; ks++) {
@@ -698,7 +752,7 @@ void attn_bf16_wide(Args a) {
     const unsigned q = q0 + wave * 32 + n;
     bool bad = false;
     if (q < qrows) {
-        uint16_t *dst = a.out + (a.head_major ? ((size_t)head * a.seq + q) * D : ((size_t)q * a.heads + head) * D);
+        uint16_t *dst = a.out + (a.head_major ? ((size_t)head * a.seq + q) * D : query_at<SEQ>(a, head, q));
 #pragma unroll
         for (int md = 0; md < 4; md++)
 #pragma unroll
@@ -728,11 +782,11 @@ void attn_bf16_wide(Args a) {
     if (a.lse && hf == 0 && q < qrows) a.lse[(size_t)head * qrows + q] = (m + log2f(total)) * 0.6931471805599453f;
 }
 
-template <int KT, bool SPARSE, bool MSUM, bool NOMAX, int WAVES = 8>
+template <int KT, bool SPARSE, bool MSUM, bool NOMAX, int WAVES = 8, bool SEQ = false>
 int configure_wide(h3_gpu *g) {
     static bool configured = false;
     if (!configured) {
-        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)attn_bf16_wide<KT, SPARSE, MSUM, NOMAX, WAVES>,
+        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)attn_bf16_wide<KT, SPARSE, MSUM, NOMAX, WAVES, SEQ>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * KT * STAGE_BYTES)),
                           "attention shared memory"))
             return 0;
@@ -1036,19 +1090,19 @@ constexpr int PIPE_STAGE = 2 * (K_BYTES + V_BYTES);   // 64 KB: two 64-key tiles
     AP_CL10(a, 11), "a120", "a121", "a122", "a123", "a124", "a125", "a126", "a127",                               \
     "m0", "vcc", "scc", "memory"
 
+template <bool SEQ>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1)))
 void attn_bf16_pipe(Args a) {
     constexpr int WAVES = 4, BM = 256;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
     const unsigned n = lane % 32, hf = lane / 32;
-    const unsigned nqb = (a.seq + BM - 1) / BM;
-    const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
-    const unsigned head = __builtin_amdgcn_readfirstlane(id / nqb), qb = __builtin_amdgcn_readfirstlane(id % nqb);
-    const unsigned q0 = qb * BM;
-    uint8_t *const retry = a.retry + ((size_t)head * nqb + qb) * 8;
+    unsigned head, qb;
+    size_t retry_at;
+    enter_sequence<SEQ>(a, BM, head, qb, retry_at);
+    const unsigned rows = SEQ ? a.qrows : a.seq, q0 = qb * BM;
+    uint8_t *const retry = a.retry + retry_at * 8;
     const size_t stride = (size_t)a.heads * D;
-    const uint16_t *qh = a.q + (size_t)head * D;
     const float c = a.scale_log2;
     const unsigned count = (a.seq + BN - 1) / BN;        // 64-key tiles
     const unsigned groups = (count + 1) / 2;             // the launcher ensures groups >= 3
@@ -1060,8 +1114,8 @@ void attn_bf16_pipe(Args a) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             unsigned row = q0 + wave * 64 + b * 32 + n;
-            row = row < a.seq ? row : a.seq - 1;
-            const uint16_t *p = qh + (size_t)row * stride + hf * 8;
+            row = row < rows ? row : rows - 1;
+            const uint16_t *p = a.q + query_at<SEQ>(a, head, row) + hf * 8;
 #pragma unroll
             for (int ks = 0; ks < 8; ks++) {
                 qf[b][ks] = *reinterpret_cast<const bf16x8 *>(p + ks * 16);
@@ -1218,8 +1272,8 @@ void attn_bf16_pipe(Args a) {
         const float inv = total > 0.f ? 1.f / total : 0.f;
         const unsigned q = q0 + wave * 64 + b * 32 + n;
         bool bad = false;
-        if (q < a.seq) {
-            uint16_t *dst = a.out + (a.head_major ? ((size_t)head * a.seq + q) * D : ((size_t)q * a.heads + head) * D);
+        if (q < rows) {
+            uint16_t *dst = a.out + (a.head_major ? ((size_t)head * a.seq + q) * D : query_at<SEQ>(a, head, q));
 #pragma unroll
             for (int md = 0; md < 4; md++)
 #pragma unroll
@@ -1240,27 +1294,27 @@ void attn_bf16_pipe(Args a) {
     }
 }
 
-int launch_pipe_attention(h3_gpu *g, const Args &a) {
+template <bool SEQ> int launch_pipe_attention(h3_gpu *g, const Args &a) {
     constexpr size_t shared = 2 * PIPE_STAGE;
     static bool configured = false;
     if (!configured) {
-        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)attn_bf16_pipe, hipFuncAttributeMaxDynamicSharedMemorySize,
+        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)attn_bf16_pipe<SEQ>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                  (int)shared), "attention shared memory"))
             return 0;
         configured = true;
     }
-    if (!configure_wide<2, false, false, false, 8>(g)) return 0;
-    const unsigned groups = (a.seq + 255) / 256 * a.heads;
+    if (!configure_wide<2, false, false, false, 8, SEQ>(g)) return 0;
+    const unsigned groups = SEQ ? a.item_count * a.heads : (a.seq + 255) / 256 * a.heads;
     h3_note_kernel(g, "attn_bf16_pipe");
     hipEvent_t timing = h3_kernel_timing_begin(g);
-    hipLaunchKernelGGL(attn_bf16_pipe, dim3(groups), dim3(256), shared, g->compute, a);
+    hipLaunchKernelGGL(attn_bf16_pipe<SEQ>, dim3(groups), dim3(256), shared, g->compute, a);
     if (!h3_launch_status(g, "BF16 attention")) {
         h3_kernel_timing_end(g, timing);
         return 0;
     }
     // The recomputation launch: the wide kernel with a per-tile max over the
     // 32-query blocks flagged above (same retry bytes, 256 queries per workgroup).
-    hipLaunchKernelGGL((attn_bf16_wide<2, false, false, false, 8>), dim3(groups), dim3(512), 2 * 2 * STAGE_BYTES,
+    hipLaunchKernelGGL((attn_bf16_wide<2, false, false, false, 8, SEQ>), dim3(groups), dim3(512), 2 * 2 * STAGE_BYTES,
                        g->compute, a);
     h3_kernel_timing_end(g, timing);
     return h3_launch_status(g, "BF16 attention");
@@ -1965,8 +2019,24 @@ int h3_launch_attention_bf16(h3_gpu *g, void *workspace, uint16_t *out, const ui
     if (g->attention_variant == 9 && a.buffered) return launch_pingpong<1>(g, a, (seq + 255) / 256 * heads);
     // The hand-scheduled kernel needs at least three 128-key groups; variant
     // 14 keeps the wide kernel.
-    if (a.buffered && seq > 256 && g->attention_variant != 14) return launch_pipe_attention(g, a);
+    if (a.buffered && seq > 256 && g->attention_variant != 14) return launch_pipe_attention<false>(g, a);
     return launch_wide<2, false, false, true>(g, a, (seq + 255) / 256 * heads);
+}
+
+int h3_launch_attention_sequence_tiles(h3_gpu *g, uint16_t *out, const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                                       const h3_sequence_tiles &t, float scale) {
+    Args a{};
+    a.out = out; a.q = q; a.k = k; a.vt = t.vt;
+    a.heads = t.kv_heads;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.fault = g->fault;
+    a.retry = t.retry;
+    a.buffered = 1;
+    a.sequences = t.sequences; a.items = t.items;
+    a.item_count = t.count; a.q_heads = t.heads; a.share = t.heads / t.kv_heads;
+    hipLaunchKernelGGL(transpose_sequences, dim3(t.key_count * t.kv_heads), dim3(256), 0, g->compute, v, k, t.vt, t.sequences,
+                       t.key_items, t.kv_heads, g->fault);
+    return h3_launch_status(g, "V transpose") && launch_pipe_attention<true>(g, a);
 }
 
 // Dense attention of query rows [first, first + qrows) (q and out already

@@ -18,22 +18,46 @@ namespace {
 
 constexpr int D = 128, BN = 64, TILE = BN * D * 2, WAVES = 4;
 constexpr float RESCALE_SLACK = 8.0f;
+constexpr uint32_t WHOLE = UINT32_MAX, PARTS_MOST = 128;
+constexpr size_t PART_FLOATS = 32 * (D + 2);   // of 32 rows: O, the running max and the sum
 
-struct Sequence {
-    uint32_t q0, lq, k0, lk;
+// A workgroup's share: 32 rows of a sequence and its key tiles [first, last); part: where its
+// partial result goes, WHOLE if it has all tiles.
+struct RowItem {
+    uint32_t sequence, block, first, last, part;
 };
-// A workgroup's share: a block of rows of a sequence.
-struct Item {
-    uint32_t sequence, block;
+// 32 rows whose tiles were shared out to parts [part, part + parts).
+struct JoinItem {
+    uint32_t sequence, block, part, parts;
+};
+
+// What a call does, made on the host.
+struct Plan {
+    std::vector<h3_sequence> sequences;
+    std::vector<h3_sequence_item> tiles, keys;   // by the 256-row tile kernel
+    std::vector<RowItem> rows;                   // by the kernel here
+    std::vector<JoinItem> joins;
+    uint64_t vt = 0;                             // elements of transposed V
+    uint32_t parts = 0;
+    size_t table_bytes() const {
+        return sequences.size() * sizeof(h3_sequence) + (tiles.size() + keys.size()) * sizeof(h3_sequence_item) +
+               rows.size() * sizeof(RowItem) + joins.size() * sizeof(JoinItem);
+    }
+    size_t retry_at() const { return (vt * 2 + 255) / 256 * 256; }
+    size_t parts_at(uint32_t kv_heads) const { return (retry_at() + tiles.size() * kv_heads * 8 + 255) / 256 * 256; }
+    size_t workspace_bytes(uint32_t kv_heads) const { return parts_at(kv_heads) + (size_t)parts * kv_heads * PART_FLOATS * 4; }
 };
 
 }  // namespace
 
 struct h3_hip_sequences {
     h3_gpu *owner;
-    uint32_t heads, kv_heads, count, items;
+    uint32_t heads, kv_heads, count;
+    uint32_t tiles, keys, rows, joins;
     uint64_t q_rows, k_rows;      // rows that the tensors must hold
-    h3_gpu_tensor *table;         // u32: Sequence [count], Item [items]
+    size_t retry_at, parts_at;
+    h3_gpu_tensor *table;         // h3_sequence, tiles, keys, rows, joins, behind one another
+    h3_gpu_tensor *workspace;     // transposed V, retry bytes, partial results
 };
 
 namespace {
@@ -41,9 +65,11 @@ namespace {
 struct SeqArgs {
     uint16_t *out;
     const uint16_t *q, *k, *v;
-    const Sequence *sequences;
-    const Item *items;
-    unsigned count, heads, kv_heads, share;
+    const h3_sequence *sequences;
+    const RowItem *items;
+    const JoinItem *joins;
+    float *partial;
+    unsigned count, join_count, heads, kv_heads, share;
     float scale_log2;
     unsigned *fault;
 };
@@ -73,12 +99,13 @@ void attn_sequences(SeqArgs a) {
     const unsigned n = lane % 32, hf = lane / 32;
     const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
     const unsigned kv = __builtin_amdgcn_readfirstlane(id / a.count);
-    const Item item = a.items[__builtin_amdgcn_readfirstlane(id % a.count)];
-    const Sequence s = a.sequences[item.sequence];
+    const RowItem item = a.items[__builtin_amdgcn_readfirstlane(id % a.count)];
+    const h3_sequence s = a.sequences[item.sequence];
     const unsigned lq = __builtin_amdgcn_readfirstlane(s.lq), lk = __builtin_amdgcn_readfirstlane(s.lk);
     const unsigned q0 = __builtin_amdgcn_readfirstlane(s.q0), k0 = __builtin_amdgcn_readfirstlane(s.k0);
     const unsigned block = __builtin_amdgcn_readfirstlane(item.block);
-    const unsigned rows = lq * a.share, blocks = (rows + 31) / 32, count = (lk + BN - 1) / BN;
+    const unsigned part = __builtin_amdgcn_readfirstlane(item.part);
+    const unsigned rows = lq * a.share, blocks = (rows + 31) / 32, count = __builtin_amdgcn_readfirstlane(item.last);
     const size_t kstride = (size_t)a.kv_heads * D * 2;   // bytes
     const float c = a.scale_log2;
     uint8_t *const kt = smem + wave * 2 * TILE, *const vt = kt + TILE;
@@ -124,7 +151,7 @@ void attn_sequences(SeqArgs a) {
     const size_t qrow = ((size_t)q0 + vrow_id / a.share) * a.heads + kv * a.share + vrow_id % a.share;
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) qf[ks] = *reinterpret_cast<const bf16x8 *>(a.q + qrow * D + hf * 8 + ks * 16);
-    unsigned t = wave;
+    unsigned t = __builtin_amdgcn_readfirstlane(item.first) + wave;
     if (t < count) {
         load(a.k, kt, t);
         load(a.v, vt, t);
@@ -247,6 +274,28 @@ void attn_sequences(SeqArgs a) {
     float total = lpart[0][n];
 #pragma unroll
     for (int w = 1; w < WAVES; w++) total += lpart[w][n];
+    if (part != WHOLE) {
+        // The sums over this part's tiles, with their maximum, for attn_sequences_join.
+        float *const mine = a.partial + ((size_t)part * a.kv_heads + kv) * PART_FLOATS;
+        if (block * 32 + n < rows)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                f32x4 x{};
+#pragma unroll
+                for (int w = 0; w < WAVES; w++)
+                    x += *reinterpret_cast<const f32x4 *>(smem + w * 2 * TILE + ((wave * 4 + g) * 64 + lane) * 16);
+                *reinterpret_cast<f32x4 *>(mine + n * D + wave * 32 + g * 8 + hf * 4) = x;
+            }
+        if (wave == 0 && hf == 0) {
+            float top = mpart[0][n];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) top = fmaxf(top, mpart[w][n]);
+            mine[32 * D + n] = top;
+            mine[32 * D + 32 + n] = total;
+        }
+        if (worst >= 0x7f800000u) a.fault[0] = 1u;
+        return;
+    }
     const float inv = total > 0.f ? 1.f / total : 0.f;
     uint16_t *dst = a.out + qrow * D;
 #pragma unroll
@@ -267,6 +316,54 @@ void attn_sequences(SeqArgs a) {
     if (worst >= 0x7f800000u) a.fault[0] = 1u;
 }
 
+// 32 rows from their parts, in the parts' order: each brought to the common maximum.
+__global__ __launch_bounds__(256) void attn_sequences_join(SeqArgs a) {
+    __shared__ float weight[32][PARTS_MOST + 1];
+    const unsigned tid = threadIdx.x, kv = blockIdx.x % a.kv_heads;
+    const JoinItem item = a.joins[blockIdx.x / a.kv_heads];
+    const h3_sequence s = a.sequences[item.sequence];
+    const unsigned rows = min(32u, s.lq * a.share - item.block * 32);
+    const float *const first = a.partial + ((size_t)item.part * a.kv_heads + kv) * PART_FLOATS;
+    const size_t step = (size_t)a.kv_heads * PART_FLOATS;
+    {
+        const unsigned r = tid / 8;
+        float top = -INFINITY, total = 0.f;
+        for (unsigned p = tid % 8; p < item.parts; p += 8) top = fmaxf(top, first[p * step + 32 * D + r]);
+#pragma unroll
+        for (int off = 4; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+        for (unsigned p = tid % 8; p < item.parts; p += 8) {
+            const float w = exp2f_fast(first[p * step + 32 * D + r] - top);
+            weight[r][p] = w;
+            total = fmaf(w, first[p * step + 32 * D + 32 + r], total);
+        }
+#pragma unroll
+        for (int off = 4; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
+        if (tid % 8 == 0) weight[r][PARTS_MOST] = total > 0.f ? 1.f / total : 0.f;
+    }
+    __syncthreads();
+    unsigned worst = 0;
+    for (unsigned i = tid; i < rows * (D / 4); i += 256) {
+        const unsigned r = i / (D / 4), d = i % (D / 4) * 4, v = item.block * 32 + r;
+        f32x4 x{};
+#pragma unroll 4
+        for (unsigned p = 0; p < item.parts; p++) {
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(first + p * step + r * D + d);
+            const float w = weight[r][p];
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = fmaf(w, y[e], x[e]);
+        }
+        u16x4 out;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float y = x[e] * weight[r][PARTS_MOST];
+            worst = max(worst, __builtin_bit_cast(uint32_t, y) & 0x7f800000u);
+            out[e] = f32_to_bf16(y);
+        }
+        *reinterpret_cast<u16x4 *>(a.out + (((size_t)s.q0 + v / a.share) * a.heads + kv * a.share + v % a.share) * D + d) = out;
+    }
+    if (worst >= 0x7f800000u) a.fault[0] = 1u;
+}
+
 int launch(h3_gpu *g, const SeqArgs &a) {
     constexpr size_t shared = WAVES * 2 * TILE;
     static bool configured = false;
@@ -276,11 +373,88 @@ int launch(h3_gpu *g, const SeqArgs &a) {
             return 0;
         configured = true;
     }
-    h3_note_kernel(g, "attn_sequences");
+    h3_note_kernel(g, "attn_sequences", 32, a.join_count ? 2 : 1);
     hipEvent_t timing = h3_kernel_timing_begin(g);
     hipLaunchKernelGGL(attn_sequences, dim3(a.count * a.kv_heads), dim3(64 * WAVES), shared, g->compute, a);
     h3_kernel_timing_end(g, timing);
+    if (!h3_launch_status(g, "BF16 attention of sequences") || !a.join_count) return h3_launch_status(g, "BF16 attention of sequences");
+    hipLaunchKernelGGL(attn_sequences_join, dim3(a.join_count * a.kv_heads), dim3(256), 0, g->compute, a);
     return h3_launch_status(g, "BF16 attention of sequences");
+}
+
+// Microseconds of a workgroup: here 32 rows, each wave a 64-key tile in four; 256 rows by 128
+// keys in the tile kernel.
+double row_cost(uint64_t tiles) { return 6.0 + 2.2 * (double)((tiles + 3) / 4); }
+double tile_cost(uint64_t keys) { return 2.0 + 2.13 * (double)((keys + 127) / 128); }
+
+// Which sequences the tile kernel takes, and how the others' keys are shared out.
+const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_offsets, uint32_t count, uint32_t heads,
+                      uint32_t kv_heads, uint32_t cus) {
+    if (!q_offsets || !count || count > (1u << 20) || !kv_heads || !heads || heads > 65535 || heads % kv_heads)
+        return "need 1 to 2^20 of them and heads a multiple of the key heads";
+    if (!k_offsets) k_offsets = q_offsets;
+    const uint32_t share = heads / kv_heads;
+    for (uint32_t i = 0; i < count; i++) {
+        if (q_offsets[i + 1] < q_offsets[i] || k_offsets[i + 1] < k_offsets[i]) return "the offsets fall";
+        const uint64_t lq = q_offsets[i + 1] - q_offsets[i], lk = k_offsets[i + 1] - k_offsets[i];
+        if (lq * share >= (1u << 31) || lk >= (1u << 31)) return "a sequence is longer than 2^31 rows";
+        plan.sequences.push_back({q_offsets[i], (uint32_t)lq, k_offsets[i], (uint32_t)lk, 0});
+    }
+    // Long sequences first, where they begin: a short one then ends the call.
+    std::vector<uint32_t> order;
+    for (uint32_t i = 0; i < count; i++)
+        if (plan.sequences[i].lq) order.push_back(i);
+    std::stable_sort(order.begin(), order.end(), [&](uint32_t x, uint32_t y) { return plan.sequences[x].lk > plan.sequences[y].lk; });
+    auto blocks = [&](uint32_t i, uint32_t size) { return ((uint64_t)plan.sequences[i].lq * share + size - 1) / size; };
+    auto tiles = [&](uint32_t i) { return ((uint64_t)plan.sequences[i].lk + BN - 1) / BN; };
+    // The tile kernel takes the sequences with at least some number of rows: each number in turn, with
+    // the time of its kernels' workgroups over the compute units, or of the longest one.
+    std::vector<uint32_t> by_rows;
+    for (uint32_t i : order)
+        if (plan.sequences[i].lk > 256 && (uint64_t)plan.sequences[i].lk * kv_heads * D * 2 < (1ull << 32)) by_rows.push_back(i);
+    std::stable_sort(by_rows.begin(), by_rows.end(), [&](uint32_t x, uint32_t y) { return plan.sequences[x].lq > plan.sequences[y].lq; });
+    double rows_work = 0, tile_work = 0, tile_longest = 0;
+    for (uint32_t i : order) rows_work += (double)blocks(i, 32) * kv_heads * row_cost(tiles(i));
+    double best = rows_work / cus;
+    size_t taken = 0;
+    for (size_t j = 0; j < by_rows.size(); j++) {
+        const uint32_t i = by_rows[j];
+        rows_work -= (double)blocks(i, 32) * kv_heads * row_cost(tiles(i));
+        tile_work += (double)blocks(i, 256) * kv_heads * tile_cost(plan.sequences[i].lk);
+        tile_longest = std::max(tile_longest, tile_cost(plan.sequences[i].lk));
+        const double time = 15 + std::max(tile_work / cus, tile_longest) + rows_work / cus;
+        if (time < best) {
+            best = time;
+            taken = j + 1;
+        }
+    }
+    std::vector<bool> tiled(count, false);
+    for (size_t j = 0; j < taken; j++) tiled[by_rows[j]] = true;
+    uint64_t work = 0;   // key tiles of the others
+    for (uint32_t i : order)
+        if (!tiled[i]) work += blocks(i, 32) * kv_heads * tiles(i);
+    const uint64_t share_tiles = std::max<uint64_t>(16, (work + cus - 1) / cus);
+    for (uint32_t i : order) {
+        h3_sequence &s = plan.sequences[i];
+        // Launches hold fewer than 2^32 threads.
+        if (tiled[i]) {
+            if ((plan.tiles.size() + blocks(i, 256)) * kv_heads >= (1u << 23) || (plan.keys.size() + tiles(i)) * kv_heads >= (1u << 24))
+                return "more rows than a launch takes";
+            s.vt = plan.vt;
+            plan.vt += (uint64_t)tiles(i) * BN * D * kv_heads;
+            for (uint32_t b = 0; b < blocks(i, 256); b++) plan.tiles.push_back({i, b});
+            for (uint32_t b = 0; b < tiles(i); b++) plan.keys.push_back({i, b});
+            continue;
+        }
+        const uint64_t n = tiles(i), parts = n * 2 > share_tiles * 3 ? std::min<uint64_t>((n + share_tiles - 1) / share_tiles, PARTS_MOST) : 1;
+        if ((plan.rows.size() + blocks(i, 32) * parts) * kv_heads >= (1u << 24)) return "more rows than a launch takes";
+        for (uint32_t b = 0; b < blocks(i, 32); b++) {
+            if (parts > 1) plan.joins.push_back({i, b, plan.parts, (uint32_t)parts});
+            for (uint64_t p = 0; p < parts; p++)
+                plan.rows.push_back({i, b, (uint32_t)(n * p / parts), (uint32_t)(n * (p + 1) / parts), parts > 1 ? plan.parts++ : WHOLE});
+        }
+    }
+    return nullptr;
 }
 
 }  // namespace
@@ -288,53 +462,51 @@ int launch(h3_gpu *g, const SeqArgs &a) {
 extern "C" void h3_hip_sequences_free(h3_hip_sequences *s) {
     if (!s) return;
     h3_gpu_tensor_free(s->table);
+    h3_gpu_tensor_free(s->workspace);
     delete s;
+}
+
+extern "C" int h3_hip_sequences_layout(const uint32_t *q_offsets, const uint32_t *k_offsets, uint32_t count, uint32_t heads,
+                                       uint32_t kv_heads, size_t *bytes) try {
+    Plan plan;
+    if (make_plan(plan, q_offsets, k_offsets, count, heads, kv_heads, 256)) return 0;
+    if (bytes) *bytes = plan.table_bytes() + plan.workspace_bytes(kv_heads);
+    return 1;
+} catch (const std::bad_alloc &) {
+    return 0;
 }
 
 extern "C" h3_hip_sequences *h3_hip_sequences_new(h3_gpu *g, const uint32_t *q_offsets, const uint32_t *k_offsets, uint32_t count,
                                                   uint32_t heads, uint32_t kv_heads) {
     if (!g) return nullptr;
-    if (!q_offsets || !count || count > (1u << 20) || !kv_heads || !heads || heads > 65535 || heads % kv_heads) {
-        h3_set_error(g, "sequences: need 1 to 2^20 of them and heads a multiple of the key heads");
-        return nullptr;
-    }
-    if (!k_offsets) k_offsets = q_offsets;
-    const uint32_t share = heads / kv_heads;
     h3_hip_sequences *s = nullptr;
+    Plan plan;
     std::vector<uint32_t> words;
     try {
-        std::vector<Item> items;
-        for (uint32_t i = 0; i < count; i++) {
-            if (q_offsets[i + 1] < q_offsets[i] || k_offsets[i + 1] < k_offsets[i]) {
-                h3_set_error(g, "sequences: offsets of sequence %u fall", i);
-                return nullptr;
-            }
-            const uint64_t lq = q_offsets[i + 1] - q_offsets[i], lk = k_offsets[i + 1] - k_offsets[i];
-            if (lq * share >= (1u << 31) || lk >= (1u << 31)) {
-                h3_set_error(g, "sequences: sequence %u is longer than 2^31 rows", i);
-                return nullptr;
-            }
-            words.insert(words.end(), {q_offsets[i], (uint32_t)lq, k_offsets[i], (uint32_t)lk});
-            for (uint32_t b = 0; b < (lq * share + 31) / 32; b++) items.push_back({i, b});
-        }
-        // Long sequences first: a short one then ends the call.
-        std::stable_sort(items.begin(), items.end(), [&](const Item &x, const Item &y) {
-            return words[4 * x.sequence + 3] > words[4 * y.sequence + 3];
-        });
-        // A launch holds fewer than 2^32 threads.
-        if (items.size() * kv_heads >= (1u << 24)) {
-            h3_set_error(g, "sequences: more rows than a launch takes");
+        if (const char *why = make_plan(plan, q_offsets, k_offsets, count, heads, kv_heads, g->cus)) {
+            h3_set_error(g, "sequences: %s", why);
             return nullptr;
         }
-        for (const Item &x : items) words.insert(words.end(), {x.sequence, x.block});
-        s = new h3_hip_sequences{g, heads, kv_heads, count, (uint32_t)items.size(), q_offsets[count], k_offsets[count], nullptr};
+        auto append = [&](const auto &list) {
+            const auto *w = reinterpret_cast<const uint32_t *>(list.data());
+            words.insert(words.end(), w, w + list.size() * sizeof(list[0]) / 4);
+        };
+        append(plan.sequences);
+        append(plan.tiles);
+        append(plan.keys);
+        append(plan.rows);
+        append(plan.joins);
+        s = new h3_hip_sequences{g, heads, kv_heads, count, (uint32_t)plan.tiles.size(), (uint32_t)plan.keys.size(),
+                                 (uint32_t)plan.rows.size(), (uint32_t)plan.joins.size(), q_offsets[count],
+                                 (k_offsets ? k_offsets : q_offsets)[count], plan.retry_at(), plan.parts_at(kv_heads), nullptr, nullptr};
     } catch (const std::bad_alloc &) {
         h3_set_error(g, "sequences: out of host memory");
         return nullptr;
     }
     s->table = h3_gpu_tensor_from_u32(g, words.data(), words.size());
-    if (!s->table) {
-        delete s;
+    if (s->table && plan.workspace_bytes(kv_heads)) s->workspace = h3_gpu_tensor_alloc(g, plan.workspace_bytes(kv_heads), H3_GPU_I8, H3_GPU_DEVICE_ONLY);
+    if (!s->table || (plan.workspace_bytes(kv_heads) && !s->workspace)) {
+        h3_hip_sequences_free(s);
         return nullptr;
     }
     return s;
@@ -350,12 +522,24 @@ extern "C" int h3_hip_sdpa_sequences_bf16(h3_gpu *g, h3_gpu_tensor *out, const h
     if (!h3_require(g, q, H3_GPU_BF16, nq, "attention Q") || !h3_require(g, k, H3_GPU_BF16, nk, "attention K") ||
         !h3_require(g, v, H3_GPU_BF16, nk, "attention V") || !h3_require(g, out, H3_GPU_BF16, nq, "attention output"))
         return 0;
-    if (!s->items) return 1;
-    const SeqArgs a{(uint16_t *)out->data, (const uint16_t *)q->data, (const uint16_t *)k->data, (const uint16_t *)v->data,
-                    (const Sequence *)s->table->data, (const Item *)((const uint32_t *)s->table->data + 4 * (size_t)s->count),
-                    s->items, s->heads, s->kv_heads, s->heads / s->kv_heads, bf16_to_f32(f32_to_bf16(scale)) * 1.4426950408889634f,
-                    g->fault};
-    if (!launch(g, a)) return 0;
-    g->stats.attention_dispatches++;
+    const float rounded = bf16_to_f32(f32_to_bf16(scale));
+    const auto *sequences = (const h3_sequence *)s->table->data;
+    const auto *items = (const h3_sequence_item *)(sequences + s->count);
+    const auto *rows = (const RowItem *)(items + s->tiles + s->keys);
+    char *const workspace = s->workspace ? (char *)s->workspace->data : nullptr;
+    if (s->tiles) {
+        const h3_sequence_tiles t{sequences, items, items + s->tiles, s->tiles, s->keys, s->heads, s->kv_heads,
+                                  (uint16_t *)workspace, (uint8_t *)workspace + s->retry_at};
+        if (!h3_launch_attention_sequence_tiles(g, (uint16_t *)out->data, (const uint16_t *)q->data, (const uint16_t *)k->data,
+                                                (const uint16_t *)v->data, t, rounded))
+            return 0;
+    }
+    if (s->rows) {
+        const SeqArgs a{(uint16_t *)out->data, (const uint16_t *)q->data, (const uint16_t *)k->data, (const uint16_t *)v->data,
+                        sequences, rows, (const JoinItem *)(rows + s->rows), s->joins ? (float *)(workspace + s->parts_at) : nullptr,
+                        s->rows, s->joins, s->heads, s->kv_heads, s->heads / s->kv_heads, rounded * 1.4426950408889634f, g->fault};
+        if (!launch(g, a)) return 0;
+    }
+    if (s->tiles + s->rows) g->stats.attention_dispatches++;
     return 1;
 }

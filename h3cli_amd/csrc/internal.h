@@ -41,6 +41,30 @@ int h3_launch_attention_routed(h3_gpu *g, void *workspace, uint16_t *out, const 
                                const uint32_t *lists, const uint32_t *counts, uint32_t list_stride,
                                uint32_t head0, uint32_t group, uint32_t qb0, uint32_t qslab, bool transpose);
 
+// Packed sequences (attn_sequences.hip): query rows [q0, q0 + lq) attend to key rows
+// [k0, k0 + lk). Row v of (sequence, key head) is query v / share of head share * key head +
+// v % share, share the query heads of a key head. vt: where the tile kernels keep the
+// sequence's transposed V, in elements of the workspace.
+struct h3_sequence {
+    uint32_t q0, lq, k0, lk;
+    uint64_t vt;
+};
+// A workgroup's part of a sequence: a block of rows, or of keys.
+struct h3_sequence_item {
+    uint32_t sequence, block;
+};
+struct h3_sequence_tiles {
+    const h3_sequence *sequences;
+    const h3_sequence_item *items;       // blocks of 256 rows, each with at least 257 keys and below 4 GiB of K
+    const h3_sequence_item *key_items;   // blocks of 64 keys of the same sequences
+    uint32_t count, key_count, heads, kv_heads;
+    uint16_t *vt;                        // [kv_heads][128][lk rounded up to 64] of each sequence
+    uint8_t *retry;                      // 8 bytes an item and key head
+};
+// Attention of those blocks by the 256-row tile kernel, the transposition of V first.
+int h3_launch_attention_sequence_tiles(h3_gpu *g, uint16_t *out, const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                                       const h3_sequence_tiles &t, float scale);
+
 // SOL attention lists (see csrc/sol.hip): exact tiles per (head, query block),
 // centroid tiles with their approximate-block masks, and the centroid arrays.
 struct h3_sol_lists {

@@ -245,6 +245,9 @@ typedef struct h3_hip_sequences h3_hip_sequences;
 h3_hip_sequences *h3_hip_sequences_new(h3_gpu *gpu, const uint32_t *q_offsets, const uint32_t *k_offsets,
                                        uint32_t count, uint32_t heads, uint32_t kv_heads);
 void h3_hip_sequences_free(h3_hip_sequences *sequences);
+/* Host only: the device bytes of such a plan on a whole GPU; 0 where it is refused. */
+int h3_hip_sequences_layout(const uint32_t *q_offsets, const uint32_t *k_offsets, uint32_t count, uint32_t heads,
+                            uint32_t kv_heads, size_t *bytes);
 /* softmax(scale * Q K^T) V within each sequence: q and out [rows, heads, 128], k and v
  * [rows, kv_heads, 128] BF16, the scale rounded to BF16, as h3_gpu_sdpa_bf16 of each
  * sequence alone. A query of a sequence without keys gets zeros; rows of no

@@ -69,13 +69,17 @@ def attention_reference(q, k, v, scale):
     return out, HALF * np.abs(out) + (HALF + 2 * score + 2 * (len(k) + 64) * F32) * weight * (1 + HALF)
 
 
-def check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=1, spread=1.0, scale=SCALE, rows=None):
-    """One call against the reference; rows of no sequence hold NaN in the inputs and must stay in the output."""
+def check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=1, spread=1.0, scale=SCALE, rows=None, rising=0.0, heads_seen=None):
+    """One call against the reference; rows of no sequence hold NaN in the inputs and must stay in the
+    output. rising: how much a sequence's last keys are larger than its first."""
     at = k_offsets if k_offsets is not None else q_offsets
     rows = rows or (q_offsets[-1] + 3, at[-1] + 5)
     share = heads // kv_heads
     q, k, v = (normal(rows[i > 0] * n * 128, seed + i, scale=spread if i < 2 else 1.0).reshape(rows[i > 0], n, 128).copy()
                for i, n in ((0, heads), (1, kv_heads), (2, kv_heads)))
+    if rising:
+        for a, b in zip(at, at[1:]):
+            k[a:b] = synth.f32_to_bf16(bf16(k[a:b]) * np.linspace(1, 1 + rising, b - a, dtype=np.float32)[:, None, None])
     for t, ends in ((q, q_offsets), (k, at), (v, at)):
         t[:ends[0]] = 0x7fc0
         t[ends[-1]:] = 0x7f80
@@ -100,7 +104,7 @@ def check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=1, spread=1.0
         if at[i] == at[i + 1]:
             assert not np.any(got[qs] & 0x7fff)
             continue
-        for h in range(heads):
+        for h in range(heads) if heads_seen is None else heads_seen:
             want, bound = attention_reference(fq[qs, h], fk[ks, h // share], fv[ks, h // share], scale)
             within(bf16(got[qs, h]), want, bound, (kernel, i, h))
     for t in (tq, tk, tv, out):
@@ -129,6 +133,53 @@ def test_attention_of_sequences(q_offsets, k_offsets, heads, kv_heads):
 def test_attention_of_sequences_peaks_and_flat_rows(spread, scale):
     with Gpu() as g:
         check_attention(g, [0, 70, 135], [0, 300, 650], 2, 2, seed=5, spread=spread, scale=scale)
+
+
+@pytest.mark.parametrize("q_offsets,k_offsets,heads,kv_heads,rising", [
+    ([0, 700, 1500], None, 40, 40, 0.0),
+    ([1, 258, 258, 1000, 1513], None, 40, 40, 30.0),                # later keys' scores far above the first's
+    ([0, 600, 1000], [3, 260, 900], 60, 12, 0.0),                   # shared key heads: rows of five heads in a tile
+    ([0, 513, 770, 1500], [0, 640, 897, 2000], 42, 42, 5.0),
+    ([0, 1100, 1130, 1131, 1200], [0, 900, 1000, 2400, 2400], 40, 40, 0.0),   # and short ones beside them
+])
+def test_attention_of_sequences_by_tiles(q_offsets, k_offsets, heads, kv_heads, rising):
+    """Sequences long and many enough for the kernel of 256-row tiles, alone or with others."""
+    print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads}", flush=True)
+    size = C.c_size_t()
+    with Gpu() as g:
+        g.check(g.lib.h3_hip_sequences_layout(u32(q_offsets), None if k_offsets is None else u32(k_offsets), len(q_offsets) - 1,
+                                              heads, kv_heads, C.byref(size)))
+        assert size.value > 2 * 128 * 256 * kv_heads, size.value      # the plan holds transposed values
+        check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=7, rising=rising, heads_seen=(0, 1, heads // 2, heads - 1))
+
+
+def test_attention_of_one_sequence_is_the_dense_attention():
+    seq, heads = 4133, 6
+    with Gpu() as g:
+        ts = [g.from_bf16(normal(seq * heads * 128, i)) for i in range(3)]
+        a, b = g.empty(seq * heads * 128), g.empty(seq * heads * 128)
+        with sequences(g, [0, seq], None, heads, heads) as plan:
+            g.begin()
+            g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, a.handle, *(t.handle for t in ts), plan, C.c_float(SCALE)))
+            assert g.last_kernel() == "attn_bf16_pipe"
+            g.check(g.lib.h3_gpu_sdpa_bf16(g.handle, b.handle, *(t.handle for t in ts), seq, heads, 128, C.c_float(SCALE)))
+            assert g.last_kernel() == "attn_bf16_pipe"
+            g.submit()
+        assert np.array_equal(a.read(), b.read())
+
+
+@pytest.mark.parametrize("q_offsets,k_offsets,heads,kv_heads", [
+    ([0, 1], [0, 18225], 5, 1),
+    ([0, 1, 2, 5, 6], [0, 6000, 6001, 6001, 9000], 10, 2),
+    ([0, 40, 41], [0, 5000, 9001], 3, 1),                    # two blocks of rows, the second cut off
+    ([0, 4], [2, 8195], 1, 1),
+])
+def test_attention_of_few_rows_over_many_keys(q_offsets, k_offsets, heads, kv_heads):
+    print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads}", flush=True)
+    with Gpu() as g:
+        for rising in (0.0, 4.0):
+            kernel = check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=3, rising=rising)
+            assert kernel == "attn_sequences rows=32 shares=2", kernel     # parts, joined
 
 
 def test_attention_of_sequences_reports_values_that_are_not_finite():

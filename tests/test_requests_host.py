@@ -1,0 +1,39 @@
+"""Plans of a step that serves several requests at once: what needs no GPU."""
+import ctypes as C
+
+import pytest
+
+from h3cli_amd import _lib
+
+
+def u32(values):
+    return (C.c_uint32 * len(values))(*values)
+
+
+def layout(q, k, heads, kv_heads, count=None):
+    size = C.c_size_t()
+    ok = _lib.load().h3_hip_sequences_layout(q and u32(q), k and u32(k), len(q) - 1 if count is None else count, heads, kv_heads,
+                                             C.byref(size))
+    return size.value if ok else None
+
+
+@pytest.mark.parametrize("q,k,heads,kv_heads,count", [
+    ([0, 4], None, 3, 2, None), ([0, 4], None, 0, 1, None), ([0, 4], None, 4, 0, None), ([4, 3], None, 1, 1, None),
+    ([0, 4], [5, 4], 1, 1, None), ([0, 4, 3], None, 1, 1, None), ([0, 4], None, 65536, 1, None), ([0], None, 1, 1, 0),
+    (None, [0, 1], 1, 1, 1), ([0, 2 ** 31], None, 1, 1, None), ([0, 2 ** 30], None, 2, 1, None), ([0, 1], [0, 2 ** 31], 1, 1, None),
+    ([0, 2 ** 29], [0, 1], 1, 1, None), ([0, 2 ** 25], [0, 0], 60000, 60000, None), ([0, 2 ** 31 - 1], [0, 2 ** 31 - 1], 1, 1, None),
+])
+def test_refused_sequences(q, k, heads, kv_heads, count):
+    assert layout(q, k, heads, kv_heads, count) is None
+
+
+def test_sequences_hold_what_their_kernels_need():
+    assert 0 < layout([0, 1], None, 1, 1) < 1000
+    assert layout([0, 0, 0], None, 1, 1) > 0                     # no rows at all
+    assert layout([5, 5, 9], [7, 20, 20], 4, 2) > 0
+    # Transposed values of 4133 keys in whole tiles of 64, and retry bytes.
+    assert layout([0, 4133], None, 6, 6) > 65 * 64 * 6 * 256
+    # One row over many keys: parts of 32 rows, and no transposed values.
+    assert 2 * 130 * 128 < layout([0, 1], [0, 18225], 5, 1) < 128 * 32 * 130 * 4 + 4096
+    # A K of 4 GiB and more, in which a tile's offsets would not fit 32 bits, goes without them too.
+    assert layout([0, 300], [0, 2 ** 24], 1, 1) < 1 << 25
