@@ -161,8 +161,157 @@ __global__ __launch_bounds__(256) void rope_axes_any(AxesArgs a) {
     }
 }
 
+// Sums over the 16 / 8 / 32 lanes of a head by row rotations of the VALU; every lane gets the
+// same bits, since both sides of each addition are the same two values.
+template <int CTRL> __device__ inline float rotated(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int LANES> __device__ inline float head_sum(float v) {
+    static_assert(LANES >= 1 && LANES <= 32, "lanes of a head");
+    if constexpr (LANES >= 2) v += rotated<0xb1>(v);                    // quad_perm [1, 0, 3, 2]
+    if constexpr (LANES >= 4) v += rotated<0x4e>(v);                    // quad_perm [2, 3, 0, 1]
+    if constexpr (LANES >= 8) v += rotated<0x141>(v);                   // row_half_mirror
+    if constexpr (LANES >= 16) v += rotated<0x140>(v);                  // row_mirror
+    if constexpr (LANES >= 32) v += __shfl_xor(v, 16, 64);
+    return v;
+}
+
+// Heads of 8 * CHUNKS channels, CHUNKS <= LANES a power of two: LANES lanes a head, a 16-byte chunk each.
+// A workgroup takes a row (or a share of its heads) and goes through the heads 256 / LANES at
+// a time, UNROLL of them in flight a lane. Pairs of halves need pairs % 8 == 0 (a chunk's partner
+// is a chunk, fetched from its lane), interleaved ones pairs % 4 == 0 (partners are in the chunk).
+template <int LANES, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rope_axes_chunks(AxesArgs a) {
+    constexpr int GROUPS = 256 / LANES, UNROLL = 4;
+    const unsigned lane = threadIdx.x % 64, c = lane % LANES, group = threadIdx.x / LANES;
+    const unsigned items = a.heads + 2 * a.kv_heads, chunks = a.dim / 8;
+    const bool held = c < chunks;
+    const unsigned half = INTERLEAVED ? 0 : a.pairs / 8;
+    const bool turned = INTERLEAVED ? c < a.pairs / 4 : c < 2 * half;
+    const bool second = !INTERLEAVED && c >= half;
+    const int partner = (int)(turned && !INTERLEAVED ? lane + (second ? 0u - half : half) : lane) * 4;
+    const float inv_dim = 1.f / (float)a.dim;
+    u16x8 wq{}, wk{}, pq{}, pk{};
+    if (a.qw && held) {
+        const unsigned pc = turned && !INTERLEAVED ? (second ? c - half : c + half) : c;
+        wq = *reinterpret_cast<const u16x8 *>(a.qw + c * 8);
+        wk = *reinterpret_cast<const u16x8 *>(a.kw + c * 8);
+        pq = *reinterpret_cast<const u16x8 *>(a.qw + pc * 8);
+        pk = *reinterpret_cast<const u16x8 *>(a.kw + pc * 8);
+    }
+    for (size_t block = blockIdx.x; block < (size_t)a.rows * a.splits; block += gridDim.x) {
+        const size_t row = block / a.splits;
+        const unsigned part = block % a.splits;
+        // Channel e of the chunk: what it and its partner are multiplied with.
+        float oq[8], tq[8], ok[8], tk[8];
+        {
+            float cs[8], sn[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                cs[e] = 1.f;
+                sn[e] = 0.f;
+            }
+            if (turned) {
+#pragma unroll
+                for (int e = 0; e < 8; e += INTERLEAVED ? 2 : 1) {
+                    const unsigned pair = INTERLEAVED ? c * 4 + e / 2 : (second ? c - half : c) * 8 + e;
+                    phase(a, row, pair, cs[e], sn[e]);
+                    if constexpr (INTERLEAVED) {
+                        cs[e + 1] = cs[e];
+                        sn[e + 1] = sn[e];
+                        sn[e] = -sn[e];
+                    } else if (!second) {
+                        sn[e] = -sn[e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int pe = INTERLEAVED ? e ^ 1 : e;
+                oq[e] = a.qw ? cs[e] * bf16_to_f32(wq[e]) : cs[e];
+                ok[e] = a.qw ? cs[e] * bf16_to_f32(wk[e]) : cs[e];
+                tq[e] = a.qw ? sn[e] * bf16_to_f32(pq[pe]) : sn[e];
+                tk[e] = a.qw ? sn[e] * bf16_to_f32(pk[pe]) : sn[e];
+            }
+        }
+        const uint16_t *const src = a.qkv + row * items * a.dim + c * 8;
+        for (unsigned first = part * GROUPS + group; first < items; first += a.splits * GROUPS * UNROLL) {
+            u16x8 raw[UNROLL] = {};
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                const unsigned item = first + u * a.splits * GROUPS;
+                unsigned head;
+                int kind;
+                if (item < items && held)
+                    raw[u] = *reinterpret_cast<const u16x8 *>(src + (size_t)source_head(a, item, head, kind) * a.dim);
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                const unsigned item = first + u * a.splits * GROUPS;
+                if (item >= items) break;
+                unsigned head;
+                int kind;
+                source_head(a, item, head, kind);
+                uint16_t *const dst = (kind == QUERY ? a.q + (row * a.heads + head) * a.dim
+                                                     : (kind == KEY ? a.k : a.v) + (row * a.kv_heads + head) * a.dim) + c * 8;
+                if (kind != VALUE) {
+                    float x[8], sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[e] = bf16_to_f32(raw[u][e]);
+                        sum = fmaf(x[e], x[e], sum);
+                    }
+                    const float r = a.qw ? rsqrtf(head_sum<LANES>(sum) * inv_dim + a.eps) : 1.f;
+                    float y[8];
+                    if constexpr (INTERLEAVED) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) y[e] = turned ? x[e ^ 1] : 0.f;
+                    } else {
+                        const i32x4 own = __builtin_bit_cast(i32x4, raw[u]);
+                        i32x4 other;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) other[e] = __builtin_amdgcn_ds_bpermute(partner, own[e]);
+                        // Channels behind the pairs pass as they are, infinities too.
+#pragma unroll
+                        for (int e = 0; e < 4; e++) other[e] = turned ? other[e] : 0;
+                        const u16x8 o = __builtin_bit_cast(u16x8, other);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) y[e] = bf16_to_f32(o[e]);
+                    }
+                    if (kind == QUERY)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) raw[u][e] = f32_to_bf16(r * fmaf(x[e], oq[e], y[e] * tq[e]));
+                    else
+#pragma unroll
+                        for (int e = 0; e < 8; e++) raw[u][e] = f32_to_bf16(r * fmaf(x[e], ok[e], y[e] * tk[e]));
+                }
+                if (held) *reinterpret_cast<u16x8 *>(dst) = raw[u];
+            }
+        }
+    }
+}
+
+template <int LANES> void launch_chunks(h3_gpu *g, AxesArgs a) {
+    const unsigned items = a.heads + 2 * a.kv_heads;
+    constexpr unsigned GROUPS = 256 / LANES;
+    // A row's heads go to more workgroups where the rows alone would not fill the chip.
+    a.splits = (unsigned)std::min<size_t>((items + GROUPS - 1) / GROUPS, (2048 + (size_t)a.rows - 1) / a.rows);
+    const unsigned blocks = (unsigned)std::min<size_t>((size_t)a.rows * a.splits, 1 << 20);
+    if (a.interleaved) hipLaunchKernelGGL((rope_axes_chunks<LANES, true>), dim3(blocks), dim3(256), 0, g->compute, a);
+    else hipLaunchKernelGGL((rope_axes_chunks<LANES, false>), dim3(blocks), dim3(256), 0, g->compute, a);
+}
+
 int rope_axes(h3_gpu *g, const AxesArgs &args) {
     AxesArgs a = args;
+    if (a.dim % 8 == 0 && a.pairs % (a.interleaved ? 4 : 8) == 0) {
+        const unsigned chunks = a.dim / 8;
+        if (chunks <= 2) launch_chunks<2>(g, a);
+        else if (chunks <= 4) launch_chunks<4>(g, a);
+        else if (chunks <= 8) launch_chunks<8>(g, a);
+        else if (chunks <= 16) launch_chunks<16>(g, a);
+        else launch_chunks<32>(g, a);
+        return h3_launch_status(g, "QKV norm/RoPE by axes");
+    }
     const unsigned items = a.heads + 2 * a.kv_heads;
     // A row's heads go to more workgroups where the rows alone would not fill the chip.
     a.splits = (unsigned)std::min<size_t>((items + 3) / 4, (4096 + (size_t)a.rows - 1) / a.rows);
