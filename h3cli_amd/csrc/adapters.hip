@@ -22,16 +22,16 @@
 
 struct AdapterEntry {
     uint64_t down, up;     // elements from the start of the packed matrices
-    uint32_t blocks;       // 32 ranks each
+    uint32_t ranks;        // up to the next 16
     float scale;
 };
 
 struct h3_hip_adapters {
     h3_gpu *owner;
-    uint32_t count, k, n, k_padded;
+    uint32_t count, k, n, k_padded, n_padded;
     std::vector<uint32_t> ranks;
     std::vector<AdapterEntry> entries;
-    h3_gpu_tensor *weights;   // BF16: A_a [32 blocks, k_padded] of every adapter, then B_a [n, 32 blocks]
+    h3_gpu_tensor *weights;   // BF16: of each A_a, then B_a, as adapter_pack orders them
     h3_gpu_tensor *table;     // AdapterEntry [count]
 };
 
@@ -48,6 +48,7 @@ namespace {
 
 constexpr uint32_t NONE = UINT32_MAX;
 constexpr unsigned KC = 64;                // channels of K a step: one cache line of a row
+constexpr unsigned COLS = 64;              // columns of N a step: one cache line of a row
 constexpr uint32_t RANK_MOST = 256;
 
 uint32_t rank_blocks(uint32_t rank) { return (rank + 31) / 32; }
@@ -59,155 +60,274 @@ struct AdapterArgs {
     const AdapterEntry *table;
     const uint32_t *order, *adapter;       // [32 tiles], [tiles]
     float *sums;
-    unsigned rows, count, k, n, k_padded, tiles, passes, splits, rank_padded;
+    unsigned k, n, k_padded, tiles, passes, splits, rank_padded;
+    unsigned groups, span;                 // adapter_up: workgroups of a tile, their steps of columns
 };
 
-// Eight values of a row from channel c on, zeros from `end` on; WIDE: rows start on 16 bytes.
-template <bool WIDE> __device__ inline bf16x8 load8(const uint16_t *row, unsigned c, unsigned end) {
-    u16x8 v{};
-    if constexpr (WIDE) {
-        if (c < end) v = *reinterpret_cast<const u16x8 *>(row + c);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (c + e < end) v[e] = row[c + e];
-    }
-    return __builtin_bit_cast(bf16x8, v);
+// Eight values from any element on. Global memory takes 16-byte accesses at any two bytes; what
+// lies behind a tensor's end is within its allocation.
+struct __attribute__((packed, aligned(2))) Loose { i32x4 v; };
+__device__ inline i32x4 load_loose(const uint16_t *p) { return reinterpret_cast<const Loose *>(p)->v; }
+
+// The wave's own LDS writes are there, for all its lanes.
+__device__ inline void wait_lds() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
 }
 
-// t of a tile and up to 64 ranks over a share of K: four waves take its 64-channel steps in
-// turn and add their sums in LDS, in wave order.
-template <bool WIDE>
-__global__ __launch_bounds__(256) void adapter_down(AdapterArgs a) {
-    __shared__ float part[4][8][64][4];    // [wave][32-rank block * 4 + rows' group][lane]
-    const unsigned wave = threadIdx.x / 64, lane = threadIdx.x % 64, n = lane % 32, hf = lane / 32;
+// t of a tile and up to 64 ranks over a share of K: four waves take its 64-channel steps in turn, the
+// next two steps' values of x in flight, and add their sums in LDS, in wave order. x is loaded by
+// whole cache lines, eight lanes a row, and goes through 4 KB of LDS a wave (16-byte chunks
+// XOR-swizzled) to the lanes that multiply it: loaded as these lanes need it, each line is asked for
+// four times, and evicted from the L1 in between.
+constexpr unsigned DOWN_WAVES = 4;
+__global__ __launch_bounds__(64 * DOWN_WAVES, 2) void adapter_down(AdapterArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float part[];   // [wave][32-rank block * 4 + rows' group][lane][4]
+    const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, n = lane % 32, hf = lane / 32;
     const unsigned split = blockIdx.x % a.splits, pass = blockIdx.x / a.splits % a.passes, tile = blockIdx.x / a.splits / a.passes;
-    const AdapterEntry entry = a.table[a.adapter[tile]];
-    if (pass * 2 >= entry.blocks) return;
-    const bool both = pass * 2 + 1 < entry.blocks;
-    const uint32_t row = a.order[tile * 32 + n];
-    const uint16_t *xr = a.x + (size_t)(row == NONE ? a.order[tile * 32] : row) * a.k;
-    const uint16_t *down = a.weights + entry.down + (size_t)(pass * 64 + n) * a.k_padded;
-    f32x16 acc[2] = {};
-    for (unsigned step = split * 4 + wave; step * KC < a.k; step += a.splits * 4) {
+    const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
+    if (pass * 64 >= entry.ranks) return;
+    const bool both = pass * 64 + 32 < entry.ranks;
+    // Lane's chunk lane % 8 of rows lane / 8 + 8 i; row r keeps chunk c at c ^ r % 8.
+    const unsigned chunk = lane % 8 * 8;
+    const uint16_t *xr[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const unsigned c = step * KC + j * 16 + hf * 8;
-            const bf16x8 xv = load8<WIDE>(xr, c, a.k);
+    for (int i = 0; i < 4; i++) {
+        uint32_t row = a.order[tile * 32 + lane / 8 + 8 * i];
+        if (row == NONE) row = a.order[tile * 32];
+        xr[i] = a.x + (size_t)row * a.k + chunk;
+    }
+    i32x4 *const buffer = reinterpret_cast<i32x4 *>(part + wave * 1024);
+    const size_t block_size = (size_t)a.k_padded * 32;
+    const uint16_t *const down = a.weights + entry.down + pass * 2 * block_size + lane * 8;
+    f32x16 acc[2] = {};
+    i32x4 x[2][4];
+    auto load = [&](int slot, unsigned step) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[slot][i] = i32x4{};
+            if (step * KC + chunk < a.k) x[slot][i] = load_loose(xr[i] + step * KC);
+        }
+    };
+    auto multiply = [&](int slot, unsigned step) {
+        i32x4 w[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int b = 0; b < 2; b++)
-                if (b == 0 || both) {
-                    const bf16x8 w = *reinterpret_cast<const bf16x8 *>(down + (size_t)b * 32 * a.k_padded + c);
-                    acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, xv, acc[b], 0, 0, 0);
-                }
+                if (b == 0 || both) w[b][j] = *reinterpret_cast<const i32x4 *>(down + b * block_size + (size_t)(step * 4 + j) * 512);
+        if (step * KC + KC > a.k)   // what lies behind the row's end is another row's
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (unsigned e = 0; e < 8; e++)
+                    if (step * KC + chunk + e >= a.k) x[slot][i][e / 2] &= e % 2 ? 0x0000ffff : 0xffff0000;
+        wait_lds();                     // the last step's reads
+#pragma unroll
+        for (int i = 0; i < 4; i++) buffer[(lane / 8 + 8 * i) * 8 + (lane % 8 ^ lane / 8)] = x[slot][i];
+        wait_lds();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const bf16x8 v = __builtin_bit_cast(bf16x8, buffer[n * 8 + ((j * 2 + hf) ^ n % 8)]);
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+                if (b == 0 || both)
+                    acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w[b][j]), v, acc[b], 0, 0, 0);
         }
+    };
+    const unsigned steps = a.k_padded / KC, stride = a.splits * DOWN_WAVES;
+    unsigned step = split * DOWN_WAVES + wave;
+    if (step < steps) load(0, step);
+    for (; step < steps; step += 2 * stride) {
+        if (step + stride < steps) load(1, step + stride);
+        multiply(0, step);
+        if (step + stride >= steps) break;
+        if (step + 2 * stride < steps) load(0, step + 2 * stride);
+        multiply(1, step + stride);
     }
+    __syncthreads();                    // the sums take the buffers' place
 #pragma unroll
     for (int b = 0; b < 2; b++)
+        if (b == 0 || both)
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-            *reinterpret_cast<f32x4 *>(part[wave][b * 4 + q][lane]) =
-                f32x4{acc[b][4 * q], acc[b][4 * q + 1], acc[b][4 * q + 2], acc[b][4 * q + 3]};
+            for (int q = 0; q < 4; q++)
+                *reinterpret_cast<f32x4 *>(part + ((wave * 8 + b * 4 + q) * 64 + lane) * 4) =
+                    f32x4{acc[b][4 * q], acc[b][4 * q + 1], acc[b][4 * q + 2], acc[b][4 * q + 3]};
     __syncthreads();
-    float *sums = a.sums + ((size_t)(split * a.tiles + tile) * 32 + n) * a.rank_padded + pass * 64;
+    float *const sums = a.sums + ((size_t)(split * a.tiles + tile) * 32 + n) * a.rank_padded + pass * 64 + hf * 4;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const unsigned q = wave * 2 + i;   // ranks 32 (q / 4) + 8 (q % 4) + 4 hf + 0..3 of row n
-        if (q >= 4 && !both) continue;
+    for (unsigned b = 0; b < 2; b++) {
+        if (b && !both) break;
         f32x4 t{};
 #pragma unroll
-        for (int w = 0; w < 4; w++) t += *reinterpret_cast<const f32x4 *>(part[w][q][lane]);
-        *reinterpret_cast<f32x4 *>(sums + q / 4 * 32 + q % 4 * 8 + hf * 4) = t;
+        for (unsigned v = 0; v < DOWN_WAVES; v++) t += *reinterpret_cast<const f32x4 *>(part + ((v * 8 + b * 4 + wave) * 64 + lane) * 4);
+        *reinterpret_cast<f32x4 *>(sums + b * 32 + wave * 8) = t;     // ranks 32 b + 8 wave + 4 hf + 0..3 of row n
     }
 }
 
-constexpr unsigned COLS = 128;             // columns of a wave's step
-constexpr unsigned LDS_ROW = COLS + 4;     // floats: rows of a step shift by four banks
+constexpr unsigned STAGE_ROW = COLS + 4;   // floats: rows shift by four banks
+constexpr unsigned UP_STAGE = 32 * STAGE_ROW;
 
-// out = base + scale * t . B^T for a tile's rows and 128 columns a wave; tiles behind the
-// adapters' are copied.
+// out = base + scale * t . B^T for a tile's rows, 64 columns a wave and step; tiles behind the
+// adapters' are copied. t is summed over its shares once per workgroup and kept in LDS as the
+// two BF16 operands, in the matrix instruction's order. The products go through LDS too, so that base
+// and out are read and written by whole cache lines, eight lanes a row. The next weights, and the
+// next step's base, are on their way while these are multiplied.
 template <bool WIDE>
-__global__ __launch_bounds__(256) void adapter_up(AdapterArgs a) {
-    extern __shared__ __attribute__((aligned(16))) float stage[];
-    const unsigned wave = threadIdx.x / 64, lane = threadIdx.x % 64, n = lane % 32, hf = lane / 32;
-    const unsigned groups = (a.n + 4 * COLS - 1) / (4 * COLS);
-    const unsigned tile = blockIdx.x / groups, c0 = (blockIdx.x % groups * 4 + wave) * COLS;
-    if (c0 >= a.n) return;
-    float *const mine = stage + wave * 32 * LDS_ROW;
+__global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float shared[];   // [wave] stage, then operands [rank / 16][2][lane]
+    const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, n = lane % 32, hf = lane / 32;
+    float *const stage = shared + wave * UP_STAGE;
+    i32x4 *const operand = reinterpret_cast<i32x4 *>(shared + 4 * UP_STAGE);
+    const unsigned tile = blockIdx.x / a.groups, group = blockIdx.x % a.groups;
+    const unsigned steps = (a.n + COLS - 1) / COLS, last = min(steps, (group + 1) * a.span);
     const bool adapted = tile < a.tiles;
+    // Lane's chunk lane % 8 of rows lane / 8 + 8 i.
+    const unsigned chunk = lane % 8 * 8;
+    uint32_t row[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) row[i] = a.order[tile * 32 + lane / 8 + 8 * i];
+    AdapterEntry entry{};
+    if (adapted) entry = a.table[load_uniform(a.adapter + tile)];
+    const unsigned sixteens = entry.ranks / 16;
+    const uint16_t *const up = a.weights + entry.up + lane * 8;
+    i32x4 next_v[4] = {}, next_w[4] = {};
+    auto load_base = [&](unsigned step) {
+        const unsigned c = step * COLS + chunk;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (row[i] != NONE && c < a.n) {
+                const uint16_t *const p = a.base + (size_t)row[i] * a.n + c;
+                if constexpr (WIDE) next_v[i] = *reinterpret_cast<const i32x4 *>(p);
+                else next_v[i] = load_loose(p);
+            }
+    };
+    // 32 ranks of the step's 64 columns, or the last 16.
+    auto load_up = [&](unsigned step, unsigned r) {
+#pragma unroll
+        for (unsigned i = 0; i < 4; i++)
+            if (i < 2 || r + 1 < sixteens) next_w[i] = *reinterpret_cast<const i32x4 *>(up + (((size_t)step * sixteens + r) * 2 + i) * 512);
+    };
+    unsigned step = group * a.span + wave;
+    if (step < last) {
+        load_base(step);
+        if (adapted) load_up(step, 0);
+    }
     if (adapted) {
-        const AdapterEntry entry = a.table[a.adapter[tile]];
-        const unsigned ranks = entry.blocks * 32;
-        f32x16 acc[4] = {};
-        for (unsigned r = 0; r < ranks; r += 16) {
+        for (unsigned i = threadIdx.x; i < sixteens * 64; i += 256) {
+            // Lane i % 64 of rank step i / 64: eight ranks of its row.
+            const unsigned from = i / 64 * 16 + i % 64 / 32 * 8;
+            const float *p = a.sums + ((size_t)tile * 32 + i % 32) * a.rank_padded + from;
             f32x4 t[2] = {};
+#pragma unroll 4
             for (unsigned split = 0; split < a.splits; split++) {
-                const float *p = a.sums + ((size_t)(split * a.tiles + tile) * 32 + n) * a.rank_padded + r + hf * 8;
                 t[0] += *reinterpret_cast<const f32x4 *>(p);
                 t[1] += *reinterpret_cast<const f32x4 *>(p + 4);
+                p += (size_t)a.tiles * 32 * a.rank_padded;
             }
             bf16x8 high, low;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float v = t[e / 4][e % 4] * entry.scale;
-                high[e] = (__bf16)v;
-                low[e] = (__bf16)(v - (float)high[e]);
+                const float f = t[e / 4][e % 4] * entry.scale;
+                high[e] = (__bf16)f;
+                low[e] = (__bf16)(f - (float)high[e]);
             }
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                const unsigned c = min(c0 + b * 32 + n, a.n - 1);
-                const bf16x8 w = *reinterpret_cast<const bf16x8 *>(a.weights + entry.up + (size_t)c * ranks + r + hf * 8);
-                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, high, acc[b], 0, 0, 0);
-                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, low, acc[b], 0, 0, 0);
-            }
+            operand[i / 64 * 128 + i % 64] = __builtin_bit_cast(i32x4, high);
+            operand[i / 64 * 128 + 64 + i % 64] = __builtin_bit_cast(i32x4, low);
         }
-        // Row n's columns 32 b + 8 q + 4 hf + 0..3, to be read by whole rows.
-#pragma unroll
-        for (int b = 0; b < 4; b++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                *reinterpret_cast<f32x4 *>(mine + n * LDS_ROW + b * 32 + q * 8 + hf * 4) =
-                    f32x4{acc[b][4 * q], acc[b][4 * q + 1], acc[b][4 * q + 2], acc[b][4 * q + 3]};
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own stores
-        __builtin_amdgcn_wave_barrier();
+        __syncthreads();
     }
+    for (; step < last; step += 4) {
+        i32x4 v[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const unsigned r = 4 * i + lane / 16, c = c0 + lane % 16 * 8;
-        const uint32_t row = a.order[tile * 32 + r];
-        if (row == NONE || c >= a.n) continue;
-        const uint16_t *src = a.base + (size_t)row * a.n;
-        uint16_t *dst = a.out + (size_t)row * a.n + c;
-        u16x8 v = __builtin_bit_cast(u16x8, load8<WIDE>(src, c, a.n));
+        for (int i = 0; i < 4; i++) v[i] = next_v[i];
+        const bool more = step + 4 < last;
         if (adapted) {
-            const f32x4 d0 = *reinterpret_cast<const f32x4 *>(mine + r * LDS_ROW + lane % 16 * 8);
-            const f32x4 d1 = *reinterpret_cast<const f32x4 *>(mine + r * LDS_ROW + lane % 16 * 8 + 4);
+            f32x16 acc[2] = {};
+            for (unsigned first = 0; first < sixteens; first += 2) {
+                i32x4 w[4];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = f32_to_bf16(bf16_to_f32(v[e]) + (e < 4 ? d0[e] : d1[e - 4]));
+                for (int i = 0; i < 4; i++) w[i] = next_w[i];
+                if (first + 2 < sixteens) load_up(step, first + 2);
+                else if (more) {
+                    load_base(step + 4);
+                    load_up(step + 4, 0);
+                }
+#pragma unroll
+                for (unsigned r = 0; r < 2; r++) {
+                    if (first + r >= sixteens) break;
+                    const bf16x8 high = __builtin_bit_cast(bf16x8, operand[(first + r) * 128 + lane]);
+                    const bf16x8 low = __builtin_bit_cast(bf16x8, operand[(first + r) * 128 + 64 + lane]);
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        const bf16x8 u = __builtin_bit_cast(bf16x8, w[r * 2 + b]);
+                        acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, high, acc[b], 0, 0, 0);
+                        acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, low, acc[b], 0, 0, 0);
+                    }
+                }
+            }
+            // Row n's columns 32 b + 8 q + 4 hf + 0..3.
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    *reinterpret_cast<f32x4 *>(stage + n * STAGE_ROW + b * 32 + q * 8 + hf * 4) =
+                        f32x4{acc[b][4 * q], acc[b][4 * q + 1], acc[b][4 * q + 2], acc[b][4 * q + 3]};
+            wait_lds();
+        } else if (more) {
+            load_base(step + 4);
         }
-        if constexpr (WIDE) *reinterpret_cast<u16x8 *>(dst) = v;
-        else
+        const unsigned c = step * COLS + chunk;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (c + e < a.n) dst[e] = v[e];
+        for (int i = 0; i < 4; i++) {
+            if (adapted) {
+                const f32x4 *const d = reinterpret_cast<const f32x4 *>(stage + (lane / 8 + 8 * i) * STAGE_ROW + chunk);
+                const f32x4 d0 = d[0], d1 = d[1];
+                bf16x8 y;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t word = (uint32_t)v[i][e / 2];
+                    y[e] = (__bf16)(__builtin_bit_cast(float, e % 2 ? word & 0xffff0000u : word << 16) + (e < 4 ? d0[e % 4] : d1[e % 4]));
+                }
+                v[i] = __builtin_bit_cast(i32x4, y);
+            }
+            if (row[i] == NONE || c >= a.n) continue;
+            uint16_t *const out = a.out + (size_t)row[i] * a.n + c;
+            if constexpr (WIDE) *reinterpret_cast<i32x4 *>(out) = v[i];
+            else if (c + 8 <= a.n) reinterpret_cast<Loose *>(out)->v = v[i];
+            else
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (c + e < a.n) out[e] = (uint16_t)((uint32_t)v[i][e / 2] >> (e % 2 * 16));
+        }
+        wait_lds();                     // the stage's reads, before the next step's products
     }
 }
 
-// A [rank, k] into 32 * blocks rows of k_padded values and B [n, rank] into n rows of
-// 32 * blocks, zeros behind the ends; without a source (a new adapter) zeros.
-__global__ __launch_bounds__(256) void adapter_pack(uint16_t *dst, const uint16_t *src, size_t rows, size_t columns,
-                                                    size_t rows_padded, size_t columns_padded) {
-    const size_t total = rows_padded * columns_padded;
+// A [rank, k] or B [n, rank] in the order in which the kernels' matrix instructions take them, 1 KB each,
+// eight values a lane: A's as [32-rank block][16 channels][lane], lane l having rank l % 32 and channels
+// 8 (l / 32) on; B's as [64-column step][16 ranks][32 columns of the step][lane], lane l having column
+// l % 32 and ranks 8 (l / 32) on. Zeros behind the ends, and without a source (a new adapter).
+__global__ __launch_bounds__(256) void adapter_pack(uint16_t *dst, const uint16_t *src, size_t total, size_t rank, size_t other,
+                                                    size_t inner, int second) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-        const size_t r = i / columns_padded, c = i % columns_padded;
-        dst[i] = src && r < rows && c < columns ? src[r * columns + c] : (uint16_t)0;
+        const size_t e = i % 8, lane = i / 8 % 64, at = i / 512;
+        uint16_t v = 0;
+        if (!second) {
+            const size_t r = at / inner * 32 + lane % 32, k = at % inner * 16 + lane / 32 * 8 + e;
+            if (src && r < rank && k < other) v = src[r * other + k];
+        } else {
+            const size_t c = at / 2 / inner * COLS + at % 2 * 32 + lane % 32;
+            const size_t r = at / 2 % inner * 16 + lane / 32 * 8 + e;
+            if (src && r < rank && c < other) v = src[c * rank + r];
+        }
+        dst[i] = v;
     }
 }
 
-void pack(h3_gpu *g, uint16_t *dst, const uint16_t *src, size_t rows, size_t columns, size_t rows_padded, size_t columns_padded) {
-    const size_t blocks = std::min<size_t>((rows_padded * columns_padded + 255) / 256, 4096);
-    hipLaunchKernelGGL(adapter_pack, dim3((unsigned)blocks), dim3(256), 0, g->compute, dst, src, rows, columns, rows_padded,
-                       columns_padded);
+void pack(h3_gpu *g, uint16_t *dst, const uint16_t *src, size_t total, size_t rank, size_t other, size_t inner, int second) {
+    const size_t blocks = std::min<size_t>((total + 255) / 256, 4096);
+    hipLaunchKernelGGL(adapter_pack, dim3((unsigned)blocks), dim3(256), 0, g->compute, dst, src, total, rank, other, inner, second);
 }
 
 // Shares of K for `tiles` tiles of up to `passes` * 64 ranks: about two workgroups a compute unit.
@@ -239,11 +359,13 @@ extern "C" h3_hip_adapters *h3_hip_adapters_new(h3_gpu *g, const uint32_t *ranks
     h3_hip_adapters *a = nullptr;
     size_t elements = 0;
     try {
-        a = new h3_hip_adapters{g, count, k, n, (k + KC - 1) / KC * KC, std::vector<uint32_t>(ranks, ranks + count), {}, nullptr, nullptr};
+        a = new h3_hip_adapters{g, count, k, n, (k + KC - 1) / KC * KC, (n + COLS - 1) / COLS * COLS,
+                                std::vector<uint32_t>(ranks, ranks + count), {}, nullptr, nullptr};
         for (uint32_t i = 0; i < count; i++) {
-            const uint64_t blocks = rank_blocks(ranks[i]);
-            a->entries.push_back({elements, elements + blocks * 32 * a->k_padded, (uint32_t)blocks, 0.f});
-            elements += blocks * 32 * ((size_t)a->k_padded + n);
+            const uint32_t padded = (ranks[i] + 15) / 16 * 16;
+            const size_t down = (size_t)rank_blocks(ranks[i]) * 32 * a->k_padded;
+            a->entries.push_back({elements, elements + down, padded, 0.f});
+            elements += down + (size_t)padded * a->n_padded;
         }
     } catch (const std::bad_alloc &) {
         delete a;
@@ -252,7 +374,7 @@ extern "C" h3_hip_adapters *h3_hip_adapters_new(h3_gpu *g, const uint32_t *ranks
     }
     a->weights = h3_gpu_tensor_new_bf16(g, elements);
     if (a->weights) {
-        pack(g, (uint16_t *)a->weights->data, nullptr, 0, 0, 1, elements);
+        pack(g, (uint16_t *)a->weights->data, nullptr, elements, 0, 0, 1, 0);
         a->table = h3_gpu_tensor_from_u32(g, (const uint32_t *)a->entries.data(), count * sizeof(AdapterEntry) / 4);
     }
     if (!a->table || !h3_hip_check(g, hipGetLastError(), "adapters") ||
@@ -276,8 +398,8 @@ extern "C" int h3_hip_adapters_set(h3_gpu *g, h3_hip_adapters *a, uint32_t index
         return 0;
     AdapterEntry &e = a->entries[index];
     uint16_t *w = (uint16_t *)a->weights->data;
-    pack(g, w + e.down, (const uint16_t *)down->data, rank, a->k, (size_t)e.blocks * 32, a->k_padded);
-    pack(g, w + e.up, (const uint16_t *)up->data, a->n, rank, a->n, (size_t)e.blocks * 32);
+    pack(g, w + e.down, (const uint16_t *)down->data, (size_t)rank_blocks(rank) * 32 * a->k_padded, rank, a->k, a->k_padded / 16, 0);
+    pack(g, w + e.up, (const uint16_t *)up->data, (size_t)e.ranks * a->n_padded, rank, a->n, e.ranks / 16, 1);
     hipLaunchKernelGGL(adapter_entry_scale, dim3(1), dim3(1), 0, g->compute, (AdapterEntry *)a->table->data + index, scale);
     e.scale = scale;
     return h3_launch_status(g, "adapter");
@@ -344,22 +466,23 @@ static int adapters_valid(h3_gpu *g, const h3_hip_adapters *w, const h3_hip_adap
     return 1;
 }
 
-template <bool WIDE_X, bool WIDE_OUT> static int launch_adapters(h3_gpu *g, const AdapterArgs &a, uint32_t copied) {
-    constexpr unsigned shared = 4 * 32 * LDS_ROW * 4;
+template <bool WIDE> static int launch_adapters(h3_gpu *g, const AdapterArgs &a, uint32_t copied, uint32_t blocks) {
+    constexpr unsigned shared = DOWN_WAVES * 8 * 64 * 16;
     static bool configured = false;
     if (!configured) {
-        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)adapter_up<WIDE_OUT>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)shared), "adapters' shared memory"))
+        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)adapter_down, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)shared), "adapters' shared memory") ||
+            !h3_hip_check(g, hipFuncSetAttribute((const void *)adapter_up<WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)(4 * UP_STAGE * 4 + RANK_MOST / 32 * 4096)), "adapters' shared memory"))
             return 0;
         configured = true;
     }
     if (a.tiles) {
-        hipLaunchKernelGGL(adapter_down<WIDE_X>, dim3(a.tiles * a.passes * a.splits), dim3(256), 0, g->compute, a);
+        hipLaunchKernelGGL(adapter_down, dim3(a.tiles * a.passes * a.splits), dim3(64 * DOWN_WAVES), shared, g->compute, a);
         if (!h3_launch_status(g, "adapters' first product")) return 0;
     }
-    const unsigned groups = (a.n + 4 * COLS - 1) / (4 * COLS);
     if (a.tiles + copied)
-        hipLaunchKernelGGL(adapter_up<WIDE_OUT>, dim3((a.tiles + copied) * groups), dim3(256), shared, g->compute, a);
+        hipLaunchKernelGGL(adapter_up<WIDE>, dim3((a.tiles + copied) * a.groups), dim3(256), 4 * UP_STAGE * 4 + blocks * 4096, g->compute, a);
     return h3_launch_status(g, "adapters' second product");
 }
 
@@ -374,18 +497,22 @@ extern "C" int h3_hip_adapters_add_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_
     if (out == in) return h3_set_error(g, "adapters: output aliases input");
     uint32_t blocks = 0;
     for (uint32_t rank : w->ranks) blocks = std::max(blocks, rank_blocks(rank));
-    const uint32_t groups = (n + 4 * COLS - 1) / (4 * COLS), copied = out->data == base->data ? 0 : p->plain;
+    const uint32_t copied = out->data == base->data ? 0 : p->plain, tiles = p->tiles + copied;
     const uint32_t passes = (blocks + 1) / 2, splits = std::min(p->splits, splits_for(g, p->tiles, passes));
+    // A workgroup's share of the columns, in steps of 64: few rows in one round of the three
+    // workgroups that a compute unit holds, many in four rounds and more.
+    const uint32_t steps = (n + COLS - 1) / COLS;
+    const uint64_t quads = (uint64_t)tiles * ((steps + 3) / 4), round = 3ull * g->cus;
+    const uint32_t span = 4 * (uint32_t)std::min<uint64_t>(8, std::max<uint64_t>(1, quads <= 4 * round ? (quads + round - 1) / round : quads / (4 * round)));
+    const uint32_t groups = (steps + span - 1) / span;
     // Launches hold fewer than 2^32 threads.
-    if ((uint64_t)(p->tiles + copied) * groups >= (1u << 24) || (uint64_t)p->tiles * passes * splits >= (1u << 24))
+    if ((uint64_t)tiles * groups >= (1u << 24) || (uint64_t)p->tiles * passes * splits >= (1u << 23))
         return h3_set_error(g, "adapters: %u rows by %u columns are more than a launch takes", rows, n);
     const AdapterArgs a{(uint16_t *)out->data, (const uint16_t *)base->data, (const uint16_t *)in->data,
                         (const uint16_t *)w->weights->data, (const AdapterEntry *)w->table->data,
                         (const uint32_t *)p->order->data, (const uint32_t *)p->order->data + (size_t)32 * (p->tiles + p->plain),
-                        (float *)p->sums->data, rows, w->count, k, n, w->k_padded, p->tiles, passes, splits,
-                        rank_blocks(p->max_rank) * 32};
-    if (k % 8 == 0) return n % 8 == 0 ? launch_adapters<true, true>(g, a, copied) : launch_adapters<true, false>(g, a, copied);
-    return n % 8 == 0 ? launch_adapters<false, true>(g, a, copied) : launch_adapters<false, false>(g, a, copied);
+                        (float *)p->sums->data, k, n, w->k_padded, p->tiles, passes, splits, rank_blocks(p->max_rank) * 32, groups, span};
+    return n % 8 == 0 ? launch_adapters<true>(g, a, copied, blocks) : launch_adapters<false>(g, a, copied, blocks);
 }
 
 extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *weight,

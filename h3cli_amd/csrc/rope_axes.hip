@@ -20,6 +20,7 @@
 #include "internal.h"
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 struct h3_hip_rope_axes {
@@ -37,128 +38,18 @@ struct AxesArgs {
     const float *turns;          // [pairs][2]
     const uint32_t *axis;        // [pairs]
     const float *positions;      // [rows][axes]
-    unsigned rows, heads, kv_heads, dim, pairs, axes, splits;
+    unsigned rows, heads, kv_heads, share, dim, pairs, axes, splits;
     float eps;
     int grouped, interleaved;
 };
 
 enum Kind { QUERY, KEY, VALUE };
 
-// Item i of a row's heads, queries first, then keys, then values: its source head within the
-// row, its head within its own output.
-__device__ inline unsigned source_head(const AxesArgs &a, unsigned i, unsigned &head, int &kind) {
-    kind = i < a.heads ? QUERY : i < a.heads + a.kv_heads ? KEY : VALUE;
-    head = kind == QUERY ? i : kind == KEY ? i - a.heads : i - a.heads - a.kv_heads;
-    if (!a.grouped) return i;
-    const unsigned share = a.heads / a.kv_heads;
+// Where a row has a head of its queries, keys or values.
+__device__ inline unsigned source_head(const AxesArgs &a, Kind kind, unsigned head) {
+    if (!a.grouped) return kind == QUERY ? head : kind == KEY ? a.heads + head : a.heads + a.kv_heads + head;
+    const unsigned share = a.share;
     return kind == QUERY ? head / share * (share + 2) + head % share : head * (share + 2) + share + (kind == VALUE);
-}
-
-__device__ inline void phase(const AxesArgs &a, size_t row, unsigned pair, float &c, float &s) {
-    const float p = a.positions[row * a.axes + a.axis[pair]];
-    const float hi = a.turns[2 * pair], lo = a.turns[2 * pair + 1];
-    const float t = fmaf(p, lo, fmaf(p, hi, -rintf(p * hi)));
-    c = __builtin_amdgcn_cosf(t);
-    s = __builtin_amdgcn_sinf(t);
-}
-
-__device__ inline float wave_sum(float v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
-}
-
-// Any head width up to 256 and any number of pairs: a wave per head, two channels a lane and
-// 128 channels a step; partners go through LDS.
-__global__ __launch_bounds__(256) void rope_axes_any(AxesArgs a) {
-    __shared__ float stage[4][256];
-    const unsigned wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-    const unsigned items = a.heads + 2 * a.kv_heads;
-    const bool wide = a.dim % 2 == 0;                      // every head then starts on four bytes
-    for (size_t block = blockIdx.x; block < (size_t)a.rows * a.splits; block += gridDim.x) {
-        const size_t row = block / a.splits;
-        const unsigned part = block % a.splits;
-        // Channel d = 128 i + 2 lane + e: its partner and the factors of both.
-        unsigned partner[2][2];
-        float own[2][2], other[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const unsigned d = 128 * i + 2 * lane + e;
-                partner[i][e] = min(d, a.dim - 1);
-                own[i][e] = 1.f;
-                other[i][e] = 0.f;
-                if (d < 2 * a.pairs) {
-                    const bool second = a.interleaved ? d % 2 : d >= a.pairs;
-                    const unsigned pair = a.interleaved ? d / 2 : second ? d - a.pairs : d;
-                    phase(a, row, pair, own[i][e], other[i][e]);
-                    if (!second) other[i][e] = -other[i][e];
-                    partner[i][e] = a.interleaved ? d ^ 1 : second ? d - a.pairs : d + a.pairs;
-                }
-            }
-        for (unsigned item = part * 4 + wave; item < items; item += a.splits * 4) {
-            unsigned head;
-            int kind;
-            const unsigned from = source_head(a, item, head, kind);
-            const uint16_t *src = a.qkv + (row * items + from) * a.dim;
-            uint16_t *dst = kind == QUERY ? a.q + (row * a.heads + head) * a.dim
-                                          : (kind == KEY ? a.k : a.v) + (row * a.kv_heads + head) * a.dim;
-            const uint16_t *w = kind == QUERY ? a.qw : kind == KEY ? a.kw : nullptr;
-            uint16_t raw[2][2] = {};
-            float x[2][2], sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const unsigned d = 128 * i + 2 * lane;
-                if (d >= a.dim) continue;
-                if (wide) {
-                    const uint32_t both = *reinterpret_cast<const uint32_t *>(src + d);
-                    raw[i][0] = both & 0xffff;
-                    raw[i][1] = both >> 16;
-                } else {
-                    raw[i][0] = src[d];
-                    if (d + 1 < a.dim) raw[i][1] = src[d + 1];
-                }
-            }
-            if (kind != VALUE) {
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const unsigned d = 128 * i + 2 * lane + e;
-                        x[i][e] = bf16_to_f32(raw[i][e]);
-                        sum = fmaf(x[i][e], x[i][e], sum);
-                        if (w && d < a.dim) x[i][e] *= bf16_to_f32(w[d]);
-                        stage[wave][d] = x[i][e];
-                    }
-                const float r = w ? rsqrtf(wave_sum(sum) / (float)a.dim + a.eps) : 1.f;
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own stores
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-                    {
-                        // Channels behind the pairs pass as they are, infinities too.
-                        const bool turned = 128 * i + 2 * lane + e < 2 * a.pairs;
-                        raw[i][e] = f32_to_bf16(r * (turned ? fmaf(x[i][e], own[i][e], stage[wave][partner[i][e]] * other[i][e])
-                                                            : x[i][e]));
-                    }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the next head's
-                __builtin_amdgcn_wave_barrier();
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const unsigned d = 128 * i + 2 * lane;
-                if (d >= a.dim) continue;
-                if (wide) *reinterpret_cast<uint32_t *>(dst + d) = raw[i][0] | (uint32_t)raw[i][1] << 16;
-                else {
-                    dst[d] = raw[i][0];
-                    if (d + 1 < a.dim) dst[d + 1] = raw[i][1];
-                }
-            }
-        }
-    }
 }
 
 // Sums over the 16 / 8 / 32 lanes of a head by row rotations of the VALU; every lane gets the
@@ -176,147 +67,179 @@ template <int LANES> __device__ inline float head_sum(float v) {
     return v;
 }
 
-// Heads of 8 * CHUNKS channels, CHUNKS <= LANES a power of two: LANES lanes a head, a 16-byte chunk each.
-// A workgroup takes a row (or a share of its heads) and goes through the heads 256 / LANES at
-// a time, UNROLL of them in flight a lane. Pairs of halves need pairs % 8 == 0 (a chunk's partner
-// is a chunk, fetched from its lane), interleaved ones pairs % 4 == 0 (partners are in the chunk).
-template <int LANES, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void rope_axes_chunks(AxesArgs a) {
+// Eight values from any element on. Global memory takes 16-byte accesses at any two bytes; what
+// lies behind a tensor's end is within its allocation.
+// Values stay packed, two a register, until they are used.
+struct __attribute__((packed, aligned(2))) Loose { i32x4 v; };
+__device__ inline i32x4 load_loose(const uint16_t *p) { return reinterpret_cast<const Loose *>(p)->v; }
+__device__ inline float value(const i32x4 &v, int e) {
+    return __builtin_bit_cast(float, e % 2 ? (uint32_t)v[e / 2] & 0xffff0000u : (uint32_t)v[e / 2] << 16);
+}
+__device__ inline void put(i32x4 &v, int e, uint16_t bits) { v[e / 2] |= (uint32_t)bits << (e % 2 * 16); }
+
+// How a channel finds its partner.
+enum Pairing {
+    HALVES,          // j and j + pairs, pairs % 8 == 0: a chunk's partner is another lane's chunk
+    HALVES_LOOSE,    // any number of pairs: loaded again, from the caches
+    NEIGHBOURS,      // 2 j and 2 j + 1: in the chunk
+};
+
+// LANES lanes a head, a chunk of eight channels each (the last one cut off where the head ends).
+// A workgroup takes rows, or a share of their heads, and goes through a row's queries, keys and
+// values 256 / LANES heads at a time, UNROLL of them in flight a lane. Thread d makes what channel
+// d and its partner are multiplied with in the next row, the norms' weights included, while this
+// one's heads are on their way; lanes take their chunk's from LDS.
+template <int LANES, Pairing PAIRING>
+__global__ __launch_bounds__(256, PAIRING == HALVES_LOOSE ? 4 : 5) void rope_axes_chunks(AxesArgs a) {
     constexpr int GROUPS = 256 / LANES, UNROLL = 4;
-    const unsigned lane = threadIdx.x % 64, c = lane % LANES, group = threadIdx.x / LANES;
-    const unsigned items = a.heads + 2 * a.kv_heads, chunks = a.dim / 8;
-    const bool held = c < chunks;
-    const unsigned half = INTERLEAVED ? 0 : a.pairs / 8;
-    const bool turned = INTERLEAVED ? c < a.pairs / 4 : c < 2 * half;
-    const bool second = !INTERLEAVED && c >= half;
-    const int partner = (int)(turned && !INTERLEAVED ? lane + (second ? 0u - half : half) : lane) * 4;
+    // [buffer][query, key][channel, partner][channel]
+    __shared__ __attribute__((aligned(16))) float factors[2][2][2][256];
+    const unsigned tid = threadIdx.x, lane = tid % 64, c = lane % LANES, d0 = c * 8, group = tid / LANES;
+    const unsigned items = a.heads + 2 * a.kv_heads;
+    const bool held = d0 < a.dim, whole = d0 + 8 <= a.dim;
     const float inv_dim = 1.f / (float)a.dim;
-    u16x8 wq{}, wk{}, pq{}, pk{};
-    if (a.qw && held) {
-        const unsigned pc = turned && !INTERLEAVED ? (second ? c - half : c + half) : c;
-        wq = *reinterpret_cast<const u16x8 *>(a.qw + c * 8);
-        wk = *reinterpret_cast<const u16x8 *>(a.kw + c * 8);
-        pq = *reinterpret_cast<const u16x8 *>(a.qw + pc * 8);
-        pk = *reinterpret_cast<const u16x8 *>(a.kw + pc * 8);
+    // Channel tid: its pair, whether it is the pair's first, its partner.
+    const bool turns = tid < 2 * a.pairs, first_channel = PAIRING == NEIGHBOURS ? tid % 2 == 0 : tid < a.pairs;
+    const unsigned pair = PAIRING == NEIGHBOURS ? tid / 2 : first_channel ? tid : tid - a.pairs;
+    const unsigned partner_channel = !turns ? tid : PAIRING == NEIGHBOURS ? tid ^ 1 : first_channel ? tid + a.pairs : tid - a.pairs;
+    float hi = 0.f, lo = 0.f, weight[2] = {1.f, 1.f}, partner_weight[2] = {1.f, 1.f};
+    unsigned axis = 0;
+    if (turns) {
+        hi = a.turns[2 * pair];
+        lo = a.turns[2 * pair + 1];
+        axis = a.axis[pair];
     }
-    for (size_t block = blockIdx.x; block < (size_t)a.rows * a.splits; block += gridDim.x) {
+    if (a.qw && tid < a.dim) {
+        weight[QUERY] = bf16_to_f32(a.qw[tid]);
+        weight[KEY] = bf16_to_f32(a.kw[tid]);
+        partner_weight[QUERY] = bf16_to_f32(a.qw[partner_channel]);
+        partner_weight[KEY] = bf16_to_f32(a.kw[partner_channel]);
+    }
+    const size_t blocks = (size_t)a.rows * a.splits;
+    auto position = [&](size_t block) { return turns && block < blocks ? a.positions[block / a.splits * a.axes + axis] : 0.f; };
+    auto turn = [&](float p, int buffer) {
+        const float t = fmaf(p, lo, fmaf(p, hi, -rintf(p * hi)));
+        const float cs = turns ? __builtin_amdgcn_cosf(t) : 1.f, sn = turns ? __builtin_amdgcn_sinf(t) : 0.f;
+#pragma unroll
+        for (int kind = QUERY; kind <= KEY; kind++) {
+            factors[buffer][kind][0][tid] = cs * weight[kind];
+            factors[buffer][kind][1][tid] = (first_channel ? -sn : sn) * partner_weight[kind];
+        }
+    };
+    turn(position(blockIdx.x), 0);
+    __syncthreads();
+    int buffer = 0;
+    for (size_t block = blockIdx.x; block < blocks; block += gridDim.x, buffer ^= 1) {
         const size_t row = block / a.splits;
         const unsigned part = block % a.splits;
-        // Channel e of the chunk: what it and its partner are multiplied with.
-        float oq[8], tq[8], ok[8], tk[8];
-        {
-            float cs[8], sn[8];
+        const float next = position(block + gridDim.x);
+        const size_t row_at = row * items * a.dim;
+        auto heads = [&](auto kind_tag) {
+            constexpr Kind kind = decltype(kind_tag)::value;
+            const unsigned count = kind == QUERY ? a.heads : a.kv_heads;
+            f32x4 own[2], other[2];
+            if constexpr (kind != VALUE)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                cs[e] = 1.f;
-                sn[e] = 0.f;
-            }
-            if (turned) {
+                for (int i = 0; i < 2; i++) {
+                    own[i] = *reinterpret_cast<const f32x4 *>(&factors[buffer][kind][0][d0 + 4 * i]);
+                    other[i] = *reinterpret_cast<const f32x4 *>(&factors[buffer][kind][1][d0 + 4 * i]);
+                }
+            uint16_t *const out = (kind == QUERY ? a.q : kind == KEY ? a.k : a.v) + row * count * a.dim + d0;
+            for (unsigned first = part * GROUPS + group; first < count; first += a.splits * GROUPS * UNROLL) {
+                i32x4 raw[UNROLL] = {}, up[UNROLL] = {}, low[UNROLL] = {};
 #pragma unroll
-                for (int e = 0; e < 8; e += INTERLEAVED ? 2 : 1) {
-                    const unsigned pair = INTERLEAVED ? c * 4 + e / 2 : (second ? c - half : c) * 8 + e;
-                    phase(a, row, pair, cs[e], sn[e]);
-                    if constexpr (INTERLEAVED) {
-                        cs[e + 1] = cs[e];
-                        sn[e + 1] = sn[e];
-                        sn[e] = -sn[e];
-                    } else if (!second) {
-                        sn[e] = -sn[e];
+                for (int u = 0; u < UNROLL; u++) {
+                    const unsigned head = first + u * a.splits * GROUPS;
+                    if (head >= count || !held) continue;
+                    const size_t at = row_at + (size_t)source_head(a, kind, head) * a.dim + d0;
+                    raw[u] = load_loose(a.qkv + at);
+                    if (PAIRING == HALVES_LOOSE && kind != VALUE) {
+                        if (d0 < a.pairs) up[u] = load_loose(a.qkv + at + a.pairs);
+                        if (d0 + 7 >= a.pairs && d0 < 2 * a.pairs) {
+                            if (at >= a.pairs) low[u] = load_loose(a.qkv + (at - a.pairs));
+                            else   // the first head's chunk across the middle: its partners start behind the tensor's first value
+#pragma unroll
+                                for (int e = 0; e < 8; e++)
+                                    if (at + e >= a.pairs) put(low[u], e, a.qkv[at + e - a.pairs]);
+                        }
                     }
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int pe = INTERLEAVED ? e ^ 1 : e;
-                oq[e] = a.qw ? cs[e] * bf16_to_f32(wq[e]) : cs[e];
-                ok[e] = a.qw ? cs[e] * bf16_to_f32(wk[e]) : cs[e];
-                tq[e] = a.qw ? sn[e] * bf16_to_f32(pq[pe]) : sn[e];
-                tk[e] = a.qw ? sn[e] * bf16_to_f32(pk[pe]) : sn[e];
-            }
-        }
-        const uint16_t *const src = a.qkv + row * items * a.dim + c * 8;
-        for (unsigned first = part * GROUPS + group; first < items; first += a.splits * GROUPS * UNROLL) {
-            u16x8 raw[UNROLL] = {};
+                for (int u = 0; u < UNROLL; u++) {
+                    const unsigned head = first + u * a.splits * GROUPS;
+                    if (head >= count) break;
+                    if constexpr (kind != VALUE) {
+                        float x[8], y[8], sum = 0.f;
 #pragma unroll
-            for (int u = 0; u < UNROLL; u++) {
-                const unsigned item = first + u * a.splits * GROUPS;
-                unsigned head;
-                int kind;
-                if (item < items && held)
-                    raw[u] = *reinterpret_cast<const u16x8 *>(src + (size_t)source_head(a, item, head, kind) * a.dim);
-            }
+                        for (int e = 0; e < 8; e++) {
+                            x[e] = PAIRING == HALVES || d0 + e < a.dim ? value(raw[u], e) : 0.f;
+                            sum = fmaf(x[e], x[e], sum);
+                        }
+                        const float r = a.qw ? rsqrtf(head_sum<LANES>(sum) * inv_dim + a.eps) : 1.f;
+                        if constexpr (PAIRING == HALVES) {
+                            const bool turned = d0 < 2 * a.pairs;
+                            const int partner = (int)(turned ? d0 < a.pairs ? lane + a.pairs / 8 : lane - a.pairs / 8 : lane) * 4;
+                            i32x4 theirs;
 #pragma unroll
-            for (int u = 0; u < UNROLL; u++) {
-                const unsigned item = first + u * a.splits * GROUPS;
-                if (item >= items) break;
-                unsigned head;
-                int kind;
-                source_head(a, item, head, kind);
-                uint16_t *const dst = (kind == QUERY ? a.q + (row * a.heads + head) * a.dim
-                                                     : (kind == KEY ? a.k : a.v) + (row * a.kv_heads + head) * a.dim) + c * 8;
-                if (kind != VALUE) {
-                    float x[8], sum = 0.f;
+                            for (int e = 0; e < 4; e++) {
+                                theirs[e] = __builtin_amdgcn_ds_bpermute(partner, raw[u][e]);
+                                theirs[e] = turned ? theirs[e] : 0;
+                            }
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[e] = bf16_to_f32(raw[u][e]);
-                        sum = fmaf(x[e], x[e], sum);
+                            for (int e = 0; e < 8; e++) y[e] = value(theirs, e);
+                        } else {
+                            // Channels behind the pairs pass as they are, infinities too.
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                const unsigned d = d0 + e;
+                                const float theirs = PAIRING == NEIGHBOURS ? x[e ^ 1] : d < a.pairs ? value(up[u], e) : value(low[u], e);
+                                y[e] = d < 2 * a.pairs ? theirs : 0.f;
+                            }
+                        }
+                        bf16x8 result;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) result[e] = (__bf16)(r * fmaf(x[e], own[e / 4][e % 4], y[e] * other[e / 4][e % 4]));
+                        raw[u] = __builtin_bit_cast(i32x4, result);
                     }
-                    const float r = a.qw ? rsqrtf(head_sum<LANES>(sum) * inv_dim + a.eps) : 1.f;
-                    float y[8];
-                    if constexpr (INTERLEAVED) {
+                    uint16_t *const dst = out + (size_t)head * a.dim;
+                    if (whole) reinterpret_cast<Loose *>(dst)->v = raw[u];
+                    else if (held)
 #pragma unroll
-                        for (int e = 0; e < 8; e++) y[e] = turned ? x[e ^ 1] : 0.f;
-                    } else {
-                        const i32x4 own = __builtin_bit_cast(i32x4, raw[u]);
-                        i32x4 other;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) other[e] = __builtin_amdgcn_ds_bpermute(partner, own[e]);
-                        // Channels behind the pairs pass as they are, infinities too.
-#pragma unroll
-                        for (int e = 0; e < 4; e++) other[e] = turned ? other[e] : 0;
-                        const u16x8 o = __builtin_bit_cast(u16x8, other);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) y[e] = bf16_to_f32(o[e]);
-                    }
-                    if (kind == QUERY)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) raw[u][e] = f32_to_bf16(r * fmaf(x[e], oq[e], y[e] * tq[e]));
-                    else
-#pragma unroll
-                        for (int e = 0; e < 8; e++) raw[u][e] = f32_to_bf16(r * fmaf(x[e], ok[e], y[e] * tk[e]));
+                        for (int e = 0; e < 8; e++)
+                            if (d0 + e < a.dim) dst[e] = (uint16_t)((uint32_t)raw[u][e / 2] >> (e % 2 * 16));
                 }
-                if (held) *reinterpret_cast<u16x8 *>(dst) = raw[u];
             }
-        }
+        };
+        heads(std::integral_constant<Kind, QUERY>{});
+        heads(std::integral_constant<Kind, KEY>{});
+        heads(std::integral_constant<Kind, VALUE>{});
+        turn(next, buffer ^ 1);
+        __syncthreads();
     }
 }
 
 template <int LANES> void launch_chunks(h3_gpu *g, AxesArgs a) {
-    const unsigned items = a.heads + 2 * a.kv_heads;
     constexpr unsigned GROUPS = 256 / LANES;
     // A row's heads go to more workgroups where the rows alone would not fill the chip.
-    a.splits = (unsigned)std::min<size_t>((items + GROUPS - 1) / GROUPS, (2048 + (size_t)a.rows - 1) / a.rows);
-    const unsigned blocks = (unsigned)std::min<size_t>((size_t)a.rows * a.splits, 1 << 20);
-    if (a.interleaved) hipLaunchKernelGGL((rope_axes_chunks<LANES, true>), dim3(blocks), dim3(256), 0, g->compute, a);
-    else hipLaunchKernelGGL((rope_axes_chunks<LANES, false>), dim3(blocks), dim3(256), 0, g->compute, a);
+    a.splits = (unsigned)std::min<size_t>((a.heads + GROUPS - 1) / GROUPS, (2048 + (size_t)a.rows - 1) / a.rows);
+    // A few rows a workgroup: with as many workgroups as run at once the last ones end the call (18,225
+    // rows: 311 us, 313 with twice, 307 with four times and 293 with twenty times as many).
+    const size_t tasks = (size_t)a.rows * a.splits, each = (tasks + 64 * g->cus - 1) / (64 * g->cus);
+    const unsigned blocks = (unsigned)((tasks + each - 1) / each);
+    const Pairing pairing = a.interleaved ? NEIGHBOURS : a.dim % 8 == 0 && a.pairs % 8 == 0 ? HALVES : HALVES_LOOSE;
+    auto *kernel = pairing == NEIGHBOURS ? rope_axes_chunks<LANES, NEIGHBOURS>
+                   : pairing == HALVES   ? rope_axes_chunks<LANES, HALVES>
+                                         : rope_axes_chunks<LANES, HALVES_LOOSE>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, g->compute, a);
 }
 
-int rope_axes(h3_gpu *g, const AxesArgs &args) {
-    AxesArgs a = args;
-    if (a.dim % 8 == 0 && a.pairs % (a.interleaved ? 4 : 8) == 0) {
-        const unsigned chunks = a.dim / 8;
-        if (chunks <= 2) launch_chunks<2>(g, a);
-        else if (chunks <= 4) launch_chunks<4>(g, a);
-        else if (chunks <= 8) launch_chunks<8>(g, a);
-        else if (chunks <= 16) launch_chunks<16>(g, a);
-        else launch_chunks<32>(g, a);
-        return h3_launch_status(g, "QKV norm/RoPE by axes");
-    }
-    const unsigned items = a.heads + 2 * a.kv_heads;
-    // A row's heads go to more workgroups where the rows alone would not fill the chip.
-    a.splits = (unsigned)std::min<size_t>((items + 3) / 4, (4096 + (size_t)a.rows - 1) / a.rows);
-    const size_t blocks = std::min<size_t>((size_t)a.rows * a.splits, 1 << 20);
-    hipLaunchKernelGGL(rope_axes_any, dim3((unsigned)blocks), dim3(256), 0, g->compute, a);
+int rope_axes(h3_gpu *g, const AxesArgs &a) {
+    const unsigned chunks = (a.dim + 7) / 8;
+    if (chunks <= 2) launch_chunks<2>(g, a);
+    else if (chunks <= 4) launch_chunks<4>(g, a);
+    else if (chunks <= 8) launch_chunks<8>(g, a);
+    else if (chunks <= 16) launch_chunks<16>(g, a);
+    else launch_chunks<32>(g, a);
     return h3_launch_status(g, "QKV norm/RoPE by axes");
 }
 
@@ -374,7 +297,8 @@ extern "C" int h3_hip_qkv_rope_axes_bf16(h3_gpu *g, h3_gpu_tensor *q, h3_gpu_ten
     const AxesArgs a{(uint16_t *)q->data, (uint16_t *)k->data, (uint16_t *)v->data, (const uint16_t *)qkv->data,
                      qw ? (const uint16_t *)qw->data : nullptr, kw ? (const uint16_t *)kw->data : nullptr,
                      (const float *)rope->table->data, (const uint32_t *)rope->table->data + 2 * rope->pairs,
-                     (const float *)positions->data, rows, heads, kv_heads, dim, rope->pairs, rope->axes, 1, eps, grouped,
+                     (const float *)positions->data, rows, heads, kv_heads, heads / kv_heads, dim, rope->pairs,
+                     rope->axes, 1, eps, grouped,
                      rope->interleaved};
     return rope_axes(g, a);
 }
