@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
             }
             if (row[i] == NONE || c >= a.n) continue;
             uint16_t *const out = a.out + (size_t)row[i] * a.n + c;
-            if constexpr (WIDE) *reinterpret_cast<i32x4 *>(out) = v[i];
+            if constexpr (WIDE) __builtin_nontemporal_store(v[i], reinterpret_cast<i32x4 *>(out));
             else if (c + 8 <= a.n) reinterpret_cast<Loose *>(out)->v = v[i];
             else
 #pragma unroll

@@ -345,12 +345,17 @@ __global__ __launch_bounds__(256) void attn_sequences_join(SeqArgs a) {
     for (unsigned i = tid; i < rows * (D / 4); i += 256) {
         const unsigned r = i / (D / 4), d = i % (D / 4) * 4, v = item.block * 32 + r;
         f32x4 x{};
-#pragma unroll 4
-        for (unsigned p = 0; p < item.parts; p++) {
-            const f32x4 y = *reinterpret_cast<const f32x4 *>(first + p * step + r * D + d);
-            const float w = weight[r][p];
+        // Eight parts on their way at a time; those behind the last are the last again, for nothing.
+        for (unsigned p0 = 0; p0 < item.parts; p0 += 8) {
+            f32x4 y[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = fmaf(w, y[e], x[e]);
+            for (unsigned p = 0; p < 8; p++) y[p] = *reinterpret_cast<const f32x4 *>(first + min(p0 + p, item.parts - 1) * step + r * D + d);
+#pragma unroll
+            for (unsigned p = 0; p < 8; p++) {
+                const float w = p0 + p < item.parts ? weight[r][p0 + p] : 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = p0 + p < item.parts ? fmaf(w, y[p][e], x[e]) : x[e];
+            }
         }
         u16x4 out;
 #pragma unroll
