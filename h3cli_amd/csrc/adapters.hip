@@ -18,6 +18,7 @@
 #include "internal.h"
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 struct AdapterEntry {
@@ -60,14 +61,20 @@ struct AdapterArgs {
     const AdapterEntry *table;
     const uint32_t *order, *adapter;       // [32 tiles], [tiles]
     float *sums;
+    const uint16_t *w, *bias;              // adapter_gemm
+    unsigned plain;
     unsigned k, n, k_padded, tiles, passes, splits, rank_padded;
     unsigned groups, span;                 // adapter_up: workgroups of a tile, their steps of columns
 };
 
-// Eight values from any element on. Global memory takes 16-byte accesses at any two bytes; what
-// lies behind a tensor's end is within its allocation.
+// Eight values from any element on. Global memory takes 16-byte accesses at any two bytes. What lies up
+// to 256 bytes behind a tensor's end, more than a step of 64 values, is within its allocation.
 struct __attribute__((packed, aligned(2))) Loose { i32x4 v; };
 __device__ inline i32x4 load_loose(const uint16_t *p) { return reinterpret_cast<const Loose *>(p)->v; }
+
+// Where chunk c of row r is in LDS, rows of eight 16-byte chunks: sixteen rows' reads of one chunk meet
+// sixteen groups of banks.
+__device__ inline unsigned swizzled(unsigned r, unsigned c) { return r * 8 + (c ^ r / 2 % 8); }
 
 // The wave's own LDS writes are there, for all its lanes.
 __device__ inline void wait_lds() {
@@ -88,7 +95,7 @@ __global__ __launch_bounds__(64 * DOWN_WAVES, 2) void adapter_down(AdapterArgs a
     const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
     if (pass * 64 >= entry.ranks) return;
     const bool both = pass * 64 + 32 < entry.ranks;
-    // Lane's chunk lane % 8 of rows lane / 8 + 8 i; row r keeps chunk c at c ^ r % 8.
+    // Lane's chunk lane % 8 of rows lane / 8 + 8 i; row r keeps chunk c at swizzled(r, c).
     const unsigned chunk = lane % 8 * 8;
     const uint16_t *xr[4];
 #pragma unroll
@@ -100,51 +107,56 @@ __global__ __launch_bounds__(64 * DOWN_WAVES, 2) void adapter_down(AdapterArgs a
     i32x4 *const buffer = reinterpret_cast<i32x4 *>(part + wave * 1024);
     const size_t block_size = (size_t)a.k_padded * 32;
     const uint16_t *const down = a.weights + entry.down + pass * 2 * block_size + lane * 8;
+    const unsigned steps = a.k_padded / KC, stride = a.splits * DOWN_WAVES, begin = split * DOWN_WAVES + wave;
     f32x16 acc[2] = {};
-    i32x4 x[2][4];
-    auto load = [&](int slot, unsigned step) {
+    // Loads are made whatever comes of them (behind a row's end, behind the last step): under a
+    // condition each would be waited for where it is made.
+    auto sum = [&](auto blocks_tag) {
+        constexpr int BLOCKS = decltype(blocks_tag)::value;
+        i32x4 x[2][4];
+        auto load = [&](int slot, unsigned step) {
+            step = min(step, steps - 1);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[slot][i] = i32x4{};
-            if (step * KC + chunk < a.k) x[slot][i] = load_loose(xr[i] + step * KC);
-        }
-    };
-    auto multiply = [&](int slot, unsigned step) {
-        i32x4 w[2][4];
+            for (int i = 0; i < 4; i++) x[slot][i] = load_loose(xr[i] + step * KC);
+        };
+        auto multiply = [&](int slot, unsigned step) {
+            i32x4 w[BLOCKS][4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int b = 0; b < 2; b++)
-                if (b == 0 || both) w[b][j] = *reinterpret_cast<const i32x4 *>(down + b * block_size + (size_t)(step * 4 + j) * 512);
-        if (step * KC + KC > a.k)   // what lies behind the row's end is another row's
+                for (int b = 0; b < BLOCKS; b++)
+                    w[b][j] = *reinterpret_cast<const i32x4 *>(down + b * block_size + (size_t)(step * 4 + j) * 512);
+            if (step * KC + KC > a.k)   // what lies behind the row's end is another row's
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (unsigned e = 0; e < 8; e++)
-                    if (step * KC + chunk + e >= a.k) x[slot][i][e / 2] &= e % 2 ? 0x0000ffff : 0xffff0000;
-        wait_lds();                     // the last step's reads
+                    for (unsigned e = 0; e < 8; e++)
+                        if (step * KC + chunk + e >= a.k) x[slot][i][e / 2] &= e % 2 ? 0x0000ffff : 0xffff0000;
+            wait_lds();                 // the last step's reads
 #pragma unroll
-        for (int i = 0; i < 4; i++) buffer[(lane / 8 + 8 * i) * 8 + (lane % 8 ^ lane / 8)] = x[slot][i];
-        wait_lds();
+            for (int i = 0; i < 4; i++) buffer[swizzled(lane / 8 + 8 * i, lane % 8)] = x[slot][i];
+            wait_lds();
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bf16x8 v = __builtin_bit_cast(bf16x8, buffer[n * 8 + ((j * 2 + hf) ^ n % 8)]);
+            for (int j = 0; j < 4; j++) {
+                const bf16x8 v = __builtin_bit_cast(bf16x8, buffer[swizzled(n, j * 2 + hf)]);
 #pragma unroll
-            for (int b = 0; b < 2; b++)
-                if (b == 0 || both)
+                for (int b = 0; b < BLOCKS; b++)
                     acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w[b][j]), v, acc[b], 0, 0, 0);
+            }
+        };
+        if (begin >= steps) return;
+        load(0, begin);
+        load(1, begin + stride);
+        for (unsigned step = begin; step < steps; step += 2 * stride) {
+            multiply(0, step);
+            load(0, step + 2 * stride);
+            if (step + stride >= steps) break;
+            multiply(1, step + stride);
+            load(1, step + 3 * stride);
         }
     };
-    const unsigned steps = a.k_padded / KC, stride = a.splits * DOWN_WAVES;
-    unsigned step = split * DOWN_WAVES + wave;
-    if (step < steps) load(0, step);
-    for (; step < steps; step += 2 * stride) {
-        if (step + stride < steps) load(1, step + stride);
-        multiply(0, step);
-        if (step + stride >= steps) break;
-        if (step + 2 * stride < steps) load(0, step + 2 * stride);
-        multiply(1, step + stride);
-    }
+    if (both) sum(std::integral_constant<int, 2>{});
+    else sum(std::integral_constant<int, 1>{});
     __syncthreads();                    // the sums take the buffers' place
 #pragma unroll
     for (int b = 0; b < 2; b++)
@@ -192,28 +204,26 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
     const unsigned sixteens = entry.ranks / 16;
     const uint16_t *const up = a.weights + entry.up + lane * 8;
     i32x4 next_v[4] = {}, next_w[4] = {};
+    // Loads are made whatever comes of them (padding rows read row 0, columns behind the end the next
+    // row's): under a condition each would be waited for where it is made.
     auto load_base = [&](unsigned step) {
-        const unsigned c = step * COLS + chunk;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (row[i] != NONE && c < a.n) {
-                const uint16_t *const p = a.base + (size_t)row[i] * a.n + c;
-                if constexpr (WIDE) next_v[i] = *reinterpret_cast<const i32x4 *>(p);
-                else next_v[i] = load_loose(p);
-            }
+        for (int i = 0; i < 4; i++) {
+            const uint16_t *const p = a.base + (size_t)(row[i] == NONE ? 0 : row[i]) * a.n + step * COLS + chunk;
+            if constexpr (WIDE) next_v[i] = *reinterpret_cast<const i32x4 *>(p);
+            else next_v[i] = load_loose(p);
+        }
     };
-    // 32 ranks of the step's 64 columns, or the last 16.
+    // 32 ranks of the step's 64 columns, the last 16 once more where they end.
     auto load_up = [&](unsigned step, unsigned r) {
 #pragma unroll
         for (unsigned i = 0; i < 4; i++)
-            if (i < 2 || r + 1 < sixteens) next_w[i] = *reinterpret_cast<const i32x4 *>(up + (((size_t)step * sixteens + r) * 2 + i) * 512);
+            next_w[i] = *reinterpret_cast<const i32x4 *>(up + (((size_t)step * sixteens + min(r + i / 2, sixteens - 1)) * 2 + i % 2) * 512);
     };
     unsigned step = group * a.span + wave;
-    if (step < last) {
-        load_base(step);
-        if (adapted) load_up(step, 0);
-    }
+    load_base(min(step, steps - 1));
     if (adapted) {
+        load_up(min(step, steps - 1), 0);
         for (unsigned i = threadIdx.x; i < sixteens * 64; i += 256) {
             // Lane i % 64 of rank step i / 64: eight ranks of its row.
             const unsigned from = i / 64 * 16 + i % 64 / 32 * 8;
@@ -241,7 +251,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
         i32x4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = next_v[i];
-        const bool more = step + 4 < last;
+        const unsigned following = step + 4 < last ? step + 4 : step;   // behind the last one this one, for nothing
         if (adapted) {
             f32x16 acc[2] = {};
             for (unsigned first = 0; first < sixteens; first += 2) {
@@ -249,9 +259,9 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) w[i] = next_w[i];
                 if (first + 2 < sixteens) load_up(step, first + 2);
-                else if (more) {
-                    load_base(step + 4);
-                    load_up(step + 4, 0);
+                else {
+                    load_base(following);
+                    load_up(following, 0);
                 }
 #pragma unroll
                 for (unsigned r = 0; r < 2; r++) {
@@ -274,8 +284,8 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
                     *reinterpret_cast<f32x4 *>(stage + n * STAGE_ROW + b * 32 + q * 8 + hf * 4) =
                         f32x4{acc[b][4 * q], acc[b][4 * q + 1], acc[b][4 * q + 2], acc[b][4 * q + 3]};
             wait_lds();
-        } else if (more) {
-            load_base(step + 4);
+        } else {
+            load_base(following);
         }
         const unsigned c = step * COLS + chunk;
 #pragma unroll
@@ -301,6 +311,151 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
                     if (c + e < a.n) out[e] = (uint16_t)((uint32_t)v[i][e / 2] >> (e % 2 * 16));
         }
         wait_lds();                     // the stage's reads, before the next step's products
+    }
+}
+
+// out = x . W^T + bias + the adapters' parts in one sum and one rounding, for BF16 weights whose K is
+// no multiple of 64, which the tiled projections do not take. Four waves hold 64 R rows (tiles of
+// the rows' plan, so rows of any order) by 64 R columns, 32 R by 32 R each, and go through K
+// 64 channels at a time: x and W through two LDS buffers (16-byte chunks XOR-swizzled), the next
+// DEPTH steps' values on their way in registers. The adapters' ranks then continue the sum, each row block with
+// its adapter's. Bound by the chip's fill at small shapes and by the matrix cores and LDS alike
+// at large ones.
+template <int R>
+__global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
+    constexpr unsigned SIDE = 64 * R, LOADS = SIDE / 32, DEPTH = R == 1 ? 4 : 2;   // LOADS: chunks of each operand a thread
+    extern __shared__ __attribute__((aligned(16))) i32x4 lds[];   // [buffer][x, W][SIDE rows of 8 chunks]; then a stage a wave
+    const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, n = lane % 32, hf = lane / 32;
+    const unsigned tiles_n = (a.n + SIDE - 1) / SIDE, tiles_m = (a.tiles + a.plain + 2 * R - 1) / (2 * R);
+    // Columns fastest in bands of eight row tiles, so that what runs together shares both operands.
+    const unsigned band = blockIdx.x / (8 * tiles_n), rows_here = min(8u, tiles_m - band * 8), in_band = blockIdx.x - band * 8 * tiles_n;
+    const unsigned tm = band * 8 + in_band % rows_here, n0 = in_band / rows_here * SIDE, tile0 = tm * 2 * R;
+    const unsigned all = a.tiles + a.plain, chunk = tid % 8 * 8;
+    const uint16_t *xr[LOADS], *wr[LOADS];
+#pragma unroll
+    for (unsigned i = 0; i < LOADS; i++) {
+        const unsigned r = tid / 8 + 32 * i, tile = min(tile0 + r / 32, all - 1);
+        uint32_t row = a.order[tile * 32 + r % 32];
+        if (row == NONE) row = a.order[tile * 32];
+        xr[i] = a.x + (size_t)row * a.k + chunk;
+        wr[i] = a.w + (size_t)min(n0 + r, a.n - 1) * a.k + chunk;
+    }
+    i32x4 x[DEPTH][LOADS], w[DEPTH][LOADS];
+    const unsigned steps = (a.k + KC - 1) / KC;
+    auto load = [&](unsigned slot, unsigned step) {   // behind the last step for nothing
+        step = min(step, steps - 1);
+#pragma unroll
+        for (unsigned i = 0; i < LOADS; i++) {
+            x[slot][i] = load_loose(xr[i] + (size_t)step * KC);
+            w[slot][i] = load_loose(wr[i] + (size_t)step * KC);
+        }
+    };
+    auto store = [&](unsigned slot, unsigned step) {
+        if (step * KC + KC > a.k)       // what lies behind a row's end is another row's
+#pragma unroll
+            for (unsigned i = 0; i < LOADS; i++)
+#pragma unroll
+                for (unsigned e = 0; e < 8; e++)
+                    if (step * KC + chunk + e >= a.k) {
+                        x[slot][i][e / 2] &= e % 2 ? 0x0000ffff : 0xffff0000;
+                        w[slot][i][e / 2] &= e % 2 ? 0x0000ffff : 0xffff0000;
+                    }
+        i32x4 *const to = lds + step % 2 * 2 * SIDE * 8;
+#pragma unroll
+        for (unsigned i = 0; i < LOADS; i++) {
+            const unsigned at = swizzled(tid / 8 + 32 * i, tid % 8);
+            to[at] = x[slot][i];
+            to[SIDE * 8 + at] = w[slot][i];
+        }
+    };
+    const unsigned wm = wave / 2 * 32 * R, wn = wave % 2 * 32 * R;
+    f32x16 acc[R][R] = {};              // [row block][column block]
+#pragma unroll
+    for (unsigned i = 0; i < DEPTH; i++) load(i, i);
+    store(0, 0);
+    __syncthreads();
+    for (unsigned first = 0; first < steps; first += DEPTH)
+#pragma unroll
+    for (unsigned slot = 0; slot < DEPTH; slot++) {
+        const unsigned step = first + slot;
+        if (step >= steps) break;
+        load(slot, step + DEPTH);
+        const i32x4 *const from = lds + step % 2 * 2 * SIDE * 8;
+#pragma unroll
+        for (unsigned j = 0; j < 4; j++) {
+            bf16x8 xf[R], wf[R];
+#pragma unroll
+            for (unsigned i = 0; i < R; i++) {
+                xf[i] = __builtin_bit_cast(bf16x8, from[swizzled(wm + 32 * i + n, j * 2 + hf)]);
+                wf[i] = __builtin_bit_cast(bf16x8, from[SIDE * 8 + swizzled(wn + 32 * i + n, j * 2 + hf)]);
+            }
+#pragma unroll
+            for (unsigned i = 0; i < R; i++)
+#pragma unroll
+                for (unsigned b = 0; b < R; b++) acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[b], xf[i], acc[i][b], 0, 0, 0);
+        }
+        if (step + 1 < steps) store((slot + 1) % DEPTH, step + 1);   // last read in the step before this one
+        __syncthreads();
+    }
+    float *const stage = reinterpret_cast<float *>(lds) + wave * 32 * (32 * R + 4);
+    constexpr unsigned STRIDE = 32 * R + 4, PER_ROW = 4 * R, AT_ONCE = 64 / PER_ROW;   // chunks of a row of the stage
+#pragma unroll
+    for (unsigned i = 0; i < R; i++) {
+        const unsigned tile = tile0 + wm / 32 + i;
+        if (tile >= all) break;
+        if (tile < a.tiles) {
+            const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
+            for (unsigned r = 0; r < entry.ranks; r += 16) {
+                const float *p = a.sums + ((size_t)tile * 32 + n) * a.rank_padded + r + hf * 8;
+                f32x4 t[2] = {};
+                for (unsigned split = 0; split < a.splits; split++) {
+                    t[0] += *reinterpret_cast<const f32x4 *>(p);
+                    t[1] += *reinterpret_cast<const f32x4 *>(p + 4);
+                    p += (size_t)a.tiles * 32 * a.rank_padded;
+                }
+                bf16x8 high, low;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float f = t[e / 4][e % 4] * entry.scale;
+                    high[e] = (__bf16)f;
+                    low[e] = (__bf16)(f - (float)high[e]);
+                }
+#pragma unroll
+                for (unsigned b = 0; b < R; b++) {
+                    // Columns past the last packed step are not stored: any block does.
+                    const unsigned c = min(n0 + wn + 32 * b, (a.n - 1) / 32 * 32);
+                    const bf16x8 u = *reinterpret_cast<const bf16x8 *>(
+                        a.weights + entry.up + (((size_t)(c / COLS) * (entry.ranks / 16) + r / 16) * 2 + c / 32 % 2) * 512 + lane * 8);
+                    acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, high, acc[i][b], 0, 0, 0);
+                    acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, low, acc[i][b], 0, 0, 0);
+                }
+            }
+        }
+        wait_lds();                     // the stage's last reads
+#pragma unroll
+        for (unsigned b = 0; b < R; b++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                *reinterpret_cast<f32x4 *>(stage + n * STRIDE + b * 32 + q * 8 + hf * 4) =
+                    f32x4{acc[i][b][4 * q], acc[i][b][4 * q + 1], acc[i][b][4 * q + 2], acc[i][b][4 * q + 3]};
+        wait_lds();
+#pragma unroll
+        for (unsigned j = 0; j < 32 / AT_ONCE; j++) {
+            const unsigned r = j * AT_ONCE + lane / PER_ROW, at = lane % PER_ROW * 8, c = n0 + wn + at;
+            const uint32_t row = a.order[tile * 32 + r];
+            if (row == NONE || c >= a.n) continue;
+            bf16x8 y;
+#pragma unroll
+            for (unsigned e = 0; e < 8; e++)
+                y[e] = (__bf16)(stage[r * STRIDE + at + e] + (a.bias && c + e < a.n ? bf16_to_f32(a.bias[c + e]) : 0.f));
+            uint16_t *const out = a.out + (size_t)row * a.n + c;
+            const i32x4 v = __builtin_bit_cast(i32x4, y);
+            if (c + 8 <= a.n) reinterpret_cast<Loose *>(out)->v = v;
+            else
+#pragma unroll
+                for (unsigned e = 0; e < 8; e++)
+                    if (c + e < a.n) out[e] = (uint16_t)((uint32_t)v[e / 2] >> (e % 2 * 16));
+        }
     }
 }
 
@@ -466,24 +621,65 @@ static int adapters_valid(h3_gpu *g, const h3_hip_adapters *w, const h3_hip_adap
     return 1;
 }
 
-template <bool WIDE> static int launch_adapters(h3_gpu *g, const AdapterArgs &a, uint32_t copied, uint32_t blocks) {
+// Launches hold fewer than 2^32 threads.
+static int adapters_fit(h3_gpu *g, const h3_hip_adapter_rows *p, uint64_t workgroups, uint32_t rows, uint32_t n) {
+    if (workgroups >= (1u << 24) || (uint64_t)p->tiles * ((rank_blocks(p->max_rank) + 1) / 2) * p->splits >= (1u << 24))
+        return h3_set_error(g, "adapters: %u rows by %u columns are more than a launch takes", rows, n);
+    return 1;
+}
+
+static int shared_memory(h3_gpu *g, const void *kernel, size_t bytes) {
+    return h3_hip_check(g, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "adapters' shared memory");
+}
+
+// The arguments of a call, and its first product.
+static int adapters_begin(h3_gpu *g, AdapterArgs &a, const h3_gpu_tensor *in, const h3_hip_adapters *w, const h3_hip_adapter_rows *p,
+                          uint32_t &blocks) {
+    blocks = 0;
+    for (uint32_t rank : w->ranks) blocks = std::max(blocks, rank_blocks(rank));
+    a.x = (const uint16_t *)in->data;
+    a.weights = (const uint16_t *)w->weights->data;
+    a.table = (const AdapterEntry *)w->table->data;
+    a.order = (const uint32_t *)p->order->data;
+    a.adapter = a.order + (size_t)32 * (p->tiles + p->plain);
+    a.sums = (float *)p->sums->data;
+    a.k = w->k;
+    a.n = w->n;
+    a.k_padded = w->k_padded;
+    a.tiles = p->tiles;
+    a.plain = p->plain;
+    a.passes = (blocks + 1) / 2;
+    a.splits = std::min(p->splits, splits_for(g, p->tiles, a.passes));
+    a.rank_padded = rank_blocks(p->max_rank) * 32;
+    if (!a.tiles) return 1;
     constexpr unsigned shared = DOWN_WAVES * 8 * 64 * 16;
     static bool configured = false;
-    if (!configured) {
-        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)adapter_down, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)shared), "adapters' shared memory") ||
-            !h3_hip_check(g, hipFuncSetAttribute((const void *)adapter_up<WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)(4 * UP_STAGE * 4 + RANK_MOST / 32 * 4096)), "adapters' shared memory"))
-            return 0;
-        configured = true;
-    }
-    if (a.tiles) {
-        hipLaunchKernelGGL(adapter_down, dim3(a.tiles * a.passes * a.splits), dim3(64 * DOWN_WAVES), shared, g->compute, a);
-        if (!h3_launch_status(g, "adapters' first product")) return 0;
-    }
-    if (a.tiles + copied)
-        hipLaunchKernelGGL(adapter_up<WIDE>, dim3((a.tiles + copied) * a.groups), dim3(256), 4 * UP_STAGE * 4 + blocks * 4096, g->compute, a);
+    if (!configured && !shared_memory(g, (const void *)adapter_down, shared)) return 0;
+    configured = true;
+    hipLaunchKernelGGL(adapter_down, dim3(a.tiles * a.passes * a.splits), dim3(64 * DOWN_WAVES), shared, g->compute, a);
+    return h3_launch_status(g, "adapters' first product");
+}
+
+template <bool WIDE> static int launch_up(h3_gpu *g, const AdapterArgs &a, uint32_t tiles, uint32_t blocks) {
+    static bool configured = false;
+    if (!configured && !shared_memory(g, (const void *)adapter_up<WIDE>, 4 * UP_STAGE * 4 + RANK_MOST / 32 * 4096)) return 0;
+    configured = true;
+    hipLaunchKernelGGL(adapter_up<WIDE>, dim3(tiles * a.groups), dim3(256), 4 * UP_STAGE * 4 + blocks * 4096, g->compute, a);
     return h3_launch_status(g, "adapters' second product");
+}
+
+template <int R> static int launch_gemm(h3_gpu *g, const AdapterArgs &a) {
+    constexpr unsigned shared = 2 * 2 * 64 * R * 128;
+    static_assert(4 * 32 * (32 * R + 4) * 4 <= shared, "the stages take the buffers' place");
+    static bool configured = false;
+    if (!configured && !shared_memory(g, (const void *)adapter_gemm<R>, shared)) return 0;
+    configured = true;
+    h3_note_kernel(g, "adapter_gemm", 64 * R);
+    hipEvent_t timing = h3_kernel_timing_begin(g);
+    hipLaunchKernelGGL(adapter_gemm<R>, dim3((a.tiles + a.plain + 2 * R - 1) / (2 * R) * ((a.n + 64 * R - 1) / (64 * R))), dim3(256),
+                       shared, g->compute, a);
+    h3_kernel_timing_end(g, timing);
+    return h3_launch_status(g, "projection with adapters");
 }
 
 extern "C" int h3_hip_adapters_add_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *base, const h3_gpu_tensor *in,
@@ -495,30 +691,50 @@ extern "C" int h3_hip_adapters_add_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_
         !h3_require(g, out, H3_GPU_BF16, (size_t)rows * n, "adapters' output"))
         return 0;
     if (out == in) return h3_set_error(g, "adapters: output aliases input");
-    uint32_t blocks = 0;
-    for (uint32_t rank : w->ranks) blocks = std::max(blocks, rank_blocks(rank));
-    const uint32_t copied = out->data == base->data ? 0 : p->plain, tiles = p->tiles + copied;
-    const uint32_t passes = (blocks + 1) / 2, splits = std::min(p->splits, splits_for(g, p->tiles, passes));
+    const uint32_t tiles = p->tiles + (out->data == base->data ? 0 : p->plain);
     // A workgroup's share of the columns, in steps of 64: few rows in one round of the three
     // workgroups that a compute unit holds, many in four rounds and more.
     const uint32_t steps = (n + COLS - 1) / COLS;
     const uint64_t quads = (uint64_t)tiles * ((steps + 3) / 4), round = 3ull * g->cus;
-    const uint32_t span = 4 * (uint32_t)std::min<uint64_t>(8, std::max<uint64_t>(1, quads <= 4 * round ? (quads + round - 1) / round : quads / (4 * round)));
-    const uint32_t groups = (steps + span - 1) / span;
-    // Launches hold fewer than 2^32 threads.
-    if ((uint64_t)tiles * groups >= (1u << 24) || (uint64_t)p->tiles * passes * splits >= (1u << 23))
-        return h3_set_error(g, "adapters: %u rows by %u columns are more than a launch takes", rows, n);
-    const AdapterArgs a{(uint16_t *)out->data, (const uint16_t *)base->data, (const uint16_t *)in->data,
-                        (const uint16_t *)w->weights->data, (const AdapterEntry *)w->table->data,
-                        (const uint32_t *)p->order->data, (const uint32_t *)p->order->data + (size_t)32 * (p->tiles + p->plain),
-                        (float *)p->sums->data, k, n, w->k_padded, p->tiles, passes, splits, rank_blocks(p->max_rank) * 32, groups, span};
-    return n % 8 == 0 ? launch_adapters<true>(g, a, copied, blocks) : launch_adapters<false>(g, a, copied, blocks);
+    AdapterArgs a{};
+    a.out = (uint16_t *)out->data;
+    a.base = (const uint16_t *)base->data;
+    a.span = 4 * (uint32_t)std::min<uint64_t>(8, std::max<uint64_t>(1, quads <= 4 * round ? (quads + round - 1) / round : quads / (4 * round)));
+    a.groups = (steps + a.span - 1) / a.span;
+    if (!adapters_fit(g, p, (uint64_t)tiles * a.groups, rows, n)) return 0;
+    uint32_t blocks;
+    if (!adapters_begin(g, a, in, w, p, blocks)) return 0;
+    if (!tiles) return 1;
+    return n % 8 == 0 ? launch_up<true>(g, a, tiles, blocks) : launch_up<false>(g, a, tiles, blocks);
 }
 
 extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *weight,
                                            const h3_gpu_tensor *bias, const h3_hip_adapters *w, const h3_hip_adapter_rows *p,
                                            uint32_t rows, uint32_t k, uint32_t n) {
-    return g && h3_launch_ready(g) && adapters_valid(g, w, p, rows, k, n) &&
-           h3_gpu_linear_bf16(g, out, in, weight, bias, rows, k, n) &&
-           h3_hip_adapters_add_bf16(g, out, out, in, w, p, rows, k, n);
+    if (!h3_launch_ready(g) || !adapters_valid(g, w, p, rows, k, n)) return 0;
+    // The tiled projections take a K of whole 64-channel steps, the others would be gemm_small's, on the
+    // vector units. With the adapters: 301 rows, 1001 -> 777: 24 us, by gemm_small 140; 8000 rows, 5001 ->
+    // 5001: 758 us, 528 TFLOP/s. Tiles of 64 rows by 64 columns where the large ones would fill few
+    // compute units: 600 rows, 2001 -> 3001: 41 us (large 50), 800 rows: 55 (50), 1200 rows, 3001 ->
+    // 3001: 93 (65).
+    if (k % KC == 0 || !weight || weight->owner != g || weight->dtype != H3_GPU_BF16 || weight->q8 || weight->quant_mode || weight->block_tile)
+        return h3_gpu_linear_bf16(g, out, in, weight, bias, rows, k, n) && h3_hip_adapters_add_bf16(g, out, out, in, w, p, rows, k, n);
+    if (!h3_require(g, in, H3_GPU_BF16, (size_t)rows * k, "linear input") ||
+        !h3_require(g, weight, H3_GPU_BF16, (size_t)n * k, "linear weight") ||
+        !h3_require(g, out, H3_GPU_BF16, (size_t)rows * n, "linear output") ||
+        (bias && !h3_require(g, bias, H3_GPU_BF16, n, "linear bias")))
+        return 0;
+    if (out == in) return h3_set_error(g, "linear: output aliases input");
+    const uint64_t tiles = p->tiles + p->plain;
+    const uint64_t large = (tiles + 3) / 4 * ((n + 127) / 128), small = (tiles + 1) / 2 * ((n + 63) / 64);
+    if (!adapters_fit(g, p, small, rows, n)) return 0;
+    AdapterArgs a{};
+    a.out = (uint16_t *)out->data;
+    a.w = (const uint16_t *)weight->data;
+    a.bias = bias ? (const uint16_t *)bias->data : nullptr;
+    uint32_t blocks;
+    if (!h3_tensor_acquire(g, weight) || !adapters_begin(g, a, in, w, p, blocks)) return 0;
+    if (!(large * 5 >= g->cus * 3ull ? launch_gemm<2>(g, a) : launch_gemm<1>(g, a))) return 0;
+    g->stats.linear_dispatches++;
+    return h3_tensor_release(g, weight);
 }

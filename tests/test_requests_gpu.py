@@ -459,6 +459,35 @@ def test_linear_with_adapters_is_the_projection_and_the_adapters(kind, rows):
             g.lib.h3_gpu_tensor_free(w)
 
 
+@pytest.mark.parametrize("rows,k,n,ranks,bias", [
+    (1, 1, 1, [1], True), (5, 65, 130, [16], False), (301, 1001, 777, [1, 40, 7, 19], True), (130, 72, 1000, [33, 64], False),
+    (33, 5000, 64, [256], True), (1000, 200, 2049, [16, 8, 100], True), (2100, 520, 4100, [32, 32], False), (64, 1000, 7, [5], True),
+])
+def test_linear_with_adapters_of_any_width(rows, k, n, ranks, bias):
+    """A BF16 weight whose K is no multiple of 64: one sum and one rounding for projection, bias and adapters."""
+    print(f"[adapters] linear {rows}x{k}x{n} {ranks}", flush=True)
+    with Gpu() as g:
+        x, w, b = normal(rows * k, 1).reshape(rows, k), normal(n * k, 2, scale=1 / math.sqrt(k)).reshape(n, k), normal(n, 3)
+        mark = normal((rows + 1) * n, 4)
+        tx, tw, tb, out = (g.from_bf16(t) for t in (x, w, b, mark))
+        at = row_map(rows, len(ranks), 5)
+        ad = Adapters(g, ranks, k, n, seed=7)
+        with adapter_rows(g, at, len(ranks), max(ranks)) as plan:
+            g.begin()
+            g.check(g.lib.h3_hip_linear_adapters_bf16(g.handle, out.handle, tx.handle, tw.handle, tb.handle if bias else None, ad.handle,
+                                                      plan, rows, k, n), "linear")
+            assert "adapter_gemm" in g.last_kernel()
+            g.submit()
+        got = out.read()
+        assert np.array_equal(got[rows * n:], mark[rows * n:])
+        fx, fw = bf16(x).astype(np.float64), bf16(w).astype(np.float64)
+        base = fx @ fw.T + (bf16(b).astype(np.float64) if bias else 0)
+        error = (k + 64) * F32 * (np.abs(fx) @ np.abs(fw).T + np.abs(bf16(b)) * bias)
+        want, bound = ad.reference(fx, at, base, error)
+        within(bf16(got[:rows * n]).reshape(rows, n), want, bound)
+        ad.close()
+
+
 # ------------------------------------------------------------------ refusals
 def refused(g, ok, text):
     assert not ok
