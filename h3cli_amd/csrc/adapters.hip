@@ -23,7 +23,7 @@
 
 struct AdapterEntry {
     uint64_t down, up;     // elements from the start of the packed matrices
-    uint32_t ranks;        // up to the next 16
+    uint32_t rank;
     float scale;
 };
 
@@ -67,6 +67,29 @@ struct AdapterArgs {
     unsigned groups, span;                 // adapter_up: workgroups of a tile, their steps of columns
 };
 
+__device__ inline unsigned sixteens_of(const AdapterEntry &e) { return (e.rank + 15) / 16; }
+
+// Ranks `from` to from + 7 of row `row` of t, its shares added in order and scaled, as two BF16 values
+// each: what the first rounding left is in the second (nothing where the first is infinite).
+// Ranks that only fill the packed weights up are nothing, whatever x holds.
+__device__ inline void operands(const AdapterArgs &a, const AdapterEntry &entry, unsigned tile, unsigned row, unsigned from,
+                                bf16x8 &high, bf16x8 &low) {
+    const float *p = a.sums + ((size_t)tile * 32 + row) * a.rank_padded + from;
+    f32x4 t[2] = {};
+#pragma unroll 4
+    for (unsigned split = 0; split < a.splits; split++) {
+        t[0] += *reinterpret_cast<const f32x4 *>(p);
+        t[1] += *reinterpret_cast<const f32x4 *>(p + 4);
+        p += (size_t)a.tiles * 32 * a.rank_padded;
+    }
+#pragma unroll
+    for (unsigned e = 0; e < 8; e++) {
+        const float f = from + e < entry.rank ? t[e / 4][e % 4] * entry.scale : 0.f;
+        high[e] = (__bf16)f;
+        low[e] = (__bf16)(finite_f32((float)high[e]) ? f - (float)high[e] : 0.f);
+    }
+}
+
 // Eight values from any element on. Global memory takes 16-byte accesses at any two bytes. What lies up
 // to 256 bytes behind a tensor's end, more than a step of 64 values, is within its allocation.
 struct __attribute__((packed, aligned(2))) Loose { i32x4 v; };
@@ -93,8 +116,8 @@ __global__ __launch_bounds__(64 * DOWN_WAVES, 2) void adapter_down(AdapterArgs a
     const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, n = lane % 32, hf = lane / 32;
     const unsigned split = blockIdx.x % a.splits, pass = blockIdx.x / a.splits % a.passes, tile = blockIdx.x / a.splits / a.passes;
     const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
-    if (pass * 64 >= entry.ranks) return;
-    const bool both = pass * 64 + 32 < entry.ranks;
+    if (pass * 64 >= entry.rank) return;
+    const bool both = pass * 64 + 32 < entry.rank;
     // Lane's chunk lane % 8 of rows lane / 8 + 8 i; row r keeps chunk c at swizzled(r, c).
     const unsigned chunk = lane % 8 * 8;
     const uint16_t *xr[4];
@@ -201,7 +224,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
     for (int i = 0; i < 4; i++) row[i] = a.order[tile * 32 + lane / 8 + 8 * i];
     AdapterEntry entry{};
     if (adapted) entry = a.table[load_uniform(a.adapter + tile)];
-    const unsigned sixteens = entry.ranks / 16;
+    const unsigned sixteens = sixteens_of(entry);
     const uint16_t *const up = a.weights + entry.up + lane * 8;
     i32x4 next_v[4] = {}, next_w[4] = {};
     // Loads are made whatever comes of them (padding rows read row 0, columns behind the end the next
@@ -227,21 +250,8 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
         for (unsigned i = threadIdx.x; i < sixteens * 64; i += 256) {
             // Lane i % 64 of rank step i / 64: eight ranks of its row.
             const unsigned from = i / 64 * 16 + i % 64 / 32 * 8;
-            const float *p = a.sums + ((size_t)tile * 32 + i % 32) * a.rank_padded + from;
-            f32x4 t[2] = {};
-#pragma unroll 4
-            for (unsigned split = 0; split < a.splits; split++) {
-                t[0] += *reinterpret_cast<const f32x4 *>(p);
-                t[1] += *reinterpret_cast<const f32x4 *>(p + 4);
-                p += (size_t)a.tiles * 32 * a.rank_padded;
-            }
             bf16x8 high, low;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float f = t[e / 4][e % 4] * entry.scale;
-                high[e] = (__bf16)f;
-                low[e] = (__bf16)(f - (float)high[e]);
-            }
+            operands(a, entry, tile, i % 32, from, high, low);
             operand[i / 64 * 128 + i % 64] = __builtin_bit_cast(i32x4, high);
             operand[i / 64 * 128 + 64 + i % 64] = __builtin_bit_cast(i32x4, low);
         }
@@ -405,27 +415,15 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
         if (tile >= all) break;
         if (tile < a.tiles) {
             const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
-            for (unsigned r = 0; r < entry.ranks; r += 16) {
-                const float *p = a.sums + ((size_t)tile * 32 + n) * a.rank_padded + r + hf * 8;
-                f32x4 t[2] = {};
-                for (unsigned split = 0; split < a.splits; split++) {
-                    t[0] += *reinterpret_cast<const f32x4 *>(p);
-                    t[1] += *reinterpret_cast<const f32x4 *>(p + 4);
-                    p += (size_t)a.tiles * 32 * a.rank_padded;
-                }
+            for (unsigned r = 0; r < entry.rank; r += 16) {
                 bf16x8 high, low;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float f = t[e / 4][e % 4] * entry.scale;
-                    high[e] = (__bf16)f;
-                    low[e] = (__bf16)(f - (float)high[e]);
-                }
+                operands(a, entry, tile, n, r + hf * 8, high, low);
 #pragma unroll
                 for (unsigned b = 0; b < R; b++) {
                     // Columns past the last packed step are not stored: any block does.
                     const unsigned c = min(n0 + wn + 32 * b, (a.n - 1) / 32 * 32);
                     const bf16x8 u = *reinterpret_cast<const bf16x8 *>(
-                        a.weights + entry.up + (((size_t)(c / COLS) * (entry.ranks / 16) + r / 16) * 2 + c / 32 % 2) * 512 + lane * 8);
+                        a.weights + entry.up + (((size_t)(c / COLS) * sixteens_of(entry) + r / 16) * 2 + c / 32 % 2) * 512 + lane * 8);
                     acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, high, acc[i][b], 0, 0, 0);
                     acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, low, acc[i][b], 0, 0, 0);
                 }
@@ -517,10 +515,9 @@ extern "C" h3_hip_adapters *h3_hip_adapters_new(h3_gpu *g, const uint32_t *ranks
         a = new h3_hip_adapters{g, count, k, n, (k + KC - 1) / KC * KC, (n + COLS - 1) / COLS * COLS,
                                 std::vector<uint32_t>(ranks, ranks + count), {}, nullptr, nullptr};
         for (uint32_t i = 0; i < count; i++) {
-            const uint32_t padded = (ranks[i] + 15) / 16 * 16;
             const size_t down = (size_t)rank_blocks(ranks[i]) * 32 * a->k_padded;
-            a->entries.push_back({elements, elements + down, padded, 0.f});
-            elements += down + (size_t)padded * a->n_padded;
+            a->entries.push_back({elements, elements + down, ranks[i], 0.f});
+            elements += down + (size_t)((ranks[i] + 15) / 16 * 16) * a->n_padded;
         }
     } catch (const std::bad_alloc &) {
         delete a;
@@ -554,7 +551,8 @@ extern "C" int h3_hip_adapters_set(h3_gpu *g, h3_hip_adapters *a, uint32_t index
     AdapterEntry &e = a->entries[index];
     uint16_t *w = (uint16_t *)a->weights->data;
     pack(g, w + e.down, (const uint16_t *)down->data, (size_t)rank_blocks(rank) * 32 * a->k_padded, rank, a->k, a->k_padded / 16, 0);
-    pack(g, w + e.up, (const uint16_t *)up->data, (size_t)e.ranks * a->n_padded, rank, a->n, e.ranks / 16, 1);
+    const uint32_t sixteens = (rank + 15) / 16;
+    pack(g, w + e.up, (const uint16_t *)up->data, (size_t)sixteens * 16 * a->n_padded, rank, a->n, sixteens, 1);
     hipLaunchKernelGGL(adapter_entry_scale, dim3(1), dim3(1), 0, g->compute, (AdapterEntry *)a->table->data + index, scale);
     e.scale = scale;
     return h3_launch_status(g, "adapter");

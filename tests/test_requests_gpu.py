@@ -424,6 +424,42 @@ def test_adapters_are_replaced_and_start_as_zero():
         w.close()
 
 
+@pytest.mark.parametrize("k,n", [(128, 200), (65, 199)])
+def test_adapters_keep_infinities_to_their_rows_and_signs(k, n):
+    """Rank 1 with weights of one sign: an infinity of x gives infinities of the formula's signs in its
+    own row, with no NaN from the ranks that fill the packed weights up; other rows are as without it."""
+    rows = 40
+    with Gpu() as g:
+        w = Adapters(g, [1, 3], k, n)
+        w.set(0, a=normal(k, 1) & 0x7fff, b=normal(n, 2), scale=1.0)
+        at = np.arange(rows) % 3
+        x = normal(rows * k, 3).reshape(rows, k).copy()
+        tw = g.from_bf16(np.zeros(n * k, np.uint16))
+        base, out = g.from_bf16(np.zeros(rows * n, np.uint16)), g.empty(rows * n)
+
+        def call(values):
+            tx = g.from_bf16(values)
+            with adapter_rows(g, at, 2, 3) as plan:
+                g.begin()
+                if k % 64:
+                    g.check(g.lib.h3_hip_linear_adapters_bf16(g.handle, out.handle, tx.handle, tw.handle, None, w.handle, plan, rows, k, n))
+                else:
+                    g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, out.handle, base.handle, tx.handle, w.handle, plan, rows, k, n))
+                g.submit()
+            return out.read().reshape(rows, n)
+
+        clean = call(x)
+        x[6, 5], x[9, k - 1] = 0x7f80, 0xff80                # rows of adapter 0
+        got = call(x)
+        others = np.setdiff1d(np.arange(rows), (6, 9))
+        assert np.array_equal(got[others], clean[others])
+        if k % 64 == 0:                                      # the projection's weights of zero make NaN of an infinity
+            positive = w.b[0].reshape(-1) < 0x8000
+            assert np.array_equal(got[6], np.where(positive, 0x7f80, 0xff80))
+            assert np.array_equal(got[9], np.where(positive, 0xff80, 0x7f80))
+        w.close()
+
+
 @pytest.mark.parametrize("kind", ["bf16", "q8", "fp8_block"])
 @pytest.mark.parametrize("rows", [1, 70, 300])
 def test_linear_with_adapters_is_the_projection_and_the_adapters(kind, rows):
@@ -486,6 +522,160 @@ def test_linear_with_adapters_of_any_width(rows, k, n, ranks, bias):
         want, bound = ad.reference(fx, at, base, error)
         within(bf16(got[:rows * n]).reshape(rows, n), want, bound)
         ad.close()
+
+
+# ------------------------------------------------------------------ together
+def fill(g, t, seed, scale=1.0):
+    g.check(g.lib.h3_hip_fill_normal_bf16(g.handle, t.handle, seed, C.c_float(scale), t.elements), "fill")
+
+
+class Step:
+    """Attention's half of a block for the rows of several requests: projection with adapters, norms and
+    rotation, attention of the sequences, projection with adapters."""
+
+    def __init__(self, g, lengths, hidden=384, heads=6, kv_heads=2, ranks=(16, 40), seed=1):
+        self.g, self.rows, self.hidden, self.heads, self.kv_heads = g, sum(lengths), hidden, heads, kv_heads
+        self.inner, self.qkv_width = heads * 128, (heads + 2 * kv_heads) * 128
+        rng = np.random.RandomState(seed)
+        ends = np.cumsum([0] + list(lengths))
+        self.w = [g.from_bf16(normal(self.qkv_width * hidden, 11, scale=1 / math.sqrt(hidden))),
+                  g.from_bf16(normal(hidden * self.inner, 12, scale=1 / math.sqrt(self.inner)))]
+        self.norms = [g.from_bf16(synth.f32_to_bf16((1 + 0.1 * np.random.RandomState(i).randn(128)).astype(np.float32))) for i in (3, 4)]
+        positions = np.concatenate([np.stack([np.arange(n) // 8 + 1000 * i, np.arange(n) % 8], axis=1) for i, n in enumerate(lengths)])
+        self.positions = g.from_f32(positions.astype(np.float32))
+        frequencies = 10000.0 ** -(np.arange(64) / 64)
+        self.adapters = [Adapters(g, list(ranks), hidden, self.qkv_width, seed=21), Adapters(g, list(ranks), self.inner, hidden, seed=31)]
+        at = np.repeat(np.arange(len(lengths)) % (len(ranks) + 1), lengths)
+        self.at = at
+        self.plans = [rope_axes(g, list(frequencies), [0, 1] * 32, 2, 0), sequences(g, ends, None, heads, kv_heads),
+                      adapter_rows(g, at, len(ranks), max(ranks))]
+        self.t = {name: g.empty(self.rows * width) for name, width in (
+            ("qkv", self.qkv_width), ("q", self.inner), ("k", kv_heads * 128), ("v", kv_heads * 128), ("o", self.inner), ("y", hidden))}
+
+    def run(self, x):
+        g, lib, t, h = self.g, self.g.lib, {n: v.handle for n, v in self.t.items()}, self.g.handle
+        rope, seqs, rows = (p.handle for p in self.plans)
+        g.check(lib.h3_hip_linear_adapters_bf16(h, t["qkv"], x.handle, self.w[0].handle, None, self.adapters[0].handle, rows, self.rows,
+                                                self.hidden, self.qkv_width), "qkv")
+        g.check(lib.h3_hip_qkv_rope_axes_bf16(h, t["q"], t["k"], t["v"], t["qkv"], self.norms[0].handle, self.norms[1].handle, rope,
+                                              self.positions.handle, self.rows, self.heads, self.kv_heads, 128, 0, C.c_float(EPS)), "rope")
+        g.check(lib.h3_hip_sdpa_sequences_bf16(h, t["o"], t["q"], t["k"], t["v"], seqs, C.c_float(SCALE)), "attention")
+        g.check(lib.h3_hip_linear_adapters_bf16(h, t["y"], t["o"], self.w[1].handle, None, self.adapters[1].handle, rows, self.rows,
+                                                self.inner, self.hidden), "out")
+
+    def close(self):
+        for p in self.plans:
+            p.__exit__()
+        for a in self.adapters:
+            a.close()
+
+
+def step_reference(step, x, lengths):
+    """The step in 64 bits, each stage's result rounded to BF16 as the operators hand it on."""
+    def rounded(v):
+        return bf16(synth.f32_to_bf16(np.asarray(v, np.float32))).astype(np.float64)
+
+    def projected(v, w, n, adapters):
+        base = rounded(v @ bf16(w.read()).astype(np.float64).reshape(n, -1).T)
+        return rounded(adapters.reference(v, step.at, base, np.zeros_like(base))[0])
+
+    qkv = projected(x, step.w[0], step.qkv_width, step.adapters[0]).reshape(step.rows, -1, 128)
+    weights = [bf16(w.read()).astype(np.float64) for w in step.norms]
+    (q, _), (k, _), (v, _) = rope_reference(qkv, weights, 10000.0 ** -(np.arange(64) / 64), np.array([0, 1] * 32),
+                                            step.positions.read().reshape(-1, 2), step.heads, step.kv_heads, 0, 0)
+    q, k, out, ends = rounded(q), rounded(k), np.zeros(q.shape), np.cumsum([0] + list(lengths))
+    for a, b in zip(ends, ends[1:]):
+        for h in range(step.heads if b > a else 0):
+            kv = h // (step.heads // step.kv_heads)
+            out[a:b, h] = attention_reference(q[a:b, h], k[a:b, kv], v[a:b, kv], SCALE)[0]
+    return projected(rounded(out).reshape(step.rows, -1), step.w[1], step.hidden, step.adapters[1])
+
+
+@pytest.mark.parametrize("lengths", [(1,), (70, 1, 0, 133), (300, 260, 33)])
+def test_a_step_of_several_requests(lengths):
+    """The operators one after another, against 64 bits: each stage keeps to BF16's rounding, so the
+    result is off by a few of them; and every request's rows as in a step of its own."""
+    print(f"[step] {lengths}", flush=True)
+    with Gpu() as g:
+        step = Step(g, lengths)
+        x = normal(step.rows * step.hidden, 5)
+        tx = g.from_bf16(x)
+        g.begin()
+        step.run(tx)
+        g.submit()
+        got = bf16(step.t["y"].read()).astype(np.float64).reshape(step.rows, -1)
+        want = step_reference(step, bf16(x).astype(np.float64).reshape(step.rows, -1), lengths)
+        # Six stages round (two of them twice), P once more: at most nine half steps if all went one way,
+        # relative to the result's size.
+        assert np.linalg.norm(got - want) <= 9 * HALF * np.linalg.norm(want)
+        step.close()
+
+
+def test_steps_captured_into_two_graphs():
+    """Two graphs of one context with plans of their own, replayed in turn between eager work that uses
+    the context's workspaces: every replay gives the same bits. (Captured projections are not split
+    over K, so the eager step's bits may differ, by what rounding allows.)"""
+    lengths = [(150, 90, 31), (400, 520)]
+    with Gpu() as g:
+        steps = [Step(g, n, seed=i) for i, n in enumerate(lengths)]
+        xs = [g.from_bf16(normal(s.rows * s.hidden, 40 + i)) for i, s in enumerate(steps)]
+        other = [g.empty(900 * 4096), g.empty(4096 * 4096), g.empty(900 * 4096)]
+        want = []
+        for s, x in zip(steps, xs):
+            g.begin()
+            s.run(x)
+            g.submit()
+            want.append(s.t["y"].read())
+        graphs = []
+        g.begin()
+        for s, x in zip(steps, xs):
+            graphs.append(Graph(g))
+            with graphs[-1]:
+                s.run(x)
+        first = [None, None]
+        for turn in range(3):
+            for i in (0, 1, 0):
+                fill(g, steps[i].t["y"], turn + 9)
+                fill(g, other[0], turn)
+                g.check(g.lib.h3_gpu_linear_bf16(g.handle, other[2].handle, other[0].handle, other[1].handle, None, 900, 4096, 4096))
+                graphs[i].launch()
+                g.submit()
+                got = steps[i].t["y"].read()
+                first[i] = got if first[i] is None else first[i]
+                assert np.array_equal(got, first[i]), (turn, i)
+                a, b = bf16(got).astype(np.float64), bf16(want[i]).astype(np.float64)
+                assert np.linalg.norm(a - b) <= 18 * HALF * np.linalg.norm(b), (turn, i)
+                g.begin()
+        g.submit()
+        for graph in graphs:
+            graph.close()
+        for s in steps:
+            s.close()
+
+
+def test_steps_of_two_contexts_at_once():
+    """Two contexts, whose streams run side by side: the same bits as each alone."""
+    with Gpu() as a, Gpu() as b:
+        pairs = []
+        for i, g in enumerate((a, b)):
+            s = Step(g, (200 + 100 * i, 77), seed=i)
+            x = g.from_bf16(normal(s.rows * s.hidden, 60 + i))
+            g.begin()
+            s.run(x)
+            g.submit()
+            pairs.append((g, s, x, s.t["y"].read()))
+        for _ in range(3):
+            for g, s, x, _ in pairs:
+                g.begin()
+                fill(g, s.t["y"], 3)
+            for _ in range(4):
+                for g, s, x, _ in pairs:
+                    s.run(x)
+            for g, s, x, want in pairs:
+                g.submit()
+                assert np.array_equal(s.t["y"].read(), want)
+        for _, s, _, _ in pairs:
+            s.close()
 
 
 # ------------------------------------------------------------------ refusals
