@@ -43,6 +43,7 @@ struct h3_hip_adapter_rows {
     h3_gpu_tensor *order;     // u32 [32 (tiles + plain)]: row, or UINT32_MAX; then the adapter of each tile
     h3_gpu_tensor *sums;      // F32 [splits][32 tiles][padded rank]
     uint32_t splits;          // most K shares of a tile that `sums` holds
+    size_t sums_at;           // behind them adapter_gemm's shared tiles, [SHARED_TILES][64 x 64]
 };
 
 namespace {
@@ -51,6 +52,7 @@ constexpr uint32_t NONE = UINT32_MAX;
 constexpr unsigned KC = 64;                // channels of K a step: one cache line of a row
 constexpr unsigned COLS = 64;              // columns of N a step: one cache line of a row
 constexpr uint32_t RANK_MOST = 256;
+constexpr uint32_t SHARED_TILES = 256;
 
 uint32_t rank_blocks(uint32_t rank) { return (rank + 31) / 32; }
 
@@ -62,6 +64,8 @@ struct AdapterArgs {
     const uint32_t *order, *adapter;       // [32 tiles], [tiles]
     float *sums;
     const uint16_t *w, *bias;              // adapter_gemm
+    float *shared_sums;
+    unsigned shares;
     unsigned plain;
     unsigned k, n, k_padded, tiles, passes, splits, rank_padded;
     unsigned groups, span;                 // adapter_up: workgroups of a tile, their steps of columns
@@ -331,14 +335,19 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
 // DEPTH steps' values on their way in registers. The adapters' ranks then continue the sum, each row block with
 // its adapter's. Bound by the chip's fill at small shapes and by the matrix cores and LDS alike
 // at large ones.
-template <int R>
+// A compute unit takes in about 20 bytes a cycle of such rows, so few tiles over a long K are shared out
+// (part PRODUCT: a share of K, its sums to memory; then part REST: the shares added in order, and
+// what follows them).
+enum Part { ALL, PRODUCT, REST };
+template <int R, Part PART>
 __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
     constexpr unsigned SIDE = 64 * R, LOADS = SIDE / 32, DEPTH = R == 1 ? 4 : 2;   // LOADS: chunks of each operand a thread
     extern __shared__ __attribute__((aligned(16))) i32x4 lds[];   // [buffer][x, W][SIDE rows of 8 chunks]; then a stage a wave
     const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, n = lane % 32, hf = lane / 32;
+    const unsigned id = PART == PRODUCT ? blockIdx.x / a.shares : blockIdx.x;
     const unsigned tiles_n = (a.n + SIDE - 1) / SIDE, tiles_m = (a.tiles + a.plain + 2 * R - 1) / (2 * R);
     // Columns fastest in bands of eight row tiles, so that what runs together shares both operands.
-    const unsigned band = blockIdx.x / (8 * tiles_n), rows_here = min(8u, tiles_m - band * 8), in_band = blockIdx.x - band * 8 * tiles_n;
+    const unsigned band = id / (8 * tiles_n), rows_here = min(8u, tiles_m - band * 8), in_band = id - band * 8 * tiles_n;
     const unsigned tm = band * 8 + in_band % rows_here, n0 = in_band / rows_here * SIDE, tile0 = tm * 2 * R;
     const unsigned all = a.tiles + a.plain, chunk = tid % 8 * 8;
     const uint16_t *xr[LOADS], *wr[LOADS];
@@ -380,33 +389,50 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
     };
     const unsigned wm = wave / 2 * 32 * R, wn = wave % 2 * 32 * R;
     f32x16 acc[R][R] = {};              // [row block][column block]
+    if constexpr (PART != REST) {
+        const unsigned share = PART == PRODUCT ? blockIdx.x % a.shares : 0;
+        const unsigned begin = PART == PRODUCT ? steps * share / a.shares : 0, end = PART == PRODUCT ? steps * (share + 1) / a.shares : steps;
 #pragma unroll
-    for (unsigned i = 0; i < DEPTH; i++) load(i, i);
-    store(0, 0);
-    __syncthreads();
-    for (unsigned first = 0; first < steps; first += DEPTH)
-#pragma unroll
-    for (unsigned slot = 0; slot < DEPTH; slot++) {
-        const unsigned step = first + slot;
-        if (step >= steps) break;
-        load(slot, step + DEPTH);
-        const i32x4 *const from = lds + step % 2 * 2 * SIDE * 8;
-#pragma unroll
-        for (unsigned j = 0; j < 4; j++) {
-            bf16x8 xf[R], wf[R];
-#pragma unroll
-            for (unsigned i = 0; i < R; i++) {
-                xf[i] = __builtin_bit_cast(bf16x8, from[swizzled(wm + 32 * i + n, j * 2 + hf)]);
-                wf[i] = __builtin_bit_cast(bf16x8, from[SIDE * 8 + swizzled(wn + 32 * i + n, j * 2 + hf)]);
-            }
-#pragma unroll
-            for (unsigned i = 0; i < R; i++)
-#pragma unroll
-                for (unsigned b = 0; b < R; b++) acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[b], xf[i], acc[i][b], 0, 0, 0);
-        }
-        if (step + 1 < steps) store((slot + 1) % DEPTH, step + 1);   // last read in the step before this one
+        for (unsigned i = 0; i < DEPTH; i++) load(i, begin + i);
+        store(0, begin);
         __syncthreads();
+        for (unsigned first = begin; first < end; first += DEPTH)
+#pragma unroll
+        for (unsigned slot = 0; slot < DEPTH; slot++) {
+            const unsigned step = first + slot;
+            if (step >= end) break;
+            load(slot, step + DEPTH);
+            const i32x4 *const from = lds + step % 2 * 2 * SIDE * 8;
+#pragma unroll
+            for (unsigned j = 0; j < 4; j++) {
+                bf16x8 xf[R], wf[R];
+#pragma unroll
+                for (unsigned i = 0; i < R; i++) {
+                    xf[i] = __builtin_bit_cast(bf16x8, from[swizzled(wm + 32 * i + n, j * 2 + hf)]);
+                    wf[i] = __builtin_bit_cast(bf16x8, from[SIDE * 8 + swizzled(wn + 32 * i + n, j * 2 + hf)]);
+                }
+#pragma unroll
+                for (unsigned i = 0; i < R; i++)
+#pragma unroll
+                    for (unsigned b = 0; b < R; b++) acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[b], xf[i], acc[i][b], 0, 0, 0);
+            }
+            if (step + 1 < end) store((slot + 1) % DEPTH, step + 1);   // last read in the step before this one
+            __syncthreads();
+        }
     }
+    // Shares' sums: [tile][share][wave][register][lane].
+    if constexpr (PART == PRODUCT) {
+        float *const to = a.shared_sums + ((size_t)blockIdx.x * 4 + wave) * R * R * 16 * 64 + lane;
+#pragma unroll
+        for (unsigned i = 0; i < R * R * 16; i++) to[i * 64] = acc[i / 16 / R][i / 16 % R][i % 16];
+        return;
+    }
+    if constexpr (PART == REST)
+        for (unsigned share = 0; share < a.shares; share++) {
+            const float *const from = a.shared_sums + (((size_t)id * a.shares + share) * 4 + wave) * R * R * 16 * 64 + lane;
+#pragma unroll
+            for (unsigned i = 0; i < R * R * 16; i++) acc[i / 16 / R][i / 16 % R][i % 16] += from[i * 64];
+        }
     float *const stage = reinterpret_cast<float *>(lds) + wave * 32 * (32 * R + 4);
     constexpr unsigned STRIDE = 32 * R + 4, PER_ROW = 4 * R, AT_ONCE = 64 / PER_ROW;   // chunks of a row of the stage
 #pragma unroll
@@ -576,7 +602,7 @@ extern "C" h3_hip_adapter_rows *h3_hip_adapter_rows_new(h3_gpu *g, const uint32_
     h3_hip_adapter_rows *p = nullptr;
     std::vector<uint32_t> order;
     try {
-        p = new h3_hip_adapter_rows{g, rows, count, max_rank, 0, 0, nullptr, nullptr, 1};
+        p = new h3_hip_adapter_rows{g, rows, count, max_rank, 0, 0, nullptr, nullptr, 1, 0};
         // Rows by adapter, those without (an index past the last) behind them, each in whole tiles.
         std::vector<size_t> start(count + 2, 0);
         for (uint32_t r = 0; r < rows; r++) start[std::min(map[r], count) + 1]++;
@@ -599,7 +625,8 @@ extern "C" h3_hip_adapter_rows *h3_hip_adapter_rows_new(h3_gpu *g, const uint32_
     const uint32_t blocks = rank_blocks(max_rank);
     p->splits = splits_for(g, p->tiles, (blocks + 1) / 2);
     p->order = h3_gpu_tensor_from_u32(g, order.data(), order.size());
-    p->sums = p->order ? h3_gpu_tensor_new_f32(g, std::max<size_t>((size_t)p->splits * p->tiles * 32 * blocks * 32, 1)) : nullptr;
+    p->sums_at = (size_t)p->splits * p->tiles * 32 * blocks * 32;
+    p->sums = p->order ? h3_gpu_tensor_new_f32(g, p->sums_at + (size_t)SHARED_TILES * 64 * 64) : nullptr;
     if (!p->sums) {
         h3_hip_adapter_rows_free(p);
         return nullptr;
@@ -666,17 +693,14 @@ template <bool WIDE> static int launch_up(h3_gpu *g, const AdapterArgs &a, uint3
     return h3_launch_status(g, "adapters' second product");
 }
 
-template <int R> static int launch_gemm(h3_gpu *g, const AdapterArgs &a) {
+template <int R, Part PART> static int launch_gemm(h3_gpu *g, const AdapterArgs &a, uint32_t workgroups) {
     constexpr unsigned shared = 2 * 2 * 64 * R * 128;
     static_assert(4 * 32 * (32 * R + 4) * 4 <= shared, "the stages take the buffers' place");
     static bool configured = false;
-    if (!configured && !shared_memory(g, (const void *)adapter_gemm<R>, shared)) return 0;
+    if (!configured && !shared_memory(g, (const void *)adapter_gemm<R, PART>, shared)) return 0;
     configured = true;
-    h3_note_kernel(g, "adapter_gemm", 64 * R);
-    hipEvent_t timing = h3_kernel_timing_begin(g);
-    hipLaunchKernelGGL(adapter_gemm<R>, dim3((a.tiles + a.plain + 2 * R - 1) / (2 * R) * ((a.n + 64 * R - 1) / (64 * R))), dim3(256),
-                       shared, g->compute, a);
-    h3_kernel_timing_end(g, timing);
+    h3_note_kernel(g, "adapter_gemm", 64 * R, a.shares);
+    hipLaunchKernelGGL((adapter_gemm<R, PART>), dim3(workgroups), dim3(256), shared, g->compute, a);
     return h3_launch_status(g, "projection with adapters");
 }
 
@@ -730,9 +754,18 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
     a.out = (uint16_t *)out->data;
     a.w = (const uint16_t *)weight->data;
     a.bias = bias ? (const uint16_t *)bias->data : nullptr;
+    a.shared_sums = (float *)p->sums->data + p->sums_at;
+    // Four steps of 64 channels a share at least, in one round of the compute units.
+    a.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint32_t>(SHARED_TILES, g->cus) / small, (k + KC - 1) / KC / 4));
+    if ((k + KC - 1) / KC < 20) a.shares = 1;
     uint32_t blocks;
     if (!h3_tensor_acquire(g, weight) || !adapters_begin(g, a, in, w, p, blocks)) return 0;
-    if (!(large * 5 >= g->cus * 3ull ? launch_gemm<2>(g, a) : launch_gemm<1>(g, a))) return 0;
+    hipEvent_t timing = h3_kernel_timing_begin(g);
+    const int ok = a.shares > 1                  ? launch_gemm<1, PRODUCT>(g, a, (uint32_t)small * a.shares) && launch_gemm<1, REST>(g, a, (uint32_t)small)
+                   : large * 5 >= g->cus * 3ull ? launch_gemm<2, ALL>(g, a, (uint32_t)large)
+                                                : launch_gemm<1, ALL>(g, a, (uint32_t)small);
+    h3_kernel_timing_end(g, timing);
+    if (!ok) return 0;
     g->stats.linear_dispatches++;
     return h3_tensor_release(g, weight);
 }

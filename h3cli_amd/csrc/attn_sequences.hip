@@ -19,6 +19,7 @@ namespace {
 constexpr int D = 128, BN = 64, TILE = BN * D * 2, WAVES = 4;
 constexpr float RESCALE_SLACK = 8.0f;
 constexpr uint32_t WHOLE = UINT32_MAX, PARTS_MOST = 128;
+constexpr uint64_t JOIN_TILES = 8;             // what a join costs, in tiles of a workgroup
 constexpr size_t PART_FLOATS = 32 * (D + 2);   // of 32 rows: O, the running max and the sum
 
 // A workgroup's share: 32 rows of a sequence and its key tiles [first, last); part: where its
@@ -438,7 +439,8 @@ const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_o
     uint64_t work = 0;   // key tiles of the others
     for (uint32_t i : order)
         if (!tiled[i]) work += blocks(i, 32) * kv_heads * tiles(i);
-    const uint64_t share_tiles = std::max<uint64_t>(16, (work + cus - 1) / cus);
+    // A workgroup's share of them: a round of the compute units, each wave with as many tiles as the others.
+    const uint64_t share_tiles = (std::max<uint64_t>(1, (work + cus - 1) / cus) + WAVES - 1) / WAVES * WAVES;
     for (uint32_t i : order) {
         h3_sequence &s = plan.sequences[i];
         // Launches hold fewer than 2^32 threads.
@@ -451,7 +453,7 @@ const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_o
             for (uint32_t b = 0; b < tiles(i); b++) plan.keys.push_back({i, b});
             continue;
         }
-        const uint64_t n = tiles(i), parts = n * 2 > share_tiles * 3 ? std::min<uint64_t>((n + share_tiles - 1) / share_tiles, PARTS_MOST) : 1;
+        const uint64_t n = tiles(i), parts = n >= share_tiles + JOIN_TILES ? std::min<uint64_t>((n + share_tiles - 1) / share_tiles, PARTS_MOST) : 1;
         if ((plan.rows.size() + blocks(i, 32) * parts) * kv_heads >= (1u << 24)) return "more rows than a launch takes";
         for (uint32_t b = 0; b < blocks(i, 32); b++) {
             if (parts > 1) plan.joins.push_back({i, b, plan.parts, (uint32_t)parts});

@@ -38,18 +38,27 @@ struct AxesArgs {
     const float *turns;          // [pairs][2]
     const uint32_t *axis;        // [pairs]
     const float *positions;      // [rows][axes]
-    unsigned rows, heads, kv_heads, share, dim, pairs, axes, splits;
+    unsigned rows, heads, kv_heads, share, dim, pairs, axes, splits, together;
     float eps;
     int grouped, interleaved;
 };
 
 enum Kind { QUERY, KEY, VALUE };
 
-// Where a row has a head of its queries, keys or values.
-__device__ inline unsigned source_head(const AxesArgs &a, Kind kind, unsigned head) {
-    if (!a.grouped) return kind == QUERY ? head : kind == KEY ? a.heads + head : a.heads + a.kv_heads + head;
-    const unsigned share = a.share;
-    return kind == QUERY ? head / share * (share + 2) + head % share : head * (share + 2) + share + (kind == VALUE);
+// Head i of rows from row0 on, each row's queries first, then its keys and values.
+struct Item {
+    int kind;
+    unsigned row;          // behind row0
+    size_t from, to;       // its first channel in qkv, and in its own output
+};
+__device__ inline Item item_of(const AxesArgs &a, unsigned i, unsigned items, size_t row0) {
+    const unsigned row = a.together == 1 ? 0 : i / items, h = i - row * items;
+    const int kind = h < a.heads ? QUERY : h < a.heads + a.kv_heads ? KEY : VALUE;
+    const unsigned head = kind == QUERY ? h : kind == KEY ? h - a.heads : h - a.heads - a.kv_heads;
+    const unsigned source = !a.grouped        ? h
+                            : kind == QUERY ? head / a.share * (a.share + 2) + head % a.share
+                                            : head * (a.share + 2) + a.share + (kind == VALUE);
+    return {kind, row, ((row0 + row) * items + source) * a.dim, ((row0 + row) * (kind == QUERY ? a.heads : a.kv_heads) + head) * a.dim};
 }
 
 // Sums over the 16 / 8 / 32 lanes of a head by row rotations of the VALU; every lane gets the
@@ -85,15 +94,16 @@ enum Pairing {
 };
 
 // LANES lanes a head, a chunk of eight channels each (the last one cut off where the head ends).
-// A workgroup takes rows, or a share of their heads, and goes through a row's queries, keys and
-// values 256 / LANES heads at a time, UNROLL of them in flight a lane. Thread d makes what channel
-// d and its partner are multiplied with in the next row, the norms' weights included, while this
-// one's heads are on their way; lanes take their chunk's from LDS.
+// A workgroup takes `together` rows at a time (more than one where a row's heads would leave lanes
+// idle), or a share of a row's heads, and goes through their queries, keys and values 256 / LANES at a
+// time, UNROLL of them in flight a lane. Thread d makes what channel d and its partner are multiplied
+// with in the next rows, the norms' weights included, while these rows' heads are on their way;
+// lanes take their chunk's from LDS.
+constexpr unsigned TOGETHER = 4;
 template <int LANES, Pairing PAIRING>
-__global__ __launch_bounds__(256, PAIRING == HALVES_LOOSE ? 4 : 5) void rope_axes_chunks(AxesArgs a) {
+__global__ __launch_bounds__(256, 4) void rope_axes_chunks(AxesArgs a) {
     constexpr int GROUPS = 256 / LANES, UNROLL = 4;
-    // [buffer][query, key][channel, partner][channel]
-    __shared__ __attribute__((aligned(16))) float factors[2][2][2][256];
+    extern __shared__ __attribute__((aligned(16))) float factors[];   // [buffer][row][query, key][channel, partner][256]
     const unsigned tid = threadIdx.x, lane = tid % 64, c = lane % LANES, d0 = c * 8, group = tid / LANES;
     const unsigned items = a.heads + 2 * a.kv_heads;
     const bool held = d0 < a.dim, whole = d0 + 8 <= a.dim;
@@ -115,122 +125,126 @@ __global__ __launch_bounds__(256, PAIRING == HALVES_LOOSE ? 4 : 5) void rope_axe
         partner_weight[QUERY] = bf16_to_f32(a.qw[partner_channel]);
         partner_weight[KEY] = bf16_to_f32(a.kw[partner_channel]);
     }
-    const size_t blocks = (size_t)a.rows * a.splits;
-    auto position = [&](size_t block) { return turns && block < blocks ? a.positions[block / a.splits * a.axes + axis] : 0.f; };
-    auto turn = [&](float p, int buffer) {
-        const float t = fmaf(p, lo, fmaf(p, hi, -rintf(p * hi)));
-        const float cs = turns ? __builtin_amdgcn_cosf(t) : 1.f, sn = turns ? __builtin_amdgcn_sinf(t) : 0.f;
+    // Task: `together` rows, or a share of one row.
+    const size_t tasks = (size_t)(a.rows + a.together - 1) / a.together * a.splits;
+    float next[TOGETHER] = {};
+    auto positions = [&](size_t task) {
 #pragma unroll
-        for (int kind = QUERY; kind <= KEY; kind++) {
-            factors[buffer][kind][0][tid] = cs * weight[kind];
-            factors[buffer][kind][1][tid] = (first_channel ? -sn : sn) * partner_weight[kind];
+        for (unsigned r = 0; r < TOGETHER; r++) {
+            const size_t row = task / a.splits * a.together + r;
+            if (r < a.together && turns && row < a.rows) next[r] = a.positions[row * a.axes + axis];
         }
     };
-    turn(position(blockIdx.x), 0);
+    auto turn = [&](unsigned buffer) {
+#pragma unroll
+        for (unsigned r = 0; r < TOGETHER; r++) {
+            if (r >= a.together) break;
+            const float t = fmaf(next[r], lo, fmaf(next[r], hi, -rintf(next[r] * hi)));
+            const float cs = turns ? __builtin_amdgcn_cosf(t) : 1.f, sn = turns ? __builtin_amdgcn_sinf(t) : 0.f;
+#pragma unroll
+            for (int kind = QUERY; kind <= KEY; kind++) {
+                float *const f = factors + ((buffer * a.together + r) * 2 + kind) * 512 + tid;
+                f[0] = cs * weight[kind];
+                f[256] = (first_channel ? -sn : sn) * partner_weight[kind];
+            }
+        }
+    };
+    positions(blockIdx.x);
+    turn(0);
     __syncthreads();
-    int buffer = 0;
-    for (size_t block = blockIdx.x; block < blocks; block += gridDim.x, buffer ^= 1) {
-        const size_t row = block / a.splits;
-        const unsigned part = block % a.splits;
-        const float next = position(block + gridDim.x);
-        const size_t row_at = row * items * a.dim;
-        auto heads = [&](auto kind_tag) {
-            constexpr Kind kind = decltype(kind_tag)::value;
-            const unsigned count = kind == QUERY ? a.heads : a.kv_heads;
-            f32x4 own[2], other[2];
-            if constexpr (kind != VALUE)
+    unsigned buffer = 0;
+    for (size_t task = blockIdx.x; task < tasks; task += gridDim.x, buffer ^= 1) {
+        const size_t row0 = task / a.splits * a.together;
+        const unsigned part = task % a.splits, count = (unsigned)min((size_t)a.together, a.rows - row0) * items;
+        positions(task + gridDim.x);
+        for (unsigned first = part * GROUPS + group; first < count; first += a.splits * GROUPS * UNROLL) {
+            i32x4 raw[UNROLL] = {}, up[UNROLL] = {}, low[UNROLL] = {};
+            Item at[UNROLL];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    own[i] = *reinterpret_cast<const f32x4 *>(&factors[buffer][kind][0][d0 + 4 * i]);
-                    other[i] = *reinterpret_cast<const f32x4 *>(&factors[buffer][kind][1][d0 + 4 * i]);
-                }
-            uint16_t *const out = (kind == QUERY ? a.q : kind == KEY ? a.k : a.v) + row * count * a.dim + d0;
-            for (unsigned first = part * GROUPS + group; first < count; first += a.splits * GROUPS * UNROLL) {
-                i32x4 raw[UNROLL] = {}, up[UNROLL] = {}, low[UNROLL] = {};
+            for (int u = 0; u < UNROLL; u++) {
+                at[u] = item_of(a, first + u * a.splits * GROUPS, items, row0);
+                if (first + u * a.splits * GROUPS >= count || !held) continue;
+                const size_t from = at[u].from + d0;
+                raw[u] = load_loose(a.qkv + from);
+                if (PAIRING == HALVES_LOOSE && at[u].kind != VALUE) {
+                    if (d0 < a.pairs) up[u] = load_loose(a.qkv + from + a.pairs);
+                    if (d0 + 7 >= a.pairs && d0 < 2 * a.pairs) {
+                        if (from >= a.pairs) low[u] = load_loose(a.qkv + (from - a.pairs));
+                        else   // the first head's chunk across the middle: its partners start behind the tensor's first value
 #pragma unroll
-                for (int u = 0; u < UNROLL; u++) {
-                    const unsigned head = first + u * a.splits * GROUPS;
-                    if (head >= count || !held) continue;
-                    const size_t at = row_at + (size_t)source_head(a, kind, head) * a.dim + d0;
-                    raw[u] = load_loose(a.qkv + at);
-                    if (PAIRING == HALVES_LOOSE && kind != VALUE) {
-                        if (d0 < a.pairs) up[u] = load_loose(a.qkv + at + a.pairs);
-                        if (d0 + 7 >= a.pairs && d0 < 2 * a.pairs) {
-                            if (at >= a.pairs) low[u] = load_loose(a.qkv + (at - a.pairs));
-                            else   // the first head's chunk across the middle: its partners start behind the tensor's first value
-#pragma unroll
-                                for (int e = 0; e < 8; e++)
-                                    if (at + e >= a.pairs) put(low[u], e, a.qkv[at + e - a.pairs]);
-                        }
+                            for (int e = 0; e < 8; e++)
+                                if (from + e >= a.pairs) put(low[u], e, a.qkv[from + e - a.pairs]);
                     }
-                }
-#pragma unroll
-                for (int u = 0; u < UNROLL; u++) {
-                    const unsigned head = first + u * a.splits * GROUPS;
-                    if (head >= count) break;
-                    if constexpr (kind != VALUE) {
-                        float x[8], y[8], sum = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            x[e] = PAIRING == HALVES || d0 + e < a.dim ? value(raw[u], e) : 0.f;
-                            sum = fmaf(x[e], x[e], sum);
-                        }
-                        const float r = a.qw ? rsqrtf(head_sum<LANES>(sum) * inv_dim + a.eps) : 1.f;
-                        if constexpr (PAIRING == HALVES) {
-                            const bool turned = d0 < 2 * a.pairs;
-                            const int partner = (int)(turned ? d0 < a.pairs ? lane + a.pairs / 8 : lane - a.pairs / 8 : lane) * 4;
-                            i32x4 theirs;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                theirs[e] = __builtin_amdgcn_ds_bpermute(partner, raw[u][e]);
-                                theirs[e] = turned ? theirs[e] : 0;
-                            }
-#pragma unroll
-                            for (int e = 0; e < 8; e++) y[e] = value(theirs, e);
-                        } else {
-                            // Channels behind the pairs pass as they are, infinities too.
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                const unsigned d = d0 + e;
-                                const float theirs = PAIRING == NEIGHBOURS ? x[e ^ 1] : d < a.pairs ? value(up[u], e) : value(low[u], e);
-                                y[e] = d < 2 * a.pairs ? theirs : 0.f;
-                            }
-                        }
-                        bf16x8 result;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) result[e] = (__bf16)(r * fmaf(x[e], own[e / 4][e % 4], y[e] * other[e / 4][e % 4]));
-                        raw[u] = __builtin_bit_cast(i32x4, result);
-                    }
-                    uint16_t *const dst = out + (size_t)head * a.dim;
-                    if (whole) reinterpret_cast<Loose *>(dst)->v = raw[u];
-                    else if (held)
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (d0 + e < a.dim) dst[e] = (uint16_t)((uint32_t)raw[u][e / 2] >> (e % 2 * 16));
                 }
             }
-        };
-        heads(std::integral_constant<Kind, QUERY>{});
-        heads(std::integral_constant<Kind, KEY>{});
-        heads(std::integral_constant<Kind, VALUE>{});
-        turn(next, buffer ^ 1);
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                if (first + u * a.splits * GROUPS >= count) break;
+                if (at[u].kind != VALUE) {
+                    const f32x4 *const f = reinterpret_cast<const f32x4 *>(factors + ((buffer * a.together + at[u].row) * 2 + at[u].kind) * 512 + d0);
+                    const f32x4 own[2] = {f[0], f[1]}, other[2] = {f[64], f[65]};
+                    float x[8], y[8], sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[e] = PAIRING == HALVES || d0 + e < a.dim ? value(raw[u], e) : 0.f;
+                        sum = fmaf(x[e], x[e], sum);
+                    }
+                    const float r = a.qw ? rsqrtf(head_sum<LANES>(sum) * inv_dim + a.eps) : 1.f;
+                    if constexpr (PAIRING == HALVES) {
+                        const bool turned = d0 < 2 * a.pairs;
+                        const int partner = (int)(turned ? d0 < a.pairs ? lane + a.pairs / 8 : lane - a.pairs / 8 : lane) * 4;
+                        i32x4 theirs;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            theirs[e] = __builtin_amdgcn_ds_bpermute(partner, raw[u][e]);
+                            theirs[e] = turned ? theirs[e] : 0;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; e++) y[e] = value(theirs, e);
+                    } else {
+                        // Channels behind the pairs pass as they are, infinities too.
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const unsigned d = d0 + e;
+                            const float theirs = PAIRING == NEIGHBOURS ? x[e ^ 1] : d < a.pairs ? value(up[u], e) : value(low[u], e);
+                            y[e] = d < 2 * a.pairs ? theirs : 0.f;
+                        }
+                    }
+                    bf16x8 result;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) result[e] = (__bf16)(r * fmaf(x[e], own[e / 4][e % 4], y[e] * other[e / 4][e % 4]));
+                    raw[u] = __builtin_bit_cast(i32x4, result);
+                }
+                uint16_t *const dst = (at[u].kind == QUERY ? a.q : at[u].kind == KEY ? a.k : a.v) + at[u].to + d0;
+                if (whole) reinterpret_cast<Loose *>(dst)->v = raw[u];
+                else if (held)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (d0 + e < a.dim) dst[e] = (uint16_t)((uint32_t)raw[u][e / 2] >> (e % 2 * 16));
+            }
+        }
+        turn(buffer ^ 1);
         __syncthreads();
     }
 }
 
 template <int LANES> void launch_chunks(h3_gpu *g, AxesArgs a) {
     constexpr unsigned GROUPS = 256 / LANES;
-    // A row's heads go to more workgroups where the rows alone would not fill the chip.
-    a.splits = (unsigned)std::min<size_t>((a.heads + GROUPS - 1) / GROUPS, (2048 + (size_t)a.rows - 1) / a.rows);
+    const unsigned items = a.heads + 2 * a.kv_heads;
+    // A row's heads go to more workgroups where the rows alone would not fill the chip; rows of few
+    // heads share a workgroup's lanes where there are rows enough.
+    a.splits = (unsigned)std::min<size_t>((items + GROUPS - 1) / GROUPS, (2048 + (size_t)a.rows - 1) / a.rows);
+    a.together = 1;
+    while (a.together < TOGETHER && a.splits == 1 && items * a.together * 2 <= 2 * GROUPS && a.rows >= 2 * a.together * 4 * g->cus) a.together *= 2;
     // A few rows a workgroup: with as many workgroups as run at once the last ones end the call (18,225
     // rows: 311 us, 313 with twice, 307 with four times and 293 with twenty times as many).
-    const size_t tasks = (size_t)a.rows * a.splits, each = (tasks + 64 * g->cus - 1) / (64 * g->cus);
+    const size_t tasks = (size_t)(a.rows + a.together - 1) / a.together * a.splits, each = (tasks + 64 * g->cus - 1) / (64 * g->cus);
     const unsigned blocks = (unsigned)((tasks + each - 1) / each);
     const Pairing pairing = a.interleaved ? NEIGHBOURS : a.dim % 8 == 0 && a.pairs % 8 == 0 ? HALVES : HALVES_LOOSE;
     auto *kernel = pairing == NEIGHBOURS ? rope_axes_chunks<LANES, NEIGHBOURS>
                    : pairing == HALVES   ? rope_axes_chunks<LANES, HALVES>
                                          : rope_axes_chunks<LANES, HALVES_LOOSE>;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, g->compute, a);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 2 * a.together * 1024 * sizeof(float), g->compute, a);
 }
 
 int rope_axes(h3_gpu *g, const AxesArgs &a) {
@@ -298,7 +312,7 @@ extern "C" int h3_hip_qkv_rope_axes_bf16(h3_gpu *g, h3_gpu_tensor *q, h3_gpu_ten
                      qw ? (const uint16_t *)qw->data : nullptr, kw ? (const uint16_t *)kw->data : nullptr,
                      (const float *)rope->table->data, (const uint32_t *)rope->table->data + 2 * rope->pairs,
                      (const float *)positions->data, rows, heads, kv_heads, heads / kv_heads, dim, rope->pairs,
-                     rope->axes, 1, eps, grouped,
+                     rope->axes, 1, 1, eps, grouped,
                      rope->interleaved};
     return rope_axes(g, a);
 }
