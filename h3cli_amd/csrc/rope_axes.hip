@@ -48,17 +48,16 @@ enum Kind { QUERY, KEY, VALUE };
 // Head i of rows from row0 on, each row's queries first, then its keys and values.
 struct Item {
     int kind;
-    unsigned row;          // behind row0
-    size_t from, to;       // its first channel in qkv, and in its own output
+    unsigned row, from, to;   // its row, and its first channel in qkv and in its own output, behind row0's
 };
-__device__ inline Item item_of(const AxesArgs &a, unsigned i, unsigned items, size_t row0) {
+__device__ inline Item item_of(const AxesArgs &a, unsigned i, unsigned items) {
     const unsigned row = a.together == 1 ? 0 : i / items, h = i - row * items;
     const int kind = h < a.heads ? QUERY : h < a.heads + a.kv_heads ? KEY : VALUE;
     const unsigned head = kind == QUERY ? h : kind == KEY ? h - a.heads : h - a.heads - a.kv_heads;
     const unsigned source = !a.grouped        ? h
                             : kind == QUERY ? head / a.share * (a.share + 2) + head % a.share
                                             : head * (a.share + 2) + a.share + (kind == VALUE);
-    return {kind, row, ((row0 + row) * items + source) * a.dim, ((row0 + row) * (kind == QUERY ? a.heads : a.kv_heads) + head) * a.dim};
+    return {kind, row, (row * items + source) * a.dim, (row * (kind == QUERY ? a.heads : a.kv_heads) + head) * a.dim};
 }
 
 // Sums over the 16 / 8 / 32 lanes of a head by row rotations of the VALU; every lane gets the
@@ -101,8 +100,8 @@ enum Pairing {
 // lanes take their chunk's from LDS.
 constexpr unsigned TOGETHER = 4;
 template <int LANES, Pairing PAIRING>
-__global__ __launch_bounds__(256, 4) void rope_axes_chunks(AxesArgs a) {
-    constexpr int GROUPS = 256 / LANES, UNROLL = 4;
+__global__ __launch_bounds__(256, 5) void rope_axes_chunks(AxesArgs a) {
+    constexpr int GROUPS = 256 / LANES, UNROLL = PAIRING == HALVES_LOOSE ? 2 : 4;   // in five waves' registers
     extern __shared__ __attribute__((aligned(16))) float factors[];   // [buffer][row][query, key][channel, partner][256]
     const unsigned tid = threadIdx.x, lane = tid % 64, c = lane % LANES, d0 = c * 8, group = tid / LANES;
     const unsigned items = a.heads + 2 * a.kv_heads;
@@ -157,23 +156,25 @@ __global__ __launch_bounds__(256, 4) void rope_axes_chunks(AxesArgs a) {
         const size_t row0 = task / a.splits * a.together;
         const unsigned part = task % a.splits, count = (unsigned)min((size_t)a.together, a.rows - row0) * items;
         positions(task + gridDim.x);
+        const uint16_t *const qkv = a.qkv + row0 * items * a.dim;
+        uint16_t *const q = a.q + row0 * a.heads * a.dim, *const k = a.k + row0 * a.kv_heads * a.dim, *const v = a.v + row0 * a.kv_heads * a.dim;
         for (unsigned first = part * GROUPS + group; first < count; first += a.splits * GROUPS * UNROLL) {
             i32x4 raw[UNROLL] = {}, up[UNROLL] = {}, low[UNROLL] = {};
             Item at[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) {
-                at[u] = item_of(a, first + u * a.splits * GROUPS, items, row0);
+                at[u] = item_of(a, first + u * a.splits * GROUPS, items);
                 if (first + u * a.splits * GROUPS >= count || !held) continue;
-                const size_t from = at[u].from + d0;
-                raw[u] = load_loose(a.qkv + from);
+                const unsigned from = at[u].from + d0;
+                raw[u] = load_loose(qkv + from);
                 if (PAIRING == HALVES_LOOSE && at[u].kind != VALUE) {
-                    if (d0 < a.pairs) up[u] = load_loose(a.qkv + from + a.pairs);
+                    if (d0 < a.pairs) up[u] = load_loose(qkv + from + a.pairs);
                     if (d0 + 7 >= a.pairs && d0 < 2 * a.pairs) {
-                        if (from >= a.pairs) low[u] = load_loose(a.qkv + (from - a.pairs));
-                        else   // the first head's chunk across the middle: its partners start behind the tensor's first value
+                        if (row0 || from >= a.pairs) low[u] = load_loose(qkv + from - a.pairs);
+                        else   // the very first head's chunk across the middle: its partners start behind the tensor's first value
 #pragma unroll
                             for (int e = 0; e < 8; e++)
-                                if (from + e >= a.pairs) put(low[u], e, a.qkv[from + e - a.pairs]);
+                                if (from + e >= a.pairs) put(low[u], e, qkv[from + e - a.pairs]);
                     }
                 }
             }
@@ -215,7 +216,7 @@ __global__ __launch_bounds__(256, 4) void rope_axes_chunks(AxesArgs a) {
                     for (int e = 0; e < 8; e++) result[e] = (__bf16)(r * fmaf(x[e], own[e / 4][e % 4], y[e] * other[e / 4][e % 4]));
                     raw[u] = __builtin_bit_cast(i32x4, result);
                 }
-                uint16_t *const dst = (at[u].kind == QUERY ? a.q : at[u].kind == KEY ? a.k : a.v) + at[u].to + d0;
+                uint16_t *const dst = (at[u].kind == QUERY ? q : at[u].kind == KEY ? k : v) + at[u].to + d0;
                 if (whole) reinterpret_cast<Loose *>(dst)->v = raw[u];
                 else if (held)
 #pragma unroll
@@ -235,10 +236,10 @@ template <int LANES> void launch_chunks(h3_gpu *g, AxesArgs a) {
     // heads share a workgroup's lanes where there are rows enough.
     a.splits = (unsigned)std::min<size_t>((items + GROUPS - 1) / GROUPS, (2048 + (size_t)a.rows - 1) / a.rows);
     a.together = 1;
-    while (a.together < TOGETHER && a.splits == 1 && items * a.together * 2 <= 2 * GROUPS && a.rows >= 2 * a.together * 4 * g->cus) a.together *= 2;
-    // A few rows a workgroup: with as many workgroups as run at once the last ones end the call (18,225
-    // rows: 311 us, 313 with twice, 307 with four times and 293 with twenty times as many).
-    const size_t tasks = (size_t)(a.rows + a.together - 1) / a.together * a.splits, each = (tasks + 64 * g->cus - 1) / (64 * g->cus);
+    while (a.together < TOGETHER && a.splits == 1 && items * a.together * 2 <= 4 * GROUPS && a.rows >= 2 * a.together * 4 * g->cus) a.together *= 2;
+    // Many workgroups of a row or few: with as many as run at once the last ones end the call (18,225 rows
+    // of 56 heads: 305 us with 4 workgroups a compute unit, 303 with 16, 298 with 64, 291 with one a row).
+    const size_t tasks = (size_t)(a.rows + a.together - 1) / a.together * a.splits, each = (tasks + 256 * g->cus - 1) / (256 * g->cus);
     const unsigned blocks = (unsigned)((tasks + each - 1) / each);
     const Pairing pairing = a.interleaved ? NEIGHBOURS : a.dim % 8 == 0 && a.pairs % 8 == 0 ? HALVES : HALVES_LOOSE;
     auto *kernel = pairing == NEIGHBOURS ? rope_axes_chunks<LANES, NEIGHBOURS>
