@@ -36,12 +36,13 @@ struct JoinItem {
 struct Plan {
     std::vector<h3_sequence> sequences;
     std::vector<h3_sequence_item> tiles, keys;   // by the 256-row tile kernel
-    std::vector<RowItem> rows;                   // by the kernel here
+    std::vector<h3_sequence_item> mid;           // by attn_sequences_mid
+    std::vector<RowItem> rows;                   // by attn_sequences
     std::vector<JoinItem> joins;
     uint64_t vt = 0;                             // elements of transposed V
     uint32_t parts = 0;
     size_t table_bytes() const {
-        return sequences.size() * sizeof(h3_sequence) + (tiles.size() + keys.size()) * sizeof(h3_sequence_item) +
+        return sequences.size() * sizeof(h3_sequence) + (tiles.size() + keys.size() + mid.size()) * sizeof(h3_sequence_item) +
                rows.size() * sizeof(RowItem) + joins.size() * sizeof(JoinItem);
     }
     size_t retry_at() const { return (vt * 2 + 255) / 256 * 256; }
@@ -54,10 +55,10 @@ struct Plan {
 struct h3_hip_sequences {
     h3_gpu *owner;
     uint32_t heads, kv_heads, count;
-    uint32_t tiles, keys, rows, joins;
+    uint32_t tiles, keys, mid, rows, joins;
     uint64_t q_rows, k_rows;      // rows that the tensors must hold
     size_t retry_at, parts_at;
-    h3_gpu_tensor *table;         // h3_sequence, tiles, keys, rows, joins, behind one another
+    h3_gpu_tensor *table;         // h3_sequence, tiles, keys, mid, rows, joins, behind one another
     h3_gpu_tensor *workspace;     // transposed V, retry bytes, partial results
 };
 
@@ -68,6 +69,7 @@ struct SeqArgs {
     const uint16_t *q, *k, *v;
     const h3_sequence *sequences;
     const RowItem *items;
+    const h3_sequence_item *mid_items;
     const JoinItem *joins;
     float *partial;
     unsigned count, join_count, heads, kv_heads, share;
@@ -317,6 +319,165 @@ void attn_sequences(SeqArgs a) {
     if (worst >= 0x7f800000u) a.fault[0] = 1u;
 }
 
+// A workgroup of four waves takes 128 rows, 32 a wave, and goes through the key tiles together: each
+// tile is loaded once for all waves, the next one on its way in the other of two LDS stages. Two
+// workgroups share a compute unit, so that one's softmax runs beside the other's products. Takes the
+// sequences that are too short for the 256-row tiles' transposed V and recomputation to pay.
+__global__ __attribute__((amdgpu_flat_work_group_size(64 * WAVES, 64 * WAVES), amdgpu_waves_per_eu(2, 2)))
+void attn_sequences_mid(SeqArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+    const unsigned n = lane % 32, hf = lane / 32;
+    const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
+    const unsigned kv = __builtin_amdgcn_readfirstlane(id / a.count);
+    const h3_sequence_item item = a.mid_items[__builtin_amdgcn_readfirstlane(id % a.count)];
+    const h3_sequence s = a.sequences[item.sequence];
+    const unsigned lk = __builtin_amdgcn_readfirstlane(s.lk), k0 = __builtin_amdgcn_readfirstlane(s.k0);
+    const unsigned block = __builtin_amdgcn_readfirstlane(item.block);
+    const unsigned rows = __builtin_amdgcn_readfirstlane(s.lq) * a.share, blocks = (rows + 127) / 128, count = (lk + BN - 1) / BN;
+    const size_t kstride = (size_t)a.kv_heads * D * 2;   // bytes
+    const float c = a.scale_log2;
+
+    // Wave's 1 KB blocks 4 wave + j of a tile: keys 16 wave + 4 j + lane / 16, chunk lane % 16 (swizzled).
+    unsigned off[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const unsigned key = 16 * wave + 4 * j + lane / 16;
+        off[j] = key * (unsigned)kstride + chunk(key, lane % 16) * 16;
+    }
+    auto load = [&](const uint16_t *base, uint8_t *dst, unsigned tile) {
+        const unsigned key0 = tile * BN;
+        const size_t bytes = (size_t)(lk - key0) * kstride - kv * D * 2;
+        const uint16_t *first = base + ((size_t)k0 + key0) * (kstride / 2) + kv * D;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)first, (short)0, (int)__builtin_amdgcn_readfirstlane((unsigned)(bytes < 0xFFFFFFE0u ? bytes : 0xFFFFFFE0u)), 0x00020000);
+#pragma unroll
+        for (unsigned j = 0; j < 4; j++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                r, (__attribute__((address_space(3))) void *)(dst + (wave * 4 + j) * 1024), 16,
+                key0 + 16 * wave + 4 * j + lane / 16 < lk ? off[j] : BUFFER_OOB, 0, 0, 0);
+    };
+    unsigned worst = 0;
+    auto screen = [&](const uint8_t *tile) {
+#pragma unroll
+        for (unsigned j = 0; j < 4; j++) {
+            const i32x4 w = *reinterpret_cast<const i32x4 *>(tile + ((wave * 4 + j) * 64 + lane) * 16);
+            note_bf16(worst, &w, 4);
+        }
+    };
+    bf16x8 qf[8];
+    const unsigned row = block * 128 + wave * 32 + n, held = min(row, rows - 1);
+    const size_t qrow = ((size_t)s.q0 + held / a.share) * a.heads + kv * a.share + held % a.share;
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++) qf[ks] = *reinterpret_cast<const bf16x8 *>(a.q + qrow * D + hf * 8 + ks * 16);
+    load(a.k, smem, 0);
+    load(a.v, smem + TILE, 0);
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++) note_bf16(worst, &qf[ks], 4);
+    f32x16 o[4] = {};
+    float m = -1e30f, l = 0.f;
+    const unsigned p16 = lane % 16, vrow = hf * 4 + p16 / 4, vch = 2 * (lane / 16 % 2) + p16 % 4 / 2;
+    wait_vm_loads();
+    __syncthreads();
+
+    for (unsigned t = 0; t < count; t++) {
+        const uint8_t *const kt = smem + t % 2 * 2 * TILE, *const vt = kt + TILE;
+        if (t + 1 < count) {
+            uint8_t *const next = smem + (t + 1) % 2 * 2 * TILE;
+            load(a.k, next, t + 1);
+            load(a.v, next + TILE, t + 1);
+        }
+        // Each tile's K and V are screened for Inf and NaN by one of the key head's workgroups.
+        if (t % blocks == block) {
+            screen(kt);
+            screen(vt);
+        }
+        f32x16 sc[2] = {};
+        {
+            bf16x8 kf[16];
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                const unsigned key = x % 2 * 32 + n;
+                kf[x] = *reinterpret_cast<const bf16x8 *>(kt + key * 256 + chunk(key, x / 2 * 2 + hf) * 16);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+                for (int mb = 0; mb < 2; mb++)
+                    sc[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks * 2 + mb], qf[ks], sc[mb], 0, 0, 0);
+        }
+        if (t * BN + BN > lk)
+#pragma unroll
+            for (int mb = 0; mb < 2; mb++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (t * BN + mb * 32 + (r / 4) * 8 + hf * 4 + r % 4 >= lk) sc[mb][r] = -INFINITY;
+        bf16x8 pb[4];
+        {
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                mx0 = fmaxf(fmaxf(mx0, sc[0][r]), sc[0][r + 1]);
+                mx1 = fmaxf(fmaxf(mx1, sc[1][r]), sc[1][r + 1]);
+            }
+            const float mx = half_max_swap(fmaxf(mx0, mx1)) * c;
+            if (__builtin_amdgcn_ballot_w64(mx > m + RESCALE_SLACK)) {
+                const float mnew = fmaxf(m, mx), alpha = exp2f_fast(m - mnew);
+                m = mnew;
+                l *= alpha;
+#pragma unroll
+                for (int md = 0; md < 4; md++) o[md] *= alpha;
+            }
+            const float neg = -m - RESCALE_SLACK;
+            float sum = 0.f;
+#pragma unroll
+            for (int mb = 0; mb < 2; mb++)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float p0 = exp2f_fast(fmaf(sc[mb][r], c, neg)), p1 = exp2f_fast(fmaf(sc[mb][r + 1], c, neg));
+                    sum += p0 + p1;
+                    pb[mb * 2 + r / 8][r % 8] = (__bf16)p0;
+                    pb[mb * 2 + r / 8][r % 8 + 1] = (__bf16)p1;
+                }
+            l += sum;
+        }
+        // V^T fragments: keys 16 kk + 4 hf + 0..3 and 8 further on, the order of P's registers. Read after the
+        // softmax: read before it they cost registers (4000 rows of 40 heads 388 us, so 368).
+        i16x4 vh[16][2];
+#pragma unroll
+        for (int x = 0; x < 16; x++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const unsigned r = 16 * (x / 4) + 8 * h + vrow;
+                vh[x][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) i16x4 *)(vt + r * 256 + chunk(r, x % 4 * 4 + vch) * 16 + p16 % 2 * 8));
+            }
+#pragma unroll
+        for (int x = 0; x < 16; x++) {
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(vh[x][0], vh[x][1], 0, 1, 2, 3, 4, 5, 6, 7));
+            o[x % 4] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[x / 4], o[x % 4], 0, 0, 0);
+        }
+        wait_vm_loads();
+        __syncthreads();
+    }
+    const float total = half_sum_swap(l), inv = total > 0.f ? 1.f / total : 0.f;
+    uint16_t *const dst = a.out + qrow * D;
+#pragma unroll
+    for (int md = 0; md < 4; md++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            u16x4 out;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float y = o[md][g * 4 + e] * inv;
+                worst = max(worst, __builtin_bit_cast(uint32_t, y) & 0x7f800000u);
+                out[e] = f32_to_bf16(y);
+            }
+            if (row < rows) *reinterpret_cast<u16x4 *>(dst + md * 32 + g * 8 + hf * 4) = out;
+        }
+    if (worst >= 0x7f800000u) a.fault[0] = 1u;
+}
+
 // 32 rows from their parts, in the parts' order: each brought to the common maximum.
 __global__ __launch_bounds__(256) void attn_sequences_join(SeqArgs a) {
     __shared__ float weight[32][PARTS_MOST + 1];
@@ -370,6 +531,22 @@ __global__ __launch_bounds__(256) void attn_sequences_join(SeqArgs a) {
     if (worst >= 0x7f800000u) a.fault[0] = 1u;
 }
 
+int launch_mid(h3_gpu *g, const SeqArgs &a) {
+    constexpr size_t shared = 4 * TILE;
+    static bool configured = false;
+    if (!configured) {
+        if (!h3_hip_check(g, hipFuncSetAttribute((const void *)attn_sequences_mid, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)shared), "attention shared memory"))
+            return 0;
+        configured = true;
+    }
+    h3_note_kernel(g, "attn_sequences", 128);
+    hipEvent_t timing = h3_kernel_timing_begin(g);
+    hipLaunchKernelGGL(attn_sequences_mid, dim3(a.count * a.kv_heads), dim3(64 * WAVES), shared, g->compute, a);
+    h3_kernel_timing_end(g, timing);
+    return h3_launch_status(g, "BF16 attention of sequences");
+}
+
 int launch(h3_gpu *g, const SeqArgs &a) {
     constexpr size_t shared = WAVES * 2 * TILE;
     static bool configured = false;
@@ -388,14 +565,39 @@ int launch(h3_gpu *g, const SeqArgs &a) {
     return h3_launch_status(g, "BF16 attention of sequences");
 }
 
-// Microseconds of a workgroup: here 32 rows, each wave a 64-key tile in four; 256 rows by 128
-// keys in the tile kernel.
-double row_cost(uint64_t tiles) { return 6.0 + 2.2 * (double)((tiles + 3) / 4); }
-double tile_cost(uint64_t keys) { return 2.0 + 2.13 * (double)((keys + 127) / 128); }
+// Modelled microseconds of the kernels' workgroups, by 64-key tiles, and of a kernel's launches: as many
+// workgroups as run at once, and half a round more behind whole rounds. Measured, all rows by one kernel
+// (32 / 128 / 256 rows a workgroup): 300 rows of 4 heads 11.2 / 13.4 / 23.5 us, of 40 heads 19.5 /
+// 14.8 / 27.0; 1000 rows of 8 heads 15.6 / 28.2 / 33.2, of 40 heads 65 / 45 / 45; 729 and 806 rows of
+// 56 heads 129 / 61 / 76; eight times 250 rows of 40 heads 72 / 30 / 72; 4000 rows of 40 heads 656 /
+// 368 / 332; 5000 rows of 8 heads 199 / 157 / 116.
+struct Load {
+    double sum = 0, longest = 0, workgroups = 0;
+    void add(double cost, double count) {
+        sum += cost * count;
+        longest = std::max(longest, cost);
+        workgroups += count;
+    }
+};
+double row_cost(uint64_t tiles) { return 6 + 1.75 * (double)((tiles + WAVES - 1) / WAVES); }
+double mid_cost(uint64_t tiles) { return 4 + 2.3 * (double)tiles; }              // two on a compute unit
+double tile_cost(uint64_t tiles) { return 5 + 2.1 * (double)((tiles + 1) / 2); }
+double row_time(const Load &l, double cus) {
+    return l.workgroups ? 3 + (l.workgroups > cus ? l.sum / cus + l.longest / 2 : l.longest) : 0;
+}
+double mid_time(const Load &l, double cus) {
+    if (!l.workgroups) return 0;
+    return 3 + (l.workgroups > 2 * cus ? l.sum / (2 * cus) + l.longest / 4 : l.workgroups > cus ? l.longest : l.longest * 0.75);
+}
+// Also the transposition of `keys` keys' V, and the recomputation. Busy compute units draw more power.
+double tile_time(const Load &l, double cus, double keys) {
+    if (!l.workgroups) return 0;
+    return 11 + keys * 1.7e-4 + (1 + 0.45 * std::min(1.0, l.workgroups / cus)) * (l.workgroups > cus ? l.sum / cus + l.longest / 2 : l.longest);
+}
 
-// Which sequences the tile kernel takes, and how the others' keys are shared out.
+// Which kernel takes which sequences, and how the keys of those with few rows are shared out.
 const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_offsets, uint32_t count, uint32_t heads,
-                      uint32_t kv_heads, uint32_t cus) {
+                      uint32_t kv_heads, uint32_t cus, int variant) {
     if (!q_offsets || !count || count > (1u << 20) || !kv_heads || !heads || heads > 65535 || heads % kv_heads)
         return "need 1 to 2^20 of them and heads a multiple of the key heads";
     if (!k_offsets) k_offsets = q_offsets;
@@ -413,38 +615,72 @@ const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_o
     std::stable_sort(order.begin(), order.end(), [&](uint32_t x, uint32_t y) { return plan.sequences[x].lk > plan.sequences[y].lk; });
     auto blocks = [&](uint32_t i, uint32_t size) { return ((uint64_t)plan.sequences[i].lq * share + size - 1) / size; };
     auto tiles = [&](uint32_t i) { return ((uint64_t)plan.sequences[i].lk + BN - 1) / BN; };
-    // The tile kernel takes the sequences with at least some number of rows: each number in turn, with
-    // the time of its kernels' workgroups over the compute units, or of the longest one.
-    std::vector<uint32_t> by_rows;
-    for (uint32_t i : order)
-        if (plan.sequences[i].lk > 256 && (uint64_t)plan.sequences[i].lk * kv_heads * D * 2 < (1ull << 32)) by_rows.push_back(i);
+    // Kernels in the order of their row blocks: 256, 128 and 32 rows. With the sequences by their rows each
+    // kernel takes a range of them; every choice of the two borders (of up to 65 evenly spread ones).
+    std::vector<uint32_t> by_rows = order;
+    auto tileable = [&](uint32_t i) { return plan.sequences[i].lk > 256 && (uint64_t)plan.sequences[i].lk * kv_heads * D * 2 < (1ull << 32); };
     std::stable_sort(by_rows.begin(), by_rows.end(), [&](uint32_t x, uint32_t y) { return plan.sequences[x].lq > plan.sequences[y].lq; });
-    double rows_work = 0, tile_work = 0, tile_longest = 0;
-    for (uint32_t i : order) rows_work += (double)blocks(i, 32) * kv_heads * row_cost(tiles(i));
-    double best = rows_work / cus;
-    size_t taken = 0;
-    for (size_t j = 0; j < by_rows.size(); j++) {
-        const uint32_t i = by_rows[j];
-        rows_work -= (double)blocks(i, 32) * kv_heads * row_cost(tiles(i));
-        tile_work += (double)blocks(i, 256) * kv_heads * tile_cost(plan.sequences[i].lk);
-        tile_longest = std::max(tile_longest, tile_cost(plan.sequences[i].lk));
-        const double time = 15 + std::max(tile_work / cus, tile_longest) + rows_work / cus;
-        if (time < best) {
-            best = time;
-            taken = j + 1;
+    const size_t n = by_rows.size(), stride = std::max<size_t>(1, (n + 63) / 64);
+    // Rows' time from each border on.
+    std::vector<size_t> borders;
+    for (size_t j = 0; j < n; j += stride) borders.push_back(j);
+    borders.push_back(n);
+    std::vector<double> rows_from(borders.size(), 0.0);
+    Load rows;
+    for (size_t b = borders.size() - 1, j = n; b-- > 0;) {
+        while (j > borders[b]) {
+            j--;
+            rows.add(row_cost(tiles(by_rows[j])), (double)blocks(by_rows[j], 32) * kv_heads);
+        }
+        rows_from[b] = row_time(rows, cus);
+    }
+    double best = 1e300, tile_keys = 0;
+    size_t first_mid = 0, first_row = 0, taken = 0;
+    Load tile;
+    for (size_t i = 0; i < borders.size(); i++) {
+        bool fits = true;
+        for (; taken < borders[i]; taken++) {
+            const uint32_t x = by_rows[taken];
+            if (!(fits = tileable(x))) break;
+            tile.add(tile_cost(tiles(x)), (double)blocks(x, 256) * kv_heads);
+            tile_keys += (double)plan.sequences[x].lk * kv_heads;
+        }
+        if (!fits) break;
+        Load mid;
+        size_t j = borders[i];
+        for (size_t b = i; b < borders.size(); b++) {
+            for (; j < borders[b]; j++) mid.add(mid_cost(tiles(by_rows[j])), (double)blocks(by_rows[j], 128) * kv_heads);
+            const double time = tile_time(tile, cus, tile_keys) + mid_time(mid, cus) + rows_from[b];
+            if (time < best) {
+                best = time;
+                first_mid = borders[i];
+                first_row = j;
+            }
         }
     }
-    std::vector<bool> tiled(count, false);
-    for (size_t j = 0; j < taken; j++) tiled[by_rows[j]] = true;
+    // Measurement: variants 20, 21 and 22 take the kernel of 32 rows, of 128, and of 256 wherever it can.
+    if (variant == 20) first_mid = first_row = 0;
+    if (variant == 21) first_mid = 0, first_row = n;
+    if (variant == 22) {
+        for (first_mid = 0; first_mid < n && tileable(by_rows[first_mid]);) first_mid++;
+        first_row = n;
+    }
+    std::vector<uint8_t> kernel(count, 0);
+    for (size_t j = 0; j < n; j++) kernel[by_rows[j]] = j < first_mid ? 2 : j < first_row ? 1 : 0;
     uint64_t work = 0;   // key tiles of the others
     for (uint32_t i : order)
-        if (!tiled[i]) work += blocks(i, 32) * kv_heads * tiles(i);
+        if (!kernel[i]) work += blocks(i, 32) * kv_heads * tiles(i);
     // A workgroup's share of them: a round of the compute units, each wave with as many tiles as the others.
     const uint64_t share_tiles = (std::max<uint64_t>(1, (work + cus - 1) / cus) + WAVES - 1) / WAVES * WAVES;
     for (uint32_t i : order) {
         h3_sequence &s = plan.sequences[i];
         // Launches hold fewer than 2^32 threads.
-        if (tiled[i]) {
+        if (kernel[i] == 1) {
+            if ((plan.mid.size() + blocks(i, 128)) * kv_heads >= (1u << 24)) return "more rows than a launch takes";
+            for (uint32_t b = 0; b < blocks(i, 128); b++) plan.mid.push_back({i, b});
+            continue;
+        }
+        if (kernel[i] == 2) {
             if ((plan.tiles.size() + blocks(i, 256)) * kv_heads >= (1u << 23) || (plan.keys.size() + tiles(i)) * kv_heads >= (1u << 24))
                 return "more rows than a launch takes";
             s.vt = plan.vt;
@@ -476,7 +712,7 @@ extern "C" void h3_hip_sequences_free(h3_hip_sequences *s) {
 extern "C" int h3_hip_sequences_layout(const uint32_t *q_offsets, const uint32_t *k_offsets, uint32_t count, uint32_t heads,
                                        uint32_t kv_heads, size_t *bytes) try {
     Plan plan;
-    if (make_plan(plan, q_offsets, k_offsets, count, heads, kv_heads, 256)) return 0;
+    if (make_plan(plan, q_offsets, k_offsets, count, heads, kv_heads, 256, 0)) return 0;
     if (bytes) *bytes = plan.table_bytes() + plan.workspace_bytes(kv_heads);
     return 1;
 } catch (const std::bad_alloc &) {
@@ -490,7 +726,7 @@ extern "C" h3_hip_sequences *h3_hip_sequences_new(h3_gpu *g, const uint32_t *q_o
     Plan plan;
     std::vector<uint32_t> words;
     try {
-        if (const char *why = make_plan(plan, q_offsets, k_offsets, count, heads, kv_heads, g->cus)) {
+        if (const char *why = make_plan(plan, q_offsets, k_offsets, count, heads, kv_heads, g->cus, g->attention_variant)) {
             h3_set_error(g, "sequences: %s", why);
             return nullptr;
         }
@@ -501,10 +737,11 @@ extern "C" h3_hip_sequences *h3_hip_sequences_new(h3_gpu *g, const uint32_t *q_o
         append(plan.sequences);
         append(plan.tiles);
         append(plan.keys);
+        append(plan.mid);
         append(plan.rows);
         append(plan.joins);
         s = new h3_hip_sequences{g, heads, kv_heads, count, (uint32_t)plan.tiles.size(), (uint32_t)plan.keys.size(),
-                                 (uint32_t)plan.rows.size(), (uint32_t)plan.joins.size(), q_offsets[count],
+                                 (uint32_t)plan.mid.size(), (uint32_t)plan.rows.size(), (uint32_t)plan.joins.size(), q_offsets[count],
                                  (k_offsets ? k_offsets : q_offsets)[count], plan.retry_at(), plan.parts_at(kv_heads), nullptr, nullptr};
     } catch (const std::bad_alloc &) {
         h3_set_error(g, "sequences: out of host memory");
@@ -532,7 +769,7 @@ extern "C" int h3_hip_sdpa_sequences_bf16(h3_gpu *g, h3_gpu_tensor *out, const h
     const float rounded = bf16_to_f32(f32_to_bf16(scale));
     const auto *sequences = (const h3_sequence *)s->table->data;
     const auto *items = (const h3_sequence_item *)(sequences + s->count);
-    const auto *rows = (const RowItem *)(items + s->tiles + s->keys);
+    const auto *rows = (const RowItem *)(items + s->tiles + s->keys + s->mid);
     char *const workspace = s->workspace ? (char *)s->workspace->data : nullptr;
     if (s->tiles) {
         const h3_sequence_tiles t{sequences, items, items + s->tiles, s->tiles, s->keys, s->heads, s->kv_heads,
@@ -541,12 +778,12 @@ extern "C" int h3_hip_sdpa_sequences_bf16(h3_gpu *g, h3_gpu_tensor *out, const h
                                                 (const uint16_t *)v->data, t, rounded))
             return 0;
     }
-    if (s->rows) {
-        const SeqArgs a{(uint16_t *)out->data, (const uint16_t *)q->data, (const uint16_t *)k->data, (const uint16_t *)v->data,
-                        sequences, rows, (const JoinItem *)(rows + s->rows), s->joins ? (float *)(workspace + s->parts_at) : nullptr,
-                        s->rows, s->joins, s->heads, s->kv_heads, s->heads / s->kv_heads, rounded * 1.4426950408889634f, g->fault};
-        if (!launch(g, a)) return 0;
-    }
-    if (s->tiles + s->rows) g->stats.attention_dispatches++;
+    SeqArgs a{(uint16_t *)out->data, (const uint16_t *)q->data, (const uint16_t *)k->data, (const uint16_t *)v->data, sequences, rows,
+              items + s->tiles + s->keys, (const JoinItem *)(rows + s->rows), s->joins ? (float *)(workspace + s->parts_at) : nullptr,
+              s->mid, s->joins, s->heads, s->kv_heads, s->heads / s->kv_heads, rounded * 1.4426950408889634f, g->fault};
+    if (s->mid && !launch_mid(g, a)) return 0;
+    a.count = s->rows;
+    if (s->rows && !launch(g, a)) return 0;
+    if (s->tiles + s->mid + s->rows) g->stats.attention_dispatches++;
     return 1;
 }

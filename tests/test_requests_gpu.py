@@ -123,38 +123,41 @@ def check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=1, spread=1.0
     ([0, 300, 1100, 1130], None, 4, 4),
     ([0, 200], [0, 900], 40, 8),
 ])
-def test_attention_of_sequences(q_offsets, k_offsets, heads, kv_heads):
-    print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads}", flush=True)
+@pytest.mark.parametrize("variant", [0, 20, 21, 22])
+def test_attention_of_sequences(q_offsets, k_offsets, heads, kv_heads, variant, monkeypatch):
+    """By the kernel that the plan chooses, and by those of 32, 128 and (from 257 keys on) 256 rows."""
+    print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads} {variant}", flush=True)
+    monkeypatch.setenv("H3_HIP_ATTENTION_VARIANT", str(variant))
     with Gpu() as g:
         check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=len(q_offsets) * 17 + heads)
 
 
+@pytest.mark.parametrize("variant", [20, 21, 22])
 @pytest.mark.parametrize("spread,scale", [(6.0, SCALE), (0.01, SCALE), (1.0, 3.0), (1.0, 2.0 ** -20)])
-def test_attention_of_sequences_peaks_and_flat_rows(spread, scale):
+def test_attention_of_sequences_peaks_and_flat_rows(spread, scale, variant, monkeypatch):
+    monkeypatch.setenv("H3_HIP_ATTENTION_VARIANT", str(variant))
     with Gpu() as g:
         check_attention(g, [0, 70, 135], [0, 300, 650], 2, 2, seed=5, spread=spread, scale=scale)
 
 
 @pytest.mark.parametrize("q_offsets,k_offsets,heads,kv_heads,rising", [
-    ([0, 700, 1500], None, 40, 40, 0.0),
-    ([1, 258, 258, 1000, 1513], None, 40, 40, 30.0),                # later keys' scores far above the first's
-    ([0, 600, 1000], [3, 260, 900], 60, 12, 0.0),                   # shared key heads: rows of five heads in a tile
-    ([0, 513, 770, 1500], [0, 640, 897, 2000], 42, 42, 5.0),
-    ([0, 1100, 1130, 1131, 1200], [0, 900, 1000, 2400, 2400], 40, 40, 0.0),   # and short ones beside them
+    ([0, 700, 1500], None, 4, 4, 0.0),
+    ([1, 258, 258, 1000, 1513], None, 3, 3, 30.0),                  # later keys' scores far above the first's
+    ([0, 600, 1000], [3, 260, 900], 10, 2, 0.0),                    # shared key heads: rows of five heads in a tile
+    ([0, 513, 770, 1500], [0, 640, 897, 2000], 2, 2, 5.0),
+    ([0, 1100, 1130, 1131, 1200], [0, 900, 1000, 2400, 2400], 4, 4, 0.0),   # and short ones beside them
 ])
-def test_attention_of_sequences_by_tiles(q_offsets, k_offsets, heads, kv_heads, rising):
-    """Sequences long and many enough for the kernel of 256-row tiles, alone or with others."""
+def test_attention_of_sequences_by_tiles(q_offsets, k_offsets, heads, kv_heads, rising, monkeypatch):
+    """The kernel of 256-row tiles, with the recomputation where a row's scores rise."""
     print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads}", flush=True)
-    size = C.c_size_t()
+    monkeypatch.setenv("H3_HIP_ATTENTION_VARIANT", "22")
     with Gpu() as g:
-        g.check(g.lib.h3_hip_sequences_layout(u32(q_offsets), None if k_offsets is None else u32(k_offsets), len(q_offsets) - 1,
-                                              heads, kv_heads, C.byref(size)))
-        assert size.value > 2 * 128 * 256 * kv_heads, size.value      # the plan holds transposed values
-        check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=7, rising=rising, heads_seen=(0, 1, heads // 2, heads - 1))
+        kernel = check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=7, rising=rising)
+        assert kernel in ("attn_bf16_pipe", "attn_sequences rows=128"), kernel
 
 
 def test_attention_of_one_sequence_is_the_dense_attention():
-    seq, heads = 4133, 6
+    seq, heads = 4133, 12
     with Gpu() as g:
         ts = [g.from_bf16(normal(seq * heads * 128, i)) for i in range(3)]
         a, b = g.empty(seq * heads * 128), g.empty(seq * heads * 128)
@@ -166,6 +169,33 @@ def test_attention_of_one_sequence_is_the_dense_attention():
             assert g.last_kernel() == "attn_bf16_pipe"
             g.submit()
         assert np.array_equal(a.read(), b.read())
+
+
+@pytest.mark.parametrize("q_offsets,k_offsets,heads,kv_heads,rising", [
+    ([0, 729, 1535], None, 3, 3, 0.0),
+    ([2, 131, 131, 260, 700], None, 4, 4, 20.0),                    # 128 rows and one more
+    ([0, 100, 250, 251], [0, 64, 64, 700], 10, 2, 0.0),             # queries without keys; rows of five heads in a block
+    ([0, 128, 400], [0, 65, 330], 9, 3, 6.0),
+])
+def test_attention_of_sequences_by_128_rows(q_offsets, k_offsets, heads, kv_heads, rising, monkeypatch):
+    print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads}", flush=True)
+    monkeypatch.setenv("H3_HIP_ATTENTION_VARIANT", "21")
+    with Gpu() as g:
+        kernel = check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=11, rising=rising)
+        assert kernel == "attn_sequences rows=128", kernel
+
+
+@pytest.mark.parametrize("lengths,heads,kernel", [((1000,), 8, "rows=32"), ((729, 806), 56, "rows=128"), ((8193,), 12, "attn_bf16_pipe")])
+def test_plans_choose_by_rows_and_heads(lengths, heads, kernel):
+    with Gpu() as g:
+        rows = sum(lengths)
+        t, out = g.empty(rows * heads * 128), g.empty(rows * heads * 128)
+        with sequences(g, np.cumsum([0] + list(lengths)), None, heads, heads) as plan:
+            g.begin()
+            g.check(g.lib.h3_hip_fill_normal_bf16(g.handle, t.handle, 1, C.c_float(1.0), t.elements))
+            g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, out.handle, t.handle, t.handle, t.handle, plan, C.c_float(SCALE)))
+            assert kernel in g.last_kernel(), g.last_kernel()
+            g.submit()
 
 
 @pytest.mark.parametrize("q_offsets,k_offsets,heads,kv_heads", [
@@ -182,16 +212,19 @@ def test_attention_of_few_rows_over_many_keys(q_offsets, k_offsets, heads, kv_he
             assert kernel == "attn_sequences rows=32 shares=2", kernel     # parts, joined
 
 
-def test_attention_of_sequences_reports_values_that_are_not_finite():
+@pytest.mark.parametrize("variant", [20, 21, 22])
+def test_attention_of_sequences_reports_values_that_are_not_finite(variant, monkeypatch):
     """In a query, key or value of any sequence; the others' results stay whole."""
+    monkeypatch.setenv("H3_HIP_ATTENTION_VARIANT", str(variant))
+    rows, cut = 400, 60
     for which in range(3):
         with Gpu() as g:
-            ts = [normal(100 * 256, 3 + i).reshape(100, 2, 128).copy() for i in range(3)]
+            ts = [normal(rows * 256, 3 + i).reshape(rows, 2, 128).copy() for i in range(3)]
             clean = [g.from_bf16(t) for t in ts]
-            ts[which][77, 1, 5] = 0x7f80 if which else 0x7fc0
+            ts[which][77 + 4 * variant, 1, 5] = 0x7f80 if which else 0x7fc0
             dirty = [g.from_bf16(t) for t in ts]
-            out, other = g.empty(100 * 256), g.empty(100 * 256)
-            with sequences(g, [0, 40, 100], None, 2, 2) as plan:
+            out, other = g.empty(rows * 256), g.empty(rows * 256)
+            with sequences(g, [0, cut, rows], None, 2, 2) as plan:
                 args = (plan, C.c_float(SCALE))
                 g.begin()
                 g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, out.handle, *(t.handle for t in clean), *args))
@@ -201,8 +234,8 @@ def test_attention_of_sequences_reports_values_that_are_not_finite():
                 with pytest.raises(H3Error, match="nonfinite attention"):
                     g.submit()
                 g.cancel()
-                a, b = out.read().reshape(100, 2, 128), other.read().reshape(100, 2, 128)
-                assert np.array_equal(a[:40], b[:40]) and np.array_equal(a[40:, 0], b[40:, 0])
+                a, b = out.read().reshape(rows, 2, 128), other.read().reshape(rows, 2, 128)
+                assert np.array_equal(a[:cut], b[:cut]) and np.array_equal(a[cut:, 0], b[cut:, 0])
 
 
 # ------------------------------------------------------------------ rotation by axes

@@ -21,7 +21,7 @@ def layout(q, k, heads, kv_heads, count=None):
     ([0, 4], None, 3, 2, None), ([0, 4], None, 0, 1, None), ([0, 4], None, 4, 0, None), ([4, 3], None, 1, 1, None),
     ([0, 4], [5, 4], 1, 1, None), ([0, 4, 3], None, 1, 1, None), ([0, 4], None, 65536, 1, None), ([0], None, 1, 1, 0),
     (None, [0, 1], 1, 1, 1), ([0, 2 ** 31], None, 1, 1, None), ([0, 2 ** 30], None, 2, 1, None), ([0, 1], [0, 2 ** 31], 1, 1, None),
-    ([0, 2 ** 29], [0, 1], 1, 1, None), ([0, 2 ** 25], [0, 0], 60000, 60000, None), ([0, 2 ** 31 - 1], [0, 2 ** 31 - 1], 1, 1, None),
+    ([0, 2 ** 31 - 1], [0, 1], 1, 1, None), ([0, 2 ** 25], [0, 0], 60000, 60000, None), ([0, 2 ** 31 - 1], [0, 2 ** 31 - 1], 1, 1, None),
 ])
 def test_refused_sequences(q, k, heads, kv_heads, count):
     assert layout(q, k, heads, kv_heads, count) is None
@@ -32,7 +32,7 @@ def test_sequences_hold_what_their_kernels_need():
     assert layout([0, 0, 0], None, 1, 1) > 0                     # no rows at all
     assert layout([5, 5, 9], [7, 20, 20], 4, 2) > 0
     # Transposed values of 4133 keys in whole tiles of 64, and retry bytes.
-    assert layout([0, 4133], None, 6, 6) > 65 * 64 * 6 * 256
+    assert layout([0, 4133], None, 12, 12) > 65 * 64 * 12 * 256
     # One row over many keys: parts of 32 rows, and no transposed values.
     assert 2 * 130 * 128 < layout([0, 1], [0, 18225], 5, 1) < 128 * 32 * 130 * 4 + 4096
     # A K of 4 GiB and more, in which a tile's offsets would not fit 32 bits, goes without them too.
