@@ -77,8 +77,12 @@ struct SeqArgs {
     unsigned *fault;
 };
 
-// 16-byte chunk swizzle of a 256-byte row.
+// 16-byte chunk swizzles of a 256-byte row. K: sixteen keys' reads of one chunk meet all banks. V: a
+// transposing read takes 32 bytes of each of four keys for 16 lanes, and the 32 bytes behind them for the
+// next 16: they meet all banks too. (With K's swizzle for both, 60% of the LDS cycles of the 128-row
+// kernel were conflicts: 4000 rows of 40 heads 368 us.)
 __device__ inline unsigned chunk(unsigned key, unsigned ch) { return ch ^ (key & 15); }
+__device__ inline unsigned v_chunk(unsigned key, unsigned ch) { return ch ^ (key & 3) << 2; }
 
 // The largest exponent field seen, in place (bits 30:23 of a float): non-finite from
 // 0x7f800000 on.
@@ -115,13 +119,14 @@ void attn_sequences(SeqArgs a) {
 
     // Tile loads: 1 KB block b of a tile holds keys 4 b + lane / 16, chunk lane % 16 (swizzled).
     // A tile's descriptor starts at its first key and ends with the sequence, or 4 GiB on.
-    unsigned off[4];
+    unsigned off[4], v_off[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const unsigned key = 4 * j + lane / 16;
         off[j] = key * (unsigned)kstride + chunk(key, lane % 16) * 16;
+        v_off[j] = key * (unsigned)kstride + v_chunk(key, lane % 16) * 16;
     }
-    auto load = [&](const uint16_t *base, uint8_t *dst, unsigned tile) {
+    auto load = [&](const uint16_t *base, const unsigned *off, uint8_t *dst, unsigned tile) {
         const unsigned key0 = tile * BN;
         const size_t bytes = (size_t)(lk - key0) * kstride - kv * D * 2;
         const uint16_t *first = base + ((size_t)k0 + key0) * (kstride / 2) + kv * D;
@@ -156,8 +161,8 @@ void attn_sequences(SeqArgs a) {
     for (int ks = 0; ks < 8; ks++) qf[ks] = *reinterpret_cast<const bf16x8 *>(a.q + qrow * D + hf * 8 + ks * 16);
     unsigned t = __builtin_amdgcn_readfirstlane(item.first) + wave;
     if (t < count) {
-        load(a.k, kt, t);
-        load(a.v, vt, t);
+        load(a.k, off, kt, t);
+        load(a.v, v_off, vt, t);
     }
     if (wave == 0)
 #pragma unroll
@@ -184,7 +189,7 @@ void attn_sequences(SeqArgs a) {
             }
             if (screen) screen_tile(kt);
             wait_vm_lds<16>();              // this wave's reads: the tile may be overwritten
-            if (more) load(a.k, kt, t + WAVES);
+            if (more) load(a.k, off, kt, t + WAVES);
 #pragma unroll
             for (int ks = 0; ks < 8; ks++)
 #pragma unroll
@@ -239,14 +244,14 @@ void attn_sequences(SeqArgs a) {
                 for (int h = 0; h < 2; h++) {
                     const unsigned row = 16 * kk + 8 * h + vrow;
                     half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) i16x4 *)(vt + row * 256 + chunk(row, md * 4 + vch) * 16 +
+                        (__attribute__((address_space(3))) i16x4 *)(vt + row * 256 + v_chunk(row, md * 4 + vch) * 16 +
                                                                      p16 % 2 * 8));
                 }
                 vf[kk * 4 + md] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
             }
         if (screen) screen_tile(vt);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (more) load(a.v, vt, t + WAVES);
+        if (more) load(a.v, v_off, vt, t + WAVES);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++)
 #pragma unroll
@@ -339,13 +344,14 @@ void attn_sequences_mid(SeqArgs a) {
     const float c = a.scale_log2;
 
     // Wave's 1 KB blocks 4 wave + j of a tile: keys 16 wave + 4 j + lane / 16, chunk lane % 16 (swizzled).
-    unsigned off[4];
+    unsigned off[4], v_off[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const unsigned key = 16 * wave + 4 * j + lane / 16;
         off[j] = key * (unsigned)kstride + chunk(key, lane % 16) * 16;
+        v_off[j] = key * (unsigned)kstride + v_chunk(key, lane % 16) * 16;
     }
-    auto load = [&](const uint16_t *base, uint8_t *dst, unsigned tile) {
+    auto load = [&](const uint16_t *base, const unsigned *off, uint8_t *dst, unsigned tile) {
         const unsigned key0 = tile * BN;
         const size_t bytes = (size_t)(lk - key0) * kstride - kv * D * 2;
         const uint16_t *first = base + ((size_t)k0 + key0) * (kstride / 2) + kv * D;
@@ -370,8 +376,8 @@ void attn_sequences_mid(SeqArgs a) {
     const size_t qrow = ((size_t)s.q0 + held / a.share) * a.heads + kv * a.share + held % a.share;
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) qf[ks] = *reinterpret_cast<const bf16x8 *>(a.q + qrow * D + hf * 8 + ks * 16);
-    load(a.k, smem, 0);
-    load(a.v, smem + TILE, 0);
+    load(a.k, off, smem, 0);
+    load(a.v, v_off, smem + TILE, 0);
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) note_bf16(worst, &qf[ks], 4);
     f32x16 o[4] = {};
@@ -384,8 +390,8 @@ void attn_sequences_mid(SeqArgs a) {
         const uint8_t *const kt = smem + t % 2 * 2 * TILE, *const vt = kt + TILE;
         if (t + 1 < count) {
             uint8_t *const next = smem + (t + 1) % 2 * 2 * TILE;
-            load(a.k, next, t + 1);
-            load(a.v, next + TILE, t + 1);
+            load(a.k, off, next, t + 1);
+            load(a.v, v_off, next + TILE, t + 1);
         }
         // Each tile's K and V are screened for Inf and NaN by one of the key head's workgroups.
         if (t % blocks == block) {
@@ -450,7 +456,7 @@ void attn_sequences_mid(SeqArgs a) {
             for (int h = 0; h < 2; h++) {
                 const unsigned r = 16 * (x / 4) + 8 * h + vrow;
                 vh[x][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) i16x4 *)(vt + r * 256 + chunk(r, x % 4 * 4 + vch) * 16 + p16 % 2 * 8));
+                    (__attribute__((address_space(3))) i16x4 *)(vt + r * 256 + v_chunk(r, x % 4 * 4 + vch) * 16 + p16 % 2 * 8));
             }
 #pragma unroll
         for (int x = 0; x < 16; x++) {
