@@ -7,6 +7,17 @@
 // Query heads that share a key head are rows of one tile: row v of (sequence, key head) is
 // query v / share of head share * key head + v % share, so that a key tile is read once for
 // all of them and one query of several heads fills more of a matrix instruction.
+//
+// Three kernels, by how many rows a call has (make_plan):
+//  * attn_bf16_pipe (attn_bf16.hip), 256 rows a workgroup, for long sequences: the fastest by row,
+//    bound by the matrix cores, but V is transposed first and flagged rows are computed again
+//    after it. Four clips of 8193, 301, 2917 and one row, 40 heads: 1.37-1.42 ms, 1.1 PFLOP/s;
+//  * attn_sequences_mid, 128 rows, for frames and short clips, one launch. Its matrix and vector
+//    instructions take about as long as one another (52 and 50% of the time at 4000 rows) and
+//    overlap by two waves a SIMD only. 729 and 806 rows of 56 heads: 54 us;
+//  * attn_sequences, 32 rows, its four waves taking the key tiles in turn, for few rows: bound by
+//    the keys' reads. Long key ranges go to several workgroups, joined by attn_sequences_join. One to
+//    three rows over 18225, 4001, 729 and 9000 keys of 8 key heads (131 MB): 37 us, 3.5 TB/s.
 #include "common.h"
 #include "internal.h"
 #include "attn_common.h"
@@ -412,6 +423,17 @@ void attn_sequences_mid(SeqArgs a) {
                 for (int mb = 0; mb < 2; mb++)
                     sc[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks * 2 + mb], qf[ks], sc[mb], 0, 0, 0);
         }
+        // V^T fragments, on their way during the softmax: keys 16 kk + 4 hf + 0..3 and 8 further on, the order
+        // of P's registers. (Read after it: 729 and 806 rows of 56 heads 55 us, so 54.)
+        i16x4 vh[16][2];
+#pragma unroll
+        for (int x = 0; x < 16; x++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const unsigned r = 16 * (x / 4) + 8 * h + vrow;
+                vh[x][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) i16x4 *)(vt + r * 256 + v_chunk(r, x % 4 * 4 + vch) * 16 + p16 % 2 * 8));
+            }
         if (t * BN + BN > lk)
 #pragma unroll
             for (int mb = 0; mb < 2; mb++)
@@ -447,17 +469,6 @@ void attn_sequences_mid(SeqArgs a) {
                 }
             l += sum;
         }
-        // V^T fragments: keys 16 kk + 4 hf + 0..3 and 8 further on, the order of P's registers. Read after the
-        // softmax: read before it they cost registers (4000 rows of 40 heads 388 us, so 368).
-        i16x4 vh[16][2];
-#pragma unroll
-        for (int x = 0; x < 16; x++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const unsigned r = 16 * (x / 4) + 8 * h + vrow;
-                vh[x][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) i16x4 *)(vt + r * 256 + v_chunk(r, x % 4 * 4 + vch) * 16 + p16 % 2 * 8));
-            }
 #pragma unroll
         for (int x = 0; x < 16; x++) {
             const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(vh[x][0], vh[x][1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -573,10 +584,10 @@ int launch(h3_gpu *g, const SeqArgs &a) {
 
 // Modelled microseconds of the kernels' workgroups, by 64-key tiles, and of a kernel's launches: as many
 // workgroups as run at once, and half a round more behind whole rounds. Measured, all rows by one kernel
-// (32 / 128 / 256 rows a workgroup): 300 rows of 4 heads 11.2 / 13.4 / 23.5 us, of 40 heads 19.5 /
-// 14.8 / 27.0; 1000 rows of 8 heads 15.6 / 28.2 / 33.2, of 40 heads 65 / 45 / 45; 729 and 806 rows of
-// 56 heads 129 / 61 / 76; eight times 250 rows of 40 heads 72 / 30 / 72; 4000 rows of 40 heads 656 /
-// 368 / 332; 5000 rows of 8 heads 199 / 157 / 116.
+// (32 / 128 / 256 rows a workgroup): 300 rows of 4 heads 11 / 13 / 24 us, of 40 heads 19 / 14 / 27;
+// 1000 rows of 8 heads 15 / 26 / 34, of 40 heads 62 / 41 / 45; 729 and 806 rows of 56 heads 124 / 56 /
+// 76; eight times 250 rows of 40 heads 70 / 29 / 72; 4000 rows of 40 heads 634 / 346 / 332; 5000
+// rows of 8 heads 195 / 144 / 118.
 struct Load {
     double sum = 0, longest = 0, workgroups = 0;
     void add(double cost, double count) {
@@ -586,7 +597,7 @@ struct Load {
     }
 };
 double row_cost(uint64_t tiles) { return 6 + 1.75 * (double)((tiles + WAVES - 1) / WAVES); }
-double mid_cost(uint64_t tiles) { return 4 + 2.3 * (double)tiles; }              // two on a compute unit
+double mid_cost(uint64_t tiles) { return 4 + 2.1 * (double)tiles; }              // two on a compute unit
 double tile_cost(uint64_t tiles) { return 5 + 2.1 * (double)((tiles + 1) / 2); }
 double row_time(const Load &l, double cus) {
     return l.workgroups ? 3 + (l.workgroups > cus ? l.sum / cus + l.longest / 2 : l.longest) : 0;
