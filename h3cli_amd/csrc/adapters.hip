@@ -29,7 +29,7 @@ struct AdapterEntry {
 
 struct h3_hip_adapters {
     h3_gpu *owner;
-    uint32_t count, k, n, k_padded, n_padded;
+    uint32_t count, k, n, k_padded, n_padded, max_rank;
     std::vector<uint32_t> ranks;
     std::vector<AdapterEntry> entries;
     h3_gpu_tensor *weights;   // BF16: of each A_a, then B_a, as adapter_pack orders them
@@ -539,7 +539,7 @@ extern "C" h3_hip_adapters *h3_hip_adapters_new(h3_gpu *g, const uint32_t *ranks
     size_t elements = 0;
     try {
         a = new h3_hip_adapters{g, count, k, n, (k + KC - 1) / KC * KC, (n + COLS - 1) / COLS * COLS,
-                                std::vector<uint32_t>(ranks, ranks + count), {}, nullptr, nullptr};
+                                *std::max_element(ranks, ranks + count), std::vector<uint32_t>(ranks, ranks + count), {}, nullptr, nullptr};
         for (uint32_t i = 0; i < count; i++) {
             const size_t down = (size_t)rank_blocks(ranks[i]) * 32 * a->k_padded;
             a->entries.push_back({elements, elements + down, ranks[i], 0.f});
@@ -641,8 +641,7 @@ static int adapters_valid(h3_gpu *g, const h3_hip_adapters *w, const h3_hip_adap
     if (w->k != k || w->n != n || p->rows != rows || p->count != w->count)
         return h3_set_error(g, "adapters are for %ux%u, %u of them and the rows for %u of %u, need %ux%u and %u rows", w->k, w->n,
                             w->count, p->rows, p->count, k, n, rows);
-    for (uint32_t rank : w->ranks)
-        if (rank > p->max_rank) return h3_set_error(g, "adapters: rank %u, the rows' plan holds %u", rank, p->max_rank);
+    if (w->max_rank > p->max_rank) return h3_set_error(g, "adapters: rank %u, the rows' plan holds %u", w->max_rank, p->max_rank);
     return 1;
 }
 
@@ -660,8 +659,7 @@ static int shared_memory(h3_gpu *g, const void *kernel, size_t bytes) {
 // The arguments of a call, and its first product.
 static int adapters_begin(h3_gpu *g, AdapterArgs &a, const h3_gpu_tensor *in, const h3_hip_adapters *w, const h3_hip_adapter_rows *p,
                           uint32_t &blocks) {
-    blocks = 0;
-    for (uint32_t rank : w->ranks) blocks = std::max(blocks, rank_blocks(rank));
+    blocks = rank_blocks(w->max_rank);
     a.x = (const uint16_t *)in->data;
     a.weights = (const uint16_t *)w->weights->data;
     a.table = (const AdapterEntry *)w->table->data;

@@ -8,14 +8,15 @@
 //
 // All in FP32, one rounding to BF16. The pass is bound by HBM (4 bytes a value), so the
 // rotation must stay below the loads: cosines and sines are made once per row and channel
-// and kept in registers for all heads, with the norm's weights folded into them:
+// and kept in LDS for all its heads, with the norms' weights folded into them:
 //   x'_d cos +- x'_p sin = r (x_d (w_d cos) + x_p (+-w_p sin)),   r the head's norm factor.
 //
 // Angles. A position may be far (2^24 and beyond), where an FP32 angle has lost its phase. With
-// f / 2 pi = hi + lo in two floats, n = rint(p hi), the phase in turns is
+// f / 2 pi = hi + lo in two floats and n = rint(p hi), the phase in turns is
 //   fma(p, lo, fma(p, hi, -n)),
-// whose inner fma is exact but for one rounding of a value of at most a half (2^-25 turns); the
-// hardware's sine and cosine take turns.
+// whose inner fma is exact (the product's rounding, or what follows the point) and, beyond 2^24
+// turns, once more brought near zero. What is left is the last rounding and that of lo: up to
+// 2^24 turns 2^-23 turns, beyond them 2^-47 of the angle. The hardware's sine and cosine take turns.
 #include "common.h"
 #include "internal.h"
 #include <algorithm>
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(256, 5) void rope_axes_chunks(AxesArgs a) {
         partner_weight[KEY] = bf16_to_f32(a.kw[partner_channel]);
     }
     // Task: `together` rows, or a share of one row.
-    const size_t tasks = (size_t)(a.rows + a.together - 1) / a.together * a.splits;
+    const size_t tasks = ((size_t)a.rows + a.together - 1) / a.together * a.splits;
     float next[TOGETHER] = {};
     auto positions = [&](size_t task) {
 #pragma unroll
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(256, 5) void rope_axes_chunks(AxesArgs a) {
 #pragma unroll
         for (unsigned r = 0; r < TOGETHER; r++) {
             if (r >= a.together) break;
-            const float t = fmaf(next[r], lo, fmaf(next[r], hi, -rintf(next[r] * hi)));
+            const float near = fmaf(next[r], hi, -rintf(next[r] * hi)), t = fmaf(next[r], lo, near - rintf(near));
             const float cs = turns ? __builtin_amdgcn_cosf(t) : 1.f, sn = turns ? __builtin_amdgcn_sinf(t) : 0.f;
 #pragma unroll
             for (int kind = QUERY; kind <= KEY; kind++) {
@@ -239,7 +240,7 @@ template <int LANES> void launch_chunks(h3_gpu *g, AxesArgs a) {
     while (a.together < TOGETHER && a.splits == 1 && items * a.together * 2 <= 4 * GROUPS && a.rows >= 2 * a.together * 4 * g->cus) a.together *= 2;
     // Many workgroups of a row or few: with as many as run at once the last ones end the call (18,225 rows
     // of 56 heads: 305 us with 4 workgroups a compute unit, 303 with 16, 298 with 64, 291 with one a row).
-    const size_t tasks = (size_t)(a.rows + a.together - 1) / a.together * a.splits, each = (tasks + 256 * g->cus - 1) / (256 * g->cus);
+    const size_t tasks = ((size_t)a.rows + a.together - 1) / a.together * a.splits, each = (tasks + 256 * g->cus - 1) / (256 * g->cus);
     const unsigned blocks = (unsigned)((tasks + each - 1) / each);
     const Pairing pairing = a.interleaved ? NEIGHBOURS : a.dim % 8 == 0 && a.pairs % 8 == 0 ? HALVES : HALVES_LOOSE;
     auto *kernel = pairing == NEIGHBOURS ? rope_axes_chunks<LANES, NEIGHBOURS>

@@ -266,9 +266,9 @@ void h3_hip_rope_axes_free(h3_hip_rope_axes *rope);
 /* h3_gpu_qkv_rope_bf16 with each row's positions (F32 [rows, axes]) for its tables and
  * with kv_heads key heads. qkv rows are [heads + 2 * kv_heads, dim], queries first, then
  * keys, then values; grouped 1: for each key head its query heads, its key and its
- * value, [kv_heads, heads / kv_heads + 2, dim]. The angles' phase is exact to 2^-23 of
- * a turn for positions of any size. dim <= 256; rows of a multiple of 8 channels
- * and pairs are several times as fast as others. */
+ * value, [kv_heads, heads / kv_heads + 2, dim]. The angles' phase is off by at most 2^-23 of
+ * a turn up to 2^24 turns, by 2^-47 of the angle beyond. dim <= 256; heads of 16, 32, 64, 128 or 256
+ * channels use all lanes, others up to twice as long for a channel. */
 int h3_hip_qkv_rope_axes_bf16(h3_gpu *gpu, h3_gpu_tensor *query, h3_gpu_tensor *key, h3_gpu_tensor *value,
                               const h3_gpu_tensor *qkv, const h3_gpu_tensor *q_norm, const h3_gpu_tensor *k_norm,
                               const h3_hip_rope_axes *rope, const h3_gpu_tensor *positions, uint32_t rows,
@@ -297,7 +297,9 @@ void h3_hip_adapter_rows_free(h3_hip_adapter_rows *rows);
 int h3_hip_adapters_add_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *base, const h3_gpu_tensor *input,
                              const h3_hip_adapters *adapters, const h3_hip_adapter_rows *adapter_rows, uint32_t rows,
                              uint32_t input_dim, uint32_t output_dim);
-/* h3_gpu_linear_bf16 and the adapters' parts, which are added to its BF16 output. */
+/* h3_gpu_linear_bf16 and the adapters' parts. They are added to its BF16 output, but for
+ * BF16 weights of an input_dim that is no multiple of 64: there all is one FP32 sum,
+ * rounded once. output may not be input. */
 int h3_hip_linear_adapters_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
                                 const h3_gpu_tensor *weight, const h3_gpu_tensor *bias,
                                 const h3_hip_adapters *adapters, const h3_hip_adapter_rows *adapter_rows,

@@ -212,6 +212,27 @@ def test_attention_of_few_rows_over_many_keys(q_offsets, k_offsets, heads, kv_he
             assert kernel == "attn_sequences rows=32 shares=2", kernel     # parts, joined
 
 
+@pytest.mark.parametrize("variant,q_rows,keys", [(20, 3, 700), (21, 130, 700), (22, 300, 700)])
+def test_attention_of_keys_behind_4_gib(variant, q_rows, keys, monkeypatch):
+    monkeypatch.setenv("H3_HIP_ATTENTION_VARIANT", str(variant))
+    first = (1 << 32) // 256 + 5                            # a row of K is 256 bytes
+    with Gpu() as g:
+        q = g.from_bf16(normal(q_rows * 128, 1))
+        k, v, out = g.empty((first + keys) * 128), g.empty((first + keys) * 128), g.empty(q_rows * 128)
+        for t, seed in ((k, 2), (v, 3)):
+            g.begin()
+            g.check(g.lib.h3_hip_fill_normal_bf16(g.handle, t.handle, seed, C.c_float(1), (first + keys) * 128), "fill")
+            g.submit()
+        with sequences(g, [0, q_rows], [first, first + keys], 1, 1) as plan:
+            g.begin()
+            g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, out.handle, q.handle, k.handle, v.handle, plan, C.c_float(SCALE)),
+                    "attention")
+            g.submit()
+        fq, fk, fv = (bf16(t.read()[-rows * 128:]).reshape(rows, 128).astype(np.float64)
+                      for t, rows in ((q, q_rows), (k, keys), (v, keys)))
+        within(bf16(out.read()).reshape(q_rows, 128), *attention_reference(fq, fk, fv, SCALE))
+
+
 @pytest.mark.parametrize("variant", [20, 21, 22])
 def test_attention_of_sequences_reports_values_that_are_not_finite(variant, monkeypatch):
     """In a query, key or value of any sequence; the others' results stay whole."""
@@ -788,16 +809,3 @@ def test_refusals():
         lib.h3_hip_adapters_free(ad)
         lib.h3_hip_adapter_rows_free(rows)
         lib.h3_hip_adapter_rows_free(low)
-
-
-def test_no_context():
-    from h3cli_amd import _lib
-    lib = _lib.load()
-    assert not lib.h3_hip_sequences_new(None, u32([0, 1]), None, 1, 1, 1)
-    assert not lib.h3_hip_sdpa_sequences_bf16(None, None, None, None, None, None, C.c_float(1))
-    assert not lib.h3_hip_rope_axes_new(None, None, None, 1, 1, 0)
-    assert not lib.h3_hip_adapters_new(None, u32([1]), 1, 1, 1)
-    assert not lib.h3_hip_adapter_rows_new(None, u32([0]), 1, 1, 1)
-    assert not lib.h3_hip_linear_adapters_bf16(None, None, None, None, None, None, None, 1, 1, 1)
-    for free in (lib.h3_hip_sequences_free, lib.h3_hip_rope_axes_free, lib.h3_hip_adapters_free, lib.h3_hip_adapter_rows_free):
-        free(None)

@@ -37,3 +37,18 @@ def test_sequences_hold_what_their_kernels_need():
     assert 2 * 130 * 128 < layout([0, 1], [0, 18225], 5, 1) < 128 * 32 * 130 * 4 + 4096
     # A K of 4 GiB and more, in which a tile's offsets would not fit 32 bits, goes without them too.
     assert layout([0, 300], [0, 2 ** 24], 1, 1) < 1 << 25
+
+
+def test_no_context():
+    lib = _lib.load()
+    assert not lib.h3_hip_sequences_new(None, u32([0, 1]), None, 1, 1, 1)
+    assert not lib.h3_hip_sdpa_sequences_bf16(None, None, None, None, None, None, C.c_float(1))
+    assert not lib.h3_hip_rope_axes_new(None, None, None, 1, 1, 0)
+    assert not lib.h3_hip_qkv_rope_axes_bf16(None, None, None, None, None, None, None, None, None, 1, 1, 1, 1, 0, C.c_float(0))
+    assert not lib.h3_hip_adapters_new(None, u32([1]), 1, 1, 1)
+    assert not lib.h3_hip_adapters_set(None, None, 0, None, None, C.c_float(1))
+    assert not lib.h3_hip_adapter_rows_new(None, u32([0]), 1, 1, 1)
+    assert not lib.h3_hip_adapters_add_bf16(None, None, None, None, None, None, 1, 1, 1)
+    assert not lib.h3_hip_linear_adapters_bf16(None, None, None, None, None, None, None, 1, 1, 1)
+    for free in (lib.h3_hip_sequences_free, lib.h3_hip_rope_axes_free, lib.h3_hip_adapters_free, lib.h3_hip_adapter_rows_free):
+        free(None)
