@@ -61,15 +61,27 @@ struct AdapterArgs {
     const uint16_t *base, *x;
     const uint16_t *weights;
     const AdapterEntry *table;
+    unsigned count;                        // of adapters
     const uint32_t *order, *adapter;       // [32 tiles], [tiles]
     float *sums;
     const uint16_t *w, *bias;              // adapter_gemm
     float *shared_sums;
-    unsigned shares;
+    unsigned shares, products;             // and the workgroups of all shares
     unsigned plain;
     unsigned k, n, k_padded, tiles, passes, splits, rank_padded;
     unsigned groups, span;                 // adapter_up: workgroups of a tile, their steps of columns
 };
+
+// The adapter of a tile. A table of up to 64 is read whole beside the tile's index, an entry a lane, so
+// that few rows wait for memory once less (9 rows, 5376 -> 16128: XX us, by the index YY).
+__device__ inline AdapterEntry entry_of(const AdapterArgs &a, unsigned tile) {
+    if (a.count > 64) return a.table[load_uniform(a.adapter + tile)];
+    const AdapterEntry held = a.table[min(threadIdx.x % 64, a.count - 1)];
+    const unsigned index = load_uniform(a.adapter + tile);
+    auto word = [&](unsigned v) { return (unsigned)__builtin_amdgcn_readlane((int)v, (int)index); };
+    auto wide = [&](uint64_t v) { return (uint64_t)word((unsigned)(v >> 32)) << 32 | word((unsigned)v); };
+    return {wide(held.down), wide(held.up), word(held.rank), __builtin_bit_cast(float, word(__builtin_bit_cast(unsigned, held.scale)))};
+}
 
 __device__ inline unsigned sixteens_of(const AdapterEntry &e) { return (e.rank + 15) / 16; }
 
@@ -115,11 +127,10 @@ __device__ inline void wait_lds() {
 // XOR-swizzled) to the lanes that multiply it: loaded as these lanes need it, each line is asked for
 // four times, and evicted from the L1 in between.
 constexpr unsigned DOWN_WAVES = 4;
-__global__ __launch_bounds__(64 * DOWN_WAVES, 2) void adapter_down(AdapterArgs a) {
-    extern __shared__ __attribute__((aligned(16))) float part[];   // [wave][32-rank block * 4 + rows' group][lane][4]
+__device__ void first_product(const AdapterArgs &a, unsigned id, float *part) {   // part: [wave][32-rank block * 4 + rows' group][lane][4]
     const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, n = lane % 32, hf = lane / 32;
-    const unsigned split = blockIdx.x % a.splits, pass = blockIdx.x / a.splits % a.passes, tile = blockIdx.x / a.splits / a.passes;
-    const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
+    const unsigned split = id % a.splits, pass = id / a.splits % a.passes, tile = id / a.splits / a.passes;
+    const AdapterEntry entry = entry_of(a, tile);
     if (pass * 64 >= entry.rank) return;
     const bool both = pass * 64 + 32 < entry.rank;
     // Lane's chunk lane % 8 of rows lane / 8 + 8 i; row r keeps chunk c at swizzled(r, c).
@@ -204,6 +215,11 @@ __global__ __launch_bounds__(64 * DOWN_WAVES, 2) void adapter_down(AdapterArgs a
     }
 }
 
+__global__ __launch_bounds__(64 * DOWN_WAVES, 2) void adapter_down(AdapterArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float part[];
+    first_product(a, blockIdx.x, part);
+}
+
 constexpr unsigned STAGE_ROW = COLS + 4;   // floats: rows shift by four banks
 constexpr unsigned UP_STAGE = 32 * STAGE_ROW;
 
@@ -227,7 +243,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; i++) row[i] = a.order[tile * 32 + lane / 8 + 8 * i];
     AdapterEntry entry{};
-    if (adapted) entry = a.table[load_uniform(a.adapter + tile)];
+    if (adapted) entry = entry_of(a, tile);
     const unsigned sixteens = sixteens_of(entry);
     const uint16_t *const up = a.weights + entry.up + lane * 8;
     i32x4 next_v[4] = {}, next_w[4] = {};
@@ -344,6 +360,10 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
     constexpr unsigned SIDE = 64 * R, LOADS = SIDE / 32, DEPTH = R == 1 ? 4 : 2;   // LOADS: chunks of each operand a thread
     extern __shared__ __attribute__((aligned(16))) i32x4 lds[];   // [buffer][x, W][SIDE rows of 8 chunks]; then a stage a wave
     const unsigned tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, n = lane % 32, hf = lane / 32;
+    if (PART == PRODUCT && blockIdx.x >= a.products) {
+        first_product(a, blockIdx.x - a.products, reinterpret_cast<float *>(lds));
+        return;
+    }
     const unsigned id = PART == PRODUCT ? blockIdx.x / a.shares : blockIdx.x;
     const unsigned tiles_n = (a.n + SIDE - 1) / SIDE, tiles_m = (a.tiles + a.plain + 2 * R - 1) / (2 * R);
     // Columns fastest in bands of eight row tiles, so that what runs together shares both operands.
@@ -440,7 +460,7 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
         const unsigned tile = tile0 + wm / 32 + i;
         if (tile >= all) break;
         if (tile < a.tiles) {
-            const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
+            const AdapterEntry entry = entry_of(a, tile);
             for (unsigned r = 0; r < entry.rank; r += 16) {
                 bf16x8 high, low;
                 operands(a, entry, tile, n, r + hf * 8, high, low);
@@ -663,6 +683,7 @@ static int adapters_begin(h3_gpu *g, AdapterArgs &a, const h3_gpu_tensor *in, co
     a.x = (const uint16_t *)in->data;
     a.weights = (const uint16_t *)w->weights->data;
     a.table = (const AdapterEntry *)w->table->data;
+    a.count = w->count;
     a.order = (const uint32_t *)p->order->data;
     a.adapter = a.order + (size_t)32 * (p->tiles + p->plain);
     a.sums = (float *)p->sums->data;
@@ -674,7 +695,7 @@ static int adapters_begin(h3_gpu *g, AdapterArgs &a, const h3_gpu_tensor *in, co
     a.passes = (blocks + 1) / 2;
     a.splits = std::min(p->splits, splits_for(g, p->tiles, a.passes));
     a.rank_padded = rank_blocks(p->max_rank) * 32;
-    if (!a.tiles) return 1;
+    if (!a.tiles || a.products) return 1;   // a shared projection's first launch takes it along
     constexpr unsigned shared = DOWN_WAVES * 8 * 64 * 16;
     static bool configured = false;
     if (!configured && !shared_memory(g, (const void *)adapter_down, shared)) return 0;
@@ -755,11 +776,12 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
     a.shared_sums = (float *)p->sums->data + p->sums_at;
     // Four steps of 64 channels a share at least, in one round of the compute units.
     a.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint32_t>(SHARED_TILES, g->cus) / small, (k + KC - 1) / KC / 4));
-    if ((k + KC - 1) / KC < 20) a.shares = 1;
+    if ((k + KC - 1) / KC < 8) a.shares = 1;
+    a.products = a.shares > 1 ? (uint32_t)small * a.shares : 0;
     uint32_t blocks;
     if (!h3_tensor_acquire(g, weight) || !adapters_begin(g, a, in, w, p, blocks)) return 0;
     hipEvent_t timing = h3_kernel_timing_begin(g);
-    const int ok = a.shares > 1                  ? launch_gemm<1, PRODUCT>(g, a, (uint32_t)small * a.shares) && launch_gemm<1, REST>(g, a, (uint32_t)small)
+    const int ok = a.shares > 1                  ? launch_gemm<1, PRODUCT>(g, a, a.products + a.tiles * a.passes * a.splits) && launch_gemm<1, REST>(g, a, (uint32_t)small)
                    : large * 5 >= g->cus * 3ull ? launch_gemm<2, ALL>(g, a, (uint32_t)large)
                                                 : launch_gemm<1, ALL>(g, a, (uint32_t)small);
     h3_kernel_timing_end(g, timing);

@@ -34,27 +34,31 @@ constexpr uint64_t JOIN_TILES = 8;             // what a join costs, in tiles of
 constexpr size_t PART_FLOATS = 32 * (D + 2);   // of 32 rows: O, the running max and the sum
 
 // A workgroup's share: 32 rows of a sequence and its key tiles [first, last); part: where its
-// partial result goes, WHOLE if it has all tiles.
+// partial result goes, WHOLE if it has all tiles. (The sequence is in the item: looked up by its
+// index, it would cost a small call one more wait for memory.)
 struct RowItem {
-    uint32_t sequence, block, first, last, part;
+    uint32_t q0, lq, k0, lk, block, first, last, part;
+};
+struct MidItem {
+    uint32_t q0, lq, k0, lk, block;   // 128 rows
 };
 // 32 rows whose tiles were shared out to parts [part, part + parts).
 struct JoinItem {
-    uint32_t sequence, block, part, parts;
+    uint32_t q0, lq, block, part, parts;
 };
 
 // What a call does, made on the host.
 struct Plan {
     std::vector<h3_sequence> sequences;
     std::vector<h3_sequence_item> tiles, keys;   // by the 256-row tile kernel
-    std::vector<h3_sequence_item> mid;           // by attn_sequences_mid
+    std::vector<MidItem> mid;                    // by attn_sequences_mid
     std::vector<RowItem> rows;                   // by attn_sequences
     std::vector<JoinItem> joins;
     uint64_t vt = 0;                             // elements of transposed V
     uint32_t parts = 0;
     size_t table_bytes() const {
-        return sequences.size() * sizeof(h3_sequence) + (tiles.size() + keys.size() + mid.size()) * sizeof(h3_sequence_item) +
-               rows.size() * sizeof(RowItem) + joins.size() * sizeof(JoinItem);
+        return sequences.size() * sizeof(h3_sequence) + (tiles.size() + keys.size()) * sizeof(h3_sequence_item) +
+               mid.size() * sizeof(MidItem) + rows.size() * sizeof(RowItem) + joins.size() * sizeof(JoinItem);
     }
     size_t retry_at() const { return (vt * 2 + 255) / 256 * 256; }
     size_t parts_at(uint32_t kv_heads) const { return (retry_at() + tiles.size() * kv_heads * 8 + 255) / 256 * 256; }
@@ -78,9 +82,8 @@ namespace {
 struct SeqArgs {
     uint16_t *out;
     const uint16_t *q, *k, *v;
-    const h3_sequence *sequences;
     const RowItem *items;
-    const h3_sequence_item *mid_items;
+    const MidItem *mid_items;
     const JoinItem *joins;
     float *partial;
     unsigned count, join_count, heads, kv_heads, share;
@@ -118,9 +121,8 @@ void attn_sequences(SeqArgs a) {
     const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
     const unsigned kv = __builtin_amdgcn_readfirstlane(id / a.count);
     const RowItem item = a.items[__builtin_amdgcn_readfirstlane(id % a.count)];
-    const h3_sequence s = a.sequences[item.sequence];
-    const unsigned lq = __builtin_amdgcn_readfirstlane(s.lq), lk = __builtin_amdgcn_readfirstlane(s.lk);
-    const unsigned q0 = __builtin_amdgcn_readfirstlane(s.q0), k0 = __builtin_amdgcn_readfirstlane(s.k0);
+    const unsigned lq = __builtin_amdgcn_readfirstlane(item.lq), lk = __builtin_amdgcn_readfirstlane(item.lk);
+    const unsigned q0 = __builtin_amdgcn_readfirstlane(item.q0), k0 = __builtin_amdgcn_readfirstlane(item.k0);
     const unsigned block = __builtin_amdgcn_readfirstlane(item.block);
     const unsigned part = __builtin_amdgcn_readfirstlane(item.part);
     const unsigned rows = lq * a.share, blocks = (rows + 31) / 32, count = __builtin_amdgcn_readfirstlane(item.last);
@@ -346,11 +348,10 @@ void attn_sequences_mid(SeqArgs a) {
     const unsigned n = lane % 32, hf = lane / 32;
     const unsigned id = xcd_remap(blockIdx.x, gridDim.x);
     const unsigned kv = __builtin_amdgcn_readfirstlane(id / a.count);
-    const h3_sequence_item item = a.mid_items[__builtin_amdgcn_readfirstlane(id % a.count)];
-    const h3_sequence s = a.sequences[item.sequence];
-    const unsigned lk = __builtin_amdgcn_readfirstlane(s.lk), k0 = __builtin_amdgcn_readfirstlane(s.k0);
+    const MidItem item = a.mid_items[__builtin_amdgcn_readfirstlane(id % a.count)];
+    const unsigned lk = __builtin_amdgcn_readfirstlane(item.lk), k0 = __builtin_amdgcn_readfirstlane(item.k0);
     const unsigned block = __builtin_amdgcn_readfirstlane(item.block);
-    const unsigned rows = __builtin_amdgcn_readfirstlane(s.lq) * a.share, blocks = (rows + 127) / 128, count = (lk + BN - 1) / BN;
+    const unsigned rows = __builtin_amdgcn_readfirstlane(item.lq) * a.share, blocks = (rows + 127) / 128, count = (lk + BN - 1) / BN;
     const size_t kstride = (size_t)a.kv_heads * D * 2;   // bytes
     const float c = a.scale_log2;
 
@@ -384,7 +385,7 @@ void attn_sequences_mid(SeqArgs a) {
     };
     bf16x8 qf[8];
     const unsigned row = block * 128 + wave * 32 + n, held = min(row, rows - 1);
-    const size_t qrow = ((size_t)s.q0 + held / a.share) * a.heads + kv * a.share + held % a.share;
+    const size_t qrow = ((size_t)item.q0 + held / a.share) * a.heads + kv * a.share + held % a.share;
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) qf[ks] = *reinterpret_cast<const bf16x8 *>(a.q + qrow * D + hf * 8 + ks * 16);
     load(a.k, off, smem, 0);
@@ -500,8 +501,7 @@ __global__ __launch_bounds__(256) void attn_sequences_join(SeqArgs a) {
     __shared__ float weight[32][PARTS_MOST + 1];
     const unsigned tid = threadIdx.x, kv = blockIdx.x % a.kv_heads;
     const JoinItem item = a.joins[blockIdx.x / a.kv_heads];
-    const h3_sequence s = a.sequences[item.sequence];
-    const unsigned rows = min(32u, s.lq * a.share - item.block * 32);
+    const unsigned rows = min(32u, item.lq * a.share - item.block * 32);
     const float *const first = a.partial + ((size_t)item.part * a.kv_heads + kv) * PART_FLOATS;
     const size_t step = (size_t)a.kv_heads * PART_FLOATS;
     {
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(256) void attn_sequences_join(SeqArgs a) {
             worst = max(worst, __builtin_bit_cast(uint32_t, y) & 0x7f800000u);
             out[e] = f32_to_bf16(y);
         }
-        *reinterpret_cast<u16x4 *>(a.out + (((size_t)s.q0 + v / a.share) * a.heads + kv * a.share + v % a.share) * D + d) = out;
+        *reinterpret_cast<u16x4 *>(a.out + (((size_t)item.q0 + v / a.share) * a.heads + kv * a.share + v % a.share) * D + d) = out;
     }
     if (worst >= 0x7f800000u) a.fault[0] = 1u;
 }
@@ -694,7 +694,7 @@ const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_o
         // Launches hold fewer than 2^32 threads.
         if (kernel[i] == 1) {
             if ((plan.mid.size() + blocks(i, 128)) * kv_heads >= (1u << 24)) return "more rows than a launch takes";
-            for (uint32_t b = 0; b < blocks(i, 128); b++) plan.mid.push_back({i, b});
+            for (uint32_t b = 0; b < blocks(i, 128); b++) plan.mid.push_back({s.q0, s.lq, s.k0, s.lk, b});
             continue;
         }
         if (kernel[i] == 2) {
@@ -709,9 +709,10 @@ const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_o
         const uint64_t n = tiles(i), parts = n >= share_tiles + JOIN_TILES ? std::min<uint64_t>((n + share_tiles - 1) / share_tiles, PARTS_MOST) : 1;
         if ((plan.rows.size() + blocks(i, 32) * parts) * kv_heads >= (1u << 24)) return "more rows than a launch takes";
         for (uint32_t b = 0; b < blocks(i, 32); b++) {
-            if (parts > 1) plan.joins.push_back({i, b, plan.parts, (uint32_t)parts});
+            if (parts > 1) plan.joins.push_back({s.q0, s.lq, b, plan.parts, (uint32_t)parts});
             for (uint64_t p = 0; p < parts; p++)
-                plan.rows.push_back({i, b, (uint32_t)(n * p / parts), (uint32_t)(n * (p + 1) / parts), parts > 1 ? plan.parts++ : WHOLE});
+                plan.rows.push_back({s.q0, s.lq, s.k0, s.lk, b, (uint32_t)(n * p / parts), (uint32_t)(n * (p + 1) / parts),
+                                     parts > 1 ? plan.parts++ : WHOLE});
         }
     }
     return nullptr;
@@ -786,7 +787,8 @@ extern "C" int h3_hip_sdpa_sequences_bf16(h3_gpu *g, h3_gpu_tensor *out, const h
     const float rounded = bf16_to_f32(f32_to_bf16(scale));
     const auto *sequences = (const h3_sequence *)s->table->data;
     const auto *items = (const h3_sequence_item *)(sequences + s->count);
-    const auto *rows = (const RowItem *)(items + s->tiles + s->keys + s->mid);
+    const auto *mid = (const MidItem *)(items + s->tiles + s->keys);
+    const auto *rows = (const RowItem *)(mid + s->mid);
     char *const workspace = s->workspace ? (char *)s->workspace->data : nullptr;
     if (s->tiles) {
         const h3_sequence_tiles t{sequences, items, items + s->tiles, s->tiles, s->keys, s->heads, s->kv_heads,
@@ -795,8 +797,8 @@ extern "C" int h3_hip_sdpa_sequences_bf16(h3_gpu *g, h3_gpu_tensor *out, const h
                                                 (const uint16_t *)v->data, t, rounded))
             return 0;
     }
-    SeqArgs a{(uint16_t *)out->data, (const uint16_t *)q->data, (const uint16_t *)k->data, (const uint16_t *)v->data, sequences, rows,
-              items + s->tiles + s->keys, (const JoinItem *)(rows + s->rows), s->joins ? (float *)(workspace + s->parts_at) : nullptr,
+    SeqArgs a{(uint16_t *)out->data, (const uint16_t *)q->data, (const uint16_t *)k->data, (const uint16_t *)v->data, rows, mid,
+              (const JoinItem *)(rows + s->rows), s->joins ? (float *)(workspace + s->parts_at) : nullptr,
               s->mid, s->joins, s->heads, s->kv_heads, s->heads / s->kv_heads, rounded * 1.4426950408889634f, g->fault};
     if (s->mid && !launch_mid(g, a)) return 0;
     a.count = s->rows;
