@@ -61,7 +61,6 @@ struct AdapterArgs {
     const uint16_t *base, *x;
     const uint16_t *weights;
     const AdapterEntry *table;
-    unsigned count;                        // of adapters
     const uint32_t *order, *adapter;       // [32 tiles], [tiles]
     float *sums;
     const uint16_t *w, *bias;              // adapter_gemm
@@ -71,17 +70,6 @@ struct AdapterArgs {
     unsigned k, n, k_padded, tiles, passes, splits, rank_padded;
     unsigned groups, span;                 // adapter_up: workgroups of a tile, their steps of columns
 };
-
-// The adapter of a tile. A table of up to 64 is read whole beside the tile's index, an entry a lane, so
-// that few rows wait for memory once less (9 rows, 5376 -> 16128: XX us, by the index YY).
-__device__ inline AdapterEntry entry_of(const AdapterArgs &a, unsigned tile) {
-    if (a.count > 64) return a.table[load_uniform(a.adapter + tile)];
-    const AdapterEntry held = a.table[min(threadIdx.x % 64, a.count - 1)];
-    const unsigned index = load_uniform(a.adapter + tile);
-    auto word = [&](unsigned v) { return (unsigned)__builtin_amdgcn_readlane((int)v, (int)index); };
-    auto wide = [&](uint64_t v) { return (uint64_t)word((unsigned)(v >> 32)) << 32 | word((unsigned)v); };
-    return {wide(held.down), wide(held.up), word(held.rank), __builtin_bit_cast(float, word(__builtin_bit_cast(unsigned, held.scale)))};
-}
 
 __device__ inline unsigned sixteens_of(const AdapterEntry &e) { return (e.rank + 15) / 16; }
 
@@ -130,7 +118,7 @@ constexpr unsigned DOWN_WAVES = 4;
 __device__ void first_product(const AdapterArgs &a, unsigned id, float *part) {   // part: [wave][32-rank block * 4 + rows' group][lane][4]
     const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, n = lane % 32, hf = lane / 32;
     const unsigned split = id % a.splits, pass = id / a.splits % a.passes, tile = id / a.splits / a.passes;
-    const AdapterEntry entry = entry_of(a, tile);
+    const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
     if (pass * 64 >= entry.rank) return;
     const bool both = pass * 64 + 32 < entry.rank;
     // Lane's chunk lane % 8 of rows lane / 8 + 8 i; row r keeps chunk c at swizzled(r, c).
@@ -243,7 +231,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; i++) row[i] = a.order[tile * 32 + lane / 8 + 8 * i];
     AdapterEntry entry{};
-    if (adapted) entry = entry_of(a, tile);
+    if (adapted) entry = a.table[load_uniform(a.adapter + tile)];
     const unsigned sixteens = sixteens_of(entry);
     const uint16_t *const up = a.weights + entry.up + lane * 8;
     i32x4 next_v[4] = {}, next_w[4] = {};
@@ -353,7 +341,9 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
 // at large ones.
 // A compute unit takes in about 20 bytes a cycle of such rows, so few tiles over a long K are shared out
 // (part PRODUCT: a share of K, its sums to memory; then part REST: the shares added in order, and
-// what follows them).
+// what follows them). The adapters' first product needs nothing of it and is part of PRODUCT's launch,
+// its workgroups behind the shares'. (301 rows, 1001 -> 777: 16 us in three shares, unshared, the adapters'
+// product before it, 18; 10 rows, 5337 -> 47, 21 shares: 18, 38.)
 enum Part { ALL, PRODUCT, REST };
 template <int R, Part PART>
 __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
@@ -460,7 +450,7 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
         const unsigned tile = tile0 + wm / 32 + i;
         if (tile >= all) break;
         if (tile < a.tiles) {
-            const AdapterEntry entry = entry_of(a, tile);
+            const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
             for (unsigned r = 0; r < entry.rank; r += 16) {
                 bf16x8 high, low;
                 operands(a, entry, tile, n, r + hf * 8, high, low);
@@ -683,7 +673,6 @@ static int adapters_begin(h3_gpu *g, AdapterArgs &a, const h3_gpu_tensor *in, co
     a.x = (const uint16_t *)in->data;
     a.weights = (const uint16_t *)w->weights->data;
     a.table = (const AdapterEntry *)w->table->data;
-    a.count = w->count;
     a.order = (const uint32_t *)p->order->data;
     a.adapter = a.order + (size_t)32 * (p->tiles + p->plain);
     a.sums = (float *)p->sums->data;
@@ -754,7 +743,7 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
                                            uint32_t rows, uint32_t k, uint32_t n) {
     if (!h3_launch_ready(g) || !adapters_valid(g, w, p, rows, k, n)) return 0;
     // The tiled projections take a K of whole 64-channel steps, the others would be gemm_small's, on the
-    // vector units. With the adapters: 301 rows, 1001 -> 777: 24 us, by gemm_small 140; 8000 rows, 5001 ->
+    // vector units. With the adapters: 301 rows, 1001 -> 777: 16 us, by gemm_small 140; 8000 rows, 5001 ->
     // 5001: 758 us, 528 TFLOP/s. Tiles of 64 rows by 64 columns where the large ones would fill few
     // compute units: 600 rows, 2001 -> 3001: 41 us (large 50), 800 rows: 55 (50), 1200 rows, 3001 ->
     // 3001: 93 (65).
@@ -776,7 +765,6 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
     a.shared_sums = (float *)p->sums->data + p->sums_at;
     // Four steps of 64 channels a share at least, in one round of the compute units.
     a.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint32_t>(SHARED_TILES, g->cus) / small, (k + KC - 1) / KC / 4));
-    if ((k + KC - 1) / KC < 8) a.shares = 1;
     a.products = a.shares > 1 ? (uint32_t)small * a.shares : 0;
     uint32_t blocks;
     if (!h3_tensor_acquire(g, weight) || !adapters_begin(g, a, in, w, p, blocks)) return 0;
