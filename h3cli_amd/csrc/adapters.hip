@@ -53,6 +53,7 @@ constexpr unsigned KC = 64;                // channels of K a step: one cache li
 constexpr unsigned COLS = 64;              // columns of N a step: one cache line of a row
 constexpr uint32_t RANK_MOST = 256;
 constexpr uint32_t SHARED_TILES = 256;
+constexpr uint32_t SPLITS_MOST = 8;
 
 uint32_t rank_blocks(uint32_t rank) { return (rank + 31) / 32; }
 
@@ -78,14 +79,21 @@ __device__ inline unsigned sixteens_of(const AdapterEntry &e) { return (e.rank +
 // Ranks that only fill the packed weights up are nothing, whatever x holds.
 __device__ inline void operands(const AdapterArgs &a, const AdapterEntry &entry, unsigned tile, unsigned row, unsigned from,
                                 bf16x8 &high, bf16x8 &low) {
-    const float *p = a.sums + ((size_t)tile * 32 + row) * a.rank_padded + from;
-    f32x4 t[2] = {};
-#pragma unroll 4
-    for (unsigned split = 0; split < a.splits; split++) {
-        t[0] += *reinterpret_cast<const f32x4 *>(p);
-        t[1] += *reinterpret_cast<const f32x4 *>(p + 4);
-        p += (size_t)a.tiles * 32 * a.rank_padded;
-    }
+    const float *const p = a.sums + ((size_t)tile * 32 + row) * a.rank_padded + from;
+    const size_t stride = (size_t)a.tiles * 32 * a.rank_padded;
+    f32x4 t[2] = {}, v[SPLITS_MOST][2];
+#pragma unroll
+    for (unsigned split = 0; split < SPLITS_MOST; split++)   // all on their way at once
+        if (split < a.splits) {
+            v[split][0] = *reinterpret_cast<const f32x4 *>(p + split * stride);
+            v[split][1] = *reinterpret_cast<const f32x4 *>(p + split * stride + 4);
+        }
+#pragma unroll
+    for (unsigned split = 0; split < SPLITS_MOST; split++)
+        if (split < a.splits) {
+            t[0] += v[split][0];
+            t[1] += v[split][1];
+        }
 #pragma unroll
     for (unsigned e = 0; e < 8; e++) {
         const float f = from + e < entry.rank ? t[e / 4][e % 4] * entry.scale : 0.f;
@@ -438,17 +446,32 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
         return;
     }
     if constexpr (PART == REST)
-        for (unsigned share = 0; share < a.shares; share++) {
-            const float *const from = a.shared_sums + (((size_t)id * a.shares + share) * 4 + wave) * R * R * 16 * 64 + lane;
+        for (unsigned share0 = 0; share0 < a.shares; share0 += 4) {   // four on their way at a time
+            float v[4][R * R * 16];
 #pragma unroll
-            for (unsigned i = 0; i < R * R * 16; i++) acc[i / 16 / R][i / 16 % R][i % 16] += from[i * 64];
+            for (unsigned u = 0; u < 4; u++) {
+                const float *const from = a.shared_sums + (((size_t)id * a.shares + min(share0 + u, a.shares - 1)) * 4 + wave) * R * R * 16 * 64 + lane;
+#pragma unroll
+                for (unsigned i = 0; i < R * R * 16; i++) v[u][i] = from[i * 64];
+            }
+#pragma unroll
+            for (unsigned u = 0; u < 4; u++)
+                if (share0 + u < a.shares)
+#pragma unroll
+                    for (unsigned i = 0; i < R * R * 16; i++) acc[i / 16 / R][i / 16 % R][i % 16] += v[u][i];
         }
     float *const stage = reinterpret_cast<float *>(lds) + wave * 32 * (32 * R + 4);
     constexpr unsigned STRIDE = 32 * R + 4, PER_ROW = 4 * R, AT_ONCE = 64 / PER_ROW;   // chunks of a row of the stage
+    const unsigned at = lane % PER_ROW * 8, c = n0 + wn + at;
+    i32x4 bias{};
+    if (a.bias) bias = load_loose(a.bias + (c < a.n ? c : 0));
 #pragma unroll
     for (unsigned i = 0; i < R; i++) {
         const unsigned tile = tile0 + wm / 32 + i;
         if (tile >= all) break;
+        uint32_t row[32 / AT_ONCE];
+#pragma unroll
+        for (unsigned j = 0; j < 32 / AT_ONCE; j++) row[j] = a.order[tile * 32 + j * AT_ONCE + lane / PER_ROW];
         if (tile < a.tiles) {
             const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
             for (unsigned r = 0; r < entry.rank; r += 16) {
@@ -475,14 +498,15 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
         wait_lds();
 #pragma unroll
         for (unsigned j = 0; j < 32 / AT_ONCE; j++) {
-            const unsigned r = j * AT_ONCE + lane / PER_ROW, at = lane % PER_ROW * 8, c = n0 + wn + at;
-            const uint32_t row = a.order[tile * 32 + r];
-            if (row == NONE || c >= a.n) continue;
+            const unsigned r = j * AT_ONCE + lane / PER_ROW;
+            if (row[j] == NONE || c >= a.n) continue;
             bf16x8 y;
 #pragma unroll
-            for (unsigned e = 0; e < 8; e++)
-                y[e] = (__bf16)(stage[r * STRIDE + at + e] + (a.bias && c + e < a.n ? bf16_to_f32(a.bias[c + e]) : 0.f));
-            uint16_t *const out = a.out + (size_t)row * a.n + c;
+            for (unsigned e = 0; e < 8; e++) {
+                const uint32_t word = (uint32_t)bias[e / 2];
+                y[e] = (__bf16)(stage[r * STRIDE + at + e] + __builtin_bit_cast(float, e % 2 ? word & 0xffff0000u : word << 16));
+            }
+            uint16_t *const out = a.out + (size_t)row[j] * a.n + c;
             const i32x4 v = __builtin_bit_cast(i32x4, y);
             if (c + 8 <= a.n) reinterpret_cast<Loose *>(out)->v = v;
             else
@@ -521,7 +545,7 @@ void pack(h3_gpu *g, uint16_t *dst, const uint16_t *src, size_t total, size_t ra
 
 // Shares of K for `tiles` tiles of up to `passes` * 64 ranks: about two workgroups a compute unit.
 uint32_t splits_for(const h3_gpu *g, uint32_t tiles, uint32_t passes) {
-    return std::max(1u, std::min(8u, 2 * g->cus / std::max(1u, tiles * passes)));
+    return std::max(1u, std::min(SPLITS_MOST, 2 * g->cus / std::max(1u, tiles * passes)));
 }
 
 }  // namespace
@@ -682,7 +706,8 @@ static int adapters_begin(h3_gpu *g, AdapterArgs &a, const h3_gpu_tensor *in, co
     a.tiles = p->tiles;
     a.plain = p->plain;
     a.passes = (blocks + 1) / 2;
-    a.splits = std::min(p->splits, splits_for(g, p->tiles, a.passes));
+    // No share without a step of 64 channels for each of its waves.
+    a.splits = std::min({p->splits, splits_for(g, p->tiles, a.passes), (w->k_padded / KC + DOWN_WAVES - 1) / DOWN_WAVES});
     a.rank_padded = rank_blocks(p->max_rank) * 32;
     if (!a.tiles || a.products) return 1;   // a shared projection's first launch takes it along
     constexpr unsigned shared = DOWN_WAVES * 8 * 64 * 16;
