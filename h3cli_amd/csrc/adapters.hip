@@ -608,6 +608,7 @@ extern "C" int h3_hip_adapters_set(h3_gpu *g, h3_hip_adapters *a, uint32_t index
     if (!h3_require(g, down, H3_GPU_BF16, (size_t)rank * a->k, "adapter A") ||
         !h3_require(g, up, H3_GPU_BF16, (size_t)a->n * rank, "adapter B"))
         return 0;
+    if (!h3_tensors_acquire(g, {down, up})) return 0;
     AdapterEntry &e = a->entries[index];
     uint16_t *w = (uint16_t *)a->weights->data;
     pack(g, w + e.down, (const uint16_t *)down->data, (size_t)rank_blocks(rank) * 32 * a->k_padded, rank, a->k, a->k_padded / 16, 0);
@@ -615,7 +616,7 @@ extern "C" int h3_hip_adapters_set(h3_gpu *g, h3_hip_adapters *a, uint32_t index
     pack(g, w + e.up, (const uint16_t *)up->data, (size_t)sixteens * 16 * a->n_padded, rank, a->n, sixteens, 1);
     hipLaunchKernelGGL(adapter_entry_scale, dim3(1), dim3(1), 0, g->compute, (AdapterEntry *)a->table->data + index, scale);
     e.scale = scale;
-    return h3_launch_status(g, "adapter");
+    return h3_launch_status(g, "adapter") && h3_tensors_release(g, {down, up});
 }
 
 // ------------------------------------------------------------------ rows
@@ -758,9 +759,9 @@ extern "C" int h3_hip_adapters_add_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_
     a.groups = (steps + a.span - 1) / a.span;
     if (!adapters_fit(g, p, (uint64_t)tiles * a.groups, rows, n)) return 0;
     uint32_t blocks;
-    if (!adapters_begin(g, a, in, w, p, blocks)) return 0;
-    if (!tiles) return 1;
-    return n % 8 == 0 ? launch_up<true>(g, a, tiles, blocks) : launch_up<false>(g, a, tiles, blocks);
+    if (!h3_tensors_acquire(g, {base, in}) || !adapters_begin(g, a, in, w, p, blocks)) return 0;
+    if (tiles && !(n % 8 == 0 ? launch_up<true>(g, a, tiles, blocks) : launch_up<false>(g, a, tiles, blocks))) return 0;
+    return h3_tensors_release(g, {base, in});
 }
 
 extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const h3_gpu_tensor *in, const h3_gpu_tensor *weight,
@@ -792,7 +793,7 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
     a.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint32_t>(SHARED_TILES, g->cus) / small, (k + KC - 1) / KC / 4));
     a.products = a.shares > 1 ? (uint32_t)small * a.shares : 0;
     uint32_t blocks;
-    if (!h3_tensor_acquire(g, weight) || !adapters_begin(g, a, in, w, p, blocks)) return 0;
+    if (!h3_tensors_acquire(g, {in, weight, bias}) || !adapters_begin(g, a, in, w, p, blocks)) return 0;
     hipEvent_t timing = h3_kernel_timing_begin(g);
     const int ok = a.shares > 1                  ? launch_gemm<1, PRODUCT>(g, a, a.products + a.tiles * a.passes * a.splits) && launch_gemm<1, REST>(g, a, (uint32_t)small)
                    : large * 5 >= g->cus * 3ull ? launch_gemm<2, ALL>(g, a, (uint32_t)large)
@@ -800,5 +801,5 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
     h3_kernel_timing_end(g, timing);
     if (!ok) return 0;
     g->stats.linear_dispatches++;
-    return h3_tensor_release(g, weight);
+    return h3_tensors_release(g, {in, weight, bias});
 }

@@ -810,6 +810,7 @@ extern "C" int h3_hip_sdpa_sequences_bf16(h3_gpu *g, h3_gpu_tensor *out, const h
     const auto *mid = (const MidItem *)(items + s->tiles + s->keys);
     const auto *rows = (const RowItem *)(mid + s->mid);
     char *const workspace = s->workspace ? (char *)s->workspace->data : nullptr;
+    if (!h3_tensors_acquire(g, {q, k, v})) return 0;
     if (s->tiles) {
         const h3_sequence_tiles t{sequences, items, items + s->tiles, s->tiles, s->keys, s->heads, s->kv_heads,
                                   (uint16_t *)workspace, (uint8_t *)workspace + s->retry_at};
@@ -824,5 +825,5 @@ extern "C" int h3_hip_sdpa_sequences_bf16(h3_gpu *g, h3_gpu_tensor *out, const h
     a.count = s->rows;
     if (s->rows && !launch(g, a)) return 0;
     if (s->tiles + s->mid + s->rows) g->stats.attention_dispatches++;
-    return 1;
+    return h3_tensors_release(g, {q, k, v});
 }

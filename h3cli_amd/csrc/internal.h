@@ -1,6 +1,7 @@
 // Cross-translation-unit hooks inside the backend (not exported).
 #pragma once
 #include "common.h"
+#include <initializer_list>
 
 int h3_attention_init(h3_gpu *g);
 void h3_attention_destroy(h3_gpu *g);
@@ -12,6 +13,17 @@ void h3_streaming_destroy(h3_gpu *g);
 int h3_tensor_events(h3_gpu *g, h3_gpu_tensor *t);
 int h3_tensor_acquire(h3_gpu *g, const h3_gpu_tensor *t);
 int h3_tensor_release(h3_gpu *g, const h3_gpu_tensor *t);
+// All of a call's inputs, any of which may be absent.
+inline int h3_tensors_acquire(h3_gpu *g, std::initializer_list<const h3_gpu_tensor *> tensors) {
+    for (const h3_gpu_tensor *t : tensors)
+        if (!h3_tensor_acquire(g, t)) return 0;
+    return 1;
+}
+inline int h3_tensors_release(h3_gpu *g, std::initializer_list<const h3_gpu_tensor *> tensors) {
+    for (const h3_gpu_tensor *t : tensors)
+        if (!h3_tensor_release(g, t)) return 0;
+    return 1;
+}
 
 // Launch helpers of the kernel translation units (all enqueue on g->compute).
 // The workspace of the tile kernels; a dense call that h3_attention_small_blocks takes

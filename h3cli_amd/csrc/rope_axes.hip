@@ -316,5 +316,5 @@ extern "C" int h3_hip_qkv_rope_axes_bf16(h3_gpu *g, h3_gpu_tensor *q, h3_gpu_ten
                      (const float *)positions->data, rows, heads, kv_heads, heads / kv_heads, dim, rope->pairs,
                      rope->axes, 1, 1, eps, grouped,
                      rope->interleaved};
-    return rope_axes(g, a);
+    return h3_tensors_acquire(g, {qkv, qw, kw, positions}) && rope_axes(g, a) && h3_tensors_release(g, {qkv, qw, kw, positions});
 }

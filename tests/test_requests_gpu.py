@@ -707,6 +707,74 @@ def test_steps_captured_into_two_graphs():
             s.close()
 
 
+class Streamed:
+    """A BF16 tensor that is filled from pinned memory, again and again."""
+
+    def __init__(self, g, versions):
+        self.g, self.size = g, versions[0].size * 2
+        self.tensor = g.empty(versions[0].size)
+        self.sources = [g.check(g.lib.h3_hip_host_alloc(g.handle, self.size), "pinned memory") for _ in versions]
+        for p, v in zip(self.sources, versions):
+            C.memmove(p, np.ascontiguousarray(v).ctypes.data, self.size)
+
+    def fill(self, i):
+        self.g.check(self.g.lib.h3_hip_tensor_stream_host(self.tensor.handle, self.sources[i], self.size), "stream")
+
+    def close(self):
+        for p in self.sources:
+            self.g.lib.h3_hip_host_free(self.g.handle, p, self.size)
+
+
+def test_streamed_inputs_are_waited_for():
+    """Adapters, keys and rows that are on their way when a call is made, and are filled anew behind it."""
+    with Gpu() as g:
+        # Two adapters from one tensor of 32 MB.
+        rows, k, n, rank = 3, 1 << 16, 72, 256
+        downs, up = [normal(rank * k, 5 + i, scale=0.01) for i in range(2)], g.from_bf16(normal(n * rank, 7))
+        x, base = g.from_bf16(normal(rows * k, 8)), g.from_bf16(normal(rows * n, 9))
+        streamed, plain = Streamed(g, downs), [g.from_bf16(d) for d in downs]
+        outs = [g.empty(rows * n) for _ in range(2)]
+        weights = [g.check(g.lib.h3_hip_adapters_new(g.handle, u32([rank, rank]), 2, k, n)) for _ in range(2)]
+        with adapter_rows(g, [0, 1, 0], 2, rank) as plan:
+            g.begin()
+            for w, out, late in zip(weights, outs, (True, False)):
+                for i in range(2):
+                    if late:
+                        streamed.fill(i)
+                    a = streamed.tensor if late else plain[i]
+                    g.check(g.lib.h3_hip_adapters_set(g.handle, w, i, a.handle, up.handle, C.c_float(1)), "set")
+                g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, out.handle, base.handle, x.handle, w, plan, rows, k, n), "adapters")
+            g.submit()
+        assert np.array_equal(outs[0].read(), outs[1].read()) and not np.array_equal(outs[0].read(), base.read())
+        streamed.close()
+        for w in weights:
+            g.lib.h3_hip_adapters_free(w)
+        # Keys of two contexts in one tensor of 41 MB, and the rows of a step.
+        keys, heads = 20000, 8
+        versions = [normal(keys * heads * 128, 20 + i) for i in range(2)]
+        streamed, plain, v = Streamed(g, versions), [g.from_bf16(d) for d in versions], g.from_bf16(normal(keys * heads * 128, 23))
+        q = g.from_bf16(normal(heads * 128, 24))
+        outs = [g.empty(heads * 128) for _ in range(4)]
+        turned = [[g.empty(keys // 3 * n * 128) for n in (6, 1, 1)] for _ in range(4)]
+        positions = g.from_f32(np.arange(keys // 3, dtype=np.float32))
+        with sequences(g, [0, 1], [0, keys], heads, heads) as plan, rope_axes(g, [1.0, 0.1], [0, 0], 1, 0) as rope:
+            g.begin()
+            for i in range(4):
+                if i < 2:
+                    streamed.fill(i)
+                t = streamed.tensor if i < 2 else plain[i - 2]
+                g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, outs[i].handle, q.handle, t.handle, v.handle, plan, C.c_float(SCALE)))
+                if i < 2:
+                    streamed.fill(i)
+                g.check(g.lib.h3_hip_qkv_rope_axes_bf16(g.handle, *(o.handle for o in turned[i]), t.handle, None, None, rope,
+                                                        positions.handle, keys // 3, 6, 1, 128, 0, C.c_float(EPS)))
+            g.submit()
+        for i in range(2):
+            assert np.array_equal(outs[i].read(), outs[i + 2].read())
+            assert all(np.array_equal(a.read(), b.read()) for a, b in zip(turned[i], turned[i + 2]))
+        streamed.close()
+
+
 def test_steps_of_two_contexts_at_once():
     """Two contexts, whose streams run side by side: the same bits as each alone."""
     with Gpu() as a, Gpu() as b:
