@@ -635,7 +635,8 @@ const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_o
     // Kernels in the order of their row blocks: 256, 128 and 32 rows. With the sequences by their rows each
     // kernel takes a range of them; every choice of the two borders (of up to 65 evenly spread ones).
     std::vector<uint32_t> by_rows = order;
-    auto tileable = [&](uint32_t i) { return plan.sequences[i].lk > 256 && (uint64_t)plan.sequences[i].lk * kv_heads * D * 2 < (1ull << 32); };
+    // The tile kernel's offsets into K and into whole tiles of transposed V have 32 bits.
+    auto tileable = [&](uint32_t i) { return plan.sequences[i].lk > 256 && tiles(i) * BN * kv_heads * D * 2 < (1ull << 32); };
     std::stable_sort(by_rows.begin(), by_rows.end(), [&](uint32_t x, uint32_t y) { return plan.sequences[x].lq > plan.sequences[y].lq; });
     const size_t n = by_rows.size(), stride = std::max<size_t>(1, (n + 63) / 64);
     // Rows' time from each border on.

@@ -37,6 +37,8 @@ def test_sequences_hold_what_their_kernels_need():
     assert 2 * 130 * 128 < layout([0, 1], [0, 18225], 5, 1) < 128 * 32 * 130 * 4 + 4096
     # A K of 4 GiB and more, in which a tile's offsets would not fit 32 bits, goes without them too.
     assert layout([0, 300], [0, 2 ** 24], 1, 1) < 1 << 25
+    assert layout([0, 10 ** 5], [0, 2 ** 24 - 1], 1, 1) < 1 << 25     # its transposed V, in whole tiles, would have 4 GiB
+    assert layout([0, 10 ** 5], [0, 2 ** 24 - 64], 1, 1) > 1 << 31
 
 
 def test_no_context():
