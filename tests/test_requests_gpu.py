@@ -707,6 +707,66 @@ def test_steps_captured_into_two_graphs():
             s.close()
 
 
+def test_every_kernel_captured_with_its_plan():
+    """Each kernel in one graph, adapters set within it: replays give the same bits, the eager call's but for
+    a projection, whose sum an eager call may share out."""
+    with Gpu() as g:
+        plans, calls = [], []
+
+        def attention(q_offsets, k_offsets, heads, kv_heads):
+            rows = [(q_offsets[-1], heads), (k_offsets[-1], kv_heads), (k_offsets[-1], kv_heads)]
+            t, out = [g.from_bf16(normal(n * h * 128, i)) for i, (n, h) in enumerate(rows)], g.empty(rows[0][0] * heads * 128)
+            plans.append(sequences(g, q_offsets, k_offsets, heads, kv_heads))
+            plan = plans[-1].handle
+            calls.append((lambda: g.lib.h3_hip_sdpa_sequences_bf16(g.handle, out.handle, *(x.handle for x in t), plan, C.c_float(SCALE)),
+                          out, True))
+
+        def projection(rows, k, n, rank=70):
+            x, w, out = g.from_bf16(normal(rows * k, 1)), g.from_bf16(normal(n * k, 2)), g.empty(rows * n)
+            a, b = g.from_bf16(normal(rank * k, 3, scale=0.05)), g.from_bf16(normal(n * rank, 4))
+            plans.append(Plan(g, g.lib.h3_hip_adapters_new(g.handle, u32([16, rank]), 2, k, n), g.lib.h3_hip_adapters_free))
+            plans.append(adapter_rows(g, [i % 3 for i in range(rows)], 2, rank))
+            weights, plan = plans[-2].handle, plans[-1].handle
+            calls.append((lambda: g.lib.h3_hip_adapters_set(g.handle, weights, 1, a.handle, b.handle, C.c_float(0.5)) and
+                          g.lib.h3_hip_linear_adapters_bf16(g.handle, out.handle, x.handle, w.handle, None, weights, plan, rows, k, n),
+                          out, k % 64 != 0))
+
+        attention([0, 1], [0, 18225], 5, 1)
+        attention([0, 300, 700], [0, 300, 700], 8, 8)
+        attention([0, 5000], [0, 5000], 8, 8)
+        projection(301, 1001, 777)
+        projection(300, 1024, 777)
+        projection(600, 999, 3000)
+        qkv, turned, positions = g.from_bf16(normal(40 * 3 * 128, 5)), [g.empty(40 * 128) for _ in range(3)], g.from_f32(np.arange(40.0))
+        plans.append(rope_axes(g, [1.0, 0.1], [0, 0], 1, 0))
+        calls.append((lambda: g.lib.h3_hip_qkv_rope_axes_bf16(g.handle, *(t.handle for t in turned), qkv.handle, None, None, plans[-1].handle,
+                                                              positions.handle, 40, 1, 1, 128, 0, C.c_float(EPS)), turned[0], True))
+        g.begin()
+        graph = Graph(g)
+        with graph:
+            for call, _, _ in calls:
+                g.check(call(), "captured")
+        first = None
+        for _ in range(3):
+            graph.launch()
+            g.submit()
+            got = [out.read() for _, out, _ in calls]
+            first = first or got
+            assert all(np.array_equal(a, b) for a, b in zip(got, first))
+            g.begin()
+            for call, _, _ in calls:
+                g.check(call(), "eager")
+            g.submit()
+            for i, ((_, out, same), captured) in enumerate(zip(calls, first)):
+                eager = out.read()
+                assert np.any(eager) and (not same or np.array_equal(eager, captured)), i
+            g.begin()
+        g.submit()
+        graph.close()
+        for p in plans:
+            p.free_handle(p.handle)
+
+
 class Streamed:
     """A BF16 tensor that is filled from pinned memory, again and again."""
 
