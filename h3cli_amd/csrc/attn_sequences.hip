@@ -17,7 +17,7 @@
 //    overlap by two waves a SIMD only. 729 and 806 rows of 56 heads: 54 us;
 //  * attn_sequences, 32 rows, its four waves taking the key tiles in turn, for few rows: bound by
 //    the keys' reads. Long key ranges go to several workgroups, joined by attn_sequences_join. One to
-//    three rows over 18225, 4001, 729 and 9000 keys of 8 key heads (131 MB): 37 us, 3.5 TB/s.
+//    three rows over 18225, 4001, 729 and 9000 keys of 8 key heads (131 MB): 35.5 us, 3.7 TB/s.
 #include "common.h"
 #include "internal.h"
 #include "attn_common.h"
@@ -55,7 +55,7 @@ struct Plan {
     std::vector<RowItem> rows;                   // by attn_sequences
     std::vector<JoinItem> joins;
     uint64_t vt = 0;                             // elements of transposed V
-    uint32_t parts = 0;
+    uint32_t parts = 0, most_parts = 0;          // in all, and of 32 rows
     size_t table_bytes() const {
         return sequences.size() * sizeof(h3_sequence) + (tiles.size() + keys.size()) * sizeof(h3_sequence_item) +
                mid.size() * sizeof(MidItem) + rows.size() * sizeof(RowItem) + joins.size() * sizeof(JoinItem);
@@ -70,7 +70,7 @@ struct Plan {
 struct h3_hip_sequences {
     h3_gpu *owner;
     uint32_t heads, kv_heads, count;
-    uint32_t tiles, keys, mid, rows, joins;
+    uint32_t tiles, keys, mid, rows, joins, most_parts;
     uint64_t q_rows, k_rows;      // rows that the tensors must hold
     size_t retry_at, parts_at;
     h3_gpu_tensor *table;         // h3_sequence, tiles, keys, mid, rows, joins, behind one another
@@ -86,7 +86,7 @@ struct SeqArgs {
     const MidItem *mid_items;
     const JoinItem *joins;
     float *partial;
-    unsigned count, join_count, heads, kv_heads, share;
+    unsigned count, join_count, most_parts, heads, kv_heads, share;
     float scale_log2;
     unsigned *fault;
 };
@@ -496,54 +496,79 @@ void attn_sequences_mid(SeqArgs a) {
     if (worst >= 0x7f800000u) a.fault[0] = 1u;
 }
 
-// 32 rows from their parts, in the parts' order: each brought to the common maximum.
-__global__ __launch_bounds__(256) void attn_sequences_join(SeqArgs a) {
+// 32 rows from their parts, each brought to the common maximum. JOINERS groups of 256 threads, one or four,
+// add every JOINERS-th part, in the parts' order, eight on their way at a time; then the groups' sums
+// are added. With the attention, four groups and one: one row of 8 heads over 18225 keys of one head,
+// 72 parts, 15.4 and 19.9 us; of 40 heads over 100000 keys of 8, 32 parts, 85.9 and 88.9; ten rows over
+// 2000 to 3593 keys, 2 or 3 parts, 34.2 and 33.0.
+template <unsigned JOINERS>
+__global__ __launch_bounds__(256 * JOINERS) void attn_sequences_join(SeqArgs a) {
     __shared__ float weight[32][PARTS_MOST + 1];
-    const unsigned tid = threadIdx.x, kv = blockIdx.x % a.kv_heads;
+    __shared__ f32x4 sums[JOINERS][256];
+    const unsigned tid = threadIdx.x % 256, group = __builtin_amdgcn_readfirstlane(threadIdx.x / 256), kv = blockIdx.x % a.kv_heads;
     const JoinItem item = a.joins[blockIdx.x / a.kv_heads];
     const unsigned rows = min(32u, item.lq * a.share - item.block * 32);
     const float *const first = a.partial + ((size_t)item.part * a.kv_heads + kv) * PART_FLOATS;
     const size_t step = (size_t)a.kv_heads * PART_FLOATS;
-    {
-        const unsigned r = tid / 8;
-        float top = -INFINITY, total = 0.f;
-        for (unsigned p = tid % 8; p < item.parts; p += 8) top = fmaxf(top, first[p * step + 32 * D + r]);
+    for (unsigned r = threadIdx.x / 32; r < rows; r += 8 * JOINERS) {
+        const unsigned lane = threadIdx.x % 32;
+        constexpr unsigned EACH = PARTS_MOST / 32;
+        float m[EACH], l[EACH], top = -INFINITY, total = 0.f;
 #pragma unroll
-        for (int off = 4; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-        for (unsigned p = tid % 8; p < item.parts; p += 8) {
-            const float w = exp2f_fast(first[p * step + 32 * D + r] - top);
-            weight[r][p] = w;
-            total = fmaf(w, first[p * step + 32 * D + 32 + r], total);
+        for (unsigned i = 0; i < EACH; i++) {   // behind the last part the last again, with no weight
+            const float *const at = first + min(lane + 32 * i, item.parts - 1) * step + 32 * D + r;
+            m[i] = at[0];
+            l[i] = at[32];
         }
 #pragma unroll
-        for (int off = 4; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
-        if (tid % 8 == 0) weight[r][PARTS_MOST] = total > 0.f ? 1.f / total : 0.f;
+        for (unsigned i = 0; i < EACH; i++) top = fmaxf(top, m[i]);
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+#pragma unroll
+        for (unsigned i = 0; i < EACH; i++) {
+            const float w = lane + 32 * i < item.parts ? exp2f_fast(m[i] - top) : 0.f;
+            weight[r][lane + 32 * i] = w;
+            total = fmaf(w, l[i], total);
+        }
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
+        if (lane == 0) weight[r][PARTS_MOST] = total > 0.f ? 1.f / total : 0.f;
     }
     __syncthreads();
     unsigned worst = 0;
-    for (unsigned i = tid; i < rows * (D / 4); i += 256) {
-        const unsigned r = i / (D / 4), d = i % (D / 4) * 4, v = item.block * 32 + r;
+    for (unsigned i0 = 0; i0 < rows * (D / 4); i0 += 256) {
+        const unsigned i = i0 + tid, r = min(i / (D / 4), rows - 1), d = i % (D / 4) * 4, v = item.block * 32 + r;
         f32x4 x{};
-        // Eight parts on their way at a time; those behind the last are the last again, for nothing.
-        for (unsigned p0 = 0; p0 < item.parts; p0 += 8) {
+        for (unsigned p0 = group; p0 < item.parts; p0 += 8 * JOINERS) {
             f32x4 y[8];
 #pragma unroll
-            for (unsigned p = 0; p < 8; p++) y[p] = *reinterpret_cast<const f32x4 *>(first + min(p0 + p, item.parts - 1) * step + r * D + d);
+            for (unsigned p = 0; p < 8; p++)
+                y[p] = *reinterpret_cast<const f32x4 *>(first + min(p0 + p * JOINERS, item.parts - 1) * step + r * D + d);
 #pragma unroll
             for (unsigned p = 0; p < 8; p++) {
-                const float w = p0 + p < item.parts ? weight[r][p0 + p] : 0.f;
+                const bool there = p0 + p * JOINERS < item.parts;
+                const float w = there ? weight[r][p0 + p * JOINERS] : 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = p0 + p < item.parts ? fmaf(w, y[p][e], x[e]) : x[e];
+                for (int e = 0; e < 4; e++) x[e] = there ? fmaf(w, y[p][e], x[e]) : x[e];
             }
         }
-        u16x4 out;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float y = x[e] * weight[r][PARTS_MOST];
-            worst = max(worst, __builtin_bit_cast(uint32_t, y) & 0x7f800000u);
-            out[e] = f32_to_bf16(y);
+        if constexpr (JOINERS > 1) {
+            sums[group][tid] = x;
+            __syncthreads();
         }
-        *reinterpret_cast<u16x4 *>(a.out + (((size_t)item.q0 + v / a.share) * a.heads + kv * a.share + v % a.share) * D + d) = out;
+        if (group == 0 && i < rows * (D / 4)) {
+#pragma unroll
+            for (unsigned j = 1; j < JOINERS; j++) x += sums[j][tid];
+            u16x4 out;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float y = x[e] * weight[r][PARTS_MOST];
+                worst = max(worst, __builtin_bit_cast(uint32_t, y) & 0x7f800000u);
+                out[e] = f32_to_bf16(y);
+            }
+            *reinterpret_cast<u16x4 *>(a.out + (((size_t)item.q0 + v / a.share) * a.heads + kv * a.share + v % a.share) * D + d) = out;
+        }
+        if constexpr (JOINERS > 1) __syncthreads();
     }
     if (worst >= 0x7f800000u) a.fault[0] = 1u;
 }
@@ -578,7 +603,8 @@ int launch(h3_gpu *g, const SeqArgs &a) {
     hipLaunchKernelGGL(attn_sequences, dim3(a.count * a.kv_heads), dim3(64 * WAVES), shared, g->compute, a);
     h3_kernel_timing_end(g, timing);
     if (!h3_launch_status(g, "BF16 attention of sequences") || !a.join_count) return h3_launch_status(g, "BF16 attention of sequences");
-    hipLaunchKernelGGL(attn_sequences_join, dim3(a.join_count * a.kv_heads), dim3(256), 0, g->compute, a);
+    if (a.most_parts > 8) hipLaunchKernelGGL(attn_sequences_join<4>, dim3(a.join_count * a.kv_heads), dim3(1024), 0, g->compute, a);
+    else hipLaunchKernelGGL(attn_sequences_join<1>, dim3(a.join_count * a.kv_heads), dim3(256), 0, g->compute, a);
     return h3_launch_status(g, "BF16 attention of sequences");
 }
 
@@ -692,7 +718,7 @@ const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_o
     // Where that leaves more than a few workgroups for a second round, up to a quarter more, if all then
     // run at once. (Two rows of 56 heads over 9000 keys each: 71 tiles, 224 workgroups, 99 us; 64 tiles, 336
     // workgroups, 128. Rows over 18225, 4001, 729 and 9000 keys of 8 heads: 16 tiles, 264 workgroups,
-    // 37 us; 17 tiles 39.)
+    // 37 us; 17 tiles, 39.)
     auto parts_of = [&](uint32_t i, uint64_t share) {
         const uint64_t n = tiles(i);
         return n >= share + JOIN_TILES ? std::min<uint64_t>((n + share - 1) / share, PARTS_MOST) : 1;
@@ -729,6 +755,7 @@ const char *make_plan(Plan &plan, const uint32_t *q_offsets, const uint32_t *k_o
         }
         const uint64_t n = tiles(i), parts = parts_of(i, share_tiles);
         if ((plan.rows.size() + blocks(i, 32) * parts) * kv_heads >= (1u << 24)) return "more rows than a launch takes";
+        plan.most_parts = std::max(plan.most_parts, (uint32_t)parts);
         for (uint32_t b = 0; b < blocks(i, 32); b++) {
             if (parts > 1) plan.joins.push_back({s.q0, s.lq, b, plan.parts, (uint32_t)parts});
             for (uint64_t p = 0; p < parts; p++)
@@ -780,7 +807,8 @@ extern "C" h3_hip_sequences *h3_hip_sequences_new(h3_gpu *g, const uint32_t *q_o
         append(plan.rows);
         append(plan.joins);
         s = new h3_hip_sequences{g, heads, kv_heads, count, (uint32_t)plan.tiles.size(), (uint32_t)plan.keys.size(),
-                                 (uint32_t)plan.mid.size(), (uint32_t)plan.rows.size(), (uint32_t)plan.joins.size(), q_offsets[count],
+                                 (uint32_t)plan.mid.size(), (uint32_t)plan.rows.size(), (uint32_t)plan.joins.size(),
+                                 plan.most_parts, q_offsets[count],
                                  (k_offsets ? k_offsets : q_offsets)[count], plan.retry_at(), plan.parts_at(kv_heads), nullptr, nullptr};
     } catch (const std::bad_alloc &) {
         h3_set_error(g, "sequences: out of host memory");
@@ -821,7 +849,7 @@ extern "C" int h3_hip_sdpa_sequences_bf16(h3_gpu *g, h3_gpu_tensor *out, const h
     }
     SeqArgs a{(uint16_t *)out->data, (const uint16_t *)q->data, (const uint16_t *)k->data, (const uint16_t *)v->data, rows, mid,
               (const JoinItem *)(rows + s->rows), s->joins ? (float *)(workspace + s->parts_at) : nullptr,
-              s->mid, s->joins, s->heads, s->kv_heads, s->heads / s->kv_heads, rounded * 1.4426950408889634f, g->fault};
+              s->mid, s->joins, s->most_parts, s->heads, s->kv_heads, s->heads / s->kv_heads, rounded * 1.4426950408889634f, g->fault};
     if (s->mid && !launch_mid(g, a)) return 0;
     a.count = s->rows;
     if (s->rows && !launch(g, a)) return 0;

@@ -203,6 +203,7 @@ def test_plans_choose_by_rows_and_heads(lengths, heads, kernel):
     ([0, 1, 2, 5, 6], [0, 6000, 6001, 6001, 9000], 10, 2),
     ([0, 40, 41], [0, 5000, 9001], 3, 1),                    # two blocks of rows, the second cut off
     ([0, 4], [2, 8195], 1, 1),
+    ([0, 2, 3], [0, 3000, 5200], 40, 40),                    # few parts each
 ])
 def test_attention_of_few_rows_over_many_keys(q_offsets, k_offsets, heads, kv_heads):
     print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads}", flush=True)
