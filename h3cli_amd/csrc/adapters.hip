@@ -74,25 +74,31 @@ struct AdapterArgs {
 
 __device__ inline unsigned sixteens_of(const AdapterEntry &e) { return (e.rank + 15) / 16; }
 
-// Ranks `from` to from + 7 of row `row` of t, its shares added in order and scaled, as two BF16 values
-// each: what the first rounding left is in the second (nothing where the first is infinite).
-// Ranks that only fill the packed weights up are nothing, whatever x holds.
-__device__ inline void operands(const AdapterArgs &a, const AdapterEntry &entry, unsigned tile, unsigned row, unsigned from,
-                                bf16x8 &high, bf16x8 &low) {
+// Ranks `from` to from + 7 of row `row` of t: its shares of K, all on their way at once, and then added
+// in order, scaled, and rounded to two BF16 values each: what the first rounding left is in the second
+// (nothing where the first is infinite). Ranks that only fill the packed weights up are nothing,
+// whatever x holds.
+template <unsigned MOST> struct Shares { f32x4 v[MOST][2]; };
+template <unsigned MOST> __device__ inline Shares<MOST> shares_of(const AdapterArgs &a, unsigned tile, unsigned row, unsigned from) {
     const float *const p = a.sums + ((size_t)tile * 32 + row) * a.rank_padded + from;
     const size_t stride = (size_t)a.tiles * 32 * a.rank_padded;
-    f32x4 t[2] = {}, v[SPLITS_MOST][2];
+    Shares<MOST> s;
 #pragma unroll
-    for (unsigned split = 0; split < SPLITS_MOST; split++)   // all on their way at once
-        if (split < a.splits) {
-            v[split][0] = *reinterpret_cast<const f32x4 *>(p + split * stride);
-            v[split][1] = *reinterpret_cast<const f32x4 *>(p + split * stride + 4);
+    for (unsigned split = 0; split < MOST; split++)
+        if (MOST == 1 || split < a.splits) {
+            s.v[split][0] = *reinterpret_cast<const f32x4 *>(p + split * stride);
+            s.v[split][1] = *reinterpret_cast<const f32x4 *>(p + split * stride + 4);
         }
+    return s;
+}
+template <unsigned MOST>
+__device__ inline void operands(const AdapterArgs &a, const AdapterEntry &entry, unsigned from, const Shares<MOST> &s, bf16x8 &high, bf16x8 &low) {
+    f32x4 t[2] = {};
 #pragma unroll
-    for (unsigned split = 0; split < SPLITS_MOST; split++)
-        if (split < a.splits) {
-            t[0] += v[split][0];
-            t[1] += v[split][1];
+    for (unsigned split = 0; split < MOST; split++)
+        if (MOST == 1 || split < a.splits) {
+            t[0] += s.v[split][0];
+            t[1] += s.v[split][1];
         }
 #pragma unroll
     for (unsigned e = 0; e < 8; e++) {
@@ -267,7 +273,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
             // Lane i % 64 of rank step i / 64: eight ranks of its row.
             const unsigned from = i / 64 * 16 + i % 64 / 32 * 8;
             bf16x8 high, low;
-            operands(a, entry, tile, i % 32, from, high, low);
+            operands(a, entry, from, shares_of<SPLITS_MOST>(a, tile, i % 32, from), high, low);
             operand[i / 64 * 128 + i % 64] = __builtin_bit_cast(i32x4, high);
             operand[i / 64 * 128 + 64 + i % 64] = __builtin_bit_cast(i32x4, low);
         }
@@ -350,8 +356,8 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
 // A compute unit takes in about 20 bytes a cycle of such rows, so few tiles over a long K are shared out
 // (part PRODUCT: a share of K, its sums to memory; then part REST: the shares added in order, and
 // what follows them). The adapters' first product needs nothing of it and is part of PRODUCT's launch,
-// its workgroups behind the shares'. (301 rows, 1001 -> 777: 16 us in three shares, unshared, the adapters'
-// product before it, 18; 10 rows, 5337 -> 47, 21 shares: 18, 38.)
+// its workgroups behind the shares'. (301 rows, 1001 -> 777: 12.5 us in three shares, unshared, the adapters'
+// product before it, 18; 10 rows, 5337 -> 47, 21 shares: 16, 38.)
 enum Part { ALL, PRODUCT, REST };
 template <int R, Part PART>
 __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
@@ -474,19 +480,37 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
         for (unsigned j = 0; j < 32 / AT_ONCE; j++) row[j] = a.order[tile * 32 + j * AT_ONCE + lane / PER_ROW];
         if (tile < a.tiles) {
             const AdapterEntry entry = a.table[load_uniform(a.adapter + tile)];
-            for (unsigned r = 0; r < entry.rank; r += 16) {
-                bf16x8 high, low;
-                operands(a, entry, tile, n, r + hf * 8, high, low);
+            auto ranks = [&](auto most_tag, auto ahead_tag) {
+                constexpr unsigned MOST = decltype(most_tag)::value, AHEAD = decltype(ahead_tag)::value;
+                for (unsigned r0 = 0; r0 < entry.rank; r0 += 16 * AHEAD) {
+                    Shares<MOST> t[AHEAD];
+                    bf16x8 u[AHEAD][R];
 #pragma unroll
-                for (unsigned b = 0; b < R; b++) {
-                    // Columns past the last packed step are not stored: any block does.
-                    const unsigned c = min(n0 + wn + 32 * b, (a.n - 1) / 32 * 32);
-                    const bf16x8 u = *reinterpret_cast<const bf16x8 *>(
-                        a.weights + entry.up + (((size_t)(c / COLS) * sixteens_of(entry) + r / 16) * 2 + c / 32 % 2) * 512 + lane * 8);
-                    acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, high, acc[i][b], 0, 0, 0);
-                    acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, low, acc[i][b], 0, 0, 0);
+                    for (unsigned j = 0; j < AHEAD; j++) {
+                        const unsigned r = min(r0 + 16 * j, (sixteens_of(entry) - 1) * 16);   // behind the last for nothing
+                        t[j] = shares_of<MOST>(a, tile, n, r + hf * 8);
+#pragma unroll
+                        for (unsigned b = 0; b < R; b++) {
+                            // Columns past the last packed step are not stored: any block does.
+                            const unsigned c = min(n0 + wn + 32 * b, (a.n - 1) / 32 * 32);
+                            u[j][b] = *reinterpret_cast<const bf16x8 *>(
+                                a.weights + entry.up + (((size_t)(c / COLS) * sixteens_of(entry) + r / 16) * 2 + c / 32 % 2) * 512 + lane * 8);
+                        }
+                    }
+#pragma unroll
+                    for (unsigned j = 0; j < AHEAD; j++) {
+                        bf16x8 high, low;
+                        operands(a, entry, r0 + 16 * j + hf * 8, t[j], high, low);
+#pragma unroll
+                        for (unsigned b = 0; b < R; b++) {
+                            acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[j][b], high, acc[i][b], 0, 0, 0);
+                            acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[j][b], low, acc[i][b], 0, 0, 0);
+                        }
+                    }
                 }
-            }
+            };
+            if (a.splits == 1) ranks(std::integral_constant<unsigned, 1>{}, std::integral_constant<unsigned, 4>{});
+            else ranks(std::integral_constant<unsigned, SPLITS_MOST>{}, std::integral_constant<unsigned, 1>{});
         }
         wait_lds();                     // the stage's last reads
 #pragma unroll
@@ -709,6 +733,10 @@ static int adapters_begin(h3_gpu *g, AdapterArgs &a, const h3_gpu_tensor *in, co
     a.passes = (blocks + 1) / 2;
     // No share without a step of 64 channels for each of its waves.
     a.splits = std::min({p->splits, splits_for(g, p->tiles, a.passes), (w->k_padded / KC + DOWN_WAVES - 1) / DOWN_WAVES});
+    // Up to 64 steps adapter_gemm takes t in one share, 64 ranks of it on their way at a time; in more it waits for
+    // each 16. (301 rows, 2001 -> 777, ranks 16 and 128: 16 us, in eight shares 29; 600 rows, 2001 ->
+    // 2001: 41, 61; 10 rows, 5337 -> 47, ranks 16 and 32: 23, 16.)
+    if (a.w && w->k_padded / KC <= 64) a.splits = 1;
     a.rank_padded = rank_blocks(p->max_rank) * 32;
     if (!a.tiles || a.products) return 1;   // a shared projection's first launch takes it along
     constexpr unsigned shared = DOWN_WAVES * 8 * 64 * 16;
@@ -769,8 +797,8 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
                                            uint32_t rows, uint32_t k, uint32_t n) {
     if (!h3_launch_ready(g) || !adapters_valid(g, w, p, rows, k, n)) return 0;
     // The tiled projections take a K of whole 64-channel steps, the others would be gemm_small's, on the
-    // vector units. With the adapters: 301 rows, 1001 -> 777: 16 us, by gemm_small 140; 8000 rows, 5001 ->
-    // 5001: 758 us, 528 TFLOP/s. Tiles of 64 rows by 64 columns where the large ones would fill few
+    // vector units. With the adapters: 301 rows, 1001 -> 777: 12.5 us, by gemm_small 140; 8000 rows, 5001 ->
+    // 5001: 740 us, 541 TFLOP/s. Tiles of 64 rows by 64 columns where the large ones would fill few
     // compute units: 600 rows, 2001 -> 3001: 41 us (large 50), 800 rows: 55 (50), 1200 rows, 3001 ->
     // 3001: 93 (65).
     if (k % KC == 0 || !weight || weight->owner != g || weight->dtype != H3_GPU_BF16 || weight->q8 || weight->quant_mode || weight->block_tile)
