@@ -53,7 +53,7 @@ constexpr unsigned KC = 64;                // channels of K a step: one cache li
 constexpr unsigned COLS = 64;              // columns of N a step: one cache line of a row
 constexpr uint32_t RANK_MOST = 256;
 constexpr uint32_t SHARED_TILES = 256;
-constexpr uint32_t SPLITS_MOST = 8;
+constexpr uint32_t SPLITS_MOST = 4;   // (eight: 9 rows, 5376 -> 32256, 16.6 us, so 16.0; one: 22)
 
 uint32_t rank_blocks(uint32_t rank) { return (rank + 31) / 32; }
 
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
                 }
             };
             if (a.splits == 1) ranks(std::integral_constant<unsigned, 1>{}, std::integral_constant<unsigned, 4>{});
-            else ranks(std::integral_constant<unsigned, SPLITS_MOST>{}, std::integral_constant<unsigned, 1>{});
+            else ranks(std::integral_constant<unsigned, SPLITS_MOST>{}, std::integral_constant<unsigned, 2>{});
         }
         wait_lds();                     // the stage's last reads
 #pragma unroll
@@ -733,8 +733,8 @@ static int adapters_begin(h3_gpu *g, AdapterArgs &a, const h3_gpu_tensor *in, co
     a.passes = (blocks + 1) / 2;
     // No share without a step of 64 channels for each of its waves.
     a.splits = std::min({p->splits, splits_for(g, p->tiles, a.passes), (w->k_padded / KC + DOWN_WAVES - 1) / DOWN_WAVES});
-    // Up to 64 steps adapter_gemm takes t in one share, 64 ranks of it on their way at a time; in more it waits for
-    // each 16. (301 rows, 2001 -> 777, ranks 16 and 128: 16 us, in eight shares 29; 600 rows, 2001 ->
+    // Up to 64 steps adapter_gemm takes t in one share, 64 ranks of it on their way at a time, in more shares
+    // 32. (301 rows, 2001 -> 777, ranks 16 and 128: 16 us, in eight shares 29; 600 rows, 2001 ->
     // 2001: 41, 61; 10 rows, 5337 -> 47, ranks 16 and 32: 23, 16.)
     if (a.w && w->k_padded / KC <= 64) a.splits = 1;
     a.rank_padded = rank_blocks(p->max_rank) * 32;
