@@ -92,7 +92,8 @@ template <unsigned MOST> __device__ inline Shares<MOST> shares_of(const AdapterA
     return s;
 }
 template <unsigned MOST>
-__device__ inline void operands(const AdapterArgs &a, const AdapterEntry &entry, unsigned from, const Shares<MOST> &s, bf16x8 &high, bf16x8 &low) {
+__device__ inline void operands(const AdapterArgs &a, const AdapterEntry &entry, unsigned from, const Shares<MOST> &s, bf16x8 &high,
+                                bf16x8 &low) {
     f32x4 t[2] = {};
 #pragma unroll
     for (unsigned split = 0; split < MOST; split++)
@@ -456,7 +457,8 @@ __global__ __launch_bounds__(256, 2) void adapter_gemm(AdapterArgs a) {
             float v[4][R * R * 16];
 #pragma unroll
             for (unsigned u = 0; u < 4; u++) {
-                const float *const from = a.shared_sums + (((size_t)id * a.shares + min(share0 + u, a.shares - 1)) * 4 + wave) * R * R * 16 * 64 + lane;
+                const size_t share = (size_t)id * a.shares + min(share0 + u, a.shares - 1);
+                const float *const from = a.shared_sums + (share * 4 + wave) * R * R * 16 * 64 + lane;
 #pragma unroll
                 for (unsigned i = 0; i < R * R * 16; i++) v[u][i] = from[i * 64];
             }
@@ -823,7 +825,8 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
     uint32_t blocks;
     if (!h3_tensors_acquire(g, {in, weight, bias}) || !adapters_begin(g, a, in, w, p, blocks)) return 0;
     hipEvent_t timing = h3_kernel_timing_begin(g);
-    const int ok = a.shares > 1                  ? launch_gemm<1, PRODUCT>(g, a, a.products + a.tiles * a.passes * a.splits) && launch_gemm<1, REST>(g, a, (uint32_t)small)
+    const int ok = a.shares > 1 ? launch_gemm<1, PRODUCT>(g, a, a.products + a.tiles * a.passes * a.splits) &&
+                                      launch_gemm<1, REST>(g, a, (uint32_t)small)
                    : large * 5 >= g->cus * 3ull ? launch_gemm<2, ALL>(g, a, (uint32_t)large)
                                                 : launch_gemm<1, ALL>(g, a, (uint32_t)small);
     h3_kernel_timing_end(g, timing);

@@ -815,7 +815,8 @@ extern "C" h3_hip_sequences *h3_hip_sequences_new(h3_gpu *g, const uint32_t *q_o
         return nullptr;
     }
     s->table = h3_gpu_tensor_from_u32(g, words.data(), words.size());
-    if (s->table && plan.workspace_bytes(kv_heads)) s->workspace = h3_gpu_tensor_alloc(g, plan.workspace_bytes(kv_heads), H3_GPU_I8, H3_GPU_DEVICE_ONLY);
+    if (s->table && plan.workspace_bytes(kv_heads))
+        s->workspace = h3_gpu_tensor_alloc(g, plan.workspace_bytes(kv_heads), H3_GPU_I8, H3_GPU_DEVICE_ONLY);
     if (!s->table || (plan.workspace_bytes(kv_heads) && !s->workspace)) {
         h3_hip_sequences_free(s);
         return nullptr;

@@ -552,7 +552,8 @@ def test_linear_with_adapters_is_the_projection_and_the_adapters(kind, rows):
 
 @pytest.mark.parametrize("rows,k,n,ranks,bias", [
     (1, 1, 1, [1], True), (5, 65, 130, [16], False), (301, 1001, 777, [1, 40, 7, 19], True), (130, 72, 1000, [33, 64], False),
-    (33, 5000, 64, [256], True), (1700, 4200, 1500, [70, 9], False), (1000, 200, 2049, [16, 8, 100], True), (2100, 520, 4100, [32, 32], False), (64, 1000, 7, [5], True),
+    (33, 5000, 64, [256], True), (1700, 4200, 1500, [70, 9], False), (1000, 200, 2049, [16, 8, 100], True),
+    (2100, 520, 4100, [32, 32], False), (64, 1000, 7, [5], True),
 ])
 def test_linear_with_adapters_of_any_width(rows, k, n, ranks, bias):
     """A BF16 weight whose K is no multiple of 64: one sum and one rounding for projection, bias and adapters."""
