@@ -12,11 +12,12 @@
 //   x'_d cos +- x'_p sin = r (x_d (w_d cos) + x_p (+-w_p sin)),   r the head's norm factor.
 //
 // Angles. A position may be far (2^24 and beyond), where an FP32 angle has lost its phase. With
-// f / 2 pi = hi + lo in two floats and n = rint(p hi), the phase in turns is
-//   fma(p, lo, fma(p, hi, -n)),
-// whose inner fma is exact (the product's rounding, or what follows the point) and, beyond 2^24
-// turns, once more brought near zero. What is left is the last rounding and that of lo: up to
-// 2^24 turns 2^-23 turns, beyond them 2^-47 of the angle. The hardware's sine and cosine take turns.
+// f / 2 pi = hi + lo in two floats, the phase in turns is
+//   near = fma(p, hi, -rint(p hi)),   t = fma(p, lo, near - rint(near)),   t - rint(t).
+// Up to 2^24 turns near is below one turn and off by half a bit of that, 2^-25; beyond, it is what p hi
+// was rounded by, exactly, and may be many turns. p lo is off by lo's rounding, 2^-48 of the angle, and t by its
+// own. In all up to 2^24 turns 2^-23 turns, beyond them 2^-47 of the angle. The hardware's sine and cosine
+// take turns, up to 256 of them: t alone passes that at 2^33 turns, and is brought below half a turn.
 #include "common.h"
 #include "internal.h"
 #include <algorithm>
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256, 5) void rope_axes_chunks(AxesArgs a) {
 #pragma unroll
         for (unsigned r = 0; r < TOGETHER; r++) {
             if (r >= a.together) break;
-            const float near = fmaf(next[r], hi, -rintf(next[r] * hi)), t = fmaf(next[r], lo, near - rintf(near));
+            const float near = fmaf(next[r], hi, -rintf(next[r] * hi)), far = fmaf(next[r], lo, near - rintf(near)), t = far - rintf(far);
             const float cs = turns ? __builtin_amdgcn_cosf(t) : 1.f, sn = turns ? __builtin_amdgcn_sinf(t) : 0.f;
 #pragma unroll
             for (int kind = QUERY; kind <= KEY; kind++) {

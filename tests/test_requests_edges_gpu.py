@@ -1,0 +1,69 @@
+"""Operators of a step that serves several requests at once, at the ends of their ranges: far
+positions, sequences that one kernel cannot take beside those it can, workgroups that take several
+tasks or steps in turn, every type of weight, tensors that are still being filled.
+
+Bounds as in test_requests_gpu.py: HALF is BF16's largest rounding error relative to the value, F32
+that of FP32; a sum of n products in FP32 is off by at most n * F32 times the sum of their magnitudes."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from h3cli_amd.runtime import Gpu
+from tests.helpers import bf16
+from tests.test_requests_gpu import EPS, F32, HALF, normal, rope_axes, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ rotation by axes
+def turned(g, qkv, positions, frequencies, dim, interleaved, axis=None, axes=1):
+    """Query rows of one head, without norms."""
+    rows = len(positions)
+    t, p, outs = g.from_bf16(qkv), g.from_f32(positions), [g.empty(rows * dim) for _ in range(3)]
+    with rope_axes(g, frequencies, [0] * len(frequencies) if axis is None else axis, axes, interleaved) as plan:
+        g.begin()
+        g.check(g.lib.h3_hip_qkv_rope_axes_bf16(g.handle, *(o.handle for o in outs), t.handle, None, None, plan, p.handle, rows, 1, 1,
+                                                dim, 0, C.c_float(EPS)), "rope")
+        g.submit()
+    return outs[0].read().reshape(rows, dim)
+
+
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("far", [2.0 ** 27, 3e9, 4.2e10, 1e11, 1e12, -1e12])
+def test_rope_by_axes_of_any_number_of_turns(far, interleaved):
+    """A phase is off by at most 2^-23 turns up to 2^24 turns and by 2^-47 of the angle beyond."""
+    rows, dim, pairs = 64, 128, 64
+    with Gpu() as g:
+        rng = np.random.RandomState(3)
+        qkv = normal(rows * 3 * dim, 5).reshape(rows, 3, dim)
+        positions = (far * (1 + rng.rand(rows))).astype(np.float32)
+        frequencies = np.concatenate([[1.0, 0.999], 10000.0 ** -rng.rand(pairs - 2)])
+        got = bf16(turned(g, qkv, positions, list(frequencies), dim, interleaved))
+    x = bf16(qkv[:, 0]).astype(np.float64)
+    angle = positions.astype(np.float64)[:, None] * frequencies
+    first = np.arange(pairs) * (2 if interleaved else 1)
+    second = first + (1 if interleaved else pairs)
+    a, b, c, s = x[:, first], x[:, second], np.cos(angle), np.sin(angle)
+    y = x.copy()
+    y[:, first], y[:, second] = a * c - b * s, b * c + a * s
+    # The hardware's sine and cosine to 2^-18, the phase as above; this reference's own angle to 2^-52 of it; two FP32
+    # products and their sum; one rounding to BF16.
+    phase = 2 * math.pi * np.maximum(2.0 ** -23, 2.0 ** -47 * np.abs(angle) / (2 * math.pi)) + 2.0 ** -52 * np.abs(angle)
+    size = np.empty_like(x)
+    size[:, first] = size[:, second] = (np.abs(a) + np.abs(b)) * (2.0 ** -18 + phase + 4 * F32)
+    within(got, y, HALF * np.abs(y) + size * (1 + HALF), (far, interleaved))
+
+
+def test_rope_by_axes_beyond_any_phase_still_turns():
+    """Where a turn is lost in the position's own rounding, pairs keep their lengths."""
+    rows, dim = 8, 64
+    with Gpu() as g:
+        qkv = normal(rows * 3 * dim, 5).reshape(rows, 3, dim)
+        positions = (1e20 * 10.0 ** (2 * np.arange(rows))).astype(np.float32)
+        got = bf16(turned(g, qkv, positions, list(10000.0 ** -(np.arange(32) / 32)), dim, 0)).astype(np.float64)
+    x = bf16(qkv[:, 0]).astype(np.float64)
+    want = np.hypot(x[:, :32], x[:, 32:])
+    # sin^2 + cos^2 is off by 4 * 2^-18 at most, each result by HALF of its size.
+    within(np.hypot(got[:, :32], got[:, 32:]), want, want * (HALF + 2.0 ** -15))
