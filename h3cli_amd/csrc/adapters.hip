@@ -803,12 +803,15 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
     // 5001: 740 us, 541 TFLOP/s. Tiles of 64 rows by 64 columns where the large ones would fill few
     // compute units: 600 rows, 2001 -> 3001: 41 us (large 50), 800 rows: 55 (50), 1200 rows, 3001 ->
     // 3001: 93 (65).
-    if (k % KC == 0 || !weight || weight->owner != g || weight->dtype != H3_GPU_BF16 || weight->q8 || weight->quant_mode || weight->block_tile)
-        return h3_gpu_linear_bf16(g, out, in, weight, bias, rows, k, n) && h3_hip_adapters_add_bf16(g, out, out, in, w, p, rows, k, n);
     if (!h3_require(g, in, H3_GPU_BF16, (size_t)rows * k, "linear input") ||
-        !h3_require(g, weight, H3_GPU_BF16, (size_t)n * k, "linear weight") ||
-        !h3_require(g, out, H3_GPU_BF16, (size_t)rows * n, "linear output") ||
         (bias && !h3_require(g, bias, H3_GPU_BF16, n, "linear bias")))
+        return 0;
+    if (k % KC == 0 || !weight || weight->owner != g || weight->dtype != H3_GPU_BF16 || weight->q8 || weight->quant_mode || weight->block_tile)
+        // The projection by itself waits for its weight only, the adapters for x.
+        return h3_tensors_acquire(g, {in, bias}) && h3_gpu_linear_bf16(g, out, in, weight, bias, rows, k, n) &&
+               h3_hip_adapters_add_bf16(g, out, out, in, w, p, rows, k, n) && h3_tensors_release(g, {bias});
+    if (!h3_require(g, weight, H3_GPU_BF16, (size_t)n * k, "linear weight") ||
+        !h3_require(g, out, H3_GPU_BF16, (size_t)rows * n, "linear output"))
         return 0;
     if (out == in) return h3_set_error(g, "linear: output aliases input");
     const uint64_t tiles = p->tiles + p->plain;

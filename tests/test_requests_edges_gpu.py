@@ -12,7 +12,7 @@ import pytest
 
 from h3cli_amd.runtime import Gpu
 from tests.helpers import bf16
-from tests.test_requests_gpu import EPS, F32, HALF, normal, rope_axes, within
+from tests.test_requests_gpu import EPS, F32, HALF, Adapters, Streamed, adapter_rows, normal, rope_axes, row_map, within
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,31 @@ def test_rope_by_axes_beyond_any_phase_still_turns():
     want = np.hypot(x[:, :32], x[:, 32:])
     # sin^2 + cos^2 is off by 4 * 2^-18 at most, each result by HALF of its size.
     within(np.hypot(got[:, :32], got[:, 32:]), want, want * (HALF + 2.0 ** -15))
+
+
+# ------------------------------------------------------------------ adapters
+@pytest.mark.parametrize("k", [4096, 4097])
+def test_projections_with_adapters_wait_for_streamed_rows_and_bias(k):
+    """x of 32 MB and then the bias are on their way when the call is made, and are filled anew behind it."""
+    rows, n = 4000, 72
+    with Gpu() as g:
+        xs, biases = [normal(rows * k, 5 + i) for i in range(2)], [normal(n, 8 + i) for i in range(2)]
+        sx, sb = Streamed(g, xs), Streamed(g, biases)
+        w, ad = g.from_bf16(normal(n * k, 3, scale=1 / math.sqrt(k))), Adapters(g, [8, 24], k, n)
+        plain, outs = [[g.from_bf16(x), g.from_bf16(b)] for x, b in zip(xs, biases)], [g.empty(rows * n) for _ in range(4)]
+        with adapter_rows(g, row_map(rows, 2, 3), 2, 24) as plan:
+            g.begin()
+            for i in range(4):
+                if i < 2:
+                    sx.fill(i)
+                    sb.fill(i)
+                x, b = (sx.tensor, sb.tensor) if i < 2 else plain[i - 2]
+                g.check(g.lib.h3_hip_linear_adapters_bf16(g.handle, outs[i].handle, x.handle, w.handle, b.handle, ad.handle, plan,
+                                                          rows, k, n), "linear")
+            g.submit()
+        for i in range(2):
+            assert np.array_equal(outs[i].read(), outs[i + 2].read()), i
+        assert not np.array_equal(outs[0].read(), outs[1].read())
+        for s in (sx, sb):
+            s.close()
+        ad.close()
