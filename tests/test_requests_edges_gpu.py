@@ -12,9 +12,60 @@ import pytest
 
 from h3cli_amd.runtime import Gpu
 from tests.helpers import bf16
-from tests.test_requests_gpu import EPS, F32, HALF, Adapters, Streamed, adapter_rows, normal, rope_axes, row_map, within
+from tests.test_requests_gpu import (EPS, F32, HALF, SCALE, Adapters, Streamed, adapter_rows, attention_reference, check_attention, fill,
+                                     normal, rope_axes, row_map, sequences, within)
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ attention of sequences
+@pytest.mark.parametrize("q_rows,k_rows,heads,launches,kernel", [
+    ((9000, 8193), (256, 8193), 40, 2, "attn_sequences rows=128"),       # the most queries have few keys, or none
+    ((9000, 8193), (0, 8193), 40, 2, "attn_sequences rows=128"),
+    ((5000, 5001), (5000, 200), 8, 2, "attn_sequences rows=128"),
+    ((5000, 1500, 1, 1), (5000, 250, 9000, 9000), 40, 3, "attn_sequences rows=32 shares=2"),
+])
+def test_plans_of_several_kernels(q_rows, k_rows, heads, launches, kernel):
+    """Each sequence by the kernel that suits it, all in one call: tiles of 256 rows for the long ones whatever
+    else there is. Sampled rows of three heads against 64 bits."""
+    print(f"[sequences] {q_rows} {k_rows} {heads}", flush=True)
+    q_ends, k_ends = (np.cumsum([0] + list(n)) for n in (q_rows, k_rows))
+    with Gpu() as g:
+        t = [g.empty(int(n) * heads * 128) for n in (q_ends[-1], k_ends[-1], k_ends[-1], q_ends[-1])]
+        total, count = C.c_double(), C.c_uint64()
+        with sequences(g, q_ends, k_ends, heads, heads) as plan:
+            g.check(g.lib.h3_hip_kernel_timing(g.handle, 1))
+            g.begin()
+            for i in range(4):
+                fill(g, t[i], i + 1)
+            g.check(g.lib.h3_hip_sdpa_sequences_bf16(g.handle, t[3].handle, *(x.handle for x in t[:3]), plan, C.c_float(SCALE)), "attention")
+            assert g.last_kernel() == kernel, g.last_kernel()
+            g.submit()
+            g.check(g.lib.h3_hip_kernel_timing_read(g.handle, C.byref(total), C.byref(count)))
+            g.check(g.lib.h3_hip_kernel_timing(g.handle, 0))
+        assert count.value == launches
+        q, k, v, got = (x.read().reshape(-1, heads, 128) for x in t)
+    for i, (lq, lk) in enumerate(zip(q_rows, k_rows)):
+        at = q_ends[i] + np.unique(np.append(np.arange(0, lq, 37), lq - 1))
+        for h in (0, heads // 2 + 1, heads - 1):
+            if not lk:
+                assert not np.any(got[at, h] & 0x7fff)
+                continue
+            keys = slice(k_ends[i], k_ends[i + 1])
+            fq, fk, fv = (bf16(x).astype(np.float64) for x in (q[at, h], k[keys, h], v[keys, h]))
+            within(bf16(got[at, h]), *attention_reference(fq, fk, fv, SCALE), (i, h))
+
+
+@pytest.mark.parametrize("q_offsets,k_offsets,heads,kv_heads", [
+    ([0, 900, 1600], [0, 200, 900], 4, 4),
+    ([0, 700, 1300, 1301, 1400], [3, 203, 903, 1700, 1700], 4, 2),       # a single row by tiles; queries without keys
+    ([2, 802, 803, 1500], [0, 0, 256, 700], 2, 2),
+])
+def test_sequences_by_tiles_beside_those_of_few_keys(q_offsets, k_offsets, heads, kv_heads, monkeypatch):
+    print(f"[sequences] {q_offsets} {k_offsets} {heads}/{kv_heads}", flush=True)
+    monkeypatch.setenv("H3_HIP_ATTENTION_VARIANT", "22")
+    with Gpu() as g:
+        assert check_attention(g, q_offsets, k_offsets, heads, kv_heads, seed=13) == "attn_sequences rows=128"
 
 
 # ------------------------------------------------------------------ rotation by axes

@@ -41,6 +41,15 @@ def test_sequences_hold_what_their_kernels_need():
     assert layout([0, 10 ** 5], [0, 2 ** 24 - 64], 1, 1) > 1 << 31
 
 
+@pytest.mark.parametrize("queries,keys", [(9000, 256), (9000, 100), (9000, 0), (8000, 256)])
+@pytest.mark.parametrize("first", [True, False])
+def test_a_sequence_of_few_keys_leaves_the_others_their_tiles(queries, keys, first):
+    """Transposed values of 8193 rows of self-attention, whether fewer or more queries over few keys stand beside them."""
+    lengths = [(queries, keys), (8193, 8193)][::1 if first else -1]
+    ends = [[0, lengths[0][i], lengths[0][i] + lengths[1][i]] for i in range(2)]
+    assert layout(ends[0], ends[1], 40, 40) > 129 * 64 * 40 * 256
+
+
 def test_no_context():
     lib = _lib.load()
     assert not lib.h3_hip_sequences_new(None, u32([0, 1]), None, 1, 1, 1)
