@@ -10,10 +10,12 @@ import math
 import numpy as np
 import pytest
 
+from h3cli_amd import synth
 from h3cli_amd.runtime import Gpu
 from tests.helpers import bf16
-from tests.test_requests_gpu import (EPS, F32, HALF, SCALE, Adapters, Streamed, adapter_rows, attention_reference, check_attention, fill,
-                                     normal, rope_axes, row_map, sequences, within)
+from tests.test_quant_gpu import configure, load, write_weight
+from tests.test_requests_gpu import (EPS, F32, HALF, SCALE, Adapters, Step, Streamed, adapter_rows, attention_reference, check_adapters,
+                                     check_attention, check_rope, fill, normal, rope_axes, rope_reference, row_map, sequences, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -120,7 +122,127 @@ def test_rope_by_axes_beyond_any_phase_still_turns():
     within(np.hypot(got[:, :32], got[:, 32:]), want, want * (HALF + 2.0 ** -15))
 
 
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("grouped", [0, 1])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,pairs", [
+    (2049, 3, 1, 128, 48), (4099, 3, 1, 128, 64), (4099, 2, 1, 64, 24), (4099, 2, 2, 90, 37), (2051, 1, 1, 256, 96), (4097, 1, 1, 24, 7),
+    (262151, 1, 1, 2, 1), (262146, 1, 1, 7, 3),
+])
+def test_rope_by_axes_of_rows_that_share_a_workgroup(rows, heads, kv_heads, dim, pairs, grouped, interleaved):
+    """Two or four rows of few heads at a time, the last ones fewer; a workgroup's second such rows, from 262144 rows on."""
+    print(f"[rope] {rows} {heads}/{kv_heads} {dim} {pairs} {grouped} {interleaved}", flush=True)
+    with Gpu() as g:
+        check_rope(g, rows, heads, kv_heads, dim, pairs, grouped=grouped, interleaved=interleaved, seed=dim)
+        check_rope(g, rows, heads, kv_heads, dim, pairs, axes=2, grouped=grouped, interleaved=interleaved, norm=False, seed=pairs)
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("dim,pairs,interleaved", [(136, 64, 0), (130, 45, 0), (130, 45, 1)])
+def test_rope_by_axes_of_more_rows_than_workgroups(dim, pairs, interleaved, norm):
+    """Workgroups that take a second row after their first. Sampled rows of both, the last ones among them."""
+    rows, heads, kv_heads, axes = 66001, 15, 1, 3
+    print(f"[rope] {rows} {dim} {pairs} {interleaved} {norm}", flush=True)
+    rng = np.random.RandomState(dim)
+    frequencies, axis = 10000.0 ** -rng.rand(pairs), rng.randint(0, axes, pairs)
+    positions = (rng.randint(-40, 40, (rows, axes)) * 0.37).astype(np.float32)
+    weights = [normal(dim, 3 + i) for i in range(2)] if norm else [None, None]
+    with Gpu() as g:
+        qkv, p, outs = g.empty(rows * 17 * dim), g.from_f32(positions), [g.empty(rows * n * dim) for n in (heads, kv_heads, kv_heads)]
+        w = [g.from_bf16(x).handle if norm else None for x in weights]
+        with rope_axes(g, list(frequencies), axis, axes, interleaved) as plan:
+            g.begin()
+            fill(g, qkv, 1, 2.0)
+            g.check(g.lib.h3_hip_qkv_rope_axes_bf16(g.handle, *(o.handle for o in outs), qkv.handle, *w, plan, p.handle, rows, heads,
+                                                    kv_heads, dim, 0, C.c_float(EPS)), "rope")
+            g.submit()
+        at = np.unique(np.concatenate([np.arange(64), rng.randint(0, rows, 500), np.arange(32900, 33100), np.arange(rows - 64, rows)]))
+        want = rope_reference(bf16(qkv.read().reshape(rows, 17, dim)[at]).astype(np.float64),
+                              [None if x is None else bf16(x).astype(np.float64) for x in weights], frequencies, axis, positions[at],
+                              heads, kv_heads, 0, interleaved)
+        for o, n, (y, bound) in zip(outs, (heads, kv_heads, kv_heads), want):
+            within(bf16(o.read().reshape(rows, n, dim)[at]), y, bound, (dim, n))
+
+
 # ------------------------------------------------------------------ adapters
+@pytest.mark.parametrize("rows,k,n,ranks", [(1500, 64, 6000, [16, 40, 128]), (3500, 72, 5999, [16, 40, 128]), (2900, 200, 5001, [70, 3])])
+def test_adapters_of_many_columns_a_workgroup(rows, k, n, ranks):
+    """Workgroups that go through 8 to 16 steps of 64 columns, the last one through fewer, in place too."""
+    print(f"[adapters] {rows}x{k}x{n} {ranks}", flush=True)
+    with Gpu() as g:
+        first = check_adapters(g, rows, k, n, ranks, seed=rows)
+        assert np.array_equal(check_adapters(g, rows, k, n, ranks, seed=rows, in_place=True), first)
+
+
+def test_adapters_of_the_most_columns_a_workgroup():
+    """32 steps of 64 columns: sampled rows have the bits that they get in a call of their own."""
+    rows, k, n, ranks = 17000, 64, 11999, [16, 40]
+    with Gpu() as g:
+        x, base, out = g.from_bf16(normal(rows * k, 1)), g.empty(rows * n), g.empty(rows * n)
+        at, ad = row_map(rows, 2, 5), Adapters(g, ranks, k, n)
+        some = np.unique(np.random.RandomState(2).randint(0, rows, 150))
+        with adapter_rows(g, at, 2, 40) as plan:
+            g.begin()
+            fill(g, base, 7)
+            g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, out.handle, base.handle, x.handle, ad.handle, plan, rows, k, n), "adapters")
+            g.submit()
+        few = [g.from_bf16(np.ascontiguousarray(t.read().reshape(rows, -1)[some])) for t in (base, x)]
+        got, own = out.read().reshape(rows, n)[some], g.empty(len(some) * n)
+        with adapter_rows(g, at[some], 2, 40) as plan:
+            g.begin()
+            g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, own.handle, few[0].handle, few[1].handle, ad.handle, plan, len(some), k, n))
+            g.submit()
+        assert np.array_equal(got, own.read().reshape(-1, n))
+        ad.close()
+
+
+def test_adapters_hand_their_first_product_on_in_two_roundings():
+    """base takes the rounded product away, so that what is left shows how the product was held: two BF16 values
+    leave 2^-17 of it, the second rounding of what the first, 2^-8, left."""
+    rows, k, n = 96, 64, 8
+    with Gpu() as g:
+        ad = Adapters(g, [1], k, n, scales=[1.0])
+        ad.set(0, b=np.full((n, 1), 0x3f80, np.uint16))
+        x = np.zeros((rows, k), np.uint16)
+        x[:, [3, 20, 61]] = normal(rows * 3, 4).reshape(rows, 3)
+        fx, fa = bf16(x).astype(np.float64), bf16(ad.a[0]).astype(np.float64)
+        t, size = fx @ fa.T, np.abs(fx) @ np.abs(fa).T
+        base = np.repeat(synth.f32_to_bf16(-t.astype(np.float32)), n, axis=1)
+        tx, tb, out = g.from_bf16(x), g.from_bf16(base), g.empty(rows * n)
+        with adapter_rows(g, [0] * rows, 1, 1) as plan:
+            g.begin()
+            g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, out.handle, tb.handle, tx.handle, ad.handle, plan, rows, k, n), "adapters")
+            g.submit()
+        want = t + bf16(base).astype(np.float64)
+        # Three exact products' sum, the scaling, the two values' sum and base's: FP32; one rounding to BF16.
+        bound = 2.0 ** -17 * np.abs(t) + 6 * F32 * size
+        within(bf16(out.read()).reshape(rows, n), want, bound + HALF * (np.abs(want) + bound))
+        ad.close()
+
+
+@pytest.mark.parametrize("mode", [1, 2], ids=["fp8", "nvfp4"])
+@pytest.mark.parametrize("rows", [1, 70, 300])
+def test_adapters_beside_packed_weights(mode, rows, tmp_path):
+    """Beside per-tensor FP8 and NVFP4 weights: the same bits as the two calls."""
+    k, n, ranks = 512, 1024, [16, 48]
+    write_weight(tmp_path / "w.bin", normal(n * k, 2, scale=0.05))
+    with Gpu() as g:
+        g.check(configure(g, tmp_path / "cache", mode=mode), "configure")
+        w, x, at = load(g, tmp_path / "w.bin", n, k, mode=mode), normal(rows * k, 1), row_map(rows, 2, 3)
+        tx, out, base, both = g.from_bf16(x), g.empty(rows * n), g.empty(rows * n), g.empty(rows * n)
+        ad = Adapters(g, ranks, k, n)
+        with adapter_rows(g, at, 2, 48) as plan:
+            g.begin()
+            g.check(g.lib.h3_hip_linear_adapters_bf16(g.handle, out.handle, tx.handle, w.handle, None, ad.handle, plan, rows, k, n), "linear")
+            g.check(g.lib.h3_gpu_linear_bf16(g.handle, base.handle, tx.handle, w.handle, None, rows, k, n))
+            g.check(g.lib.h3_hip_adapters_add_bf16(g.handle, both.handle, base.handle, tx.handle, ad.handle, plan, rows, k, n))
+            g.submit()
+        got = out.read()
+        assert np.array_equal(got, both.read())
+        fb = bf16(base.read()).astype(np.float64).reshape(rows, n)
+        within(bf16(got).reshape(rows, n), *ad.reference(bf16(x).astype(np.float64).reshape(rows, k), at, fb, np.zeros_like(fb)))
+        ad.close()
+
+
 @pytest.mark.parametrize("k", [4096, 4097])
 def test_projections_with_adapters_wait_for_streamed_rows_and_bias(k):
     """x of 32 MB and then the bias are on their way when the call is made, and are filled anew behind it."""
@@ -146,3 +268,37 @@ def test_projections_with_adapters_wait_for_streamed_rows_and_bias(k):
         for s in (sx, sb):
             s.close()
         ad.close()
+
+
+# ------------------------------------------------------------------ together
+@pytest.mark.parametrize("lengths", [(1,), (70, 1, 0, 133), (300, 260, 33)])
+def test_each_stage_of_a_step(lengths):
+    """Every value of every stage, against 64 bits of what the stage before it left."""
+    print(f"[step] {lengths}", flush=True)
+
+    def projected(x, w, n, adapters):
+        fx, fw = bf16(x).astype(np.float64).reshape(step.rows, -1), bf16(w.read()).astype(np.float64).reshape(n, -1)
+        base, sums = fx @ fw.T, (fw.shape[1] + 64) * F32 * (np.abs(fx) @ np.abs(fw).T)
+        return adapters.reference(fx, step.at, base, sums + HALF * (np.abs(base) + sums))
+
+    with Gpu() as g:
+        step = Step(g, lengths)
+        x = normal(step.rows * step.hidden, 5)
+        tx = g.from_bf16(x)
+        g.begin()
+        step.run(tx)
+        g.submit()
+        t = {name: v.read() for name, v in step.t.items()}
+        f = {name: bf16(v).astype(np.float64).reshape(step.rows, -1, 128) for name, v in t.items()}
+        within(f["qkv"].reshape(step.rows, -1), *projected(x, step.w[0], step.qkv_width, step.adapters[0]), "projection")
+        turned_parts = rope_reference(f["qkv"], [bf16(w.read()).astype(np.float64) for w in step.norms], 10000.0 ** -(np.arange(64) / 64),
+                                      np.array([0, 1] * 32), step.positions.read().reshape(-1, 2), step.heads, step.kv_heads, 0, 0)
+        for name, (want, bound) in zip("qkv", turned_parts):
+            within(f[name], want, bound, name)
+        ends = np.cumsum([0] + list(lengths))
+        for a, b in zip(ends, ends[1:]):
+            for h in range(step.heads if b > a else 0):
+                kv = h // (step.heads // step.kv_heads)
+                within(f["o"][a:b, h], *attention_reference(f["q"][a:b, h], f["k"][a:b, kv], f["v"][a:b, kv], SCALE), (a, h))
+        within(f["y"].reshape(step.rows, -1), *projected(t["o"], step.w[1], step.hidden, step.adapters[1]), "output")
+        step.close()
