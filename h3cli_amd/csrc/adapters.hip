@@ -3,7 +3,7 @@
 //   out[r, :] = base[r, :] + scale_a * (x[r, :] . A_a^T) . B_a^T,     a the adapter of row r
 //
 // A_a [rank_a, K], B_a [N, rank_a], ranks of their own. Two launches, for all adapters at once:
-//  * adapter_down: t = x . A^T in FP32, x read once;
+//  * adapter_down: t = x . A^T in FP32, x read once for each 64 ranks of the row's adapter;
 //  * adapter_up: out = base + scale * t . B^T, base read and out written once, whole rows.
 // Both are bound by memory: an adapter's flops per byte (rank / 2 of x, rank / 4 of base and out)
 // stay far below the matrix cores' share. The plan of the rows (h3_hip_adapter_rows_new) sorts
@@ -12,8 +12,8 @@
 // than their weights' reads.
 //
 // t enters the second product as two BF16 values, its rounding and what that left: with one,
-// the rounding of t would show in the output (2^-9 of the adapter's part), with two its error is
-// 2^-18 and the cost a second matrix instruction that memory hides.
+// the rounding of t would show in the output (2^-8 of the adapter's part), with two its error is
+// 2^-17 and the cost a second matrix instruction that memory hides.
 #include "common.h"
 #include "internal.h"
 #include <algorithm>
@@ -352,8 +352,9 @@ __global__ __launch_bounds__(256, 2) void adapter_up(AdapterArgs a) {
 // the rows' plan, so rows of any order) by 64 R columns, 32 R by 32 R each, and go through K
 // 64 channels at a time: x and W through two LDS buffers (16-byte chunks XOR-swizzled), the next
 // DEPTH steps' values on their way in registers. The adapters' ranks then continue the sum, each row block with
-// its adapter's. Bound by the chip's fill at small shapes and by the matrix cores and LDS alike
-// at large ones.
+// its adapter's. Bound by the chip's fill at small shapes. At large ones the waves wait for rows that
+// pass through registers, since their starts are aligned to two bytes only: 8000 rows, 5001 -> 5001,
+// matrix cores and LDS busy for 29% of the time each.
 // A compute unit takes in about 20 bytes a cycle of such rows, so few tiles over a long K are shared out
 // (part PRODUCT: a share of K, its sums to memory; then part REST: the shares added in order, and
 // what follows them). The adapters' first product needs nothing of it and is part of PRODUCT's launch,
@@ -798,9 +799,12 @@ extern "C" int h3_hip_linear_adapters_bf16(h3_gpu *g, h3_gpu_tensor *out, const 
                                            const h3_gpu_tensor *bias, const h3_hip_adapters *w, const h3_hip_adapter_rows *p,
                                            uint32_t rows, uint32_t k, uint32_t n) {
     if (!h3_launch_ready(g) || !adapters_valid(g, w, p, rows, k, n)) return 0;
-    // The tiled projections take a K of whole 64-channel steps, the others would be gemm_small's, on the
-    // vector units. With the adapters: 301 rows, 1001 -> 777: 12.5 us, by gemm_small 140; 8000 rows, 5001 ->
-    // 5001: 740 us, 541 TFLOP/s. Tiles of 64 rows by 64 columns where the large ones would fill few
+    // The tiled projections take a K of whole 64-channel steps and weights of any type. They write BF16, so
+    // that the adapters' parts are added to a rounded sum: one rounding more, 2^-8 of the projection (8193 rows, 7168
+    // -> 5376: off by 0.0020 of the result, in one sum 0.0017), for the bits of the projection and
+    // h3_hip_adapters_add_bf16 called in turn, whatever the weight's type. Any other K would be gemm_small's, on the
+    // vector units, and is adapter_gemm's in one sum. With the adapters: 301 rows, 1001 -> 777: 12.5 us, by
+    // gemm_small 140; 8000 rows, 5001 -> 5001: 690-740 us, 541-581 TFLOP/s. Tiles of 64 rows by 64 columns where the large ones would fill few
     // compute units: 600 rows, 2001 -> 3001: 41 us (large 50), 800 rows: 55 (50), 1200 rows, 3001 ->
     // 3001: 93 (65).
     if (!h3_require(g, in, H3_GPU_BF16, (size_t)rows * k, "linear input") ||

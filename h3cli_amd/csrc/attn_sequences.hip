@@ -1,8 +1,9 @@
 // BF16 attention of packed sequences (D = 128, non-causal): query rows [q0, q0 + lq) of a
 // sequence attend to its key rows [k0, k0 + lk), for all sequences in one call
 // (h3_hip_sdpa_sequences_bf16). Semantics as attn_bf16.hip: softmax(scale * Q K^T) V with FP32
-// scores, running max and sums, P rounded to BF16 for P.V, FP32 accumulation, BF16 output; a
-// query of a sequence without keys gets zeros.
+// scores, running max and sums, P rounded to BF16 for P.V (as the matrix instructions take it: results are
+// off by 0.0018 to 0.0023 of their size, of which BF16's own rounding is 0.0017), FP32 accumulation, BF16
+// output; a query of a sequence without keys gets zeros.
 //
 // Query heads that share a key head are rows of one tile: row v of (sequence, key head) is
 // query v / share of head share * key head + v % share, so that a key tile is read once for

@@ -234,9 +234,10 @@ int h3_hip_add_rms_norm_fp8_block(h3_gpu *gpu, h3_gpu_tensor *sum, h3_gpu_tensor
  * Projections, norms and gates take such rows as they are; these operators know
  * whose they are. Plans hold what the operators read on the device, and the
  * workspace of their calls: they allocate nothing (but for what a projection
- * beside adapters takes by itself) and may be captured into a graph. Inputs that are
- * being filled from a file or host memory are waited for. A plan serves any number of calls in turn, not two at once (calls of
- * two streams, say), and is freed before its context.
+ * beside adapters takes by itself) and may be captured into a graph. Inputs that
+ * are being filled from a file or host memory are waited for. A plan serves any
+ * number of calls in turn, not two at once (calls of two streams, say), and is
+ * freed before its context.
  *
  * Sequence i of `count` has the query rows [q_offsets[i], q_offsets[i + 1]) and
  * the key rows [k_offsets[i], k_offsets[i + 1]) (NULL: as the queries); either
